@@ -1130,7 +1130,7 @@ uint64_t kvrt_capabilities(void) {
     return KVRT_CAP_CONTIG | KVRT_CAP_RING | KVRT_CAP_PAGED | KVRT_CAP_INT8 | KVRT_CAP_FUSED_APPEND_ATTEND |
            KVRT_CAP_GATHER | KVRT_CAP_DEVICE_LENGTHS | KVRT_CAP_TENSOR_ATTEND | KVRT_CAP_PREFILL_MFMA |
            KVRT_CAP_TALKER_MASK | KVRT_CAP_PREFIX_ATTENTION | KVRT_CAP_SLOT_GENERATION | KVRT_CAP_STREAM_CONFINED |
-           KVRT_CAP_ROLLBACK_POSITION;
+           KVRT_CAP_ROLLBACK_POSITION | KVRT_CAP_BLOCK8;
 }
 
 const char *kvrt_strerror(int code) {

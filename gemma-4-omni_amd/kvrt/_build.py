@@ -1,7 +1,8 @@
 """Build libkvrt.so (gfx950) in-tree with hipcc.
 
 The library is compiled from ``csrc/kvrt_kernels.hip`` (kernels),
-``csrc/kvrt_prefill.hip`` and ``csrc/kvrt_prefill_wide.hip`` (chunked prefill)
+``csrc/kvrt_prefill.hip`` and ``csrc/kvrt_prefill_wide.hip`` (chunked prefill),
+``csrc/kvrt_block8.hip`` and ``csrc/kvrt_block8_attend.hip`` (8-bit pages)
 and ``csrc/kvrt_runtime.hip`` (host runtime, C ABI in ``include/kvrt.h``);
 kvrt_pycall.so, the calls that read torch tensors directly, from
 ``csrc/kvrt_pycall.cpp`` with the host compiler. The build also compiles
@@ -26,7 +27,8 @@ CSRC = PKG_DIR.parent / "csrc"
 INCLUDE = PKG_DIR.parent.parent / "include"
 LIB_PATH = PKG_DIR / "libkvrt.so"
 CALLS_PATH = PKG_DIR / "kvrt_pycall.so"
-SOURCES = ("kvrt_kernels.hip", "kvrt_prefill.hip", "kvrt_prefill_wide.hip", "kvrt_prefill_short.hip", "kvrt_runtime.hip")
+SOURCES = ("kvrt_kernels.hip", "kvrt_prefill.hip", "kvrt_prefill_wide.hip", "kvrt_prefill_short.hip", "kvrt_runtime.hip",
+           "kvrt_block8.hip", "kvrt_block8_attend.hip")
 
 AGPR_SOURCES = ("kvrt_prefill_wide.hip",)
 

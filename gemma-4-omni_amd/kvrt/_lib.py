@@ -38,6 +38,7 @@ DT_FP32 = 2
 DT_BOOL = 3
 DT_INT32 = 4
 DT_INT64 = 5
+DT_E4M3 = 6
 
 CAP_CONTIG = 1 << 0
 CAP_RING = 1 << 1
@@ -53,6 +54,17 @@ CAP_PREFIX_ATTENTION = 1 << 10
 CAP_SLOT_GENERATION = 1 << 11
 CAP_STREAM_CONFINED = 1 << 12
 CAP_ROLLBACK_POSITION = 1 << 13
+CAP_BLOCK8 = 1 << 14
+
+# bits of the status word of 8-bit pages and their tables (kvrt.h KVRT_BLOCK_*)
+BLOCK_BAD_INDEX = 1
+BLOCK_NO_PAGES = 2
+BLOCK_NOT_FINITE = 4
+
+
+def block_tables_work(n: int) -> int:
+    """KVRT_BLOCK_TABLES_WORK(n)."""
+    return 4 * n + 8
 
 
 class KvrtTensor(ctypes.Structure):
@@ -144,9 +156,41 @@ class KvrtTalkerMask(ctypes.Structure):
     ]
 
 
+class KvrtBlock8(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("k_scale", c_void_p),
+        ("v_scale", c_void_p),
+        ("status", c_void_p),
+        ("dtype", c_int32),
+        ("pages", c_int32),
+        ("kv_heads", c_int32),
+        ("block", c_int32),
+        ("head_dim", c_int32),
+        ("reserved", c_int32),
+    ]
+
+
+class KvrtBlockTables(ctypes.Structure):
+    _fields_ = [
+        ("table", c_void_p),
+        ("mapped", c_void_p),
+        ("free_pages", c_void_p),
+        ("free_count", c_void_p),
+        ("work", c_void_p),
+        ("status", c_void_p),
+        ("n", c_int32),
+        ("max_pages", c_int32),
+        ("pool_pages", c_int32),
+        ("block", c_int32),
+    ]
+
+
 # (name, restype, argtypes) of every symbol declared in include/kvrt.h.
 _T = POINTER(KvrtTensor)
 _I32P = POINTER(c_int32)
+_B8 = POINTER(KvrtBlock8)
 SIGNATURES = [
     ("kvrt_abi_version", c_uint32, []),
     ("kvrt_capabilities", c_uint64, []),
@@ -185,6 +229,13 @@ SIGNATURES = [
     ("kvrt_attend_tensors_noalloc_async", c_int32, [_T, _T, _T, c_void_p, _T, _T, c_float, c_int32, c_void_p]),
     ("kvrt_tensors_status", c_int32, [c_void_p]),
     ("kvrt_copy_rows_async", c_int32, [_T, _T, c_int64, c_void_p]),
+    ("kvrt_block_tables_update_async", c_int32,
+     [POINTER(KvrtBlockTables), c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    ("kvrt_block8_append_async", c_int32, [_B8, _T, _T, c_void_p, c_void_p]),
+    ("kvrt_block8_gather_async", c_int32, [_B8, _T, c_void_p, c_void_p, _T, _T, _T, c_void_p]),
+    ("kvrt_block8_attend_async", c_int32,
+     [_B8, _T, _T, c_void_p, c_void_p, c_void_p, _T, c_float, c_int32, c_int32, c_void_p, c_uint64, c_void_p]),
+    ("kvrt_block8_attend_work", c_uint64, [_B8, c_int64, c_int64, c_int64, c_int32]),
     ("kvrt_session_state", c_int32, [c_void_p, c_int32, c_int32, _I32P]),
     ("kvrt_sync_lengths", c_int32, [c_void_p]),
     ("kvrt_get_counters", c_int32, [c_void_p, POINTER(KvrtCounters)]),

@@ -79,6 +79,7 @@ extern "C" {
 #define KVRT_CAP_SLOT_GENERATION (1ull << 11)
 #define KVRT_CAP_STREAM_CONFINED (1ull << 12)
 #define KVRT_CAP_ROLLBACK_POSITION (1ull << 13) /* truncate checks expected_len; import refuses live slots */
+#define KVRT_CAP_BLOCK8 (1ull << 14) /* 8-bit pages with a scale per page and head, tables built on the GPU */
 
 /* ---- enums ------------------------------------------------------------- */
 enum kvrt_layout {
@@ -94,6 +95,7 @@ enum kvrt_dtype {
     KVRT_BOOL = 3, /* 1 byte: 0 / 1 */
     KVRT_INT32 = 4,
     KVRT_INT64 = 5,
+    KVRT_E4M3 = 6, /* OCP fp8, 3 mantissa bits; codes of kvrt_block8 pages only */
 };
 
 /* ---- descriptors --------------------------------------------------------- */
@@ -622,6 +624,119 @@ int kvrt_tensors_status(void *hip_stream);
  * (duplex_kernel/thinker_cache.py:164-170). */
 int kvrt_copy_rows_async(const kvrt_tensor *src, const kvrt_tensor *dst, int64_t rows,
                          void *hip_stream);
+
+/* ---- 8-bit pages with a scale per page and head ------------------------------- */
+/* Caller-owned pages of one layer. Codes are int8 in [-127, 127] or e4m3, and a
+ * code stands for code * scale with one fp32 scale per (page, KV head). A scale
+ * is read as within [2^-64, 2^32]. Every layer of a model has pages of its own;
+ * one page table serves all of them. The calls below are context-free: they
+ * run on the current device and the given stream, allocate nothing, return
+ * KVRT_EINVAL (nothing enqueued) for arguments they do not take and
+ * KVRT_EDEVICE when the launch fails. What only the device can see (a page id
+ * or slot outside the pool, a length outside the table) raises a bit of
+ * *status and is skipped: no access leaves the buffers. */
+typedef struct kvrt_block8 {
+    void *k, *v;              /* codes [pages, kv_heads, block, head_dim], 16-byte aligned  */
+    float *k_scale, *v_scale; /* [pages, kv_heads]                                          */
+    int32_t *status;          /* device word, KVRT_BLOCK_* bits or'ed in                    */
+    int32_t dtype;            /* KVRT_INT8 or KVRT_E4M3                                     */
+    int32_t pages;            /* pages * kv_heads * block < 2^31                            */
+    int32_t kv_heads;         /* 1..64                                                      */
+    int32_t block;            /* tokens per page: 16, 32, 64 or 128                         */
+    int32_t head_dim;         /* 64, 128, 256 or 512                                        */
+    int32_t reserved;
+} kvrt_block8;
+
+/* Page tables of n requests and the pages none of them holds. */
+typedef struct kvrt_block_tables {
+    int32_t *table;      /* [n, max_pages]: page ids of a request's mapped pages, -1 after */
+    int32_t *mapped;     /* [n]: mapped pages of each request                              */
+    int32_t *free_pages; /* [pool_pages]: free page ids, the next one taken last           */
+    int32_t *free_count; /* [1]                                                            */
+    int32_t *work;       /* [KVRT_BLOCK_TABLES_WORK(n)]: scratch of the calls              */
+    int32_t *status;     /* device word, KVRT_BLOCK_* bits or'ed in                        */
+    int32_t n;           /* 1..65536                                                       */
+    int32_t max_pages;   /* n * max_pages and max_pages * block < 2^31                     */
+    int32_t pool_pages;  /* pool_pages * block < 2^31                                      */
+    int32_t block;       /* tokens per page: 16, 32, 64 or 128                             */
+} kvrt_block_tables;
+#define KVRT_BLOCK_TABLES_WORK(n) (4 * (n) + 8)
+
+#define KVRT_BLOCK_BAD_INDEX 1 /* a page id, slot, length or row count outside its range: skipped    */
+#define KVRT_BLOCK_NO_PAGES 2  /* a request was not granted its rows: the pool ran out of pages      */
+#define KVRT_BLOCK_NOT_FINITE 4 /* an appended value was not finite: NaN stored as 0, infinities as
+                                  the largest code                                               */
+
+/* Brings the tables to a step's lengths, on the GPU and without reading anything
+ * back: request i keeps its first lengths[i] rows and takes new_rows[i] more.
+ * Pages past both are released, then pages are mapped for the new rows; in
+ * request order, the last page released is the first one taken again. A request
+ * whose new pages are no longer there is refused (KVRT_BLOCK_NO_PAGES): it keeps
+ * the pages it has and is granted no row; requests after it that need no page
+ * are still served. A request is also refused (KVRT_BLOCK_BAD_INDEX) where lengths[i] or
+ * new_rows[i] is negative, lengths[i] rows are not mapped, both exceed
+ * max_pages pages, or its new rows end past `rows`.
+ *   starts[n + 1]    first packed row of each request's new rows: running sums of
+ *                    new_rows (negative ones as 0), at most rows
+ *   slot_map[rows]   page * block + offset of each packed row; -1 where it belongs
+ *                    to a refused request or lies behind the last one's
+ *   out_lengths[n]   lengths[i] + granted[i] (a refused request: lengths[i],
+ *                    brought into its mapped pages)
+ *   granted[n]       new_rows[i], or 0 where the request was refused
+ * One or two launches; a captured call replays on the lengths it then finds.
+ * lengths and out_lengths may be the same array. The reference holds no paged
+ * KV; the host-built page tables of a context are the counterpart here. */
+int kvrt_block_tables_update_async(const kvrt_block_tables *tables, const int32_t *lengths,
+                                   const int32_t *new_rows, int64_t rows, int32_t *starts, int32_t *slot_map,
+                                   int32_t *out_lengths, int32_t *granted, void *hip_stream);
+
+/* Codes rows into their pages: k, v [T, kv_heads, head_dim] bf16 (last dim
+ * contiguous, 16-byte aligned rows), row t into slot slot_map[t] (device int32
+ * [T]; negative: skipped). Rows of consecutive slots within one page are a run;
+ * a run extends its page: rows before it in the page stay, rows behind it are
+ * dropped. The page's scale becomes
+ *   s' = max(s if the run starts past the page's first row, amax / top)
+ * clamped to [2^-64, 2^32], amax the largest finite magnitude of the run's rows
+ * of the head, top 127 (int8) or 448 (e4m3). A new code is x * (1 / s') and,
+ * where s' > s, each code before the run becomes code * (s / s'), both rounded
+ * to the nearest code (ties to even) and clamped to the largest. A page takes
+ * one run per call: slots that put two runs into one page (or name one slot
+ * twice) leave that page's rows undefined. Counterpart of kvrt_append_async's
+ * in-kernel quantisation (one scale per token and head there). */
+int kvrt_block8_append_async(const kvrt_block8 *pages, const kvrt_tensor *k, const kvrt_tensor *v,
+                             const int32_t *slot_map, void *hip_stream);
+
+/* The zero-padded batch of n requests: out_k, out_v [n, kv_heads, Lmax, head_dim],
+ * KVRT_BF16 or KVRT_FP32 (last dim contiguous, 16-byte aligned rows); row j of
+ * request i is position start_pos[i] + j (start_pos device int32 [n], or NULL
+ * for 0; a negative one is a bad index) while that lies below lengths[i],
+ * zeros after. table: KVRT_INT32 [n, width]; mask [n, Lmax] as for
+ * kvrt_gather_async, or NULL. Counterpart of kvrt_gather_async. */
+int kvrt_block8_gather_async(const kvrt_block8 *pages, const kvrt_tensor *table, const int32_t *lengths,
+                             const int32_t *start_pos, const kvrt_tensor *out_k, const kvrt_tensor *out_v,
+                             const kvrt_tensor *mask, void *hip_stream);
+
+/* Attention of packed query rows over coded pages: q, out [T, Hq, head_dim] bf16
+ * (last dim contiguous, 16-byte aligned rows; q and out do not overlap), request
+ * i's rows being starts[i] .. starts[i] + m - 1 with m = granted[i], or
+ * starts[i + 1] - starts[i] where granted is NULL; m <= max_q. Its row r sits at
+ * position p = lengths[i] - m + r and sees keys k <= p, k < lengths[i], and with
+ * window W > 0 only k > p - W; a row that sees none is written as zeros. q head
+ * h reads KV head h / (Hq / kv_heads); Hq / kv_heads <= 64. Rows of out that
+ * belong to no request are left as they were. table: KVRT_INT32 [n, width];
+ * lengths, starts [n + 1], granted: device int32. Codes enter the matrix
+ * products exactly, query rows to 2^-24 of a row's largest element, weights
+ * rounded to fp16; scores, softmax and sums in fp32. Up to 16 query rows per KV
+ * head ((Hq / kv_heads) * max_q) the keys of all requests are divided evenly
+ * over the workgroups (a decode step). work: work_bytes >= kvrt_block8_attend_work device
+ * bytes, 16-byte aligned; calls that may overlap need one each. Counterpart of
+ * kvrt_attend_tensors_async and kvrt_attend_prefill_async. */
+int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, const kvrt_tensor *table,
+                             const int32_t *lengths, const int32_t *starts, const int32_t *granted,
+                             const kvrt_tensor *out, float scale, int32_t window, int32_t max_q, void *work,
+                             uint64_t work_bytes, void *hip_stream);
+/* Bytes of kvrt_block8_attend_async's work for these arguments (0: none). */
+uint64_t kvrt_block8_attend_work(const kvrt_block8 *pages, int64_t n, int64_t width, int64_t hq, int32_t max_q);
 
 /* ---- state / diagnostics ----------------------------------------------------- */
 /* Host-authoritative length of (slot, layer). Replaces
