@@ -60,15 +60,22 @@ struct Block8AttendArgs {
     int64_t table_stride, rows;            // packed rows of q
     int n, width, group, max_q, window;
     int wgs;                               // workgroups the keys are divided over (each row tile)
+    int join_most;                         // partials of a head joined inside the launch (others: a second one)
+    int join_all;                          // divide so that every head's are
     float scale_log2;                      // scale * log2(e)
-    float *part_o;                         // partials of divided rows [tile][wg][2][D / 16][64] float4
+    float *part_o;                         // partials of divided heads [tile][wg][2][16 rows][D]
     float2 *part_ml;                       // their (max, sum) [tile][wg][2][16]
+    uint32_t *counters;                    // arrivals [wg], zero between launches
 };
+
+constexpr int kBlock8MaxWgs = 1024;  // workgroups the keys are divided over, at most
 
 hipError_t launch_block8_tables(const Block8TablesArgs &a, hipStream_t s);
 hipError_t launch_block8_append(const Block8AppendArgs &a, int dtype, int head_dim, hipStream_t s);
 hipError_t launch_block8_gather(const Block8GatherArgs &a, int dtype, int head_dim, hipStream_t s);
-hipError_t launch_block8_attend(const Block8AttendArgs &a, int dtype, int head_dim, int tiles, hipStream_t s);
+hipError_t launch_block8_attend(const Block8AttendArgs &a, int dtype, int head_dim, int tiles, bool join, hipStream_t s);
+// kBlock8MaxWgs zeroed arrival counters for a call on that stream; nullptr: none left.
+uint32_t *block8_counter_slice(hipStream_t s);
 
 // ---- codes ----------------------------------------------------------------------
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));

@@ -471,13 +471,17 @@ static bool table_ok(const kvrt_tensor *t, int shift, int64_t &n, int64_t &width
     return n <= 65535 && (width << shift) < (int64_t)1 << 31;
 }
 
-constexpr int64_t kMaxRows = (int64_t)1 << 30;
+constexpr int64_t kMaxRows = (int64_t)1 << 30, kJoinBytes = 48 << 10;
 
-// Workgroups the keys of a call are divided over, for each of its row tiles.
-static int attend_wgs(const Block8View &v, int64_t n, int64_t width, int tiles) {
-    const int64_t units = n * v.kv_heads * (((width << v.shift) + 127) / 128);
-    const int64_t most = std::max<int64_t>(1, 1024 / tiles);
-    return (int)std::max<int64_t>(1, std::min(units, most));
+// Units of 128 keys that a head of one request has at most.
+static int64_t most_units(const Block8View &v, int64_t width) { return ((width << v.shift) + 127) / 128 + 1; }
+
+// Workgroups the keys of a call are divided over, for each of its row tiles: those
+// that run at a time (their registers allow 4, 3, 2 and 1 per CU).
+static int attend_wgs(const Block8View &v, int64_t n, int64_t width, int tiles, int head_dim) {
+    const int64_t round = 256 * (head_dim == 64 ? 4 : head_dim == 128 ? 3 : head_dim == 256 ? 2 : 1);
+    const int64_t units = n * v.kv_heads * most_units(v, width);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(units, round / tiles));
 }
 static int attend_tiles(int64_t group, int64_t max_q) { return (int)std::min<int64_t>((group * max_q + 15) / 16, 65535); }
 // Partials of rows whose keys several workgroups share: none where one has them all.
@@ -582,7 +586,7 @@ uint64_t kvrt_block8_attend_work(const kvrt_block8 *pages, int64_t n, int64_t wi
     Block8View v;
     if (!view_of(pages, v) || n <= 0 || width <= 0 || hq <= 0 || hq % pages->kv_heads != 0 || max_q <= 0) return 0;
     const int tiles = attend_tiles(hq / pages->kv_heads, max_q);
-    return part_bytes(part_rows(tiles, attend_wgs(v, n, width, tiles)), pages->head_dim);
+    return part_bytes(part_rows(tiles, attend_wgs(v, n, width, tiles, pages->head_dim)), pages->head_dim);
 }
 
 int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, const kvrt_tensor *table,
@@ -606,7 +610,9 @@ int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, con
         return KVRT_EINVAL;
     a.group = (int)(hq / pages->kv_heads);
     const int tiles = attend_tiles(a.group, max_q);
-    a.wgs = attend_wgs(a.p, n, std::max<int64_t>(width, 1), tiles);
+    const int64_t most = most_units(a.p, std::max<int64_t>(width, 1)), heads = n * pages->kv_heads;
+    if (most * heads >= (int64_t)1 << 31) return KVRT_EINVAL;  // units are numbered in 32 bits
+    a.wgs = attend_wgs(a.p, n, std::max<int64_t>(width, 1), tiles, pages->head_dim);
     const uint64_t prows = part_rows(tiles, a.wgs);
     if (prows > 0 && (!aligned(work, 16) || work_bytes < part_bytes(prows, pages->head_dim))) return KVRT_EINVAL;
     a.part_o = static_cast<float *>(work);
@@ -628,8 +634,20 @@ int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, con
     a.max_q = max_q;
     a.window = window;
     a.scale_log2 = scale * 1.4426950408889634f;
-    const hipError_t e =
-        launch_block8_attend(a, pages->dtype, pages->head_dim, tiles, static_cast<hipStream_t>(stream));
+    // Joined inside the launch: heads whose partials the last workgroup reads in a few
+    // loads. Where that many workgroups per head fill the card, or a head never has
+    // more, all are; else a second launch joins the others.
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    bool join = false;
+    if (a.wgs > 1) {
+        const int64_t rows = std::min<int64_t>(16, (int64_t)a.group * max_q);
+        a.join_most = (int)std::min<int64_t>(32, kJoinBytes / (rows * pages->head_dim * 4));
+        a.counters = tiles == 1 && a.join_most > 1 ? block8_counter_slice(st) : nullptr;
+        if (!a.counters) a.join_most = 1;
+        a.join_all = most > a.join_most && heads * (a.join_most - 1) >= 512;
+        join = most > a.join_most && !a.join_all;
+    }
+    const hipError_t e = launch_block8_attend(a, pages->dtype, pages->head_dim, tiles, join, st);
     return e == hipSuccess ? KVRT_OK : KVRT_EDEVICE;
 }
 

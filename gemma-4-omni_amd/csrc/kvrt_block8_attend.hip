@@ -20,6 +20,11 @@
 // ordered in P V so that a lane's own weights are its operand: k = 8(l/16)+j is key
 // 16(j/4) + 4(l/16) + j%4. V is read row by row, D/16 bytes per lane, and
 // transposed in registers by byte permutes.
+#include <algorithm>
+#include <map>
+#include <mutex>
+#include <utility>
+
 #include "kvrt_block8.h"
 
 namespace kvrt {
@@ -39,84 +44,119 @@ struct Rows {
     int kstart;
 };
 
-__device__ __forceinline__ Rows rows_of(const Block8AttendArgs &a, int i, int tile, bool &bad) {
+__device__ __forceinline__ Rows rows_of(const Block8AttendArgs &a, int start, int count, int length, int tile) {
     Rows r;
-    const int cap = a.width << a.p.shift;
-    const int len = a.lengths[i], s0 = a.starts[i];
-    const int64_t m = a.granted ? (int64_t)a.granted[i] : (int64_t)a.starts[i + 1] - s0;
-    r.length = min(max(len, 0), cap);
-    r.start = (int)min((int64_t)max(s0, 0), a.rows);
-    r.count = (int)min(min(max(m, (int64_t)0), (int64_t)a.max_q), a.rows - r.start);
-    bad |= r.length != len || r.start != s0 || r.count != m;
-    const int all = r.count * a.group;
-    r.n = min(max(all - 16 * tile, 0), 16);
-    const int base = r.length - r.count;  // below 0: rows before the first key see nothing
+    r.start = start;
+    r.count = count;
+    r.length = length;
+    r.n = min(max(count * a.group - 16 * tile, 0), 16);
+    const int base = length - count;  // below 0: rows before the first key see nothing
     r.first = base + 16 * tile / a.group;
     r.last = base + (16 * tile + max(r.n, 1) - 1) / a.group;
-    r.kend = r.n > 0 ? min(max(r.last + 1, 0), r.length) : 0;
+    r.kend = r.n > 0 ? min(max(r.last + 1, 0), length) : 0;
     r.kstart = a.window > 0 ? min(max(r.first - a.window + 1, 0), r.kend) : 0;
     return r;
 }
-__device__ __forceinline__ int tiles_of(const Rows &r) {
-    return (r.kend + kTileKeys - 1) / kTileKeys - r.kstart / kTileKeys;
+// Request i from its words; what is out of range is brought into it and reported.
+__device__ __forceinline__ Rows load_rows(const Block8AttendArgs &a, int i, int tile, bool &bad) {
+    const int cap = a.width << a.p.shift;
+    const int len = a.lengths[i], s0 = a.starts[i];
+    const int64_t m = a.granted ? (int64_t)a.granted[i] : (int64_t)a.starts[i + 1] - s0;
+    const int length = min(max(len, 0), cap);
+    const int start = (int)min((int64_t)max(s0, 0), a.rows);
+    const int count = (int)min(min(max(m, (int64_t)0), (int64_t)a.max_q), a.rows - start);
+    bad |= length != len || start != s0 || count != m;
+    return rows_of(a, start, count, length, tile);
 }
-// Rows without keys are one unit too: their zeros have to be written.
+// Units of a head of the request. Rows without keys are one too: their zeros have to
+// be written.
 __device__ __forceinline__ int units_of(const Rows &r) {
-    return r.n == 0 ? 0 : max(1, (tiles_of(r) + kUnitTiles - 1) / kUnitTiles);
+    const int tiles = (r.kend + kTileKeys - 1) / kTileKeys - r.kstart / kTileKeys;
+    return r.n == 0 ? 0 : max(1, (tiles + kUnitTiles - 1) / kUnitTiles);
 }
 
-// Running sum over the workgroup's 256 threads (exclusive) and the total.
-__device__ __forceinline__ int64_t scan256(int64_t x, int64_t *lds, int64_t &total) {
+// How the units of all requests' heads (request, head, unit order) are divided:
+// workgroup w has units [w * per, (w + 1) * per). The host keeps their number
+// below 2^31.
+struct Division {
+    int total, per;
+};
+__device__ __forceinline__ Division divide(const Block8AttendArgs &a, int units, int most) {
+    Division d;
+    d.total = units * a.p.kv_heads;
+    d.per = (d.total + a.wgs - 1) / a.wgs;
+    // all joined in the launch: n units in a row lie over at most (n - 1) / per + 2
+    // workgroups, no head's over more than one joins (join_most >= 2)
+    if (a.join_all) d.per = max(d.per, (most + a.join_most - 2) / (a.join_most - 1));
+    return d;
+}
+
+// Running sum over the workgroup's 256 threads (exclusive), the sum and the largest.
+__device__ __forceinline__ int scan256(int x, int *lds, int &total, int &most) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t inc = x;
+    int inc = x, top = x;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int64_t y = __shfl_up(inc, d);
+        const int y = __shfl_up(inc, d);
         if (lane >= d) inc += y;
+        top = max(top, __shfl_xor(top, d));
     }
     __syncthreads();
-    if (lane == 63) lds[wave] = inc;
+    if (lane == 63) lds[wave] = inc, lds[4 + wave] = top;
     __syncthreads();
-    int64_t before = 0;
-    total = 0;
+    int before = 0;
+    total = 0, most = 0;
+#pragma unroll
     for (int w = 0; w < 4; ++w) {
         if (w < wave) before += lds[w];
         total += lds[w];
+        most = max(most, lds[4 + w]);
     }
     return before + inc - x;
 }
 
-// The units of all requests' heads for one row tile, in request, head, unit order.
-__device__ __forceinline__ int64_t units_total(const Block8AttendArgs &a, int tile, int64_t *lds, bool &bad) {
-    int64_t all = 0;
-    for (int base = 0; base < a.n; base += 256) {
-        const int i = base + threadIdx.x;
-        int64_t sum;
-        scan256(i < a.n ? units_of(rows_of(a, i, tile, bad)) : 0, lds, sum);
-        all += sum;
-    }
-    return all * a.p.kv_heads;
-}
-// The request of unit u and the units before it. Every thread of the workgroup calls.
-__device__ __forceinline__ void request_at(const Block8AttendArgs &a, int tile, int64_t u, int64_t *lds, int &req,
-                                           int64_t &before) {
-    bool bad = false;
-    int64_t all = 0;
-    __shared__ int64_t found[2];
-    for (int base = 0; base < a.n; base += 256) {
-        const int i = base + threadIdx.x;
-        const int64_t mine = i < a.n ? (int64_t)units_of(rows_of(a, i, tile, bad)) * a.p.kv_heads : 0;
-        int64_t sum;
-        const int64_t at = all + scan256(mine, lds, sum);
-        all += sum;
-        if (at <= u && u < at + mine) {
-            found[0] = i;
-            found[1] = at;
+// Keys' words that nothing in the launch writes: uniform ones load as scalars.
+typedef const __attribute__((address_space(4))) int32_t *ConstInts;
+typedef const __attribute__((address_space(4))) float *ConstFloats;
+
+// Joins partials p = 0 .. n - 1 of four output elements of a row, in their order,
+// sixteen at a time: ld(p, ml, o) reads one. The launch that makes the partials and
+// the join kernel both use it, so both give the same bits.
+template <class Ld>
+__device__ __forceinline__ void join_partials(int n, Ld ld, float &M, float &sum, float4 &o) {
+    constexpr int B = 16;
+    for (int p0 = 0; p0 < n; p0 += B) {
+        float2 ml[B];
+        float4 x[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            ml[i] = make_float2(kNegBig, 0.f);
+            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (p0 + i < n) ld(p0 + i, ml[i], x[i]);
+        }
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < B; ++i) top = fmaxf(top, ml[i].x);
+        const float c = __builtin_amdgcn_exp2f(M - top);
+        sum *= c;
+        o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
+        M = top;
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - M);
+            sum = fmaf(ml[i].y, f, sum);
+            o = make_float4(fmaf(x[i].x, f, o.x), fmaf(x[i].y, f, o.y), fmaf(x[i].z, f, o.z), fmaf(x[i].w, f, o.w));
         }
     }
-    __syncthreads();
-    req = __builtin_amdgcn_readfirstlane((int)found[0]);
-    before = found[1];
+}
+
+// Four elements of a row of the answer: dims d .. d + 3 of row `row` of the head.
+__device__ __forceinline__ void store_out(const Block8AttendArgs &a, const Rows &r, int head, int row, int d, float4 o,
+                                          float sum) {
+    const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+    const int qr = row / a.group, hr = row - qr * a.group;
+    uint16_t *out = a.out + (int64_t)(r.start + qr) * a.o_row + (int64_t)(head * a.group + hr) * a.o_head + d;
+    *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
 }
 
 // N dwords of a lane from p (N = 1, 2, 4, 8; p aligned to min(4 N, 16) bytes).
@@ -185,41 +225,100 @@ __device__ __forceinline__ void load_query(const uint16_t *row, bool valid, uint
 
 template <int CODE, int D>
 __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) {
-    constexpr int NB = D / 16;   // 16-dim blocks of the output
-    constexpr int KC = D / 64;   // 16-byte chunks of a key row per lane
-    constexpr int VW = D / 64;   // dwords of a V row per lane
-    __shared__ float4 so[4 * NB * 64];
+    constexpr int NB = D / 16;    // 16-dim blocks of the output
+    constexpr int KC = D / 64;    // 16-byte chunks of a key row per lane
+    constexpr int VW = D / 64;    // dwords of a V row per lane
+    constexpr int PITCH = D + 4;  // floats of an output row in LDS: 16 rows on 16 different bank quadruples
+    __shared__ __align__(16) float so[4 * 16 * PITCH];
     __shared__ float2 sml[4 * 16];
-    __shared__ int64_t scan_lds[4];
+    __shared__ int scan_lds[8], found[2];
+    __shared__ uint32_t arrived;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
     const int tile = blockIdx.y, wg = blockIdx.x;
-    bool bad = false;
-    const int64_t total = units_total(a, tile, scan_lds, bad);
+
+    // this workgroup's units [u, uend), the request of the first and the units before it
+    bool bad = false, unmapped = false;
+    Division div;
+    int req, before, u;
+    Rows mine{};  // of request `lane`, where there are at most 64
+    if (a.n <= 64) {
+        int units = 0;
+        if (lane < a.n) {
+            mine = load_rows(a, lane, tile, bad);
+            units = units_of(mine);
+        }
+        int inc = units, top = units;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(inc, d);
+            if (lane >= d) inc += y;
+            top = max(top, __shfl_xor(top, d));
+        }
+        div = divide(a, __builtin_amdgcn_readlane(inc, 63), __builtin_amdgcn_readfirstlane(top));
+        u = wg * div.per;
+        const int end = inc * a.p.kv_heads;
+        const uint64_t past = __ballot(end > u);
+        if (past == 0) {
+            if (bad) raise(a.p.status, KVRT_BLOCK_BAD_INDEX);
+            return;
+        }
+        req = __builtin_ctzll(past);
+        before = __builtin_amdgcn_readlane(end - units * a.p.kv_heads, req);
+    } else {
+        int all = 0, most = 0;
+        for (int base = 0; base < a.n; base += 256) {
+            const int i = base + threadIdx.x;
+            int sum, top;
+            scan256(i < a.n ? units_of(load_rows(a, i, tile, bad)) : 0, scan_lds, sum, top);
+            all += sum;
+            most = max(most, top);
+        }
+        div = divide(a, all, most);
+        u = wg * div.per;
+        if (u < div.total) {
+            int at = 0;
+            for (int base = 0; base < a.n; base += 256) {
+                const int i = base + threadIdx.x;
+                const int units = i < a.n ? units_of(load_rows(a, i, tile, bad)) * a.p.kv_heads : 0;
+                int sum, top;
+                const int first = at + scan256(units, scan_lds, sum, top);
+                at += sum;
+                if (first <= u && u < first + units) found[0] = i, found[1] = first;
+            }
+            __syncthreads();
+        } else {
+            if (bad) raise(a.p.status, KVRT_BLOCK_BAD_INDEX);
+            return;
+        }
+        req = __builtin_amdgcn_readfirstlane(found[0]);
+        before = __builtin_amdgcn_readfirstlane(found[1]);
+    }
     if (bad) raise(a.p.status, KVRT_BLOCK_BAD_INDEX);
-    const int64_t per = (total + a.wgs - 1) / a.wgs;
-    int64_t u = wg * per;
-    const int64_t uend = min(total, u + per);
-    if (u >= uend) return;
-    int req;
-    int64_t before;
-    request_at(a, tile, u, scan_lds, req, before);
+    const int uend = min(div.total, u + div.per);
     const float scale = fabsf(a.scale_log2);
     const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-    bool unmapped = false;
+    const ConstInts table = (ConstInts)(uintptr_t)a.table;
+    const ConstFloats k_scale = (ConstFloats)(uintptr_t)a.p.k_scale, v_scale = (ConstFloats)(uintptr_t)a.p.v_scale;
 
     while (u < uend) {
-        bool ignore = false;
-        const Rows r = rows_of(a, req, tile, ignore);
+        Rows r;
+        if (a.n <= 64) {
+            r = rows_of(a, __builtin_amdgcn_readlane(mine.start, req), __builtin_amdgcn_readlane(mine.count, req),
+                        __builtin_amdgcn_readlane(mine.length, req), tile);
+        } else {
+            bool ignore = false;
+            r = load_rows(a, req, tile, ignore);
+        }
         const int units = units_of(r);
-        if (u >= before + (int64_t)units * a.p.kv_heads) {
-            before += (int64_t)units * a.p.kv_heads;
+        if (u >= before + units * a.p.kv_heads) {
+            before += units * a.p.kv_heads;
             ++req;
             continue;
         }
-        const int head = (int)((u - before) / units);
-        const int64_t seg = before + (int64_t)head * units;  // the head's first unit
-        const int ua = (int)(u - seg), ub = (int)min((int64_t)units, uend - seg);
+        const int head = (u - before) / units;
+        const int seg = before + head * units;  // the head's first unit
+        const int ua = u - seg, ub = min(units, uend - seg);
         const int first_tile = r.kstart / kTileKeys;
         const int t_end = min(first_tile + ub * kUnitTiles, (r.kend + kTileKeys - 1) / kTileKeys);
         const int t_begin = first_tile + ua * kUnitTiles + wave;
@@ -229,67 +328,69 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
         const int row = 16 * tile + (valid ? col : 0);
         const int qr = row / a.group, hr = row - qr * a.group;
         const int pos = r.length - r.count + qr;
-        uint32_t qop[D / 32][4];
-        float back;
-        load_query<D>(a.q + (int64_t)(r.start + qr) * a.q_row + (int64_t)(head * a.group + hr) * a.q_head, valid, flip, qop,
-                      back);
-        const float qscale = scale * back;
-
-        float m = kNegBig, l = 0.f;
-        f32x4_t o[NB];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) o[b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 
         if (t_begin < t_end) {
             // keys every row of the tile sees
             const int all_lo = a.window > 0 ? r.last - a.window + 1 : 0, all_hi = min(r.first + 1, r.kend);
-            const int32_t *entries = a.table + (int64_t)req * a.table_stride;
+            const ConstInts entries = table + (int64_t)req * a.table_stride;
             const int64_t head_bytes = (int64_t)a.p.block * D;
-            // the pages of a tile's two 16-key halves; past the range the last key's
-            auto page_of = [&](int t, int h) __attribute__((always_inline)) {
-                const int key = min(t * kTileKeys + 16 * h, r.kend - 1);
-                return entries[key >> a.p.shift];
-            };
-            // byte offset of a half's 16 rows of this head
-            auto half_at = [&](int page, int t, int h) __attribute__((always_inline)) {
-                return ((int64_t)page * a.p.kv_heads + head) * head_bytes +
-                       (int64_t)((t * kTileKeys + 16 * h) & (a.p.block - 1)) * D;
-            };
             uint32_t kc[2][KC][4], vc[2][4][VW];
             float ks[2], vs[2];
             bool ok[2];
-            int page[2];
-            auto take_pages = [&](int t) __attribute__((always_inline)) {
+            int page[2], ids[2];
+            // the table's entries for a tile's two 16-key halves; past the range the last key's
+            auto load_ids = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) ids[h] = entries[min(t * kTileKeys + 16 * h, r.kend - 1) >> a.p.shift];
+            };
+            auto take_pages = [&]() __attribute__((always_inline)) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int p = page_of(t, h);
-                    ok[h] = (unsigned)p < (unsigned)a.p.pages;
-                    page[h] = ok[h] ? p : 0;
+                    ok[h] = (unsigned)ids[h] < (unsigned)a.p.pages;
+                    page[h] = ok[h] ? ids[h] : 0;
                 }
+            };
+            // byte offset of a half's 16 rows of this head
+            auto half_at = [&](int t, int h) __attribute__((always_inline)) {
+                return ((int64_t)page[h] * a.p.kv_heads + head) * head_bytes +
+                       (int64_t)((t * kTileKeys + 16 * h) & (a.p.block - 1)) * D;
             };
             auto load_k = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint8_t *p = a.p.k + half_at(page[h], t, h) + col * D + 16 * grp;
+                    const uint8_t *p = a.p.k + half_at(t, h) + (uint32_t)(col * D + 16 * grp);
 #pragma unroll
                     for (int c = 0; c < KC; ++c) load_dwords<4>(p + 64 * c, kc[h][c]);
-                    ks[h] = a.p.k_scale[(int64_t)page[h] * a.p.kv_heads + head];
+                    ks[h] = k_scale[(int64_t)page[h] * a.p.kv_heads + head];
                 }
             };
             auto load_v = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint8_t *p = a.p.v + half_at(page[h], t, h) + 4 * grp * D + col * (D / 16);
+                    const uint8_t *p = a.p.v + half_at(t, h) + (uint32_t)(4 * grp * D + col * (D / 16));
 #pragma unroll
                     for (int j = 0; j < 4; ++j) load_dwords<VW>(p + j * D, vc[h][j]);
-                    vs[h] = a.p.v_scale[(int64_t)page[h] * a.p.kv_heads + head];
+                    vs[h] = v_scale[(int64_t)page[h] * a.p.kv_heads + head];
                 }
             };
-            take_pages(t_begin);
+            load_ids(t_begin);
+            uint32_t qop[D / 32][4];
+            float back;
+            take_pages();
             load_k(t_begin);
             load_v(t_begin);
+            load_query<D>(a.q + (int64_t)(r.start + qr) * a.q_row + (int64_t)(head * a.group + hr) * a.q_head, valid, flip,
+                          qop, back);
+            load_ids(min(t_begin + kUnitTiles, t_end - 1));
+            const float qscale = scale * back;
+            float m = kNegBig, l = 0.f;
+            f32x4_t o[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) o[b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+
             for (int t = t_begin; t < t_end; t += kUnitTiles) {
-                const int next = min(t + kUnitTiles, t_end - 1);  // past the last: read again, not used
+                // past the last tile: read again, not used
+                const int next = min(t + kUnitTiles, t_end - 1), after = min(t + 2 * kUnitTiles, t_end - 1);
                 // scores
                 f32x4_t s[2];
                 float lv[2], inv_vs[2], cf[2];
@@ -308,12 +409,13 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
                     }
                     const float v = scale_in_range(vs[h]);
                     lv[h] = __builtin_amdgcn_logf(v);
-                    inv_vs[h] = 1.0f / v;
+                    inv_vs[h] = __builtin_amdgcn_rcpf(v);  // within 1 ulp
                     cf[h] = qscale * scale_in_range(ks[h]);
                     good[h] = ok[h];
                 }
-                take_pages(next);
+                take_pages();
                 load_k(next);
+                load_ids(after);
                 // t = S * cf + lv, masked where a row does not see the key
                 const int key0 = t * kTileKeys;
                 const bool whole = key0 >= all_lo && key0 + kTileKeys <= all_hi && good[0] && good[1];
@@ -324,10 +426,8 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
                     for (int i = 0; i < 4; ++i) w[h][i] = fmaf(s[h][i], cf[h], lv[h]);
                 if (!whole) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < 2; ++h) {
                         unmapped |= !good[h] && key0 + 16 * h < r.kend && key0 + 16 * h + 16 > r.kstart;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int key = key0 + 16 * h + 4 * grp + i;
@@ -338,6 +438,7 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
 #pragma unroll
                             for (int e = 0; e < VW; ++e) vc[h][i][e] = data ? vc[h][i][e] : 0u;
                         }
+                    }
                 }
                 float top = fmaxf(fmaxf(fmaxf(w[0][0], w[0][1]), fmaxf(w[0][2], w[0][3])),
                                   fmaxf(fmaxf(w[1][0], w[1][1]), fmaxf(w[1][2], w[1][3])));
@@ -379,148 +480,209 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
                 load_v(next);
             }
             l = pair<OpSum, 32>(pair<OpSum, 16>(l));
-        }
-
-        // combine the four waves: each scales its part to the rows' common max, and
-        // sums and stores a quarter of the dims
-        __syncthreads();  // the last segment's sums are read
-        if (grp == 0) sml[wave * 16 + col] = make_float2(m, l);
-        __syncthreads();
-        float M = kNegBig, sum = 0.f;
+            if (valid) {
+                if (grp == 0) sml[wave * 16 + col] = make_float2(m, l);
+                float *dst = so + (wave * 16 + col) * PITCH + 4 * grp * NB;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, sml[w * 16 + col].x);
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float2 x = sml[w * 16 + col];
-            sum = fmaf(x.y, __builtin_amdgcn_exp2f(x.x - M), sum);
-        }
-        const float f = __builtin_amdgcn_exp2f(m - M);
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-            so[(wave * NB + b) * 64 + lane] = make_float4(o[b][0] * f, o[b][1] * f, o[b][2] * f, o[b][3] * f);
-        __syncthreads();
-        constexpr int MB = NB / 4;  // blocks of this wave: MB wave .. MB wave + MB - 1
-        float4 x[MB];
-#pragma unroll
-        for (int b = 0; b < MB; ++b) {
-            x[b] = so[(MB * wave + b) * 64 + lane];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) {
-                const float4 y = so[(w * NB + MB * wave + b) * 64 + lane];
-                x[b] = make_float4(x[b].x + y.x, x[b].y + y.y, x[b].z + y.z, x[b].w + y.w);
+                    for (int b = 0; b < NB; b += 4)
+                        *reinterpret_cast<float4 *>(dst + i * NB + b) =
+                            make_float4(o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]);
             }
         }
+        __syncthreads();
+        // join the waves that had keys: four elements of a row per thread
+        const int parts = min(max(t_end - (t_begin - wave), 0), 4);
         const bool begins = ua == 0, ends = ub == units;
-        if (begins && ends) {
-            if (valid) {
-                const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
-                uint16_t *out = a.out + (int64_t)(r.start + qr) * a.o_row + (int64_t)(head * a.group + hr) * a.o_head +
-                                4 * grp * NB + MB * wave;
-#pragma unroll
-                for (int b = 0; b < MB; ++b) {
-                    out[b] = f32_to_bf16(x[b].x * inv);
-                    out[NB + b] = f32_to_bf16(x[b].y * inv);
-                    out[2 * NB + b] = f32_to_bf16(x[b].z * inv);
-                    out[3 * NB + b] = f32_to_bf16(x[b].w * inv);
+        const int w0 = seg / div.per, count = (seg + units - 1) / div.per - w0 + 1;  // workgroups of the head
+        const bool here = count <= a.join_most;                                       // joined in this launch
+        const int64_t slot0 = (int64_t)tile * a.wgs * 2;
+        for (int e = threadIdx.x; e < r.n * (D / 4); e += 256) {
+            const int rr = e / (D / 4), d = 4 * (e % (D / 4));
+            float M = kNegBig, sum = 0.f;
+            for (int w = 0; w < parts; ++w) M = fmaxf(M, sml[w * 16 + rr].x);
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int w = 0; w < parts; ++w) {
+                const float2 ml = sml[w * 16 + rr];
+                const float f = __builtin_amdgcn_exp2f(ml.x - M);
+                const float4 y = *reinterpret_cast<const float4 *>(so + (w * 16 + rr) * PITCH + d);
+                sum = fmaf(ml.y, f, sum);
+                x = make_float4(fmaf(y.x, f, x.x), fmaf(y.y, f, x.y), fmaf(y.z, f, x.z), fmaf(y.w, f, x.w));
+            }
+            if (begins && ends) {
+                store_out(a, r, head, 16 * tile + rr, d, x, sum);
+            } else {
+                // partial 0: the head's keys began in an earlier workgroup, 1: they begin here
+                const int64_t slot = slot0 + 2 * wg + (begins ? 1 : 0);
+                float *po = a.part_o + (slot * 16 + rr) * D + d;
+                float2 *pm = a.part_ml + slot * 16 + rr;
+                if (here) {
+                    store_agent(reinterpret_cast<float2 *>(po), make_float2(x.x, x.y));
+                    store_agent(reinterpret_cast<float2 *>(po + 2), make_float2(x.z, x.w));
+                    if (d == 0) store_agent(pm, make_float2(M, sum));
+                } else {
+                    *reinterpret_cast<float4 *>(po) = x;
+                    if (d == 0) *pm = make_float2(M, sum);
                 }
             }
-        } else {
-            // slot 0: the rows' keys began in an earlier workgroup, 1: they begin here
-            const int64_t slot = ((int64_t)tile * a.wgs + wg) * 2 + (begins ? 1 : 0);
-            float4 *po = reinterpret_cast<float4 *>(a.part_o) + (slot * NB + MB * wave) * 64 + lane;
-#pragma unroll
-            for (int b = 0; b < MB; ++b) po[b * 64] = x[b];
-            if (wave == 0 && grp == 0) a.part_ml[slot * 16 + col] = make_float2(M, sum);
+        }
+        if (here && !(begins && ends)) {
+            // the last of the head's workgroups to arrive joins their partials, in
+            // workgroup order; it leaves the counter at zero
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's partials are stored
+            __syncthreads();
+            uint32_t *counter = a.counters + w0;
+            if (threadIdx.x == 0) arrived = arrive_agent(counter);
+            __syncthreads();
+            if (arrived == (uint32_t)count - 1) {
+                if (threadIdx.x == 0) clear_agent(counter);
+                for (int e = threadIdx.x; e < r.n * (D / 4); e += 256) {
+                    const int rr = e / (D / 4), d = 4 * (e % (D / 4));
+                    float M = kNegBig, sum = 0.f;
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    join_partials(count, [&](int p, float2 &ml, float4 &y) __attribute__((always_inline)) {
+                        const int64_t at = (slot0 + 2 * (w0 + p) + (p == 0 ? 1 : 0)) * 16 + rr;
+                        ml = load_agent(a.part_ml + at);
+                        const float2 lo = load_agent(reinterpret_cast<const float2 *>(a.part_o + at * D + d));
+                        const float2 hi = load_agent(reinterpret_cast<const float2 *>(a.part_o + at * D + d + 2));
+                        y = make_float4(lo.x, lo.y, hi.x, hi.y);
+                    }, M, sum, x);
+                    store_out(a, r, head, 16 * tile + rr, d, x, sum);
+                }
+            }
         }
         u = seg + ub;
+        if (u < uend) __syncthreads();  // the sums are read before the next head's are written
     }
     if (unmapped) raise(a.p.status, KVRT_BLOCK_BAD_INDEX);
 }
 
-// Joins the partials of the rows whose keys several workgroups had: one workgroup
-// per (request, KV head, row tile), in workgroup order.
+// Joins the partials of heads that more workgroups shared than one joins inside the
+// launch: one workgroup per (request, KV head, row). Up to kFlat partials in their
+// order, as the launch does; beyond, in GROUPS interleaved orders that are then joined.
+constexpr int kFlat = 32;
+
 template <int D>
 __global__ __launch_bounds__(256) void block8_join_kernel(Block8AttendArgs a) {
-    constexpr int NB = D / 16, MB = NB / 4;
-    __shared__ int64_t scan_lds[4];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, grp = lane >> 4;
-    const int tile = blockIdx.y, head = blockIdx.x % a.p.kv_heads, req = blockIdx.x / a.p.kv_heads;
+    constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+    __shared__ int scan_lds[8];
+    __shared__ float4 so[256];
+    __shared__ float2 sml[256];
+    const int tile = blockIdx.y, rr = blockIdx.z, head = blockIdx.x % a.p.kv_heads, req = blockIdx.x / a.p.kv_heads;
     bool bad = false;
-    const Rows r = rows_of(a, req, tile, bad);
-    if (r.n == 0) return;
-    // units before the request, and all
-    int64_t all = 0, before = 0;
+    const Rows r = load_rows(a, req, tile, bad);
+    if (rr >= r.n) return;
+    // units before the request, all, and the most of a head
+    int all = 0, before = 0, most = 0;
     for (int base = 0; base < a.n; base += 256) {
         const int i = base + threadIdx.x;
-        const int64_t mine = i < a.n ? units_of(rows_of(a, i, tile, bad)) : 0;
-        int64_t sum, less;
-        scan256(mine, scan_lds, sum);
-        scan256(i < req ? mine : 0, scan_lds, less);
+        const int mine = i < a.n ? units_of(load_rows(a, i, tile, bad)) : 0;
+        int sum, less, top, ignore;
+        scan256(mine, scan_lds, sum, top);
+        scan256(i < req ? mine : 0, scan_lds, less, ignore);
         all += sum;
         before += less;
+        most = max(most, top);
     }
-    const int64_t per = (all * a.p.kv_heads + a.wgs - 1) / a.wgs;
-    const int units = units_of(r);
-    const int64_t seg = before * a.p.kv_heads + (int64_t)head * units;
-    const int w0 = (int)(seg / per), w1 = (int)((seg + units - 1) / per);
-    if (w0 == w1) return;
-    auto slot_at = [&](int w) { return ((int64_t)tile * a.wgs + w) * 2 + (w == w0 ? 1 : 0); };
-    float M = kNegBig;
-    for (int w = w0; w <= w1; ++w) M = fmaxf(M, a.part_ml[slot_at(w) * 16 + col].x);
-    float sum = 0.f;
-    float4 x[MB];
-#pragma unroll
-    for (int b = 0; b < MB; ++b) x[b] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = w0; w <= w1; ++w) {
-        const int64_t slot = slot_at(w);
-        const float2 ml = a.part_ml[slot * 16 + col];
-        const float f = __builtin_amdgcn_exp2f(ml.x - M);
-        sum = fmaf(ml.y, f, sum);
-        const float4 *po = reinterpret_cast<const float4 *>(a.part_o) + (slot * NB + MB * wave) * 64 + lane;
-#pragma unroll
-        for (int b = 0; b < MB; ++b) {
-            const float4 y = po[b * 64];
-            x[b] = make_float4(fmaf(y.x, f, x[b].x), fmaf(y.y, f, x[b].y), fmaf(y.z, f, x[b].z), fmaf(y.w, f, x[b].w));
-        }
+    const Division div = divide(a, all, most);
+    const int units = units_of(r), seg = before * a.p.kv_heads + head * units;
+    const int w0 = seg / div.per, count = (seg + units - 1) / div.per - w0 + 1;
+    if (count == 1 || count <= a.join_most) return;
+    const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
+    const int groups = count <= kFlat ? 1 : GROUPS;
+    float M = kNegBig, sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (group < groups) {
+        const int64_t slot0 = ((int64_t)tile * a.wgs + w0) * 2;
+        join_partials((count - group + groups - 1) / groups, [&](int p, float2 &ml, float4 &y) __attribute__((always_inline)) {
+            const int i = p * groups + group;
+            const int64_t at = (slot0 + 2 * i + (i == 0 ? 1 : 0)) * 16 + rr;
+            ml = a.part_ml[at];
+            y = *reinterpret_cast<const float4 *>(a.part_o + at * D + d);
+        }, M, sum, x);
     }
-    if (col >= r.n) return;
-    const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
-    const int row = 16 * tile + col, qr = row / a.group, hr = row - qr * a.group;
-    uint16_t *out = a.out + (int64_t)(r.start + qr) * a.o_row + (int64_t)(head * a.group + hr) * a.o_head + 4 * grp * NB +
-                    MB * wave;
-#pragma unroll
-    for (int b = 0; b < MB; ++b) {
-        out[b] = f32_to_bf16(x[b].x * inv);
-        out[NB + b] = f32_to_bf16(x[b].y * inv);
-        out[2 * NB + b] = f32_to_bf16(x[b].z * inv);
-        out[3 * NB + b] = f32_to_bf16(x[b].w * inv);
+    if (groups > 1) {
+        so[threadIdx.x] = x;
+        sml[threadIdx.x] = make_float2(M, sum);
+        __syncthreads();
+        if (group != 0) return;
+        M = kNegBig, sum = 0.f;
+        x = make_float4(0.f, 0.f, 0.f, 0.f);
+        join_partials(GROUPS, [&](int p, float2 &ml, float4 &y) __attribute__((always_inline)) {
+            ml = sml[p * LANES + threadIdx.x];
+            y = so[p * LANES + threadIdx.x];
+        }, M, sum, x);
+    } else if (group != 0) {
+        return;
     }
+    store_out(a, r, head, 16 * tile + rr, d, x, sum);
 }
 
 template <int CODE, int D>
-static hipError_t launch_attend(const Block8AttendArgs &a, int tiles, hipStream_t s) {
+static hipError_t launch_attend(const Block8AttendArgs &a, int tiles, bool join, hipStream_t s) {
     hipLaunchKernelGGL((block8_attend_kernel<CODE, D>), dim3(a.wgs, tiles), dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.wgs == 1) return e;
-    hipLaunchKernelGGL((block8_join_kernel<D>), dim3(a.n * a.p.kv_heads, tiles), dim3(256), 0, s, a);
+    if (e != hipSuccess || !join) return e;
+    const int rows = (int)std::min<int64_t>(16, (int64_t)a.group * a.max_q);
+    hipLaunchKernelGGL((block8_join_kernel<D>), dim3(a.n * a.p.kv_heads, tiles, rows), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
 template <int CODE>
-static hipError_t launch_attend_code(const Block8AttendArgs &a, int head_dim, int tiles, hipStream_t s) {
+static hipError_t launch_attend_code(const Block8AttendArgs &a, int head_dim, int tiles, bool join, hipStream_t s) {
     switch (head_dim) {
-        case 64: return launch_attend<CODE, 64>(a, tiles, s);
-        case 128: return launch_attend<CODE, 128>(a, tiles, s);
-        case 256: return launch_attend<CODE, 256>(a, tiles, s);
-        case 512: return launch_attend<CODE, 512>(a, tiles, s);
+        case 64: return launch_attend<CODE, 64>(a, tiles, join, s);
+        case 128: return launch_attend<CODE, 128>(a, tiles, join, s);
+        case 256: return launch_attend<CODE, 256>(a, tiles, join, s);
+        case 512: return launch_attend<CODE, 512>(a, tiles, join, s);
         default: return hipErrorInvalidValue;
     }
 }
 
-hipError_t launch_block8_attend(const Block8AttendArgs &a, int dtype, int head_dim, int tiles, hipStream_t s) {
-    return dtype == KVRT_INT8 ? launch_attend_code<KVRT_INT8>(a, head_dim, tiles, s)
-                              : launch_attend_code<KVRT_E4M3>(a, head_dim, tiles, s);
+hipError_t launch_block8_attend(const Block8AttendArgs &a, int dtype, int head_dim, int tiles, bool join, hipStream_t s) {
+    return dtype == KVRT_INT8 ? launch_attend_code<KVRT_INT8>(a, head_dim, tiles, join, s)
+                              : launch_attend_code<KVRT_E4M3>(a, head_dim, tiles, join, s);
+}
+
+// ---- arrival counters ---------------------------------------------------------------
+//
+// Zero at load and between launches. Calls on one stream run in order and share a
+// slice; a captured call has a slice of its own for good, since its graph may be
+// replayed beside anything else (a graph does not overlap itself). With the slices
+// used up, calls join in a second launch instead.
+constexpr int kSlices = 512;
+static __device__ uint32_t block8_counters[kSlices * kBlock8MaxWgs];
+
+uint32_t *block8_counter_slice(hipStream_t s) {
+    static std::mutex mu;
+    static std::map<int, uint32_t *> base;
+    static std::map<int, int> used;
+    static std::map<std::pair<int, hipStream_t>, int> of_stream;
+    int dev = 0;
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    if (hipGetDevice(&dev) != hipSuccess || hipStreamIsCapturing(s, &cs) != hipSuccess) return nullptr;
+    std::lock_guard<std::mutex> lock(mu);
+    const auto at = base.find(dev);
+    uint32_t *p;
+    if (at == base.end()) {
+        if (cs != hipStreamCaptureStatusNone) return nullptr;  // the address is looked up outside captures
+        void *sym = nullptr;
+        if (hipGetSymbolAddress(&sym, HIP_SYMBOL(block8_counters)) != hipSuccess) return nullptr;
+        p = base[dev] = static_cast<uint32_t *>(sym);
+    } else {
+        p = at->second;
+    }
+    if (cs != hipStreamCaptureStatusNone) {
+        if (used[dev] >= kSlices) return nullptr;
+        return p + (size_t)used[dev]++ * kBlock8MaxWgs;
+    }
+    const auto key = std::make_pair(dev, s);
+    const auto got = of_stream.find(key);
+    if (got != of_stream.end()) return p + (size_t)got->second * kBlock8MaxWgs;
+    if (used[dev] >= kSlices) return nullptr;
+    of_stream[key] = used[dev];
+    return p + (size_t)used[dev]++ * kBlock8MaxWgs;
 }
 
 }  // namespace kvrt
