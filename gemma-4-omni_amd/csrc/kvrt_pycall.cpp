@@ -16,6 +16,9 @@
 
 #include <climits>
 
+#include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
+#include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "kvrt.h"
@@ -286,10 +289,247 @@ PyObject *connect(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     Py_RETURN_NONE;
 }
 
+// ---- 8-bit pages (kvrt/block8.py) --------------------------------------------------
+//
+// Through ctypes and torch.empty an update of the page tables spends 14 us on the host;
+// its launches take 4 on the GPU. Here it allocates its answers, checks its tensors
+// and launches in one call. A call that is not in the plain form is
+// the general path's, which says what is wrong with it.
+
+struct BlockApi {
+    decltype(&kvrt_block_tables_update_async) update;
+    decltype(&kvrt_block8_append_async) append;
+    decltype(&kvrt_block8_gather_async) gather;
+    decltype(&kvrt_block8_attend_async) attend;
+    decltype(&kvrt_block8_attend_work) attend_work;
+} block_api;
+
+// The tensor in o where it is a plain GPU tensor on device dev.
+const at::Tensor *plain(PyObject *o, int dev) {
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (!t.defined() || !t.is_cuda() || t.get_device() != dev || t.layout() != at::kStrided || t.requires_grad())
+        return nullptr;
+    return &t;
+}
+
+// A contiguous int32 tensor of n elements on dev.
+const int32_t *ints(PyObject *o, int dev, int ndim, int64_t n) {
+    const at::Tensor *t = plain(o, dev);
+    if (!t || t->scalar_type() != at::kInt || t->dim() != ndim || t->numel() != n || !t->is_contiguous()) return nullptr;
+    return t->const_data_ptr<int32_t>();
+}
+
+bool describe(const at::Tensor *t, kvrt_tensor &d) {
+    if (!t || t->dim() > KVRT_MAX_RANK) return false;
+    d = kvrt_tensor{};
+    d.dtype = dtype_code(t->scalar_type());
+    if (d.dtype < 0) return false;
+    d.data = t->data_ptr();
+    d.ndim = (int32_t)t->dim();
+    for (int i = 0; i < d.ndim; ++i) {
+        d.dims[i] = t->size(i);
+        d.strides[i] = t->stride(i);
+    }
+    return true;
+}
+
+bool current_device(int dev) {
+    return c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getDevice().index() == dev;
+}
+
+at::Tensor fresh(at::IntArrayRef size, at::ScalarType type, int dev) {
+    return at::empty(size, at::TensorOptions().dtype(type).device(c10::DeviceType::CUDA, (c10::DeviceIndex)dev));
+}
+
+// As guarded(), for calls that answer with tensors: body's object, or the code.
+template <class F>
+PyObject *guarded_object(Py_ssize_t nargs, Py_ssize_t want, F body) {
+    PyObject *out = nullptr;
+    long rc = kGeneral;
+    try {
+        if (nargs == want) rc = body(out);
+    } catch (...) {
+        rc = kGeneral;
+    }
+    if (PyErr_Occurred()) PyErr_Clear();
+    if (rc == KVRT_OK && out) return out;
+    Py_XDECREF(out);
+    return PyLong_FromLong(rc);
+}
+
+// (tables: sizes, scratch and status, stream, device, table, mapped, free, free_count, lengths, new, rows)
+// -> (starts, slot_map, lengths, granted)
+PyObject *block_update(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded_object(nargs, 10, [&](PyObject *&out) -> long {
+        int32_t dev, rows;
+        const auto *base = static_cast<const kvrt_block_tables *>(PyLong_AsVoidPtr(a[0]));
+        void *stream = PyLong_AsVoidPtr(a[1]);
+        if (!base || !read_int(a[2], dev) || !read_int(a[9], rows) || rows < 0 || !current_device(dev)) return kGeneral;
+        kvrt_block_tables t = *base;
+        t.table = const_cast<int32_t *>(ints(a[3], dev, 2, (int64_t)t.n * t.max_pages));
+        t.mapped = const_cast<int32_t *>(ints(a[4], dev, 1, t.n));
+        t.free_pages = const_cast<int32_t *>(ints(a[5], dev, 1, t.pool_pages));
+        t.free_count = const_cast<int32_t *>(ints(a[6], dev, 1, 1));
+        const int32_t *lengths = ints(a[7], dev, 1, t.n), *fresh_rows = ints(a[8], dev, 1, t.n);
+        if (!t.table || THPVariable_Unpack(a[3]).size(0) != t.n || !t.mapped || !t.free_pages || !t.free_count ||
+            !lengths || !fresh_rows)
+            return kGeneral;
+        const at::Tensor starts = fresh({t.n + 1}, at::kInt, dev), slots = fresh({rows}, at::kInt, dev),
+                         lens = fresh({t.n}, at::kInt, dev), granted = fresh({t.n}, at::kInt, dev);
+        int32_t *const p[4] = {starts.data_ptr<int32_t>(), rows ? slots.data_ptr<int32_t>() : nullptr,
+                               lens.data_ptr<int32_t>(), granted.data_ptr<int32_t>()};
+        const long rc =
+            without_gil([&] { return block_api.update(&t, lengths, fresh_rows, rows, p[0], p[1], p[2], p[3], stream); });
+        if (rc == KVRT_OK)
+            out = Py_BuildValue("(NNNN)", THPVariable_Wrap(starts), THPVariable_Wrap(slots), THPVariable_Wrap(lens),
+                                THPVariable_Wrap(granted));
+        return rc;
+    });
+}
+
+// (pages, stream, device, k, v, slot_map)
+PyObject *block_append(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded(nargs, 6, [&]() -> long {
+        int32_t dev;
+        const auto *pages = static_cast<const kvrt_block8 *>(PyLong_AsVoidPtr(a[0]));
+        void *stream = PyLong_AsVoidPtr(a[1]);
+        kvrt_tensor k, v;
+        if (!pages || !read_int(a[2], dev) || !current_device(dev) || !describe(plain(a[3], dev), k) ||
+            !describe(plain(a[4], dev), v) || k.ndim < 1)
+            return kGeneral;
+        const int32_t *slots = ints(a[5], dev, 1, k.dims[0]);
+        if (!slots) return kGeneral;
+        return without_gil([&] { return block_api.append(pages, &k, &v, slots, stream); });
+    });
+}
+
+// What both forms of gather share.
+struct GatherHead {
+    const kvrt_block8 *pages;
+    void *stream;
+    int32_t dev;
+    kvrt_tensor table;
+    const int32_t *lengths, *from = nullptr;
+
+    bool read(PyObject *const *a) {
+        pages = static_cast<const kvrt_block8 *>(PyLong_AsVoidPtr(a[0]));
+        stream = PyLong_AsVoidPtr(a[1]);
+        if (!pages || !read_int(a[2], dev) || !current_device(dev) || !describe(plain(a[3], dev), table) || table.ndim != 2 ||
+            table.dtype != KVRT_INT32)
+            return false;
+        lengths = ints(a[4], dev, 1, table.dims[0]);
+        return lengths && (a[5] == Py_None || (from = ints(a[5], dev, 1, table.dims[0])));
+    }
+};
+
+// (pages, stream, device, table, lengths, start_pos or None, out_k, out_v, mask or None)
+PyObject *block_gather(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded(nargs, 9, [&]() -> long {
+        GatherHead h;
+        kvrt_tensor k, v, m;
+        const bool masked = a[8] != Py_None;
+        if (!h.read(a) || !describe(plain(a[6], h.dev), k) || !describe(plain(a[7], h.dev), v) ||
+            (masked && !describe(plain(a[8], h.dev), m)))
+            return kGeneral;
+        return without_gil(
+            [&] { return block_api.gather(h.pages, &h.table, h.lengths, h.from, &k, &v, masked ? &m : nullptr, h.stream); });
+    });
+}
+
+// (pages, stream, device, table, lengths, start_pos or None, lmax, fp32, mask: 0 none, 1 bool, 2 fp32, 3 bf16)
+// -> (k, v, mask or None)
+PyObject *block_gather_new(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded_object(nargs, 9, [&](PyObject *&out) -> long {
+        GatherHead h;
+        int32_t lmax, fp32, kind;
+        if (!h.read(a) || !read_int(a[6], lmax) || lmax < 0 || !read_int(a[7], fp32) || !read_int(a[8], kind) || kind < 0 ||
+            kind > 3)
+            return kGeneral;
+        const int64_t size[4] = {h.table.dims[0], h.pages->kv_heads, lmax, h.pages->head_dim}, flat[2] = {size[0], lmax};
+        const at::ScalarType kinds[3] = {at::kBool, at::kFloat, at::kBFloat16};
+        const at::Tensor kt = fresh(size, fp32 ? at::kFloat : at::kBFloat16, h.dev), vt = at::empty_like(kt);
+        at::Tensor mt;
+        if (kind) mt = fresh(flat, kinds[kind - 1], h.dev);
+        kvrt_tensor k, v, m;
+        if (!describe(&kt, k) || !describe(&vt, v) || (kind && !describe(&mt, m))) return kGeneral;
+        const long rc = without_gil(
+            [&] { return block_api.gather(h.pages, &h.table, h.lengths, h.from, &k, &v, kind ? &m : nullptr, h.stream); });
+        if (rc == KVRT_OK) {
+            PyObject *mask = Py_None;
+            if (kind) mask = THPVariable_Wrap(mt);
+            else Py_INCREF(mask);
+            out = Py_BuildValue("(NNN)", THPVariable_Wrap(kt), THPVariable_Wrap(vt), mask);
+        }
+        return rc;
+    });
+}
+
+// (pages, stream, device, scale, window, max_q, q, table, lengths, starts, granted or None, out or None) -> out
+PyObject *block_attend(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded_object(nargs, 12, [&](PyObject *&answer) -> long {
+        int32_t dev, window, max_q;
+        float scale;
+        const auto *pages = static_cast<const kvrt_block8 *>(PyLong_AsVoidPtr(a[0]));
+        void *stream = PyLong_AsVoidPtr(a[1]);
+        kvrt_tensor q, table, o;
+        const at::Tensor *qt;
+        if (!pages || !read_int(a[2], dev) || !read_float(a[3], scale) || !read_int(a[4], window) ||
+            !read_int(a[5], max_q) || !current_device(dev) || !(qt = plain(a[6], dev)) || !describe(qt, q) || q.ndim != 3 ||
+            !describe(plain(a[7], dev), table) || table.ndim != 2 || table.dtype != KVRT_INT32)
+            return kGeneral;
+        const int64_t n = table.dims[0];
+        const int32_t *lengths = ints(a[8], dev, 1, n), *starts = ints(a[9], dev, 1, n + 1), *granted = nullptr;
+        if (!lengths || !starts || (a[10] != Py_None && !(granted = ints(a[10], dev, 1, n)))) return kGeneral;
+        if (max_q > q.dims[0]) max_q = (int32_t)q.dims[0];
+        at::Tensor out;
+        if (a[11] == Py_None) {
+            out = fresh(qt->sizes(), qt->scalar_type(), dev);
+            if (!describe(&out, o)) return kGeneral;
+        } else if (!describe(plain(a[11], dev), o)) {
+            return kGeneral;
+        }
+        const uint64_t size = block_api.attend_work(pages, n, table.dims[1], q.dims[1], max_q);
+        at::Tensor work;
+        if (size) work = fresh({(int64_t)size}, at::kByte, dev);
+        const long rc = without_gil([&] {
+            return block_api.attend(pages, &q, &table, lengths, starts, granted, &o, scale, window, max_q,
+                                    size ? work.data_ptr() : nullptr, size, stream);
+        });
+        if (rc == KVRT_OK) {
+            if (out.defined()) answer = THPVariable_Wrap(out);
+            else Py_INCREF(answer = a[11]);
+        }
+        return rc;
+    });
+}
+
+// (address of each BlockApi member in order): once, after loading
+PyObject *connect_blocks(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    void *p[5];
+    if (nargs != 5) {
+        PyErr_SetString(PyExc_TypeError, "connect_blocks takes five addresses");
+        return nullptr;
+    }
+    for (int i = 0; i < 5; ++i) {
+        p[i] = PyLong_AsVoidPtr(a[i]);
+        if (PyErr_Occurred()) return nullptr;
+    }
+    block_api.update = reinterpret_cast<decltype(block_api.update)>(p[0]);
+    block_api.append = reinterpret_cast<decltype(block_api.append)>(p[1]);
+    block_api.gather = reinterpret_cast<decltype(block_api.gather)>(p[2]);
+    block_api.attend = reinterpret_cast<decltype(block_api.attend)>(p[3]);
+    block_api.attend_work = reinterpret_cast<decltype(block_api.attend_work)>(p[4]);
+    Py_RETURN_NONE;
+}
+
 #define KVRT_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {KVRT_METHOD(append_attend),   KVRT_METHOD(attend),        KVRT_METHOD(attend_talker),
                          KVRT_METHOD(write_positions), KVRT_METHOD(append_gather), KVRT_METHOD(attend_tensors),
-                         KVRT_METHOD(connect),         {nullptr, nullptr, 0, nullptr}};
+                         KVRT_METHOD(connect),         KVRT_METHOD(block_update),  KVRT_METHOD(block_append),
+                         KVRT_METHOD(block_gather),    KVRT_METHOD(block_gather_new), KVRT_METHOD(block_attend),
+                         KVRT_METHOD(connect_blocks),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "kvrt_pycall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -36,10 +36,27 @@ from typing import NamedTuple
 import torch
 
 from . import _lib as L
-from .runtime import _check, current_stream_handle, require_cuda, tensor_desc
+from .runtime import _check, calls, current_stream_handle, require_cuda, tensor_desc
+
+_calls_mod = None
+
+
+def _calls():
+    """The native call module with the entry points of this module connected."""
+    global _calls_mod
+    if _calls_mod is None:
+        lib, mod = L.load(), calls()
+        fns = (lib.kvrt_block_tables_update_async, lib.kvrt_block8_append_async, lib.kvrt_block8_gather_async,
+               lib.kvrt_block8_attend_async, lib.kvrt_block8_attend_work)
+        mod.connect_blocks(*(ctypes.cast(f, ctypes.c_void_p).value for f in fns))
+        _calls_mod = mod
+    return _calls_mod
+
 
 _CODES = {torch.int8: L.DT_INT8, torch.float8_e4m3fn: L.DT_E4M3}
 _NAMES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+_FLOATS = {torch.bfloat16: 0, torch.float32: 1}
+_MASKS = {None: 0, torch.bool: 1, torch.float32: 2, torch.bfloat16: 3}
 _I32_MAX = 2 ** 31 - 1
 
 
@@ -134,6 +151,9 @@ class BlockTables(_Status):
         self.free_count = torch.full((1,), self.pool_pages, **make)
         self._work = torch.empty(L.block_tables_work(self.n), **make)
         self._status = torch.zeros(1, **make)
+        self._call = _calls()
+        self._sizes = self._c()  # what calls read beside the four public tensors
+        self._sizes_at = ctypes.addressof(self._sizes)
 
     def _c(self) -> L.KvrtBlockTables:
         for name, size in (("mapped", self.n), ("free", self.pool_pages), ("free_count", 1)):
@@ -158,6 +178,12 @@ class BlockTables(_Status):
         longer suffice for it (``BLOCK_NO_PAGES``), or when its numbers are not
         possible or its rows end past ``rows`` (``BLOCK_BAD_INDEX``): it keeps its pages
         and is granted no row; :meth:`status` tells."""
+        got = self._call.block_update(self._sizes_at, current_stream_handle(self.device), self.device.index, self.table,
+                                      self.mapped, self.free, self.free_count, lengths, new, rows)
+        if type(got) is tuple:
+            return BlockPlan._make(got)
+        if got < 0:
+            _check(got, "kvrt_block_tables_update_async")
         rows = int(rows)
         if rows < 0:
             raise ValueError("rows must not be negative")
@@ -211,6 +237,8 @@ class Block8Pool(_Status):
         c.dtype, c.pages, c.kv_heads, c.block, c.head_dim = _CODES[k.dtype], pages, heads, block, dim
         self._c = c
         self._ref = ctypes.byref(c)
+        self._at = ctypes.addressof(c)
+        self._call = _calls()
 
     @classmethod
     def zeros(cls, pages: int, kv_heads: int, head_dim: int, *, block_size: int = 16, dtype: str = "int8",
@@ -237,6 +265,9 @@ class Block8Pool(_Status):
         them are coded anew; rows behind them (rolled back) are dropped. A page
         takes one run of consecutive slots per call; a slot map that names a slot
         twice or enters a page twice leaves that page undefined."""
+        rc = self._call.block_append(self._at, current_stream_handle(self.device), self.device.index, k, v, slot_map)
+        if rc <= 0:
+            return _check(rc, "kvrt_block8_append_async")
         for t, name in ((k, "k"), (v, "v")):
             _same(t, name, self.device)
         _int32(slot_map, "slot_map", int(k.shape[0]), self.device)
@@ -253,6 +284,19 @@ class Block8Pool(_Status):
         positions ``start_pos[i]`` (int32 [n] on the GPU, default 0) on.
         ``out``: (K, V) or (K, V, mask) destinations instead of new tensors (strided
         views with a contiguous last dimension); they then set Lmax and dtype."""
+        if out is None and dtype in _FLOATS and mask_dtype in _MASKS:
+            got = self._call.block_gather_new(self._at, current_stream_handle(self.device), self.device.index, table,
+                                              lengths, start_pos, lmax, _FLOATS[dtype], _MASKS[mask_dtype])
+            if type(got) is tuple:
+                return got
+            if got < 0:
+                _check(got, "kvrt_block8_gather_async")
+        elif out is not None and lmax is None:
+            rc = self._call.block_gather(self._at, current_stream_handle(self.device), self.device.index, table, lengths,
+                                         start_pos, out[0], out[1], out[2] if len(out) > 2 else None)
+            if rc <= 0:
+                _check(rc, "kvrt_block8_gather_async")
+                return out[0], out[1], out[2] if len(out) > 2 else None
         td = self._table(table)
         n = int(table.shape[0])
         _int32(lengths, "lengths", n, self.device)
@@ -295,6 +339,12 @@ class Block8Pool(_Status):
         request are left as they are (undefined in a new ``out``). ``max_q``: the
         most rows of one request (more raise ``BLOCK_BAD_INDEX``, the first
         ``max_q`` are computed)."""
+        got = self._call.block_attend(self._at, current_stream_handle(self.device), self.device.index, float(scale), window,
+                                      max_q, q, table, lengths, starts, granted, out)
+        if type(got) is not int:
+            return got
+        if got < 0:
+            _check(got, "kvrt_block8_attend_async")
         td = self._table(table)
         n = int(table.shape[0])
         _same(q, "q", self.device)
