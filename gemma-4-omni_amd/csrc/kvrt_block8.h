@@ -66,6 +66,9 @@ struct Block8AttendArgs {
     float *part_o;                         // partials of divided heads [tile][wg][2][16 rows][D]
     float2 *part_ml;                       // their (max, sum) [tile][wg][2][16]
     uint32_t *counters;                    // arrivals [wg], zero between launches
+    // chunks (kvrt_block8_chunk.h): tiles of 32 * row_waves rows, at most `tiles` of them,
+    // keys divided over `splits` workgroups; partials [tile][head][split][row][D]
+    int row_waves, tiles, splits;
 };
 
 constexpr int kBlock8MaxWgs = 1024;  // workgroups the keys are divided over, at most
@@ -73,7 +76,9 @@ constexpr int kBlock8MaxWgs = 1024;  // workgroups the keys are divided over, at
 hipError_t launch_block8_tables(const Block8TablesArgs &a, hipStream_t s);
 hipError_t launch_block8_append(const Block8AppendArgs &a, int dtype, int head_dim, hipStream_t s);
 hipError_t launch_block8_gather(const Block8GatherArgs &a, int dtype, int head_dim, hipStream_t s);
-hipError_t launch_block8_attend(const Block8AttendArgs &a, int dtype, int head_dim, int tiles, bool join, hipStream_t s);
+hipError_t launch_block8_attend(const Block8AttendArgs &a, int dtype, int head_dim, bool join, hipStream_t s);
+hipError_t launch_block8_chunk(const Block8AttendArgs &a, int dtype, int head_dim, hipStream_t s);
+hipError_t launch_block8_chunk_wide(const Block8AttendArgs &a, int dtype, int head_dim, hipStream_t s);
 // kBlock8MaxWgs zeroed arrival counters for a call on that stream; nullptr: none left.
 uint32_t *block8_counter_slice(hipStream_t s);
 

@@ -473,19 +473,39 @@ static bool table_ok(const kvrt_tensor *t, int shift, int64_t &n, int64_t &width
 
 constexpr int64_t kMaxRows = (int64_t)1 << 30, kJoinBytes = 48 << 10;
 
-// Units of 128 keys that a head of one request has at most.
-static int64_t most_units(const Block8View &v, int64_t width) { return ((width << v.shift) + 127) / 128 + 1; }
-
-// Workgroups the keys of a call are divided over, for each of its row tiles: those
-// that run at a time (their registers allow 4, 3, 2 and 1 per CU).
-static int attend_wgs(const Block8View &v, int64_t n, int64_t width, int tiles, int head_dim) {
-    const int64_t round = 256 * (head_dim == 64 ? 4 : head_dim == 128 ? 3 : head_dim == 256 ? 2 : 1);
-    const int64_t units = n * v.kv_heads * most_units(v, width);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(units, round / tiles));
+// How a call's rows and keys are divided.
+struct AttendPlan {
+    bool chunk;           // more than 16 query rows per KV head
+    int wgs;              // decode: workgroups the keys are divided over
+    int64_t most;         // decode: units of 128 keys that a head of one request has at most
+    int row_waves, splits;
+    int64_t tiles;        // chunk: row tiles at most
+    uint64_t part_rows;   // rows of partials in the workspace
+};
+static AttendPlan attend_plan(int kv_heads, int shift, int head_dim, int64_t n, int64_t width, int64_t rows, int64_t group,
+                              int64_t max_q) {
+    AttendPlan p{};
+    p.chunk = group * max_q > 16;
+    if (!p.chunk) {
+        // as many workgroups as run at a time (their registers allow 4, 3, 2 and 1 per CU)
+        const int64_t round = 256 * (head_dim == 64 ? 4 : head_dim == 128 ? 3 : head_dim == 256 ? 2 : 1);
+        p.most = ((width << shift) + 127) / 128 + 1;
+        p.wgs = (int)std::max<int64_t>(1, std::min(n * kv_heads * p.most, round));
+        p.part_rows = p.wgs == 1 ? 0 : (uint64_t)p.wgs * 2 * 16;
+        return p;
+    }
+    // The most rows per tile (each shares the keys' conversion) that still leave a
+    // workgroup per CU, then the keys divided as far as that takes. Every request's last
+    // tile may be a partial one.
+    for (p.row_waves = 4;; p.row_waves /= 2) {
+        const int64_t size = 32 * p.row_waves;
+        p.tiles = std::min((rows * group + size - 1) / size + n - 1, n * ((group * max_q + size - 1) / size));
+        if (p.row_waves == 1 || p.tiles * kv_heads >= 256) break;
+    }
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(16, 256 / (p.tiles * kv_heads)));
+    p.part_rows = p.splits == 1 ? 0 : (uint64_t)p.tiles * kv_heads * p.splits * 32 * p.row_waves;
+    return p;
 }
-static int attend_tiles(int64_t group, int64_t max_q) { return (int)std::min<int64_t>((group * max_q + 15) / 16, 65535); }
-// Partials of rows whose keys several workgroups share: none where one has them all.
-static uint64_t part_rows(int tiles, int wgs) { return wgs == 1 ? 0 : (uint64_t)tiles * wgs * 2 * 16; }
 static uint64_t part_bytes(uint64_t rows, int head_dim) { return rows * (4 * head_dim + 8); }
 
 }  // namespace kvrt
@@ -582,11 +602,12 @@ int kvrt_block8_gather_async(const kvrt_block8 *pages, const kvrt_tensor *table,
     return e == hipSuccess ? KVRT_OK : KVRT_EDEVICE;
 }
 
-uint64_t kvrt_block8_attend_work(const kvrt_block8 *pages, int64_t n, int64_t width, int64_t hq, int32_t max_q) {
+uint64_t kvrt_block8_attend_work(const kvrt_block8 *pages, int64_t n, int64_t width, int64_t rows, int64_t hq,
+                                 int32_t max_q) {
     Block8View v;
-    if (!view_of(pages, v) || n <= 0 || width <= 0 || hq <= 0 || hq % pages->kv_heads != 0 || max_q <= 0) return 0;
-    const int tiles = attend_tiles(hq / pages->kv_heads, max_q);
-    return part_bytes(part_rows(tiles, attend_wgs(v, n, width, tiles, pages->head_dim)), pages->head_dim);
+    if (!view_of(pages, v) || n <= 0 || width <= 0 || rows <= 0 || hq <= 0 || hq % pages->kv_heads != 0 || max_q <= 0) return 0;
+    const AttendPlan p = attend_plan(v.kv_heads, v.shift, pages->head_dim, n, width, rows, hq / v.kv_heads, max_q);
+    return part_bytes(p.part_rows, pages->head_dim);
 }
 
 int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, const kvrt_tensor *table,
@@ -603,20 +624,25 @@ int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, con
     if (q->dims[2] != pages->head_dim || hq < 1 || hq % pages->kv_heads != 0 || hq / pages->kv_heads > 64)
         return KVRT_EINVAL;
     if (!std::isfinite(scale) || window < 0 || max_q < 0 || q->dims[0] > kMaxRows) return KVRT_EINVAL;
-    if (hq / pages->kv_heads * max_q > 16 * 65535) return KVRT_EINVAL;  // row tiles are a grid dimension
+    if (hq / pages->kv_heads * max_q >= (int64_t)1 << 30) return KVRT_EINVAL;  // rows of a head are numbered in 32 bits
     if (q->dims[0] == 0 || n == 0 || max_q == 0) return KVRT_OK;
     if (!disjoint(out) || !aligned(lengths, 4) || !aligned(starts, 4) || (granted && !aligned(granted, 4)) ||
         (width > 0 && !table->data))
         return KVRT_EINVAL;
     a.group = (int)(hq / pages->kv_heads);
-    const int tiles = attend_tiles(a.group, max_q);
-    const int64_t most = most_units(a.p, std::max<int64_t>(width, 1)), heads = n * pages->kv_heads;
-    if (most * heads >= (int64_t)1 << 31) return KVRT_EINVAL;  // units are numbered in 32 bits
-    a.wgs = attend_wgs(a.p, n, std::max<int64_t>(width, 1), tiles, pages->head_dim);
-    const uint64_t prows = part_rows(tiles, a.wgs);
-    if (prows > 0 && (!aligned(work, 16) || work_bytes < part_bytes(prows, pages->head_dim))) return KVRT_EINVAL;
+    const AttendPlan plan = attend_plan(a.p.kv_heads, a.p.shift, pages->head_dim, n, std::max<int64_t>(width, 1), q->dims[0],
+                                        a.group, max_q);
+    const int64_t heads = n * pages->kv_heads;
+    if (!plan.chunk && plan.most * heads >= (int64_t)1 << 31) return KVRT_EINVAL;  // units are numbered in 32 bits
+    if (plan.chunk && plan.tiles > 65535) return KVRT_EINVAL;                      // row tiles are a grid dimension
+    if (plan.part_rows > 0 && (!aligned(work, 16) || work_bytes < part_bytes(plan.part_rows, pages->head_dim)))
+        return KVRT_EINVAL;
     a.part_o = static_cast<float *>(work);
-    a.part_ml = reinterpret_cast<float2 *>(static_cast<float *>(work) + prows * pages->head_dim);
+    a.part_ml = reinterpret_cast<float2 *>(static_cast<float *>(work) + plan.part_rows * pages->head_dim);
+    a.wgs = plan.wgs;
+    a.row_waves = plan.row_waves;
+    a.tiles = (int)plan.tiles;
+    a.splits = plan.splits;
     a.q = static_cast<const uint16_t *>(q->data);
     a.out = static_cast<uint16_t *>(out->data);
     a.q_row = q->strides[0];
@@ -634,20 +660,22 @@ int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, con
     a.max_q = max_q;
     a.window = window;
     a.scale_log2 = scale * 1.4426950408889634f;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (plan.chunk)
+        return launch_block8_chunk(a, pages->dtype, pages->head_dim, st) == hipSuccess ? KVRT_OK : KVRT_EDEVICE;
     // Joined inside the launch: heads whose partials the last workgroup reads in a few
     // loads. Where that many workgroups per head fill the card, or a head never has
     // more, all are; else a second launch joins the others.
-    const hipStream_t st = static_cast<hipStream_t>(stream);
     bool join = false;
     if (a.wgs > 1) {
         const int64_t rows = std::min<int64_t>(16, (int64_t)a.group * max_q);
         a.join_most = (int)std::min<int64_t>(32, kJoinBytes / (rows * pages->head_dim * 4));
-        a.counters = tiles == 1 && a.join_most > 1 ? block8_counter_slice(st) : nullptr;
+        a.counters = a.join_most > 1 ? block8_counter_slice(st) : nullptr;
         if (!a.counters) a.join_most = 1;
-        a.join_all = most > a.join_most && heads * (a.join_most - 1) >= 512;
-        join = most > a.join_most && !a.join_all;
+        a.join_all = plan.most > a.join_most && heads * (a.join_most - 1) >= 512;
+        join = plan.most > a.join_most && !a.join_all;
     }
-    const hipError_t e = launch_block8_attend(a, pages->dtype, pages->head_dim, tiles, join, st);
+    const hipError_t e = launch_block8_attend(a, pages->dtype, pages->head_dim, join, st);
     return e == hipSuccess ? KVRT_OK : KVRT_EDEVICE;
 }
 

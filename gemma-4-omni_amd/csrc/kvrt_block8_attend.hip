@@ -25,49 +25,14 @@
 #include <mutex>
 #include <utility>
 
-#include "kvrt_block8.h"
+#include "kvrt_block8_rows.h"
 
 namespace kvrt {
 
 namespace {
 
 constexpr int kTileKeys = 32, kUnitTiles = 4;  // a unit of division: one 32-key tile per wave
-constexpr float kWeightShift = 7.f;
 
-// A request as one row tile sees it.
-struct Rows {
-    int start, count;  // packed rows
-    int length;        // keys
-    int n;             // rows of the tile (0: none)
-    int first, last;   // positions of its first and last query
-    int kend;          // keys [kstart, kend) can be seen by some row
-    int kstart;
-};
-
-__device__ __forceinline__ Rows rows_of(const Block8AttendArgs &a, int start, int count, int length, int tile) {
-    Rows r;
-    r.start = start;
-    r.count = count;
-    r.length = length;
-    r.n = min(max(count * a.group - 16 * tile, 0), 16);
-    const int base = length - count;  // below 0: rows before the first key see nothing
-    r.first = base + 16 * tile / a.group;
-    r.last = base + (16 * tile + max(r.n, 1) - 1) / a.group;
-    r.kend = r.n > 0 ? min(max(r.last + 1, 0), length) : 0;
-    r.kstart = a.window > 0 ? min(max(r.first - a.window + 1, 0), r.kend) : 0;
-    return r;
-}
-// Request i from its words; what is out of range is brought into it and reported.
-__device__ __forceinline__ Rows load_rows(const Block8AttendArgs &a, int i, int tile, bool &bad) {
-    const int cap = a.width << a.p.shift;
-    const int len = a.lengths[i], s0 = a.starts[i];
-    const int64_t m = a.granted ? (int64_t)a.granted[i] : (int64_t)a.starts[i + 1] - s0;
-    const int length = min(max(len, 0), cap);
-    const int start = (int)min((int64_t)max(s0, 0), a.rows);
-    const int count = (int)min(min(max(m, (int64_t)0), (int64_t)a.max_q), a.rows - start);
-    bad |= length != len || start != s0 || count != m;
-    return rows_of(a, start, count, length, tile);
-}
 // Units of a head of the request. Rows without keys are one too: their zeros have to
 // be written.
 __device__ __forceinline__ int units_of(const Rows &r) {
@@ -89,74 +54,6 @@ __device__ __forceinline__ Division divide(const Block8AttendArgs &a, int units,
     // workgroups, no head's over more than one joins (join_most >= 2)
     if (a.join_all) d.per = max(d.per, (most + a.join_most - 2) / (a.join_most - 1));
     return d;
-}
-
-// Running sum over the workgroup's 256 threads (exclusive), the sum and the largest.
-__device__ __forceinline__ int scan256(int x, int *lds, int &total, int &most) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int inc = x, top = x;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(inc, d);
-        if (lane >= d) inc += y;
-        top = max(top, __shfl_xor(top, d));
-    }
-    __syncthreads();
-    if (lane == 63) lds[wave] = inc, lds[4 + wave] = top;
-    __syncthreads();
-    int before = 0;
-    total = 0, most = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (w < wave) before += lds[w];
-        total += lds[w];
-        most = max(most, lds[4 + w]);
-    }
-    return before + inc - x;
-}
-
-// Keys' words that nothing in the launch writes: uniform ones load as scalars.
-typedef const __attribute__((address_space(4))) int32_t *ConstInts;
-typedef const __attribute__((address_space(4))) float *ConstFloats;
-
-// Joins partials p = 0 .. n - 1 of four output elements of a row, in their order,
-// sixteen at a time: ld(p, ml, o) reads one. The launch that makes the partials and
-// the join kernel both use it, so both give the same bits.
-template <class Ld>
-__device__ __forceinline__ void join_partials(int n, Ld ld, float &M, float &sum, float4 &o) {
-    constexpr int B = 16;
-    for (int p0 = 0; p0 < n; p0 += B) {
-        float2 ml[B];
-        float4 x[B];
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            ml[i] = make_float2(kNegBig, 0.f);
-            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (p0 + i < n) ld(p0 + i, ml[i], x[i]);
-        }
-        float top = M;
-#pragma unroll
-        for (int i = 0; i < B; ++i) top = fmaxf(top, ml[i].x);
-        const float c = __builtin_amdgcn_exp2f(M - top);
-        sum *= c;
-        o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
-        M = top;
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const float f = __builtin_amdgcn_exp2f(ml[i].x - M);
-            sum = fmaf(ml[i].y, f, sum);
-            o = make_float4(fmaf(x[i].x, f, o.x), fmaf(x[i].y, f, o.y), fmaf(x[i].z, f, o.z), fmaf(x[i].w, f, o.w));
-        }
-    }
-}
-
-// Four elements of a row of the answer: dims d .. d + 3 of row `row` of the head.
-__device__ __forceinline__ void store_out(const Block8AttendArgs &a, const Rows &r, int head, int row, int d, float4 o,
-                                          float sum) {
-    const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
-    const int qr = row / a.group, hr = row - qr * a.group;
-    uint16_t *out = a.out + (int64_t)(r.start + qr) * a.o_row + (int64_t)(head * a.group + hr) * a.o_head + d;
-    *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
 }
 
 // N dwords of a lane from p (N = 1, 2, 4, 8; p aligned to min(4 N, 16) bytes).
@@ -182,23 +79,19 @@ __device__ __forceinline__ f32x4_t mfma16(const uint32_t (&a)[4], const uint32_t
                                                   0);
 }
 
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){lo, hi}, f16x2_t));
-}
-
 // Q^T of a row tile as fp16 operands: lane (row l%16, group l/16) holds for step c
 // the dims 64(c/2) + 16(l/16) + 8(c%2) + 0..7 of its row, scaled by 2^shift so that
-// the row's largest element lies in [2^14, 2^15). back: 2^-shift.
+// the row's largest element lies in [2^14, 2^15). back: 2^-shift. Lanes without a row
+// are given another's: loads that only some lanes make are a divergent region, and
+// the registers are too full for one.
 template <int D>
-__device__ __forceinline__ void load_query(const uint16_t *row, bool valid, uint32_t flip, uint32_t (&op)[D / 32][4],
+__device__ __forceinline__ void load_query(const uint16_t *row, uint32_t flip, uint32_t (&op)[D / 32][4],
                                            float &back) {
     const int grp = (threadIdx.x & 63) >> 4;
     uint4 raw[D / 32];
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-        raw[c] = valid ? *reinterpret_cast<const uint4 *>(row + 64 * (c / 2) + 16 * grp + 8 * (c % 2))
-                       : make_uint4(0, 0, 0, 0);
-    }
+    for (int c = 0; c < D / 32; ++c)
+        raw[c] = *reinterpret_cast<const uint4 *>(row + 64 * (c / 2) + 16 * grp + 8 * (c % 2));
     uint32_t top = 0;  // largest exponent field (with mantissa: bits of |x|)
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
@@ -235,7 +128,8 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
     __shared__ uint32_t arrived;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
-    const int tile = blockIdx.y, wg = blockIdx.x;
+    constexpr int tile = 0;  // a head's rows are one tile
+    const int wg = blockIdx.x;
 
     // this workgroup's units [u, uend), the request of the first and the units before it
     bool bad = false, unmapped = false;
@@ -245,7 +139,7 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
     if (a.n <= 64) {
         int units = 0;
         if (lane < a.n) {
-            mine = load_rows(a, lane, tile, bad);
+            mine = load_rows(a, lane, tile, 16, bad);
             units = units_of(mine);
         }
         int inc = units, top = units;
@@ -270,7 +164,7 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
         for (int base = 0; base < a.n; base += 256) {
             const int i = base + threadIdx.x;
             int sum, top;
-            scan256(i < a.n ? units_of(load_rows(a, i, tile, bad)) : 0, scan_lds, sum, top);
+            scan_wg<4>(i < a.n ? units_of(load_rows(a, i, tile, 16, bad)) : 0, scan_lds, sum, top);
             all += sum;
             most = max(most, top);
         }
@@ -280,9 +174,9 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
             int at = 0;
             for (int base = 0; base < a.n; base += 256) {
                 const int i = base + threadIdx.x;
-                const int units = i < a.n ? units_of(load_rows(a, i, tile, bad)) * a.p.kv_heads : 0;
+                const int units = i < a.n ? units_of(load_rows(a, i, tile, 16, bad)) * a.p.kv_heads : 0;
                 int sum, top;
-                const int first = at + scan256(units, scan_lds, sum, top);
+                const int first = at + scan_wg<4>(units, scan_lds, sum, top);
                 at += sum;
                 if (first <= u && u < first + units) found[0] = i, found[1] = first;
             }
@@ -305,11 +199,12 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
         Rows r;
         if (a.n <= 64) {
             r = rows_of(a, __builtin_amdgcn_readlane(mine.start, req), __builtin_amdgcn_readlane(mine.count, req),
-                        __builtin_amdgcn_readlane(mine.length, req), tile);
+                        __builtin_amdgcn_readlane(mine.length, req), tile, 16);
         } else {
             bool ignore = false;
-            r = load_rows(a, req, tile, ignore);
+            r = load_rows(a, req, tile, 16, ignore);
         }
+        r = uniform(r);
         const int units = units_of(r);
         if (u >= before + units * a.p.kv_heads) {
             before += units * a.p.kv_heads;
@@ -379,8 +274,8 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
             take_pages();
             load_k(t_begin);
             load_v(t_begin);
-            load_query<D>(a.q + (int64_t)(r.start + qr) * a.q_row + (int64_t)(head * a.group + hr) * a.q_head, valid, flip,
-                          qop, back);
+            load_query<D>(a.q + (int64_t)(r.start + qr) * a.q_row + (int64_t)(head * a.group + hr) * a.q_head, flip, qop,
+                          back);
             load_ids(min(t_begin + kUnitTiles, t_end - 1));
             const float qscale = scale * back;
             float m = kNegBig, l = 0.f;
@@ -497,7 +392,7 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
         const bool begins = ua == 0, ends = ub == units;
         const int w0 = seg / div.per, count = (seg + units - 1) / div.per - w0 + 1;  // workgroups of the head
         const bool here = count <= a.join_most;                                       // joined in this launch
-        const int64_t slot0 = (int64_t)tile * a.wgs * 2;
+        const int64_t slot0 = 0;
         for (int e = threadIdx.x; e < r.n * (D / 4); e += 256) {
             const int rr = e / (D / 4), d = 4 * (e % (D / 4));
             float M = kNegBig, sum = 0.f;
@@ -569,18 +464,19 @@ __global__ __launch_bounds__(256) void block8_join_kernel(Block8AttendArgs a) {
     __shared__ int scan_lds[8];
     __shared__ float4 so[256];
     __shared__ float2 sml[256];
-    const int tile = blockIdx.y, rr = blockIdx.z, head = blockIdx.x % a.p.kv_heads, req = blockIdx.x / a.p.kv_heads;
+    constexpr int tile = 0;
+    const int rr = blockIdx.y, head = blockIdx.x % a.p.kv_heads, req = blockIdx.x / a.p.kv_heads;
     bool bad = false;
-    const Rows r = load_rows(a, req, tile, bad);
+    const Rows r = load_rows(a, req, tile, 16, bad);
     if (rr >= r.n) return;
     // units before the request, all, and the most of a head
     int all = 0, before = 0, most = 0;
     for (int base = 0; base < a.n; base += 256) {
         const int i = base + threadIdx.x;
-        const int mine = i < a.n ? units_of(load_rows(a, i, tile, bad)) : 0;
+        const int mine = i < a.n ? units_of(load_rows(a, i, tile, 16, bad)) : 0;
         int sum, less, top, ignore;
-        scan256(mine, scan_lds, sum, top);
-        scan256(i < req ? mine : 0, scan_lds, less, ignore);
+        scan_wg<4>(mine, scan_lds, sum, top);
+        scan_wg<4>(i < req ? mine : 0, scan_lds, less, ignore);
         all += sum;
         before += less;
         most = max(most, top);
@@ -594,7 +490,7 @@ __global__ __launch_bounds__(256) void block8_join_kernel(Block8AttendArgs a) {
     float M = kNegBig, sum = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if (group < groups) {
-        const int64_t slot0 = ((int64_t)tile * a.wgs + w0) * 2;
+        const int64_t slot0 = 2 * w0;
         join_partials((count - group + groups - 1) / groups, [&](int p, float2 &ml, float4 &y) __attribute__((always_inline)) {
             const int i = p * groups + group;
             const int64_t at = (slot0 + 2 * i + (i == 0 ? 1 : 0)) * 16 + rr;
@@ -620,29 +516,29 @@ __global__ __launch_bounds__(256) void block8_join_kernel(Block8AttendArgs a) {
 }
 
 template <int CODE, int D>
-static hipError_t launch_attend(const Block8AttendArgs &a, int tiles, bool join, hipStream_t s) {
-    hipLaunchKernelGGL((block8_attend_kernel<CODE, D>), dim3(a.wgs, tiles), dim3(256), 0, s, a);
+static hipError_t launch_attend(const Block8AttendArgs &a, bool join, hipStream_t s) {
+    hipLaunchKernelGGL((block8_attend_kernel<CODE, D>), dim3(a.wgs), dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !join) return e;
     const int rows = (int)std::min<int64_t>(16, (int64_t)a.group * a.max_q);
-    hipLaunchKernelGGL((block8_join_kernel<D>), dim3(a.n * a.p.kv_heads, tiles, rows), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((block8_join_kernel<D>), dim3(a.n * a.p.kv_heads, rows), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
 template <int CODE>
-static hipError_t launch_attend_code(const Block8AttendArgs &a, int head_dim, int tiles, bool join, hipStream_t s) {
+static hipError_t launch_attend_code(const Block8AttendArgs &a, int head_dim, bool join, hipStream_t s) {
     switch (head_dim) {
-        case 64: return launch_attend<CODE, 64>(a, tiles, join, s);
-        case 128: return launch_attend<CODE, 128>(a, tiles, join, s);
-        case 256: return launch_attend<CODE, 256>(a, tiles, join, s);
-        case 512: return launch_attend<CODE, 512>(a, tiles, join, s);
+        case 64: return launch_attend<CODE, 64>(a, join, s);
+        case 128: return launch_attend<CODE, 128>(a, join, s);
+        case 256: return launch_attend<CODE, 256>(a, join, s);
+        case 512: return launch_attend<CODE, 512>(a, join, s);
         default: return hipErrorInvalidValue;
     }
 }
 
-hipError_t launch_block8_attend(const Block8AttendArgs &a, int dtype, int head_dim, int tiles, bool join, hipStream_t s) {
-    return dtype == KVRT_INT8 ? launch_attend_code<KVRT_INT8>(a, head_dim, tiles, join, s)
-                              : launch_attend_code<KVRT_E4M3>(a, head_dim, tiles, join, s);
+hipError_t launch_block8_attend(const Block8AttendArgs &a, int dtype, int head_dim, bool join, hipStream_t s) {
+    return dtype == KVRT_INT8 ? launch_attend_code<KVRT_INT8>(a, head_dim, join, s)
+                              : launch_attend_code<KVRT_E4M3>(a, head_dim, join, s);
 }
 
 // ---- arrival counters ---------------------------------------------------------------

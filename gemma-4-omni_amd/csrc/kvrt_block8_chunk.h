@@ -1,0 +1,508 @@
+// kvrt_block8_chunk.h — attention of many query rows per request over 8-bit pages.
+//
+// The mathematics is kvrt_block8_attend.hip's (codes as fp16, the V scale in the
+// exponent); here 32 rows of a (request, KV head) lie on one wave and a workgroup's
+// four waves share the keys: 32-key blocks are converted to fp16 once, into LDS, and
+// each wave takes per block
+//   S^T (32 keys x 32 rows) = K Q^T     D/16    v_mfma_f32_32x32x16_f16
+//   softmax per row (fp32, base 2)
+//   O^T (D x 32) += V^T P^T             2 D/32  v_mfma_f32_32x32x16_f16
+// A row tile is 32, 64 or 128 rows (launch) on RW = 1, 2 or 4 row blocks, fewer where
+// the request's last tile has fewer rows; the 4 / RW waves of a row block take the
+// staged blocks in turn and are combined through LDS at the end. With few tiles the
+// keys are also divided over `splits` workgroups, joined by a second launch.
+//
+// Lane layouts (32x32x16): A[row l%32][k 8(l/32)+j], B[k 8(l/32)+j][col l%32],
+// D[row 8(i/4) + 4(l/32) + i%4][col l%32].
+#pragma once
+
+#include "kvrt_block8_rows.h"
+
+namespace kvrt {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+// LDS rows: K pitched so that 16 consecutive rows' 16-byte chunks lie on all 64 banks,
+// V so that 4 rows' 64 bytes do (the transposed reads).
+template <int D>
+struct ChunkShape {
+    static constexpr int NW = D == 512 ? 8 : 4;  // waves
+    static constexpr int DS = D == 512 ? 2 : 1;  // waves that share a row block's head dims
+    static constexpr int RB = NW / DS;           // row blocks at most
+    static constexpr int NBLK = D <= 128 ? 4 : D == 256 ? 2 : 1;  // 32-key blocks staged at a time
+    static constexpr int KEYS = 32 * NBLK;
+    static constexpr int NBUF = D == 256 ? 2 : 1;  // (D <= 128: one buffer and two workgroups per CU)
+    static constexpr int KP = 2 * D + 16, VP = 2 * D + 64;  // bytes
+    static constexpr int PASSES = KEYS * D / (NW * 1024);   // 16-code chunks per thread of K (and of V)
+    static constexpr int BUF = KEYS * (KP + VP);
+    // codes wait for their step in LDS instead of in registers (D 512 has none left)
+    static constexpr bool DMA = D == 512;
+    static constexpr int RAW = DMA ? 2 * KEYS * D : 16;
+    static constexpr int QL = D == 512 ? 3 : 0;  // ... nor for the last of the Q operands
+    static constexpr int SX = DS > 1 ? NW * 4096 : 16;  // scores the waves of a row block exchange
+};
+
+struct ChunkScale {
+    float k, log_v, inv_v, ok;
+};
+
+__device__ __forceinline__ f32x16_t mfma32_f16(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0,
+                                                  0);
+}
+
+// Sixteen codes as 32 bytes of fp16.
+template <int CODE>
+__device__ __forceinline__ void write_f16(uint8_t *dst, uint4 w) {
+    uint4 a, b;
+    codes_to_f16<CODE>(w.x, a.x, a.y);
+    codes_to_f16<CODE>(w.y, a.z, a.w);
+    codes_to_f16<CODE>(w.z, b.x, b.y);
+    codes_to_f16<CODE>(w.w, b.z, b.w);
+    *reinterpret_cast<uint4 *>(dst) = a;
+    *reinterpret_cast<uint4 *>(dst + 16) = b;
+}
+
+// Tiles of `size` rows of the request.
+__device__ __forceinline__ int tiles_of(const Block8AttendArgs &a, const Rows &r, int size) {
+    return (r.count * a.group + size - 1) / size;
+}
+
+// The request that has tile u of all requests', its first tile; false past the last.
+// Every thread of the workgroup calls.
+template <int NW>
+__device__ __forceinline__ bool tile_request(const Block8AttendArgs &a, int size, int u, int &req, int &before,
+                                             bool &bad) {
+    const int lane = threadIdx.x & 63;
+    if (a.n <= 64) {
+        int tiles = 0;
+        if (lane < a.n) tiles = tiles_of(a, load_rows(a, lane, 0, size, bad), size);
+        int inc = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(inc, d);
+            if (lane >= d) inc += y;
+        }
+        const uint64_t past = __ballot(inc > u);
+        if (past == 0) return false;
+        req = __builtin_ctzll(past);
+        before = __builtin_amdgcn_readlane(inc - tiles, req);
+        return true;
+    }
+    __shared__ int lds[2 * NW], found[2];
+    int at = 0;
+    bool have = false;
+    for (int base = 0; base < a.n && !have; base += 64 * NW) {
+        const int i = base + threadIdx.x;
+        const int tiles = i < a.n ? tiles_of(a, load_rows(a, i, 0, size, bad), size) : 0;
+        int sum, top;
+        const int first = at + scan_wg<NW>(tiles, lds, sum, top);
+        at += sum;
+        if (first <= u && u < first + tiles) found[0] = i, found[1] = first;
+        have = u < at;
+    }
+    if (!have) return false;
+    __syncthreads();
+    req = __builtin_amdgcn_readfirstlane(found[0]);
+    before = __builtin_amdgcn_readfirstlane(found[1]);
+    return true;
+}
+
+// Key ranges the tile's keys are divided over (of at most a.splits).
+template <int D>
+__device__ __forceinline__ int splits_of(const Block8AttendArgs &a, const Rows &r) {
+    const int steps = (r.kend - r.kstart / 32 * 32 + ChunkShape<D>::KEYS - 1) / ChunkShape<D>::KEYS;
+    return min(a.splits, max(1, steps));
+}
+
+template <int CODE, int D>
+__global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Block8AttendArgs a) {
+    using C = ChunkShape<D>;
+    constexpr int NW = C::NW, DS = C::DS, DW = D / DS;  // head dims of a wave
+    constexpr int NB = DW / 32, NBLK = C::NBLK, KEYS = C::KEYS, PASSES = C::PASSES;
+    __shared__ __align__(16) uint8_t lds[C::NBUF * C::BUF];
+    __shared__ __align__(16) ChunkScale scales[C::NBUF][2 * NBLK];
+    __shared__ float2 sml[NW * 32];
+    __shared__ __align__(16) uint8_t sx[C::SX], raw[C::RAW];
+    __shared__ uint4 ql[C::QL ? NW * C::QL * 64 : 1];
+    constexpr int NQ = DW / 16, QR = NQ - C::QL;  // Q operands, those in registers
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    // grid (head, split, tile): heads lie on XCDs of their own where they are 8
+    const int size = 32 * a.row_waves;
+    const int head = blockIdx.x, split = blockIdx.y, u = blockIdx.z;
+    bool bad = false;
+    int req, before;
+    const bool mine = tile_request<NW>(a, size, u, req, before, bad);
+    if (bad) raise(a.p.status, KVRT_BLOCK_BAD_INDEX);
+    if (!mine) return;
+    bool ignore = false;
+    Rows r = load_rows(a, req, 0, size, ignore);
+    const int tile = tiles_of(a, r, size) - 1 - (u - before);  // most keys first
+    r = uniform(rows_of(a, r.start, r.count, r.length, tile, size));
+    const int splits = splits_of<D>(a, r);
+    if (split >= splits) return;
+
+    const int RW = NBLK == 1 || r.n > 64 ? C::RB : r.n > 32 ? 2 : 1, KS = C::RB / RW;
+    const int ds = wave & (DS - 1), rw = (wave / DS) & (RW - 1), part = wave / DS / RW;
+    const int row0 = size * tile + 32 * rw, rows = r.count * a.group;
+    const bool wlive = 32 * rw < r.n, valid = wlive && row0 + col < rows;
+    const int row = valid ? row0 + col : size * tile;
+    const int qr = row / a.group, hr = row - qr * a.group;
+    const int base = r.length - r.count, pos = base + qr;
+    // positions of this wave's first and last query
+    const int wfirst = base + row0 / a.group, wlast = base + (min(rows, row0 + 32) - 1) / a.group;
+
+    // the split's keys: steps [s0, s1) of KEYS from k0 on
+    const int k0 = r.kstart / 32 * 32;
+    const int steps = (r.kend - k0 + KEYS - 1) / KEYS;
+    const int s0 = steps * split / splits, s1 = steps * (split + 1) / splits;
+
+    // Q^T operands: lane (row col, half) holds dims 16c + 8half + 0..7 of its row, scaled
+    // by a power of two so that the row's largest element lies in [2^14, 2^15)
+    uint4 qop[QR];
+    float qscale;
+    {
+        const uint16_t *q = a.q + (int64_t)(r.start + qr) * a.q_row + (int64_t)(head * a.group + hr) * a.q_head + 8 * half +
+                            ds * DW;
+        uint4 qraw[NQ];
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(q + 16 * c);  // (lanes without a row: the tile's first)
+            qraw[c] = w;
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = max(top, max(ws[i] & 0x7fffu, (ws[i] >> 16) & 0x7fffu));
+        }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        if constexpr (DS > 1) {  // the row's largest element over both waves' dims
+            uint32_t *tops = reinterpret_cast<uint32_t *>(sx);
+            if (half == 0) tops[wave * 32 + col] = top;
+            __syncthreads();
+            top = max(top, tops[(wave ^ 1) * 32 + col]);
+            __syncthreads();
+        }
+        const int shift = 14 + 127 - (int)max(top >> 7, 1u);
+        const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+        qscale = fabsf(a.scale_log2) * ldexpf(1.0f, -shift);
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) {
+            const uint32_t ws[4] = {qraw[c].x ^ flip, qraw[c].y ^ flip, qraw[c].z ^ flip, qraw[c].w ^ flip};
+            uint32_t x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = pack_f16(ldexpf(bf16_lo(ws[i]), shift), ldexpf(bf16_hi(ws[i]), shift));
+            if (c < QR) qop[c < QR ? c : 0] = make_uint4(x[0], x[1], x[2], x[3]);
+            else ql[(wave * C::QL + c - QR) * 64 + lane] = make_uint4(x[0], x[1], x[2], x[3]);
+        }
+    }
+
+    float m = kNegBig, l = 0.f;
+    f32x16_t o[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
+
+    // ---- staging
+    const ConstInts entries = (ConstInts)(uintptr_t)a.table + (int64_t)req * a.table_stride;
+    const ConstFloats k_scale = (ConstFloats)(uintptr_t)a.p.k_scale, v_scale = (ConstFloats)(uintptr_t)a.p.v_scale;
+    constexpr int LPR = D / 16, RPP = 64 * NW / LPR, RPWV = 64 / LPR;  // lanes per row, rows per pass and per wave of it
+    const int srow = threadIdx.x / LPR, schunk = threadIdx.x % LPR;
+    uint4 kr[C::DMA ? 1 : PASSES], vr[C::DMA ? 1 : PASSES];
+    const uint32_t raw_at = lds_addr(raw) + wave * PASSES * 2048;  // this wave's [pass][K, V][lane]
+    float next_k = 0.f, next_v = 0.f;  // scales of 16-key block threadIdx.x; next_k < 0: unmapped
+    bool unmapped = false;
+    // codes of step s to registers; keys nobody sees (past the last, on unmapped pages)
+    // as zeros
+    auto fetch = [&](int s) __attribute__((always_inline)) {
+        const int key0 = k0 + s * KEYS;
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            // a wave's rows of a pass lie in one 16-key block, so on one page
+            const int wkey = key0 + p * RPP + wave * RPWV, key = key0 + p * RPP + srow;
+            const int id = entries[min(wkey, r.kend - 1) >> a.p.shift];
+            const bool ok = (unsigned)id < (unsigned)a.p.pages;
+            const int64_t at = ((((int64_t)(ok ? id : 0) * a.p.kv_heads + head) << a.p.shift) +
+                                (wkey & (a.p.block - 1))) * D;
+            const uint32_t lane_at = (uint32_t)((srow - wave * RPWV) * D + 16 * schunk);
+            if constexpr (C::DMA) {
+                dma_load16_cached(a.p.k + at + lane_at, raw_at + p * 2048);
+                dma_load16_cached(a.p.v + at + lane_at, raw_at + p * 2048 + 1024);
+                continue;
+            }
+            kr[p] = *reinterpret_cast<const uint4 *>(a.p.k + at + lane_at);
+            vr[p] = *reinterpret_cast<const uint4 *>(a.p.v + at + lane_at);
+            if (!ok || wkey + RPWV > r.kend || wkey < r.kstart) {
+                const bool data = ok && key < r.kend && key >= r.kstart;
+                kr[p] = data ? kr[p] : make_uint4(0, 0, 0, 0);
+                vr[p] = data ? vr[p] : make_uint4(0, 0, 0, 0);
+            }
+        }
+        if (threadIdx.x < 2 * NBLK) {  // the 16-key blocks' scales
+            const int key = key0 + 16 * threadIdx.x;
+            const int id = a.table[(int64_t)req * a.table_stride + (min(key, r.kend - 1) >> a.p.shift)];
+            const bool ok = (unsigned)id < (unsigned)a.p.pages;
+            unmapped |= !ok && key < r.kend && key + 16 > r.kstart;
+            const int64_t at = (int64_t)(ok ? id : 0) * a.p.kv_heads + head;
+            next_v = a.p.v_scale[at];
+            next_k = a.p.k_scale[at];
+            if (!ok) next_k = -1.f;
+            else next_k = fmaxf(next_k, 0.f);
+        }
+    };
+    auto stage = [&](int buf, int s) __attribute__((always_inline)) {
+        uint8_t *kl = lds + buf * C::BUF, *vl = kl + KEYS * C::KP;
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            const int rr = p * RPP + srow;
+            uint4 kw, vw;
+            if constexpr (C::DMA) {  // a lane reads what it fetched itself
+                if (p == 0) wait_vmem<0>();
+                const uint4 *from = reinterpret_cast<const uint4 *>(raw) + (wave * PASSES + p) * 128 + lane;
+                kw = from[0];
+                vw = from[64];
+                const int wkey = k0 + s * KEYS + p * RPP + wave * RPWV, key = k0 + s * KEYS + rr;
+                const bool ok = (unsigned)entries[min(wkey, r.kend - 1) >> a.p.shift] < (unsigned)a.p.pages;
+                if (!ok || wkey + RPWV > r.kend || wkey < r.kstart) {
+                    const bool data = ok && key < r.kend && key >= r.kstart;
+                    kw = data ? kw : make_uint4(0, 0, 0, 0);
+                    vw = data ? vw : make_uint4(0, 0, 0, 0);
+                }
+            } else {
+                kw = kr[p];
+                vw = vr[p];
+            }
+            write_f16<CODE>(kl + rr * C::KP + 32 * schunk, kw);
+            write_f16<CODE>(vl + rr * C::VP + 32 * schunk, vw);
+        }
+        if constexpr (C::DMA) wait_lds();  // read before the next step's codes land there
+        if (threadIdx.x < 2 * NBLK) {
+            const float v = scale_in_range(next_v);
+            scales[buf][threadIdx.x] = ChunkScale{scale_in_range(next_k), __builtin_amdgcn_logf(v), __builtin_amdgcn_rcpf(v),
+                                                  next_k < 0.f ? 0.f : 1.f};
+        }
+    };
+
+    // ---- one 32-key block
+    const int kadr = col * C::KP + 16 * half + 2 * ds * DW;
+    const int s16 = lane & 15;
+    const int vadr = (4 * half + (s16 >> 2)) * C::VP + 32 * ((lane >> 4) & 1) + 8 * (s16 & 3) + 2 * ds * DW;
+    // (`live` is false only where DS > 1: all waves exchange at the same time)
+    auto block = [&](int buf, int blk, int key0, bool live) __attribute__((always_inline)) {
+        const uint8_t *kl = lds + buf * C::BUF + blk * 32 * C::KP + kadr;
+        const uint8_t *vl = lds + buf * C::BUF + KEYS * C::KP + blk * 32 * C::VP + vadr;
+        f32x16_t s;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) {
+            if (DS == 1 || live)
+                s = mfma32_f16(*reinterpret_cast<const uint4 *>(kl + 32 * c),
+                               c < QR ? qop[c < QR ? c : 0] : ql[(wave * C::QL + c - QR) * 64 + lane], s);
+            if (DS > 1 && c % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // (read ahead, more operands than registers)
+        }
+        if constexpr (DS > 1) {
+            float4 *to = reinterpret_cast<float4 *>(sx) + wave * 256 + lane;
+            const float4 *from = reinterpret_cast<const float4 *>(sx) + (wave ^ 1) * 256 + lane;
+            if (live)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) to[g * 64] = make_float4(s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]);
+            __syncthreads();
+            if (!live) return;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 x = from[g * 64];
+                s[4 * g] += x.x, s[4 * g + 1] += x.y, s[4 * g + 2] += x.z, s[4 * g + 3] += x.w;
+                if (g == 1) __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        const ChunkScale sa = scales[buf][2 * blk], sb = scales[buf][2 * blk + 1];
+        const bool whole = key0 + 32 <= min(r.kend, wfirst + 1) && (a.window <= 0 || key0 > wlast - a.window) &&
+                           sa.ok + sb.ok == 2.f;
+        if (!__builtin_amdgcn_readfirstlane(whole)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = key0 + 8 * (i >> 2) + 4 * half + (i & 3);
+                const bool seen = (i < 8 ? sa.ok : sb.ok) != 0.f && key <= pos && key < r.kend &&
+                                  (a.window <= 0 || key > pos - a.window);
+                s[i] = seen ? s[i] : -INFINITY;
+            }
+        }
+        // above 0, so that a masked score stays one
+        const float ca = fmaxf(qscale * sa.k, 1e-37f), cb = fmaxf(qscale * sb.k, 1e-37f);
+        float ta = s[0], tb = s[8];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) ta = fmaxf(ta, s[i]), tb = fmaxf(tb, s[8 + i]);
+        const float top = pair<OpMax, 32>(fmaxf(fmaf(ta, ca, sa.log_v), fmaf(tb, cb, sb.log_v)));
+        const float mn = top > m + kRescaleSlack ? top : m;
+        if (__any(mn != m)) {
+            const float corr = __builtin_amdgcn_exp2f(m - mn);
+            l *= corr;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) o[b] *= corr;
+            m = mn;
+        }
+        const float da = sa.log_v + (kWeightShift - m), db = sb.log_v + (kWeightShift - m);
+        uint4 p[2];
+        float la = 0.f, lb = 0.f;
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float e0 = __builtin_amdgcn_exp2f(fmaf(s[i], i < 8 ? ca : cb, i < 8 ? da : db));
+            const float e1 = __builtin_amdgcn_exp2f(fmaf(s[i + 1], i < 8 ? ca : cb, i < 8 ? da : db));
+            if (i < 8) la += e0 + e1;
+            else lb += e0 + e1;
+            w[i / 2] = pack_f16(e0, e1);
+        }
+        l = fmaf(la, sa.inv_v, fmaf(lb, sb.inv_v, l));
+        p[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        p[1] = make_uint4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const uint2 lo = lds_read_tr16(reinterpret_cast<const uint16_t *>(vl + 16 * h * C::VP + 64 * b));
+                const uint2 hi = lds_read_tr16(reinterpret_cast<const uint16_t *>(vl + (16 * h + 8) * C::VP + 64 * b));
+                o[b] = mfma32_f16(make_uint4(lo.x, lo.y, hi.x, hi.y), p[h], o[b]);
+                if (DS > 1 && b % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+            }
+    };
+
+    if (s0 < s1) {
+        fetch(s0);
+        if constexpr (C::NBUF == 2) {
+            stage(0, s0);
+            __syncthreads();
+        }
+        for (int s = s0; s < s1; ++s) {
+            const int buf = C::NBUF == 2 ? (s - s0) & 1 : 0;
+            if constexpr (C::NBUF == 1) {
+                if (s > s0) __syncthreads();  // the last step's blocks are read
+                stage(0, s);
+                if (s + 1 < s1) fetch(s + 1);
+                __syncthreads();
+            } else {
+                if (s + 1 < s1) fetch(s + 1);
+            }
+            for (int blk = part; blk < NBLK; blk += KS) {
+                const int key0 = k0 + s * KEYS + 32 * blk;
+                // blocks that no row of the wave sees
+                const bool live = wlive && key0 <= wlast && key0 < r.kend &&
+                                  (a.window <= 0 || key0 + 32 > wfirst - a.window + 1);
+                if (DS == 1 && !live) continue;
+                block(buf, blk, key0, live);
+            }
+            if constexpr (C::NBUF == 2) {
+                if (s + 1 < s1) stage(buf ^ 1, s + 1);
+                __syncthreads();
+            }
+        }
+    }
+    if (unmapped) raise(a.p.status, KVRT_BLOCK_BAD_INDEX);
+    l = pair<OpSum, 32>(l);
+
+    // ---- the answer, or this split's partial
+    const int64_t slot = ((int64_t)u * a.p.kv_heads + head) * a.splits + split;
+    // this lane's row again: kept over the loop it would cost registers that the loop needs
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int ecol = ln & 31, ehalf = ln >> 5, erow = row0 + ecol;
+    const bool evalid = wlive && erow < rows;
+    const int eq = (evalid ? erow : 0) / a.group, eh = (evalid ? erow : 0) - eq * a.group;
+    uint16_t *const out = a.out + (int64_t)(r.start + eq) * a.o_row + (int64_t)(head * a.group + eh) * a.o_head;
+    auto store4 = [&](int b, int g, float4 x, float inv) __attribute__((always_inline)) {
+        const int d = ds * DW + 32 * b + 8 * g + 4 * ehalf;
+        if (splits == 1) {
+            *reinterpret_cast<uint2 *>(out + d) = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+        } else {
+            *reinterpret_cast<float4 *>(a.part_o + (slot * size + 32 * rw + ecol) * D + d) = x;
+        }
+    };
+    if (KS == 1) {
+        if (!evalid) return;
+        const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                store4(b, g, make_float4(o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2], o[b][4 * g + 3]), inv);
+        if (splits > 1 && ehalf == 0 && ds == 0) a.part_ml[slot * size + 32 * rw + ecol] = make_float2(m, l);
+        return;
+    }
+    if constexpr (DS == 1) {
+    // combine the parts of each row block, BS 32-dim blocks at a time
+    constexpr int BS0 = C::NBUF * C::BUF / 16384, BS = BS0 >= NB ? NB : BS0 >= 8 ? 8 : BS0 >= 4 ? 4 : BS0 >= 2 ? 2 : 1;
+    static_assert(BS * 16384 <= C::NBUF * C::BUF && NB % BS == 0, "the waves' blocks fit the buffers");
+    __syncthreads();  // every wave is done with the buffers
+    if (ehalf == 0) sml[wave * 32 + ecol] = make_float2(m, l);
+    __syncthreads();
+    float M = kNegBig, sum = 0.f;
+    for (int p = 0; p < KS; ++p) M = fmaxf(M, sml[(p * RW + rw) * 32 + ecol].x);
+    for (int p = 0; p < KS; ++p) {
+        const float2 x = sml[(p * RW + rw) * 32 + ecol];
+        sum = fmaf(x.y, __builtin_amdgcn_exp2f(x.x - M), sum);
+    }
+    const float f = __builtin_amdgcn_exp2f(m - M), inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+    float4 *xl = reinterpret_cast<float4 *>(lds);  // [wave][block][g][lane]
+#pragma unroll
+    for (int b0 = 0; b0 < NB; b0 += BS) {
+        if (b0 > 0) __syncthreads();
+#pragma unroll
+        for (int b = 0; b < BS; ++b)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                xl[((wave * BS + b) * 4 + g) * 64 + ln] = make_float4(o[b0 + b][4 * g] * f, o[b0 + b][4 * g + 1] * f,
+                                                                     o[b0 + b][4 * g + 2] * f, o[b0 + b][4 * g + 3] * f);
+        __syncthreads();
+        for (int e = part; e < 4 * BS; e += KS) {
+            float4 x = xl[(rw * BS * 4 + e) * 64 + ln];
+            for (int p = 1; p < KS; ++p) {
+                const float4 y = xl[((p * RW + rw) * BS * 4 + e) * 64 + ln];
+                x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+            }
+            if (evalid) store4(b0 + e / 4, e % 4, x, inv);
+        }
+    }
+    if (splits > 1 && part == 0 && ehalf == 0 && evalid) a.part_ml[slot * size + 32 * rw + ecol] = make_float2(M, sum);
+    }
+}
+
+// Joins the splits of a row, in their order: a row's D/4 threads each take four
+// elements; grid (head, row group, tile).
+template <int D>
+__global__ __launch_bounds__(256) void block8_chunk_join_kernel(Block8AttendArgs a) {
+    constexpr int LANES = D / 4, ROWS = 256 / LANES;
+    const int size = 32 * a.row_waves, head = blockIdx.x, u = blockIdx.z;
+    int req, before;
+    bool ignore = false;
+    if (!tile_request<4>(a, size, u, req, before, ignore)) return;
+    Rows r = load_rows(a, req, 0, size, ignore);
+    const int tile = tiles_of(a, r, size) - 1 - (u - before);
+    r = rows_of(a, r.start, r.count, r.length, tile, size);
+    const int splits = splits_of<D>(a, r), rr = blockIdx.y * ROWS + threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
+    if (splits == 1 || rr >= r.n) return;
+    const int64_t slot0 = ((int64_t)u * a.p.kv_heads + head) * a.splits;
+    float M = kNegBig, sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    join_partials(splits, [&](int p, float2 &ml, float4 &y) __attribute__((always_inline)) {
+        const int64_t at = (slot0 + p) * size + rr;
+        ml = a.part_ml[at];
+        y = *reinterpret_cast<const float4 *>(a.part_o + at * D + d);
+    }, M, sum, x);
+    store_out(a, r, head, size * tile + rr, d, x, sum);
+}
+
+template <int CODE, int D>
+static hipError_t launch_chunk(const Block8AttendArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((block8_chunk_kernel<CODE, D>), dim3(a.p.kv_heads, a.splits, a.tiles),
+                       dim3(64 * ChunkShape<D>::NW), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.splits == 1) return e;
+    const int rows = std::min(32 * a.row_waves, a.group * a.max_q), per = 1024 / D;
+    hipLaunchKernelGGL((block8_chunk_join_kernel<D>), dim3(a.p.kv_heads, (rows + per - 1) / per, a.tiles), dim3(256), 0, s,
+                       a);
+    return hipGetLastError();
+}
+
+}  // namespace kvrt

@@ -489,7 +489,7 @@ PyObject *block_attend(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
         } else if (!describe(plain(a[11], dev), o)) {
             return kGeneral;
         }
-        const uint64_t size = block_api.attend_work(pages, n, table.dims[1], q.dims[1], max_q);
+        const uint64_t size = block_api.attend_work(pages, n, table.dims[1], q.dims[0], q.dims[1], max_q);
         at::Tensor work;
         if (size) work = fresh({(int64_t)size}, at::kByte, dev);
         const long rc = without_gil([&] {

@@ -28,9 +28,9 @@ INCLUDE = PKG_DIR.parent.parent / "include"
 LIB_PATH = PKG_DIR / "libkvrt.so"
 CALLS_PATH = PKG_DIR / "kvrt_pycall.so"
 SOURCES = ("kvrt_kernels.hip", "kvrt_prefill.hip", "kvrt_prefill_wide.hip", "kvrt_prefill_short.hip", "kvrt_runtime.hip",
-           "kvrt_block8.hip", "kvrt_block8_attend.hip")
+           "kvrt_block8.hip", "kvrt_block8_attend.hip", "kvrt_block8_chunk.hip", "kvrt_block8_chunk_wide.hip")
 
-AGPR_SOURCES = ("kvrt_prefill_wide.hip",)
+AGPR_SOURCES = ("kvrt_prefill_wide.hip", "kvrt_block8_chunk_wide.hip")
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -85,13 +85,55 @@ def _resources(stderr: str) -> dict[str, dict[str, str]]:
 
 def _compile(src: Path, obj: Path) -> dict[str, dict[str, str]]:
     cmd = [hipcc(), *HIPCC_FLAGS, *mfma_flags(src.name), f"-I{INCLUDE}", "-c", str(src), "-o", str(obj),
-           "-Rpass-analysis=kernel-resource-usage"]
+           "-Rpass-analysis=kernel-resource-usage", "-save-temps=obj"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         noise = "is not a recognized feature for this target"
         err = "\n".join(l for l in res.stderr.splitlines() if noise not in l and "remark" not in l)
         raise RuntimeError(f"hipcc failed for {src.name}:\n{err}")
+    (asm,) = obj.parent.glob(f"{src.stem}-hip-amdgcn*.s")
+    errs = exec_errors(asm.read_text())
+    if errs:
+        raise RuntimeError(f"{src.name}: registers saved while lanes are off:\n  " + "\n  ".join(errs))
     return _resources(res.stderr)
+
+
+# Where a divergent region ends, the compiler puts the lanes that skipped it back
+# (s_or_b64 exec, exec, ...). Short of registers it has saved a live value to the
+# other register file ahead of that, in the lanes of the region only, and read it
+# back in all of them: a uniform value then differs between lanes (a head_dim 512
+# decode stored out of range so). No kernel of the library may hold that pattern.
+_LANES_BACK = re.compile(r"s_or_b64 exec, exec,")
+_SAVED = re.compile(r"(v_accvgpr_(write|read|mov)|scratch_)")
+
+
+def exec_errors(asm: str) -> list[str]:
+    """Register copies between the files ahead of the instruction that ends a
+    divergent region, in a device assembly listing: one line per kernel's copy."""
+    errs: list[str] = []
+    kernel, region_ends = None, set()
+    block: list[str] = []
+    for line in asm.splitlines():  # the labels that lanes without work branch to
+        t = line.split(";")[0].split()
+        if len(t) == 2 and t[0] == "s_cbranch_execz":
+            region_ends.add(t[1])
+    inside = False  # between such a label and the first change of exec
+    for line in asm.splitlines():
+        label = re.match(r"^([\w.$]+):", line)
+        if label:
+            if not label.group(1).startswith(".L"):
+                kernel = label.group(1)
+            inside, block = label.group(1) in region_ends, []
+            continue
+        t = line.split(";")[0].strip()
+        if not inside or not t or t.startswith("."):
+            continue
+        if _LANES_BACK.match(t):
+            errs += [f"{kernel}: {x}" for x in block if _SAVED.match(x)]
+        if "exec" in t.split(";")[0].replace("execz", "").replace("execnz", "") or t.startswith(("s_cbranch", "s_branch")):
+            inside = False
+        block.append(t)
+    return errs
 
 
 # The single-launch decode merge exchanges partials and arrival counts between

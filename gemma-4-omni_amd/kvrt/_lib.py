@@ -235,7 +235,7 @@ SIGNATURES = [
     ("kvrt_block8_gather_async", c_int32, [_B8, _T, c_void_p, c_void_p, _T, _T, _T, c_void_p]),
     ("kvrt_block8_attend_async", c_int32,
      [_B8, _T, _T, c_void_p, c_void_p, c_void_p, _T, c_float, c_int32, c_int32, c_void_p, c_uint64, c_void_p]),
-    ("kvrt_block8_attend_work", c_uint64, [_B8, c_int64, c_int64, c_int64, c_int32]),
+    ("kvrt_block8_attend_work", c_uint64, [_B8, c_int64, c_int64, c_int64, c_int64, c_int32]),
     ("kvrt_session_state", c_int32, [c_void_p, c_int32, c_int32, _I32P]),
     ("kvrt_sync_lengths", c_int32, [c_void_p]),
     ("kvrt_get_counters", c_int32, [c_void_p, POINTER(KvrtCounters)]),

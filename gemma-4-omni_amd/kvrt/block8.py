@@ -360,7 +360,8 @@ class Block8Pool(_Status):
         with _on(self.device):
             if out is None:
                 out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-            size = self._lib.kvrt_block8_attend_work(self._ref, n, int(table.shape[1]), int(q.shape[1]), max_q)
+            size = self._lib.kvrt_block8_attend_work(self._ref, n, int(table.shape[1]), int(q.shape[0]), int(q.shape[1]),
+                                                     max_q)
             work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
             _check(self._lib.kvrt_block8_attend_async(
                 self._ref, ctypes.byref(tensor_desc(q)), ctypes.byref(td), lengths.data_ptr(), starts.data_ptr(),

@@ -736,7 +736,8 @@ int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, con
                              const kvrt_tensor *out, float scale, int32_t window, int32_t max_q, void *work,
                              uint64_t work_bytes, void *hip_stream);
 /* Bytes of kvrt_block8_attend_async's work for these arguments (0: none). */
-uint64_t kvrt_block8_attend_work(const kvrt_block8 *pages, int64_t n, int64_t width, int64_t hq, int32_t max_q);
+uint64_t kvrt_block8_attend_work(const kvrt_block8 *pages, int64_t n, int64_t width, int64_t rows, int64_t hq,
+                                 int32_t max_q);
 
 /* ---- state / diagnostics ----------------------------------------------------- */
 /* Host-authoritative length of (slot, layer). Replaces

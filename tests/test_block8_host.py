@@ -106,7 +106,7 @@ def test_pages_are_checked(bad):
     assert lib.kvrt_block8_gather_async(p, table, AT, None, o, o, None, None) == L.KVRT_EINVAL
     q = _tensor(L, L.DT_BF16, (2, 2 * p.kv_heads, p.head_dim))
     assert lib.kvrt_block8_attend_async(p, q, table, AT, AT, None, q, 1.0, 0, 1, AT, 1 << 30, None) == L.KVRT_EINVAL
-    assert lib.kvrt_block8_attend_work(p, 2, 4, 4, 1) == 0
+    assert lib.kvrt_block8_attend_work(p, 2, 4, 2, 4, 1) == 0
 
 
 def test_append_refusals():
@@ -157,7 +157,7 @@ def test_attend_refusals():
     p = _pages(L)
     table = _tensor(L, L.DT_INT32, (2, 400))
     q = _tensor(L, L.DT_BF16, (2, 4, 128))
-    size = lib.kvrt_block8_attend_work(p, 2, 400, 4, 1)
+    size = lib.kvrt_block8_attend_work(p, 2, 400, 2, 4, 1)
     assert size > 0
 
     def call(t=table, x=q, o=q, lens=AT, starts=AT, granted=None, scale=1.0, window=0, max_q=1, work=AT, nbytes=size):
