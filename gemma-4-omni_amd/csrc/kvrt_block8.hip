@@ -497,10 +497,11 @@ static AttendPlan attend_plan(int kv_heads, int shift, int head_dim, int64_t n, 
     // The most rows per tile (each shares the keys' conversion) that still leave a
     // workgroup per CU, then the keys divided as far as that takes. Every request's last
     // tile may be a partial one.
-    for (p.row_waves = 4;; p.row_waves /= 2) {
+    const int least = head_dim == 512 ? 4 : 2;  // row blocks that keep every wave busy
+    for (p.row_waves = head_dim <= 128 ? 8 : 4;; p.row_waves /= 2) {
         const int64_t size = 32 * p.row_waves;
         p.tiles = std::min((rows * group + size - 1) / size + n - 1, n * ((group * max_q + size - 1) / size));
-        if (p.row_waves == 1 || p.tiles * kv_heads >= 256) break;
+        if (p.row_waves == least || p.tiles * kv_heads >= 256) break;
     }
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(16, 256 / (p.tiles * kv_heads)));
     p.part_rows = p.splits == 1 ? 0 : (uint64_t)p.tiles * kv_heads * p.splits * 32 * p.row_waves;

@@ -2,7 +2,7 @@
 //
 // The mathematics is kvrt_block8_attend.hip's (codes as fp16, the V scale in the
 // exponent); here 32 rows of a (request, KV head) lie on one wave and a workgroup's
-// four waves share the keys: 32-key blocks are converted to fp16 once, into LDS, and
+// eight waves share the keys: 32-key blocks are converted to fp16 once, into LDS, and
 // each wave takes per block
 //   S^T (32 keys x 32 rows) = K Q^T     D/16    v_mfma_f32_32x32x16_f16
 //   softmax per row (fp32, base 2)
@@ -26,12 +26,13 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 // V so that 4 rows' 64 bytes do (the transposed reads).
 template <int D>
 struct ChunkShape {
-    static constexpr int NW = D == 512 ? 8 : 4;  // waves
-    static constexpr int DS = D == 512 ? 2 : 1;  // waves that share a row block's head dims
+    static constexpr int NW = 8;                 // waves
+    static constexpr int DS = D >= 256 ? 2 : 1;  // waves that share a row block's head dims
     static constexpr int RB = NW / DS;           // row blocks at most
     static constexpr int NBLK = D <= 128 ? 4 : D == 256 ? 2 : 1;  // 32-key blocks staged at a time
+    static constexpr int RMIN = RB / NBLK;                        // row blocks at least (waves past the blocks idle)
     static constexpr int KEYS = 32 * NBLK;
-    static constexpr int NBUF = D == 256 ? 2 : 1;  // (D <= 128: one buffer and two workgroups per CU)
+    static constexpr int NBUF = D <= 128 ? 2 : 1;
     static constexpr int KP = 2 * D + 16, VP = 2 * D + 64;  // bytes
     static constexpr int PASSES = KEYS * D / (NW * 1024);   // 16-code chunks per thread of K (and of V)
     static constexpr int BUF = KEYS * (KP + VP);
@@ -143,7 +144,9 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
     const int splits = splits_of<D>(a, r);
     if (split >= splits) return;
 
-    const int RW = NBLK == 1 || r.n > 64 ? C::RB : r.n > 32 ? 2 : 1, KS = C::RB / RW;
+    int RW = C::RMIN;
+    while (32 * RW < r.n) RW *= 2;
+    const int KS = C::RB / RW;
     const int ds = wave & (DS - 1), rw = (wave / DS) & (RW - 1), part = wave / DS / RW;
     const int row0 = size * tile + 32 * rw, rows = r.count * a.group;
     const bool wlive = 32 * rw < r.n, valid = wlive && row0 + col < rows;
@@ -215,13 +218,17 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
     bool unmapped = false;
     // codes of step s to registers; keys nobody sees (past the last, on unmapped pages)
     // as zeros
+    int ids[PASSES];  // pages of the next step's passes
+    auto load_ids = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p)  // a wave's rows of a pass lie in one 16-key block, so on one page
+            ids[p] = entries[min(k0 + s * KEYS + p * RPP + wave * RPWV, r.kend - 1) >> a.p.shift];
+    };
     auto fetch = [&](int s) __attribute__((always_inline)) {
         const int key0 = k0 + s * KEYS;
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
-            // a wave's rows of a pass lie in one 16-key block, so on one page
-            const int wkey = key0 + p * RPP + wave * RPWV, key = key0 + p * RPP + srow;
-            const int id = entries[min(wkey, r.kend - 1) >> a.p.shift];
+            const int wkey = key0 + p * RPP + wave * RPWV, key = key0 + p * RPP + srow, id = ids[p];
             const bool ok = (unsigned)id < (unsigned)a.p.pages;
             const int64_t at = ((((int64_t)(ok ? id : 0) * a.p.kv_heads + head) << a.p.shift) +
                                 (wkey & (a.p.block - 1))) * D;
@@ -239,6 +246,7 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
                 vr[p] = data ? vr[p] : make_uint4(0, 0, 0, 0);
             }
         }
+        load_ids(s + 1);
         if (threadIdx.x < 2 * NBLK) {  // the 16-key blocks' scales
             const int key = key0 + 16 * threadIdx.x;
             const int id = a.table[(int64_t)req * a.table_stride + (min(key, r.kend - 1) >> a.p.shift)];
@@ -370,6 +378,7 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
     };
 
     if (s0 < s1) {
+        load_ids(s0);
         fetch(s0);
         if constexpr (C::NBUF == 2) {
             stage(0, s0);
@@ -430,17 +439,17 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
         if (splits > 1 && ehalf == 0 && ds == 0) a.part_ml[slot * size + 32 * rw + ecol] = make_float2(m, l);
         return;
     }
-    if constexpr (DS == 1) {
+    if constexpr (C::RMIN < C::RB) {
     // combine the parts of each row block, BS 32-dim blocks at a time
-    constexpr int BS0 = C::NBUF * C::BUF / 16384, BS = BS0 >= NB ? NB : BS0 >= 8 ? 8 : BS0 >= 4 ? 4 : BS0 >= 2 ? 2 : 1;
-    static_assert(BS * 16384 <= C::NBUF * C::BUF && NB % BS == 0, "the waves' blocks fit the buffers");
+    constexpr int BS0 = C::NBUF * C::BUF / (NW * 4096), BS = BS0 >= NB ? NB : BS0 >= 8 ? 8 : BS0 >= 4 ? 4 : BS0 >= 2 ? 2 : 1;
+    static_assert(BS * NW * 4096 <= C::NBUF * C::BUF && NB % BS == 0, "the waves' blocks fit the buffers");
     __syncthreads();  // every wave is done with the buffers
     if (ehalf == 0) sml[wave * 32 + ecol] = make_float2(m, l);
     __syncthreads();
     float M = kNegBig, sum = 0.f;
-    for (int p = 0; p < KS; ++p) M = fmaxf(M, sml[(p * RW + rw) * 32 + ecol].x);
+    for (int p = 0; p < KS; ++p) M = fmaxf(M, sml[((p * RW + rw) * DS + ds) * 32 + ecol].x);
     for (int p = 0; p < KS; ++p) {
-        const float2 x = sml[(p * RW + rw) * 32 + ecol];
+        const float2 x = sml[((p * RW + rw) * DS + ds) * 32 + ecol];
         sum = fmaf(x.y, __builtin_amdgcn_exp2f(x.x - M), sum);
     }
     const float f = __builtin_amdgcn_exp2f(m - M), inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
@@ -456,15 +465,15 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
                                                                      o[b0 + b][4 * g + 2] * f, o[b0 + b][4 * g + 3] * f);
         __syncthreads();
         for (int e = part; e < 4 * BS; e += KS) {
-            float4 x = xl[(rw * BS * 4 + e) * 64 + ln];
+            float4 x = xl[((rw * DS + ds) * BS * 4 + e) * 64 + ln];
             for (int p = 1; p < KS; ++p) {
-                const float4 y = xl[((p * RW + rw) * BS * 4 + e) * 64 + ln];
+                const float4 y = xl[(((p * RW + rw) * DS + ds) * BS * 4 + e) * 64 + ln];
                 x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
             }
             if (evalid) store4(b0 + e / 4, e % 4, x, inv);
         }
     }
-    if (splits > 1 && part == 0 && ehalf == 0 && evalid) a.part_ml[slot * size + 32 * rw + ecol] = make_float2(M, sum);
+    if (splits > 1 && part == 0 && ds == 0 && ehalf == 0 && evalid) a.part_ml[slot * size + 32 * rw + ecol] = make_float2(M, sum);
     }
 }
 

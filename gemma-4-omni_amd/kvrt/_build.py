@@ -65,37 +65,41 @@ def hipcc() -> str:
 
 
 RESOURCES_PATH = PKG_DIR / "kernel_resources.json"
-_REMARK = re.compile(r"remark:\s+(Function Name|VGPRs|AGPRs|ScratchSize \[bytes/lane\]|Occupancy \[waves/SIMD\]"
-                     r"|LDS Size \[bytes/block\]):\s+(\S+)")
+_COUNT = {"NumVgprs": "VGPRs", "NumAgprs": "AGPRs", "ScratchSize": "ScratchSize", "Occupancy": "Occupancy",
+          "LDSByteSize": "LDS"}
 
 
-def _resources(stderr: str) -> dict[str, dict[str, str]]:
-    """Per-kernel VGPR / scratch / LDS / occupancy from the compiler's resource remarks."""
+def _resources(asm: str) -> dict[str, dict[str, str]]:
+    """Per-kernel VGPR / scratch / LDS / occupancy, from the comments behind each
+    kernel of a device assembly listing."""
     out: dict[str, dict[str, str]] = {}
     name = None
-    for m in _REMARK.finditer(stderr):
-        key, val = m.group(1), m.group(2)
-        if key == "Function Name":
-            name = val
+    for line in asm.splitlines():
+        m = re.match(r"\s*\.amdhsa_kernel (\S+)", line)
+        if m:
+            name = m.group(1)
             out[name] = {}
-        elif name is not None:
-            out[name][key.split(" ")[0]] = val
+            continue
+        m = re.match(r"; (\w+): (\d+)", line)
+        if m and name is not None and m.group(1) in _COUNT:
+            out[name].setdefault(_COUNT[m.group(1)], m.group(2))
     return out
 
 
 def _compile(src: Path, obj: Path) -> dict[str, dict[str, str]]:
     cmd = [hipcc(), *HIPCC_FLAGS, *mfma_flags(src.name), f"-I{INCLUDE}", "-c", str(src), "-o", str(obj),
-           "-Rpass-analysis=kernel-resource-usage", "-save-temps=obj"]
+           "-save-temps=obj"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         noise = "is not a recognized feature for this target"
-        err = "\n".join(l for l in res.stderr.splitlines() if noise not in l and "remark" not in l)
+        err = "\n".join(l for l in res.stderr.splitlines() if noise not in l)
         raise RuntimeError(f"hipcc failed for {src.name}:\n{err}")
-    (asm,) = obj.parent.glob(f"{src.stem}-hip-amdgcn*.s")
-    errs = exec_errors(asm.read_text())
+    (listing,) = obj.parent.glob(f"{src.stem}-hip-amdgcn*.s")
+    asm = listing.read_text()
+    errs = exec_errors(asm)
     if errs:
         raise RuntimeError(f"{src.name}: registers saved while lanes are off:\n  " + "\n  ".join(errs))
-    return _resources(res.stderr)
+    return _resources(asm)
 
 
 # Where a divergent region ends, the compiler puts the lanes that skipped it back
@@ -245,7 +249,9 @@ def build(verbose: bool = False) -> Path:
         # Every kernel of the hot path must run from registers and LDS: scratch
         # (private segment) use means spilled registers or a by-value kernel
         # argument copied to memory, both of which cost a memory round trip per use.
-        spilled = {k: v["ScratchSize"] for k, v in resources.items() if v.get("ScratchSize", "0") != "0"}
+        if not resources or any("ScratchSize" not in v for v in resources.values()):
+            raise RuntimeError("the compiler's listing no longer says what a kernel's registers and scratch are")
+        spilled = {k: v["ScratchSize"] for k, v in resources.items() if v["ScratchSize"] != "0"}
         if spilled:
             raise RuntimeError(f"kernels using scratch memory: {spilled}")
         RESOURCES_PATH.write_text(json.dumps(resources, indent=1, sort_keys=True) + "\n")
