@@ -78,7 +78,6 @@ hipError_t launch_block8_append(const Block8AppendArgs &a, int dtype, int head_d
 hipError_t launch_block8_gather(const Block8GatherArgs &a, int dtype, int head_dim, hipStream_t s);
 hipError_t launch_block8_attend(const Block8AttendArgs &a, int dtype, int head_dim, bool join, hipStream_t s);
 hipError_t launch_block8_chunk(const Block8AttendArgs &a, int dtype, int head_dim, hipStream_t s);
-hipError_t launch_block8_chunk_wide(const Block8AttendArgs &a, int dtype, int head_dim, hipStream_t s);
 // kBlock8MaxWgs zeroed arrival counters for a call on that stream; nullptr: none left.
 uint32_t *block8_counter_slice(hipStream_t s);
 

@@ -497,7 +497,7 @@ static AttendPlan attend_plan(int kv_heads, int shift, int head_dim, int64_t n, 
     // The most rows per tile (each shares the keys' conversion) that still leave a
     // workgroup per CU, then the keys divided as far as that takes. Every request's last
     // tile may be a partial one.
-    const int least = head_dim == 512 ? 4 : 2;  // row blocks that keep every wave busy
+    const int least = head_dim <= 128 ? 2 : 4;  // row blocks that keep every wave busy
     for (p.row_waves = head_dim <= 128 ? 8 : 4;; p.row_waves /= 2) {
         const int64_t size = 32 * p.row_waves;
         p.tiles = std::min((rows * group + size - 1) / size + n - 1, n * ((group * max_q + size - 1) / size));

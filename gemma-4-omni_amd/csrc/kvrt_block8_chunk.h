@@ -12,6 +12,14 @@
 // staged blocks in turn and are combined through LDS at the end. With few tiles the
 // keys are also divided over `splits` workgroups, joined by a second launch.
 //
+// Bound by its vector and matrix instructions, which the two waves of a SIMD overlap only
+// in part: at D 128, 1164 keys and more per request, counters show vector issue on half of
+// all cycles and LDS on a quarter. Steps are therefore as long as LDS allows (fewer
+// barriers), and nothing in a step waits for a load of its own. Measured: 4 requests of
+// 512 rows, 16 heads over 8, D 128: 46 us over 1912 keys, 151 us over 6112 (0.64 PFLOP/s);
+// 4 of 291, 8 heads over 1, D 256: 123 us over 4969 keys; one of 512, 16 heads over 2,
+// D 512: 126 us over 4608.
+//
 // Lane layouts (32x32x16): A[row l%32][k 8(l/32)+j], B[k 8(l/32)+j][col l%32],
 // D[row 8(i/4) + 4(l/32) + i%4][col l%32].
 #pragma once
@@ -29,18 +37,30 @@ struct ChunkShape {
     static constexpr int NW = 8;                 // waves
     static constexpr int DS = D >= 256 ? 2 : 1;  // waves that share a row block's head dims
     static constexpr int RB = NW / DS;           // row blocks at most
-    static constexpr int NBLK = D <= 128 ? 4 : D == 256 ? 2 : 1;  // 32-key blocks staged at a time
-    static constexpr int RMIN = RB / NBLK;                        // row blocks at least (waves past the blocks idle)
+    static constexpr int NBLK = D <= 128 ? 4 : 1;  // 32-key blocks of a step
+    static constexpr int RMIN = RB / NBLK;                       // row blocks at least (waves past the blocks idle)
     static constexpr int KEYS = 32 * NBLK;
-    static constexpr int NBUF = D <= 128 ? 2 : 1;
+    static constexpr int SLOTS = D <= 128 ? 2 : D == 256 ? 3 : 1;  // steps whose K and V lie in LDS
     static constexpr int KP = 2 * D + 16, VP = 2 * D + 64;  // bytes
     static constexpr int PASSES = KEYS * D / (NW * 1024);   // 16-code chunks per thread of K (and of V)
-    static constexpr int BUF = KEYS * (KP + VP);
+    static constexpr int KSLOT = KEYS * KP, VSLOT = KEYS * VP, VBASE = SLOTS * KSLOT, BUF = VBASE + SLOTS * VSLOT;
     // codes wait for their step in LDS instead of in registers (D 512 has none left)
     static constexpr bool DMA = D == 512;
     static constexpr int RAW = DMA ? 2 * KEYS * D : 16;
     static constexpr int QL = D == 512 ? 3 : 0;  // ... nor for the last of the Q operands
     static constexpr int SX = DS > 1 ? NW * 4096 : 16;  // scores the waves of a row block exchange
+};
+
+// Calls f(integral_constant<int, u>) for u = U .. N - 1.
+template <int U, int N>
+struct ChunkFor {
+    template <class F>
+    __device__ __forceinline__ static void run(F &&f) {
+        if constexpr (U < N) {
+            f(std::integral_constant<int, U>{});
+            ChunkFor<U + 1, N>::run(f);
+        }
+    }
 };
 
 struct ChunkScale {
@@ -121,9 +141,9 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
     using C = ChunkShape<D>;
     constexpr int NW = C::NW, DS = C::DS, DW = D / DS;  // head dims of a wave
     constexpr int NB = DW / 32, NBLK = C::NBLK, KEYS = C::KEYS, PASSES = C::PASSES;
-    __shared__ __align__(16) uint8_t lds[C::NBUF * C::BUF];
-    __shared__ __align__(16) ChunkScale scales[C::NBUF][2 * NBLK];
-    __shared__ float2 sml[NW * 32];
+    __shared__ __align__(16) uint8_t lds[C::BUF];
+    __shared__ __align__(16) ChunkScale scales[4][2 * NBLK];
+    __shared__ float2 sml[C::RMIN < C::RB ? NW * 32 : 1];
     __shared__ __align__(16) uint8_t sx[C::SX], raw[C::RAW];
     __shared__ uint4 ql[C::QL ? NW * C::QL * 64 : 1];
     constexpr int NQ = DW / 16, QR = NQ - C::QL;  // Q operands, those in registers
@@ -208,141 +228,164 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
         for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
 
     // ---- staging
-    const ConstInts entries = (ConstInts)(uintptr_t)a.table + (int64_t)req * a.table_stride;
-    const ConstFloats k_scale = (ConstFloats)(uintptr_t)a.p.k_scale, v_scale = (ConstFloats)(uintptr_t)a.p.v_scale;
     constexpr int LPR = D / 16, RPP = 64 * NW / LPR, RPWV = 64 / LPR;  // lanes per row, rows per pass and per wave of it
     const int srow = threadIdx.x / LPR, schunk = threadIdx.x % LPR;
     uint4 kr[C::DMA ? 1 : PASSES], vr[C::DMA ? 1 : PASSES];
+    bool kok[PASSES], vok[PASSES];  // on mapped pages
+    int ids = 0;
     const uint32_t raw_at = lds_addr(raw) + wave * PASSES * 2048;  // this wave's [pass][K, V][lane]
-    float next_k = 0.f, next_v = 0.f;  // scales of 16-key block threadIdx.x; next_k < 0: unmapped
-    bool unmapped = false;
-    // codes of step s to registers; keys nobody sees (past the last, on unmapped pages)
-    // as zeros
-    int ids[PASSES];  // pages of the next step's passes
-    auto load_ids = [&](int s) __attribute__((always_inline)) {
-#pragma unroll
-        for (int p = 0; p < PASSES; ++p)  // a wave's rows of a pass lie in one 16-key block, so on one page
-            ids[p] = entries[min(k0 + s * KEYS + p * RPP + wave * RPWV, r.kend - 1) >> a.p.shift];
+    // scales of 16-key block sblk of the next step, and the page of the step after it: its
+    // entry is loaded a step before it is looked up. (All lanes load, a few store: loads
+    // under a condition are copied behind it, which waits for them.)
+    const int sblk = threadIdx.x & (2 * NBLK - 1);
+    float next_k = 0.f, next_v = 0.f;
+    int next_id = 0;
+    bool unmapped = false, next_ok = false;
+    auto load_scale_id = [&](int s) __attribute__((always_inline)) {
+        next_id = a.table[(int64_t)req * a.table_stride + (min(k0 + s * KEYS + 16 * sblk, r.kend - 1) >> a.p.shift)];
     };
-    auto fetch = [&](int s) __attribute__((always_inline)) {
+    // The pages of a step's passes, pass p's in lane p: a wave's rows of a pass lie in one
+    // 16-key block, so on one page. A vector load, since waits for LDS reads do not include it.
+    auto load_ids = [&](int s) __attribute__((always_inline)) {
+        const int key = k0 + s * KEYS + (lane & (PASSES - 1)) * RPP + wave * RPWV;
+        ids = a.table[(int64_t)req * a.table_stride + (min(key, r.kend - 1) >> a.p.shift)];
+    };
+    // Codes of step s to registers (D 512: to LDS). Nothing here may read them: that would
+    // wait for the load in front of the step's work (one request, D 512, 4608 keys:
+    // 238 us instead of 136).
+    auto fetch = [&](auto v_c, int s, int ids) __attribute__((always_inline)) {
+        constexpr bool V = decltype(v_c)::value;
+        const uint8_t *codes = V ? a.p.v : a.p.k;
         const int key0 = k0 + s * KEYS;
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
-            const int wkey = key0 + p * RPP + wave * RPWV, key = key0 + p * RPP + srow, id = ids[p];
+            const int wkey = key0 + p * RPP + wave * RPWV, id = __builtin_amdgcn_readlane(ids, p);
             const bool ok = (unsigned)id < (unsigned)a.p.pages;
-            const int64_t at = ((((int64_t)(ok ? id : 0) * a.p.kv_heads + head) << a.p.shift) +
-                                (wkey & (a.p.block - 1))) * D;
-            const uint32_t lane_at = (uint32_t)((srow - wave * RPWV) * D + 16 * schunk);
+            const int64_t at = ((((int64_t)(ok ? id : 0) * a.p.kv_heads + head) << a.p.shift) + (wkey & (a.p.block - 1))) * D;
+            const uint32_t lane_at = 16 * lane;  // a wave's rows are contiguous
             if constexpr (C::DMA) {
-                dma_load16_cached(a.p.k + at + lane_at, raw_at + p * 2048);
-                dma_load16_cached(a.p.v + at + lane_at, raw_at + p * 2048 + 1024);
-                continue;
+                dma_load16_cached(codes + at + lane_at, raw_at + p * 2048 + (V ? 1024 : 0));
+            } else {
+                (V ? vr[p] : kr[p]) = *reinterpret_cast<const uint4 *>(codes + at + lane_at);
             }
-            kr[p] = *reinterpret_cast<const uint4 *>(a.p.k + at + lane_at);
-            vr[p] = *reinterpret_cast<const uint4 *>(a.p.v + at + lane_at);
-            if (!ok || wkey + RPWV > r.kend || wkey < r.kstart) {
-                const bool data = ok && key < r.kend && key >= r.kstart;
-                kr[p] = data ? kr[p] : make_uint4(0, 0, 0, 0);
-                vr[p] = data ? vr[p] : make_uint4(0, 0, 0, 0);
-            }
-        }
-        load_ids(s + 1);
-        if (threadIdx.x < 2 * NBLK) {  // the 16-key blocks' scales
-            const int key = key0 + 16 * threadIdx.x;
-            const int id = a.table[(int64_t)req * a.table_stride + (min(key, r.kend - 1) >> a.p.shift)];
-            const bool ok = (unsigned)id < (unsigned)a.p.pages;
-            unmapped |= !ok && key < r.kend && key + 16 > r.kstart;
-            const int64_t at = (int64_t)(ok ? id : 0) * a.p.kv_heads + head;
-            next_v = a.p.v_scale[at];
-            next_k = a.p.k_scale[at];
-            if (!ok) next_k = -1.f;
-            else next_k = fmaxf(next_k, 0.f);
+            (V ? vok[p] : kok[p]) = ok;
         }
     };
-    auto stage = [&](int buf, int s) __attribute__((always_inline)) {
-        uint8_t *kl = lds + buf * C::BUF, *vl = kl + KEYS * C::KP;
-#pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-            const int rr = p * RPP + srow;
-            uint4 kw, vw;
-            if constexpr (C::DMA) {  // a lane reads what it fetched itself
-                if (p == 0) wait_vmem<0>();
-                const uint4 *from = reinterpret_cast<const uint4 *>(raw) + (wave * PASSES + p) * 128 + lane;
-                kw = from[0];
-                vw = from[64];
-                const int wkey = k0 + s * KEYS + p * RPP + wave * RPWV, key = k0 + s * KEYS + rr;
-                const bool ok = (unsigned)entries[min(wkey, r.kend - 1) >> a.p.shift] < (unsigned)a.p.pages;
-                if (!ok || wkey + RPWV > r.kend || wkey < r.kstart) {
-                    const bool data = ok && key < r.kend && key >= r.kstart;
-                    kw = data ? kw : make_uint4(0, 0, 0, 0);
-                    vw = data ? vw : make_uint4(0, 0, 0, 0);
-                }
-            } else {
-                kw = kr[p];
-                vw = vr[p];
-            }
-            write_f16<CODE>(kl + rr * C::KP + 32 * schunk, kw);
-            write_f16<CODE>(vl + rr * C::VP + 32 * schunk, vw);
+    auto fetch_scales = [&](int s) __attribute__((always_inline)) {
+        const int key = k0 + s * KEYS + 16 * sblk;
+        next_ok = (unsigned)next_id < (unsigned)a.p.pages;
+        unmapped |= !next_ok && key < r.kend && key + 16 > r.kstart;
+        const int64_t at = (int64_t)(next_ok ? next_id : 0) * a.p.kv_heads + head;
+        next_v = a.p.v_scale[at];
+        next_k = a.p.k_scale[at];
+        load_scale_id(s + 1);
+    };
+    // one pass of a step's K or V to LDS as fp16; keys nobody sees (before the window, past
+    // the last, on unmapped pages) as zeros
+    auto stage = [&](auto v_c, auto p_c, int slot, int s) __attribute__((always_inline)) {
+        constexpr bool V = decltype(v_c)::value;
+        constexpr int p = decltype(p_c)::value;
+        uint8_t *to = lds + (V ? C::VBASE + slot * C::VSLOT : slot * C::KSLOT);
+        const int rr = p * RPP + srow;
+        uint4 w;
+        const int wkey = k0 + s * KEYS + p * RPP + wave * RPWV, key = k0 + s * KEYS + rr;
+        const bool ok = V ? vok[p] : kok[p];
+        if constexpr (C::DMA) {
+            if (p == 0) wait_vmem<0>();  // a lane reads what it fetched itself
+            w = reinterpret_cast<const uint4 *>(raw)[(wave * PASSES + p) * 128 + (V ? 64 : 0) + lane];
+        } else {
+            w = V ? vr[p] : kr[p];
         }
-        if constexpr (C::DMA) wait_lds();  // read before the next step's codes land there
+        if (__builtin_amdgcn_readfirstlane(!ok || wkey + RPWV > r.kend || wkey < r.kstart)) {
+            const bool data = ok && key < r.kend && key >= r.kstart;
+            w = data ? w : make_uint4(0, 0, 0, 0);
+        }
+        write_f16<CODE>(to + rr * (V ? C::VP : C::KP) + 32 * schunk, w);
+        if constexpr (C::DMA)
+            if (p == PASSES - 1) wait_lds();  // read before the next step's codes land there
+    };
+    auto stage_scales = [&](int s) __attribute__((always_inline)) {
         if (threadIdx.x < 2 * NBLK) {
             const float v = scale_in_range(next_v);
-            scales[buf][threadIdx.x] = ChunkScale{scale_in_range(next_k), __builtin_amdgcn_logf(v), __builtin_amdgcn_rcpf(v),
-                                                  next_k < 0.f ? 0.f : 1.f};
+            scales[s & 3][sblk] = ChunkScale{scale_in_range(next_k), __builtin_amdgcn_logf(v), __builtin_amdgcn_rcpf(v),
+                                             next_ok ? 1.f : 0.f};
         }
     };
+    auto stage_all = [&](auto v_c, int slot, int s) __attribute__((always_inline)) {
+        ChunkFor<0, PASSES>::run([&](auto p_c) __attribute__((always_inline)) { stage(v_c, p_c, slot, s); });
+    };
+    constexpr std::false_type kK{};
+    constexpr std::true_type kV{};
 
-    // ---- one 32-key block
+    // ---- one 32-key block, in steps of one MFMA: operands are read PK (PV) steps ahead;
+    // sched_barrier holds that order
     const int kadr = col * C::KP + 16 * half + 2 * ds * DW;
     const int s16 = lane & 15;
-    const int vadr = (4 * half + (s16 >> 2)) * C::VP + 32 * ((lane >> 4) & 1) + 8 * (s16 & 3) + 2 * ds * DW;
-    // (`live` is false only where DS > 1: all waves exchange at the same time)
-    auto block = [&](int buf, int blk, int key0, bool live) __attribute__((always_inline)) {
-        const uint8_t *kl = lds + buf * C::BUF + blk * 32 * C::KP + kadr;
-        const uint8_t *vl = lds + buf * C::BUF + KEYS * C::KP + blk * 32 * C::VP + vadr;
-        f32x16_t s;
+    const int vadr = C::VBASE + (4 * half + (s16 >> 2)) * C::VP + 32 * ((lane >> 4) & 1) + 8 * (s16 & 3) + 2 * ds * DW;
+    constexpr int NP = 2 * NB, PK = D == 512 ? 2 : NQ, PV = D == 512 ? 2 : NP;
+    auto qk = [&](f32x16_t &s, int slot, int blk) __attribute__((always_inline)) {
+        const uint8_t *kl = lds + slot * C::KSLOT + blk * 32 * C::KP + kadr;
+        uint4 x[PK];
+#pragma unroll
+        for (int c = 0; c < PK; ++c) x[c] = *reinterpret_cast<const uint4 *>(kl + 32 * c);
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = 0.f;
+        __builtin_amdgcn_sched_barrier(0);
+        ChunkFor<0, NQ>::run([&](auto c_c) __attribute__((always_inline)) {
+            constexpr int c = decltype(c_c)::value;
+            s = mfma32_f16(x[c % PK], c < QR ? qop[c < QR ? c : 0] : ql[(wave * C::QL + c - QR) * 64 + lane], s);
+            if constexpr (c + PK < NQ) x[c % PK] = *reinterpret_cast<const uint4 *>(kl + 32 * (c + PK));
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    uint32_t w[8];  // the weights: of 16 keys in w[0 .. 3], of the next 16 in w[4 .. 7]
+    auto pv = [&](int slot, int blk) __attribute__((always_inline)) {
+        const uint8_t *vl = lds + slot * C::VSLOT + blk * 32 * C::VP + vadr;
+        auto vop = [&](int u) __attribute__((always_inline)) {
+            const uint8_t *p = vl + 16 * (u / NB) * C::VP + 64 * (u % NB);
+            const uint2 lo = lds_read_tr16(reinterpret_cast<const uint16_t *>(p));
+            const uint2 hi = lds_read_tr16(reinterpret_cast<const uint16_t *>(p + 8 * C::VP));
+            return make_uint4(lo.x, lo.y, hi.x, hi.y);
+        };
+        uint4 x[PV];
 #pragma unroll
-        for (int c = 0; c < NQ; ++c) {
-            if (DS == 1 || live)
-                s = mfma32_f16(*reinterpret_cast<const uint4 *>(kl + 32 * c),
-                               c < QR ? qop[c < QR ? c : 0] : ql[(wave * C::QL + c - QR) * 64 + lane], s);
-            if (DS > 1 && c % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // (read ahead, more operands than registers)
-        }
-        if constexpr (DS > 1) {
-            float4 *to = reinterpret_cast<float4 *>(sx) + wave * 256 + lane;
-            const float4 *from = reinterpret_cast<const float4 *>(sx) + (wave ^ 1) * 256 + lane;
-            if (live)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) to[g * 64] = make_float4(s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]);
-            __syncthreads();
-            if (!live) return;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4 x = from[g * 64];
-                s[4 * g] += x.x, s[4 * g + 1] += x.y, s[4 * g + 2] += x.z, s[4 * g + 3] += x.w;
-                if (g == 1) __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        const ChunkScale sa = scales[buf][2 * blk], sb = scales[buf][2 * blk + 1];
+        for (int u = 0; u < PV; ++u) x[u] = vop(u);
+        __builtin_amdgcn_sched_barrier(0);
+        ChunkFor<0, NP>::run([&](auto u_c) __attribute__((always_inline)) {
+            constexpr int u = decltype(u_c)::value, h = u / NB;
+            o[u % NB] = mfma32_f16(x[u % PV], make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]), o[u % NB]);
+            if constexpr (u + PV < NP) x[u % PV] = vop(u + PV);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    auto mask = [&](f32x16_t &s, int key0, const ChunkScale (&sc)[2]) __attribute__((always_inline)) {
         const bool whole = key0 + 32 <= min(r.kend, wfirst + 1) && (a.window <= 0 || key0 > wlast - a.window) &&
-                           sa.ok + sb.ok == 2.f;
-        if (!__builtin_amdgcn_readfirstlane(whole)) {
+                           sc[0].ok + sc[1].ok == 2.f;
+        if (__builtin_amdgcn_readfirstlane(whole)) return;
+        const int low = a.window > 0 ? pos - a.window : -1, high = min(pos, r.kend - 1);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+        for (int h = 0; h < 2; ++h) {
+            const int lo = sc[h].ok != 0.f ? low : high;  // (then nothing lies between them)
+#pragma unroll
+            for (int i = 8 * h; i < 8 * h + 8; ++i) {
                 const int key = key0 + 8 * (i >> 2) + 4 * half + (i & 3);
-                const bool seen = (i < 8 ? sa.ok : sb.ok) != 0.f && key <= pos && key < r.kend &&
-                                  (a.window <= 0 || key > pos - a.window);
-                s[i] = seen ? s[i] : -INFINITY;
+                s[i] = key > lo && key <= high ? s[i] : -INFINITY;
             }
         }
-        // above 0, so that a masked score stays one
-        const float ca = fmaxf(qscale * sa.k, 1e-37f), cb = fmaxf(qscale * sb.k, 1e-37f);
-        float ta = s[0], tb = s[8];
+    };
+    // the running max over s (the exponents are s * cf + log2(v scale))
+    float cf[2];
+    auto take_max = [&](const f32x16_t &s, const ChunkScale (&sc)[2]) __attribute__((always_inline)) {
+        float top = -INFINITY;
 #pragma unroll
-        for (int i = 1; i < 8; ++i) ta = fmaxf(ta, s[i]), tb = fmaxf(tb, s[8 + i]);
-        const float top = pair<OpMax, 32>(fmaxf(fmaf(ta, ca, sa.log_v), fmaf(tb, cb, sb.log_v)));
+        for (int h = 0; h < 2; ++h) {
+            cf[h] = fmaxf(qscale * sc[h].k, 1e-37f);  // above 0, so that a masked score stays one
+            float t = s[8 * h];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) t = fmaxf(t, s[8 * h + i]);
+            top = fmaxf(top, fmaf(t, cf[h], sc[h].log_v));
+        }
+        top = pair<OpMax, 32>(top);
         const float mn = top > m + kRescaleSlack ? top : m;
         if (__any(mn != m)) {
             const float corr = __builtin_amdgcn_exp2f(m - mn);
@@ -351,60 +394,164 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
             for (int b = 0; b < NB; ++b) o[b] *= corr;
             m = mn;
         }
-        const float da = sa.log_v + (kWeightShift - m), db = sb.log_v + (kWeightShift - m);
-        uint4 p[2];
-        float la = 0.f, lb = 0.f;
-        uint32_t w[8];
+    };
+    auto soft = [&](const f32x16_t &s, const ChunkScale (&sc)[2]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            const float e0 = __builtin_amdgcn_exp2f(fmaf(s[i], i < 8 ? ca : cb, i < 8 ? da : db));
-            const float e1 = __builtin_amdgcn_exp2f(fmaf(s[i + 1], i < 8 ? ca : cb, i < 8 ? da : db));
-            if (i < 8) la += e0 + e1;
-            else lb += e0 + e1;
-            w[i / 2] = pack_f16(e0, e1);
-        }
-        l = fmaf(la, sa.inv_v, fmaf(lb, sb.inv_v, l));
-        p[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        p[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        for (int h = 0; h < 2; ++h) {
+            const float d = sc[h].log_v + (kWeightShift - m);
+            float sum = 0.f;  // in fp32: a page of small values has weights that fp16 drops but the sum needs
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const uint2 lo = lds_read_tr16(reinterpret_cast<const uint16_t *>(vl + 16 * h * C::VP + 64 * b));
-                const uint2 hi = lds_read_tr16(reinterpret_cast<const uint16_t *>(vl + (16 * h + 8) * C::VP + 64 * b));
-                o[b] = mfma32_f16(make_uint4(lo.x, lo.y, hi.x, hi.y), p[h], o[b]);
-                if (DS > 1 && b % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+            for (int j = 4 * h; j < 4 * h + 4; ++j) {
+                const float e0 = __builtin_amdgcn_exp2f(fmaf(s[2 * j], cf[h], d));
+                const float e1 = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], cf[h], d));
+                sum += e0 + e1;
+                w[j] = pack_f16(e0, e1);
             }
+            l = fmaf(sum, sc[h].inv_v, l);
+            if (D == 512) __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // whether some row of the wave sees some of keys first .. first + 31
+    auto sees = [&](int first) __attribute__((always_inline)) {
+        return wlive && first <= wlast && first < r.kend && (a.window <= 0 || first + 32 > wfirst - a.window + 1);
+    };
+    // s to the weights w (DS > 1: s is this wave's half, the other's is in sx)
+    f32x16_t sc;
+    const int kx = wave * 256 + lane;
+    auto give_scores = [&]() __attribute__((always_inline)) {
+        if constexpr (DS > 1)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                reinterpret_cast<float4 *>(sx)[kx + g * 64] = make_float4(sc[4 * g], sc[4 * g + 1], sc[4 * g + 2], sc[4 * g + 3]);
+    };
+    auto weights = [&](int s, int blk) __attribute__((always_inline)) {
+        if constexpr (DS > 1) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 x = reinterpret_cast<const float4 *>(sx)[(kx ^ 256) + g * 64];
+                sc[4 * g] += x.x, sc[4 * g + 1] += x.y, sc[4 * g + 2] += x.z, sc[4 * g + 3] += x.w;
+                if (D == 512 && g == 1) __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        const ChunkScale two[2] = {scales[s & 3][2 * blk], scales[s & 3][2 * blk + 1]};
+        mask(sc, k0 + s * KEYS + 32 * blk, two);
+        take_max(sc, two);
+        soft(sc, two);
     };
 
     if (s0 < s1) {
         load_ids(s0);
-        fetch(s0);
-        if constexpr (C::NBUF == 2) {
-            stage(0, s0);
+        load_scale_id(s0);
+        int now = ids;
+        load_ids(s0 + 1);
+        fetch(kK, s0, now);
+        fetch(kV, s0, now);
+        fetch_scales(s0);
+        if constexpr (C::SLOTS == 3) {
+            // Four waves work on the matrix cores (M: P V of a block, then K Q^T of the next)
+            // while the four beside them on the same SIMDs do a softmax (V), and the other
+            // way round; a barrier ends each phase. In V the codes of K two steps ahead and
+            // of V one step ahead are staged: with three slots no slot is written that a
+            // wave one phase behind still reads, and what a wave one phase ahead reads is
+            // whole.
+            int past = ids;  // pages of the step whose V is fetched next
+            load_ids(s0 + 2);
+            stage_all(kK, 0, s0);
+            stage_scales(s0);
+            fetch(kK, s0 + 1, past);
+            fetch_scales(s0 + 1);
+            stage_all(kV, 0, s0);
+            fetch(kV, s0 + 1, past);
+            stage_all(kK, 1, s0 + 1);
+            stage_scales(s0 + 1);
+            past = ids;
+            load_ids(s0 + 3);
+            fetch(kK, s0 + 2, past);
+            fetch_scales(s0 + 2);
             __syncthreads();
-        }
-        for (int s = s0; s < s1; ++s) {
-            const int buf = C::NBUF == 2 ? (s - s0) & 1 : 0;
-            if constexpr (C::NBUF == 1) {
+            const bool behind = wave >= NW / 2;
+            if (behind) __syncthreads();
+            int slot = 0;
+            bool live = part == 0 && sees(k0 + s0 * KEYS);
+            if (live) {
+                qk(sc, 0, 0);
+                give_scores();
+            }
+            __syncthreads();
+            for (int s = s0; s < s1; ++s) {
+                const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot1 == 2 ? 0 : slot1 + 1;
+                if (live) weights(s, 0);
+                stage_all(kV, slot1, s + 1);
+                fetch(kV, s + 2, past);
+                stage_all(kK, slot2, s + 2);
+                stage_scales(s + 2);
+                past = ids;
+                load_ids(s + 4);  // looked up a step later
+                fetch(kK, s + 3, past);
+                fetch_scales(s + 3);
+                __syncthreads();
+                if (live) pv(slot, 0);
+                live = part == 0 && s + 1 < s1 && sees(k0 + (s + 1) * KEYS);
+                if (live) {
+                    qk(sc, slot1, 0);
+                    give_scores();
+                }
+                __syncthreads();
+                slot = slot1;
+            }
+            if (!behind) __syncthreads();
+        } else if constexpr (C::SLOTS == 2) {
+            // the waves run freely within a step: one's matrix work lies beside another's
+            // softmax without being told to
+            auto stage_step = [&](int slot, int s) __attribute__((always_inline)) {
+                stage_all(kK, slot, s);
+                stage_all(kV, slot, s);
+                stage_scales(s);
+            };
+            stage_step(0, s0);
+            __syncthreads();
+            for (int s = s0; s < s1; ++s) {
+                const int slot = (s - s0) & 1;
+                if (s + 1 < s1) {
+                    now = ids;
+                    load_ids(s + 2);
+                    fetch(kK, s + 1, now);
+                    fetch(kV, s + 1, now);
+                    fetch_scales(s + 1);
+                }
+                for (int blk = part; blk < NBLK; blk += KS) {
+                    if (!sees(k0 + s * KEYS + 32 * blk)) continue;
+                    qk(sc, slot, blk);
+                    weights(s, blk);
+                    pv(slot, blk);
+                }
+                if (s + 1 < s1) stage_step(slot ^ 1, s + 1);
+                __syncthreads();
+            }
+        } else {
+            for (int s = s0; s < s1; ++s) {
                 if (s > s0) __syncthreads();  // the last step's blocks are read
-                stage(0, s);
-                if (s + 1 < s1) fetch(s + 1);
+                stage_all(kK, 0, s);
+                stage_all(kV, 0, s);
+                stage_scales(s);
+                if (s + 1 < s1) {
+                    now = ids;
+                    load_ids(s + 2);
+                    fetch(kK, s + 1, now);
+                    fetch(kV, s + 1, now);
+                    fetch_scales(s + 1);
+                }
                 __syncthreads();
-            } else {
-                if (s + 1 < s1) fetch(s + 1);
-            }
-            for (int blk = part; blk < NBLK; blk += KS) {
-                const int key0 = k0 + s * KEYS + 32 * blk;
-                // blocks that no row of the wave sees
-                const bool live = wlive && key0 <= wlast && key0 < r.kend &&
-                                  (a.window <= 0 || key0 + 32 > wfirst - a.window + 1);
-                if (DS == 1 && !live) continue;
-                block(buf, blk, key0, live);
-            }
-            if constexpr (C::NBUF == 2) {
-                if (s + 1 < s1) stage(buf ^ 1, s + 1);
+                const bool live = part == 0 && sees(k0 + s * KEYS);
+                if (live) {
+                    qk(sc, 0, 0);
+                    give_scores();
+                }
                 __syncthreads();
+                if (live) {
+                    weights(s, 0);
+                    pv(0, 0);
+                }
             }
         }
     }
@@ -441,8 +588,8 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
     }
     if constexpr (C::RMIN < C::RB) {
     // combine the parts of each row block, BS 32-dim blocks at a time
-    constexpr int BS0 = C::NBUF * C::BUF / (NW * 4096), BS = BS0 >= NB ? NB : BS0 >= 8 ? 8 : BS0 >= 4 ? 4 : BS0 >= 2 ? 2 : 1;
-    static_assert(BS * NW * 4096 <= C::NBUF * C::BUF && NB % BS == 0, "the waves' blocks fit the buffers");
+    constexpr int BS0 = C::BUF / (NW * 4096), BS = BS0 >= NB ? NB : BS0 >= 8 ? 8 : BS0 >= 4 ? 4 : BS0 >= 2 ? 2 : 1;
+    static_assert(BS * NW * 4096 <= C::BUF && NB % BS == 0, "the waves' blocks fit the buffers");
     __syncthreads();  // every wave is done with the buffers
     if (ehalf == 0) sml[wave * 32 + ecol] = make_float2(m, l);
     __syncthreads();
@@ -478,7 +625,8 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
 }
 
 // Joins the splits of a row, in their order: a row's D/4 threads each take four
-// elements; grid (head, row group, tile).
+// elements; grid (head, row group, tile). Four partials at a time, for many waves on a
+// CU: with sixteen (172 registers) it took 17 us for 2328 rows of D 256 in 3 splits.
 template <int D>
 __global__ __launch_bounds__(256) void block8_chunk_join_kernel(Block8AttendArgs a) {
     constexpr int LANES = D / 4, ROWS = 256 / LANES;
@@ -494,7 +642,7 @@ __global__ __launch_bounds__(256) void block8_chunk_join_kernel(Block8AttendArgs
     const int64_t slot0 = ((int64_t)u * a.p.kv_heads + head) * a.splits;
     float M = kNegBig, sum = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    join_partials(splits, [&](int p, float2 &ml, float4 &y) __attribute__((always_inline)) {
+    join_partials<4>(splits, [&](int p, float2 &ml, float4 &y) __attribute__((always_inline)) {
         const int64_t at = (slot0 + p) * size + rr;
         ml = a.part_ml[at];
         y = *reinterpret_cast<const float4 *>(a.part_o + at * D + d);

@@ -93,11 +93,10 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 
 // Joins partials p = 0 .. n - 1 of four output elements of a row, in their order,
-// sixteen at a time: ld(p, ml, o) reads one. The launch that makes the partials and
-// the join kernel both use it, so both give the same bits.
-template <class Ld>
+// B at a time: ld(p, ml, o) reads one. The decode launch that makes the partials and its
+// join kernel both use it, with the same B, so both give the same bits.
+template <int B = 16, class Ld>
 __device__ __forceinline__ void join_partials(int n, Ld ld, float &M, float &sum, float4 &o) {
-    constexpr int B = 16;
     for (int p0 = 0; p0 < n; p0 += B) {
         float2 ml[B];
         float4 x[B];

@@ -28,9 +28,9 @@ INCLUDE = PKG_DIR.parent.parent / "include"
 LIB_PATH = PKG_DIR / "libkvrt.so"
 CALLS_PATH = PKG_DIR / "kvrt_pycall.so"
 SOURCES = ("kvrt_kernels.hip", "kvrt_prefill.hip", "kvrt_prefill_wide.hip", "kvrt_prefill_short.hip", "kvrt_runtime.hip",
-           "kvrt_block8.hip", "kvrt_block8_attend.hip", "kvrt_block8_chunk.hip", "kvrt_block8_chunk_wide.hip")
+           "kvrt_block8.hip", "kvrt_block8_attend.hip", "kvrt_block8_chunk.hip")
 
-AGPR_SOURCES = ("kvrt_prefill_wide.hip", "kvrt_block8_chunk_wide.hip")
+AGPR_SOURCES = ("kvrt_prefill_wide.hip",)
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
