@@ -704,3 +704,81 @@ def test_results_do_not_change_between_calls():
     for _ in range(20):
         got = pool.attend(q, table.cuda(), _i32([900, 3000]), _starts([2, 1]), 256 ** -0.5, max_q=2)
         assert (bits(got) == bits(out)).all()
+
+
+@pytest.mark.parametrize("name", ["int8", "e4m3"])
+@pytest.mark.parametrize("block,dim", [(64, 256), (128, 128), (128, 512)])
+def test_append_long_runs(name, block, dim):
+    """Runs longer than the slots a wave looks at together, from the middle of pages
+    too, in a call whose waves take sixteen slots each."""
+    from kvrt import Block8Pool
+
+    gen = torch.Generator().manual_seed(block + dim)
+    heads, pages = 8, 12
+    pool = Block8Pool.zeros(pages, heads, dim, block_size=block, dtype=name)
+    slots = [5] + list(range(3 * block + 2, 4 * block)) + [-1] + list(range(6 * block, 9 * block - 1)) + [11 * block]
+    slots += [-1] * (300 - len(slots))
+    x = [randn_bf16(gen, (len(slots), heads, dim)) for _ in range(2)]
+    pool.append(x[0].cuda(), x[1].cuda(), _i32(slots))
+    for codes, scale, rows in ((pool.k, pool.k_scale, x[0]), (pool.v, pool.v_scale, x[1])):
+        got, after = codes.float().cpu().double().numpy(), scale.cpu().numpy()
+        ref = _append_reference(codes, np.zeros((pages, heads), np.float32), rows.float().numpy(), slots)
+        for p in range(pages):
+            if p not in ref:
+                assert (after[p] == 0).all() and (got[p] == 0).all(), p
+                continue
+            first, m, s1, _, v = ref[p]
+            assert (after[p] == s1).all(), p
+            exact = v.transpose(1, 0, 2) / s1.astype(np.float64)[:, None, None]
+            assert _near(got[p, :, first:first + m], exact, codes.dtype).all(), p
+            assert (got[p, :, :first] == 0).all() and (got[p, :, first + m:] == 0).all(), p
+
+
+@pytest.mark.parametrize("n,block", [(3, 16), (20, 16), (70, 32)])
+def test_tables_release_many_pages(n, block):
+    """A few pages and hundreds of them go back in one call, and are handed out again
+    in the same one."""
+    from kvrt import BlockTables
+
+    rng = np.random.default_rng(n)
+    width = 700
+    t, ref = BlockTables(n, width, n * width, block_size=block), R.Tables(n, width, n * width, block)
+    full = [int(rng.integers(1, width * block + 1)) if i % 4 else 3 * block for i in range(n)]
+    want = ref.update([0] * n, full, 0)
+    plan = t.update(_i32([0] * n), _i32(full), rows=0)  # no row fits: every request is refused
+    assert plan.granted.tolist() == want[3] and t.status() != 0
+    want = ref.update([0] * n, full, sum(full))
+    _compare_tables(t, ref, t.update(_i32([0] * n), _i32(full), rows=sum(full)), want, "grown")
+    keep = [x if i % 3 == 0 else x // 2 if i % 3 == 1 else 0 for i, x in enumerate(full)]
+    new = [0 if i % 2 else min(5 * block, width * block - keep[i]) for i in range(n)]
+    want = ref.update(keep, new, sum(new))
+    _compare_tables(t, ref, t.update(_i32(keep), _i32(new), rows=sum(new)), want, "cut")
+    want = ref.update([0] * n, [1] * n, n)
+    _compare_tables(t, ref, t.update(_i32([0] * n), _i32([1] * n), rows=n), want, "emptied")
+
+
+@pytest.mark.parametrize("name,dim,n", [("int8", 64, 70), ("e4m3", 128, 65), ("int8", 256, 70), ("e4m3", 512, 66)])
+def test_chunks_of_many_requests(name, dim, n):
+    """More requests than a wave has lanes, some of them without rows."""
+    rng = np.random.default_rng(n + dim)
+    counts = [int(x) for x in rng.integers(0, 40, n)]
+    counts[3] = 0
+    lengths = [c + int(x) for c, x in zip(counts, rng.integers(0, 50, n))]
+    _attend_case(name, 2, 1, dim, 16, lengths, counts, sample=3)
+
+
+@pytest.mark.parametrize("name,hq,heads,dim,lengths,counts,window", [
+    ("int8", 8, 1, 256, [3000], [40], 0), ("e4m3", 16, 2, 512, [2100], [33], 0), ("int8", 16, 8, 128, [2500, 90], [20, 34], 0),
+    ("e4m3", 8, 1, 256, [2900, 1400], [40, 300], 1000), ("int8", 2, 1, 64, [4000], [65], 0), ("int8", 8, 1, 512, [2000], [40], 700),
+])
+def test_chunks_over_long_contexts(name, hq, heads, dim, lengths, counts, window):
+    """Keys divided over workgroups, many steps of each, joined by a second launch; and
+    the same call on another stream."""
+    pool, q, table, out = _attend_case(name, hq, heads, dim, 16, lengths, counts, window=window, sample=4)
+    lens, starts, dev = _i32(lengths), _starts(counts), table.cuda()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        again = pool.attend(q, dev, lens, starts, dim ** -0.5, max_q=max(counts), window=window)
+    s.synchronize()
+    assert torch.equal(again, out)
