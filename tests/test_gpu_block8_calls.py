@@ -66,7 +66,7 @@ def _make():
 Q = lambda: randn_bf16(torch.Generator().manual_seed(2), (4, 6, 64)).cuda()  # noqa: E731
 
 UPDATES = {
-    "plain": {}, "int64 lengths": {"lengths": torch.tensor([20, 9], device="cuda")}, "cpu new": {"new": torch.tensor([1, 1], dtype=torch.int32)},
+    "plain": {}, "int64 lengths": {"lengths": "int64"}, "cpu new": {"new": torch.tensor([1, 1], dtype=torch.int32)},
     "too few": {"new": [1]}, "strided": {"lengths": "strided"}, "negative rows": {"rows": -1}, "no rows": {"rows": 0, "new": [0, 0]},
     "table": {"table": True}, "list": {"new": "list"},
 }
@@ -78,7 +78,8 @@ def test_update(form):
 
     def call(t, p):
         lengths, new = kw.get("lengths", [20, 9]), kw.get("new", [1, 2])
-        lengths = _i32([20, 0, 9, 0])[::2] if isinstance(lengths, str) else lengths if torch.is_tensor(lengths) else _i32(lengths)
+        forms = {"strided": lambda: _i32([20, 0, 9, 0])[::2], "int64": lambda: _i32([20, 9]).long()}
+        lengths = forms[lengths]() if isinstance(lengths, str) else _i32(lengths)
         new = [1, 2] if isinstance(new, str) else new if torch.is_tensor(new) else _i32(new)
         if kw.get("table"):
             t.table = t.table.long()
