@@ -710,7 +710,8 @@ int kvrt_block8_append_async(const kvrt_block8 *pages, const kvrt_tensor *k, con
  * KVRT_BF16 or KVRT_FP32 (last dim contiguous, 16-byte aligned rows); row j of
  * request i is position start_pos[i] + j (start_pos device int32 [n], or NULL
  * for 0; a negative one is a bad index) while that lies below lengths[i],
- * zeros after. table: KVRT_INT32 [n, width]; mask [n, Lmax] as for
+ * zeros after. table: KVRT_INT32 [n, width], n <= 65535, width * block <= 2^30;
+ * mask [n, Lmax] as for
  * kvrt_gather_async, or NULL. Counterpart of kvrt_gather_async. */
 int kvrt_block8_gather_async(const kvrt_block8 *pages, const kvrt_tensor *table, const int32_t *lengths,
                              const int32_t *start_pos, const kvrt_tensor *out_k, const kvrt_tensor *out_v,

@@ -217,3 +217,12 @@ def test_python_objects_need_a_gpu():
     t = torch.zeros((4, 1, 16, 128), dtype=torch.int8)
     with pytest.raises(ValueError, match="GPU"):
         Block8Pool(t, t, t, t)
+
+
+def test_tables_hold_at_most_two_to_the_thirty_positions():
+    L, lib = _lib()
+    p = _pages(L)
+    wide = _tensor(L, L.DT_INT32, (2, (1 << 30) // p.block + 1))
+    o, q = _tensor(L, L.DT_BF16, (2, 2, 5, 128)), _tensor(L, L.DT_BF16, (2, 4, 128))
+    assert lib.kvrt_block8_gather_async(p, wide, AT, None, o, o, None, None) == L.KVRT_EINVAL
+    assert lib.kvrt_block8_attend_async(p, q, wide, AT, AT, None, q, 1.0, 0, 1, AT, 1 << 40, None) == L.KVRT_EINVAL

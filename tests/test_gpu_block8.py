@@ -782,3 +782,13 @@ def test_chunks_over_long_contexts(name, hq, heads, dim, lengths, counts, window
         again = pool.attend(q, dev, lens, starts, dim ** -0.5, max_q=max(counts), window=window)
     s.synchronize()
     assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("hq,heads,dim,count", [(2, 1, 128, 3), (8, 1, 256, 40), (4, 2, 64, 90)])
+def test_a_window_past_the_table_is_none(hq, heads, dim, count):
+    """More rows than keys, and the largest window a call can name."""
+    pool, q, table, out = _attend_case("int8", hq, heads, dim, 16, [2, count + 9], [3, count])
+    for window in (2 ** 31 - 1, 2 ** 30, 10 ** 6):
+        got = pool.attend(q, table.cuda(), _i32([2, count + 9]), _starts([3, count]), dim ** -0.5, max_q=count, window=window)
+        assert torch.equal(got, out), window
+    assert pool.status() == 0
