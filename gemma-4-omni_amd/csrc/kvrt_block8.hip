@@ -18,6 +18,11 @@ namespace kvrt {
 // orders the requests and every request works on its own: no atomics, one
 // result. A request is granted while the running sum of wanted pages is within
 // top.
+//
+// Latency bounds it: few bytes, but sums over all requests before any page has its
+// place. One workgroup keeps those on one CU without a second launch; the slot map,
+// which any thread finds by itself, takes a launch of its own from 4096 rows on.
+// Measured: 4 requests of two rows 4.7 us, 256 requests with 16608 rows 7.7 + 5.3 us.
 
 // Sum of x over the workgroup's threads before this one, and the sum over all.
 __device__ __forceinline__ int64_t scan_add(int64_t x, int64_t *lds, int64_t &total) {
@@ -264,7 +269,7 @@ hipError_t launch_block8_tables(const Block8TablesArgs &a, hipStream_t s) {
 // alone: a slot that does not follow its predecessor, or is a page's first row,
 // begins one. Latency is what it costs, so what a run needs is loaded at once: its
 // rows (held in registers, up to kHeld of a lane), the scale, and the slots of 64 rows.
-// Rows read twice, a slot at a time, took 15.6 us for 6880 rows of 16 requests, 8 heads of
+// Rows read twice, a slot at a time, took 15.6 us for 6872 rows of 16 requests, 8 heads of
 // D 128; this takes 13.6 (3.1 TB/s), and 20 with 16 rows held (232 registers, 2 waves).
 constexpr int kHeld = 4;
 template <int CODE, int D>
@@ -394,7 +399,9 @@ hipError_t launch_block8_append(const Block8AppendArgs &a, int dtype, int head_d
 
 // ---- gather -----------------------------------------------------------------------
 //
-// 16 codes per lane: a lane reads 16 bytes and writes 32 (bf16) or 64 (fp32).
+// x = code * scale, rounded once. 16 codes per lane: a lane reads 16 bytes and writes 32
+// (bf16) or 64 (fp32), and HBM bounds it: 16 requests of 430 rows padded to 512, 8 heads
+// of D 128 take 11.5 us (4.1 TB/s); two rows of four requests, 3.4 us, are latency.
 template <int CODE, int D, bool FP32>
 __global__ __launch_bounds__(256) void block8_gather_kernel(Block8GatherArgs a) {
     constexpr int LPR = D / 16, RPW = 256 / LPR;  // lanes per row, rows per workgroup

@@ -7,18 +7,18 @@
 //   S^T (32 keys x 32 rows) = K Q^T     D/16    v_mfma_f32_32x32x16_f16
 //   softmax per row (fp32, base 2)
 //   O^T (D x 32) += V^T P^T             2 D/32  v_mfma_f32_32x32x16_f16
-// A row tile is 32, 64 or 128 rows (launch) on RW = 1, 2 or 4 row blocks, fewer where
-// the request's last tile has fewer rows; the 4 / RW waves of a row block take the
-// staged blocks in turn and are combined through LDS at the end. With few tiles the
+// A row tile is 64, 128 or 256 rows at D <= 128 and 128 beyond, where two waves share a
+// row block's head dims (its Q and O fill two waves' registers). Its RW row blocks are
+// fewer where the request's last tile has fewer rows; the RB / RW waves of a row block
+// take the staged blocks in turn and are combined through LDS at the end. With few tiles the
 // keys are also divided over `splits` workgroups, joined by a second launch.
 //
 // Bound by its vector and matrix instructions, which the two waves of a SIMD overlap only
-// in part: at D 128, 1164 keys and more per request, counters show vector issue on half of
-// all cycles and LDS on a quarter. Steps are therefore as long as LDS allows (fewer
-// barriers), and nothing in a step waits for a load of its own. Measured: 4 requests of
-// 512 rows, 16 heads over 8, D 128: 46 us over 1912 keys, 151 us over 6112 (0.64 PFLOP/s);
-// 4 of 291, 8 heads over 1, D 256: 123 us over 4969 keys; one of 512, 16 heads over 2,
-// D 512: 126 us over 4608.
+// in part: at D 128 over 5600 keys counters show vector issue on half of all cycles and
+// LDS on a quarter. Steps are therefore as long as LDS allows (fewer barriers), and nothing in a step waits for a load of its own. Measured: 4 requests of
+// 512 rows, 16 heads over 8, D 128: 46 us over 1400 keys, 151 us over 5600 (0.59 PFLOP/s);
+// 4 of 291, 8 heads over 1, D 256: 123 us over 4678 keys; one of 512, 16 heads over 2,
+// D 512: 126 us over 4096.
 //
 // Lane layouts (32x32x16): A[row l%32][k 8(l/32)+j], B[k 8(l/32)+j][col l%32],
 // D[row 8(i/4) + 4(l/32) + i%4][col l%32].
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
         ids = a.table[(int64_t)req * a.table_stride + (min(key, r.kend - 1) >> a.p.shift)];
     };
     // Codes of step s to registers (D 512: to LDS). Nothing here may read them: that would
-    // wait for the load in front of the step's work (one request, D 512, 4608 keys:
+    // wait for the load in front of the step's work (one request, D 512, 4096 keys:
     // 238 us instead of 136).
     auto fetch = [&](auto v_c, int s, int ids) __attribute__((always_inline)) {
         constexpr bool V = decltype(v_c)::value;
