@@ -60,8 +60,9 @@ struct Block8AttendArgs {
     int64_t table_stride, rows;            // packed rows of q
     int n, width, group, max_q, window;
     int wgs;                               // workgroups the keys are divided over (each row tile)
-    int join_most;                         // partials of a head joined inside the launch (others: a second one)
-    int join_all;                          // divide so that every head's are
+    int join_most;                         // partials of a head that one workgroup may join (sets the division)
+    int join_all;                          // divide so that no head has more
+    int join_here;                         // join_most with counters, 1 without: a second launch joins the others
     float scale_log2;                      // scale * log2(e)
     float *part_o;                         // partials of divided heads [tile][wg][2][16 rows][D]
     float2 *part_ml;                       // their (max, sum) [tile][wg][2][16]
@@ -78,7 +79,8 @@ hipError_t launch_block8_append(const Block8AppendArgs &a, int dtype, int head_d
 hipError_t launch_block8_gather(const Block8GatherArgs &a, int dtype, int head_dim, hipStream_t s);
 hipError_t launch_block8_attend(const Block8AttendArgs &a, int dtype, int head_dim, bool join, hipStream_t s);
 hipError_t launch_block8_chunk(const Block8AttendArgs &a, int dtype, int head_dim, hipStream_t s);
-// kBlock8MaxWgs zeroed arrival counters for a call on that stream; nullptr: none left.
+// kBlock8MaxWgs zeroed arrival counters for a call on that stream; nullptr: none left
+// (the call then joins in a second launch: same division, same order, same bits).
 uint32_t *block8_counter_slice(hipStream_t s);
 
 // ---- codes ----------------------------------------------------------------------

@@ -58,8 +58,8 @@ __device__ __forceinline__ Division divide(const Block8AttendArgs &a, int units,
     Division d;
     d.total = units * a.p.kv_heads;
     d.per = (d.total + a.wgs - 1) / a.wgs;
-    // all joined in the launch: n units in a row lie over at most (n - 1) / per + 2
-    // workgroups, no head's over more than one joins (join_most >= 2)
+    // n units in a row lie over at most (n - 1) / per + 2 workgroups, no head's over more
+    // than one may join (join_most >= 2)
     if (a.join_all) d.per = max(d.per, (most + a.join_most - 2) / (a.join_most - 1));
     return d;
 }
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
         const int parts = min(max(t_end - (t_begin - wave), 0), 4);
         const bool begins = ua == 0, ends = ub == units;
         const int w0 = seg / div.per, count = (seg + units - 1) / div.per - w0 + 1;  // workgroups of the head
-        const bool here = count <= a.join_most;                                       // joined in this launch
+        const bool here = count <= a.join_here;                                       // joined in this launch
         const int64_t slot0 = 0;
         for (int e = threadIdx.x; e < r.n * (D / 4); e += 256) {
             const int rr = e / (D / 4), d = 4 * (e % (D / 4));
@@ -461,9 +461,10 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
     if (unmapped) raise(a.p.status, KVRT_BLOCK_BAD_INDEX);
 }
 
-// Joins the partials of heads that more workgroups shared than one joins inside the
-// launch: one workgroup per (request, KV head, row). Up to kFlat partials in their
-// order, as the launch does; beyond, in GROUPS interleaved orders that are then joined.
+// Joins the partials of heads that the launch did not join (more workgroups shared them
+// than one joins, or the call has no arrival counters): one workgroup per (request, KV
+// head, row). Up to kFlat partials in their order, as the launch does; beyond, in GROUPS
+// interleaved orders that are then joined.
 constexpr int kFlat = 32;
 
 template <int D>
@@ -492,7 +493,7 @@ __global__ __launch_bounds__(256) void block8_join_kernel(Block8AttendArgs a) {
     const Division div = divide(a, all, most);
     const int units = units_of(r), seg = before * a.p.kv_heads + head * units;
     const int w0 = seg / div.per, count = (seg + units - 1) / div.per - w0 + 1;
-    if (count == 1 || count <= a.join_most) return;
+    if (count <= a.join_here) return;
     const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
     const int groups = count <= kFlat ? 1 : GROUPS;
     float M = kNegBig, sum = 0.f;

@@ -1,0 +1,100 @@
+"""Decode attention over 8-bit pages in a process of its own, for what depends on the
+calls a process made before: run by tests/test_gpu_block8_captures.py as
+``python block8_capture_child.py first|many``."""
+from __future__ import annotations
+
+import sys
+from pathlib import Path
+
+ROOT = Path(__file__).resolve().parents[1]
+for p in (str(ROOT), str(ROOT / "gemma-4-omni_amd")):
+    if p not in sys.path:
+        sys.path.insert(0, p)
+
+import torch  # noqa: E402
+
+from tests.helpers import bits, randn_bf16  # noqa: E402
+
+HQ, HEADS, DIM, BLOCK = 16, 8, 128, 16
+
+
+def served(lengths, seed=0):
+    """(pool, arguments of a decode step) of one row each; pages in order."""
+    from kvrt import Block8Pool
+
+    gen = torch.Generator().manual_seed(seed)
+    pages = [-(-x // BLOCK) for x in lengths]
+    pool = Block8Pool.zeros(sum(pages), HEADS, DIM)
+    for codes, scale in ((pool.k, pool.k_scale), (pool.v, pool.v_scale)):
+        codes.copy_(torch.randint(-127, 128, codes.shape, generator=gen, dtype=torch.int8))
+        scale.copy_(0.02 * (0.5 + torch.rand(scale.shape, generator=gen)))
+    table, at = torch.full((len(lengths), max(pages)), -1, dtype=torch.int32), 0
+    for i, m in enumerate(pages):
+        table[i, :m] = torch.arange(at, at + m, dtype=torch.int32)
+        at += m
+    q = randn_bf16(gen, (len(lengths), HQ, DIM)).cuda()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    return pool, (q, table.cuda(), i32(lengths), i32(list(range(len(lengths) + 1))), DIM ** -0.5)
+
+
+# (lengths: one long request among short ones, so that where the keys are cut depends
+# on how many partials the launch may join; and equal ones)
+SHAPES = ([8100] + [100] * 63, [1500, 900, 700, 33])
+
+
+def capture(pool, args):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = pool.attend(*args, max_q=1)
+    return g, out
+
+
+def compare(name, g, out, pool, args):
+    want = pool.attend(*args, max_q=1)
+    for step in range(3):
+        out.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert (bits(out) == bits(want)).all(), (name, step, (out != want).any(-1).any(-1).nonzero().flatten().tolist())
+        assert torch.equal(pool.attend(*args, max_q=1), want), (name, step)
+    assert pool.status() == 0, name
+    print(name, "ok", flush=True)
+
+
+def first() -> None:
+    """The process's first decode calls are captured ones."""
+    made = [served(x) for x in SHAPES]
+    torch.cuda.synchronize()
+    graphs = [capture(*m) for m in made]
+    for shape, m, (g, out) in zip(SHAPES, made, graphs):
+        compare(f"first captured, {len(shape)} requests", g, out, *m)
+
+
+def many() -> None:
+    """More captured calls than a process has arrival counters for."""
+    made = [served(x) for x in SHAPES]
+    before = [m[0].attend(*m[1], max_q=1) for m in made]
+    (small, args), side = made[1], torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(600):
+        g = torch.cuda.CUDAGraph()  # (the one before is destroyed)
+        with torch.cuda.stream(side):
+            g.capture_begin()
+            small.attend(*args, max_q=1)
+            g.capture_end()
+        if i % 100 == 99:
+            print("captured", i + 1, flush=True)
+    for shape, m, want in zip(SHAPES, made, before):
+        g, out = capture(*m)
+        compare(f"captured after many, {len(shape)} requests", g, out, *m)
+        with torch.cuda.stream(torch.cuda.Stream()):  # a stream without earlier calls
+            torch.cuda.synchronize()
+            got = m[0].attend(*m[1], max_q=1)
+            torch.cuda.synchronize()
+        assert torch.equal(got, want), shape
+
+
+if __name__ == "__main__":
+    {"first": first, "many": many}[sys.argv[1]]()
+    print("done", flush=True)
