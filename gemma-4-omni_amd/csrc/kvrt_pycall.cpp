@@ -388,65 +388,90 @@ PyObject *block_update(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     });
 }
 
-// (pages, stream, device, k, v, slot_map)
+// The leading arguments of a pool's call: sizes and status, stream, device, then the pool's
+// tensors k, v, k_scale, v_scale, which may be others than the last call's.
+struct PoolHead {
+    static constexpr int kArgs = 7;
+    kvrt_block8 pages;
+    void *stream;
+    int32_t dev;
+
+    template <class T>
+    bool take(PyObject *o, at::ScalarType type, at::IntArrayRef size, T *&p) {
+        const at::Tensor *t = plain(o, dev);
+        if (!t || t->scalar_type() != type || t->sizes() != size || !t->is_contiguous()) return false;
+        p = static_cast<T *>(t->data_ptr());
+        return true;
+    }
+    bool read(PyObject *const *a) {
+        const auto *base = static_cast<const kvrt_block8 *>(PyLong_AsVoidPtr(a[0]));
+        stream = PyLong_AsVoidPtr(a[1]);
+        if (!base || !read_int(a[2], dev) || !current_device(dev)) return false;
+        pages = *base;
+        const int64_t size[4] = {pages.pages, pages.kv_heads, pages.block, pages.head_dim};
+        const at::IntArrayRef codes(size, 4), scales(size, 2);
+        const at::ScalarType type = pages.dtype == KVRT_INT8 ? at::kChar : at::kFloat8_e4m3fn;
+        return take(a[3], type, codes, pages.k) && take(a[4], type, codes, pages.v) &&
+               take(a[5], at::kFloat, scales, pages.k_scale) && take(a[6], at::kFloat, scales, pages.v_scale);
+    }
+};
+
+// (pool, k, v, slot_map)
 PyObject *block_append(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    return guarded(nargs, 6, [&]() -> long {
-        int32_t dev;
-        const auto *pages = static_cast<const kvrt_block8 *>(PyLong_AsVoidPtr(a[0]));
-        void *stream = PyLong_AsVoidPtr(a[1]);
+    return guarded(nargs, PoolHead::kArgs + 3, [&]() -> long {
+        PoolHead h;
         kvrt_tensor k, v;
-        if (!pages || !read_int(a[2], dev) || !current_device(dev) || !describe(plain(a[3], dev), k) ||
-            !describe(plain(a[4], dev), v) || k.ndim < 1)
-            return kGeneral;
-        const int32_t *slots = ints(a[5], dev, 1, k.dims[0]);
+        if (!h.read(a)) return kGeneral;
+        a += PoolHead::kArgs;
+        if (!describe(plain(a[0], h.dev), k) || !describe(plain(a[1], h.dev), v) || k.ndim < 1) return kGeneral;
+        const int32_t *slots = ints(a[2], h.dev, 1, k.dims[0]);
         if (!slots) return kGeneral;
-        return without_gil([&] { return block_api.append(pages, &k, &v, slots, stream); });
+        return without_gil([&] { return block_api.append(&h.pages, &k, &v, slots, h.stream); });
     });
 }
 
 // What both forms of gather share.
-struct GatherHead {
-    const kvrt_block8 *pages;
-    void *stream;
-    int32_t dev;
+struct GatherHead : PoolHead {
+    static constexpr int kArgs = PoolHead::kArgs + 3;
     kvrt_tensor table;
     const int32_t *lengths, *from = nullptr;
 
     bool read(PyObject *const *a) {
-        pages = static_cast<const kvrt_block8 *>(PyLong_AsVoidPtr(a[0]));
-        stream = PyLong_AsVoidPtr(a[1]);
-        if (!pages || !read_int(a[2], dev) || !current_device(dev) || !describe(plain(a[3], dev), table) || table.ndim != 2 ||
-            table.dtype != KVRT_INT32)
-            return false;
-        lengths = ints(a[4], dev, 1, table.dims[0]);
-        return lengths && (a[5] == Py_None || (from = ints(a[5], dev, 1, table.dims[0])));
+        if (!PoolHead::read(a)) return false;
+        a += PoolHead::kArgs;
+        if (!describe(plain(a[0], dev), table) || table.ndim != 2 || table.dtype != KVRT_INT32) return false;
+        lengths = ints(a[1], dev, 1, table.dims[0]);
+        return lengths && (a[2] == Py_None || (from = ints(a[2], dev, 1, table.dims[0])));
     }
 };
 
-// (pages, stream, device, table, lengths, start_pos or None, out_k, out_v, mask or None)
+// (pool, table, lengths, start_pos or None, out_k, out_v, mask or None)
 PyObject *block_gather(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    return guarded(nargs, 9, [&]() -> long {
+    return guarded(nargs, GatherHead::kArgs + 3, [&]() -> long {
         GatherHead h;
         kvrt_tensor k, v, m;
-        const bool masked = a[8] != Py_None;
-        if (!h.read(a) || !describe(plain(a[6], h.dev), k) || !describe(plain(a[7], h.dev), v) ||
-            (masked && !describe(plain(a[8], h.dev), m)))
+        if (!h.read(a)) return kGeneral;
+        a += GatherHead::kArgs;
+        const bool masked = a[2] != Py_None;
+        if (!describe(plain(a[0], h.dev), k) || !describe(plain(a[1], h.dev), v) ||
+            (masked && !describe(plain(a[2], h.dev), m)))
             return kGeneral;
         return without_gil(
-            [&] { return block_api.gather(h.pages, &h.table, h.lengths, h.from, &k, &v, masked ? &m : nullptr, h.stream); });
+            [&] { return block_api.gather(&h.pages, &h.table, h.lengths, h.from, &k, &v, masked ? &m : nullptr, h.stream); });
     });
 }
 
-// (pages, stream, device, table, lengths, start_pos or None, lmax, fp32, mask: 0 none, 1 bool, 2 fp32, 3 bf16)
+// (pool, table, lengths, start_pos or None, lmax, fp32, mask: 0 none, 1 bool, 2 fp32, 3 bf16)
 // -> (k, v, mask or None)
 PyObject *block_gather_new(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    return guarded_object(nargs, 9, [&](PyObject *&out) -> long {
+    return guarded_object(nargs, GatherHead::kArgs + 3, [&](PyObject *&out) -> long {
         GatherHead h;
         int32_t lmax, fp32, kind;
-        if (!h.read(a) || !read_int(a[6], lmax) || lmax < 0 || !read_int(a[7], fp32) || !read_int(a[8], kind) || kind < 0 ||
-            kind > 3)
+        if (!h.read(a)) return kGeneral;
+        a += GatherHead::kArgs;
+        if (!read_int(a[0], lmax) || lmax < 0 || !read_int(a[1], fp32) || !read_int(a[2], kind) || kind < 0 || kind > 3)
             return kGeneral;
-        const int64_t size[4] = {h.table.dims[0], h.pages->kv_heads, lmax, h.pages->head_dim}, flat[2] = {size[0], lmax};
+        const int64_t size[4] = {h.table.dims[0], h.pages.kv_heads, lmax, h.pages.head_dim}, flat[2] = {size[0], lmax};
         const at::ScalarType kinds[3] = {at::kBool, at::kFloat, at::kBFloat16};
         const at::Tensor kt = fresh(size, fp32 ? at::kFloat : at::kBFloat16, h.dev), vt = at::empty_like(kt);
         at::Tensor mt;
@@ -454,7 +479,7 @@ PyObject *block_gather_new(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
         kvrt_tensor k, v, m;
         if (!describe(&kt, k) || !describe(&vt, v) || (kind && !describe(&mt, m))) return kGeneral;
         const long rc = without_gil(
-            [&] { return block_api.gather(h.pages, &h.table, h.lengths, h.from, &k, &v, kind ? &m : nullptr, h.stream); });
+            [&] { return block_api.gather(&h.pages, &h.table, h.lengths, h.from, &k, &v, kind ? &m : nullptr, h.stream); });
         if (rc == KVRT_OK) {
             PyObject *mask = Py_None;
             if (kind) mask = THPVariable_Wrap(mt);
@@ -465,40 +490,42 @@ PyObject *block_gather_new(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     });
 }
 
-// (pages, stream, device, scale, window, max_q, q, table, lengths, starts, granted or None, out or None) -> out
+// (pool, scale, window, max_q, q, table, lengths, starts, granted or None, out or None) -> out
 PyObject *block_attend(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    return guarded_object(nargs, 12, [&](PyObject *&answer) -> long {
-        int32_t dev, window, max_q;
+    return guarded_object(nargs, PoolHead::kArgs + 9, [&](PyObject *&answer) -> long {
+        PoolHead h;
+        int32_t window, max_q;
         float scale;
-        const auto *pages = static_cast<const kvrt_block8 *>(PyLong_AsVoidPtr(a[0]));
-        void *stream = PyLong_AsVoidPtr(a[1]);
         kvrt_tensor q, table, o;
         const at::Tensor *qt;
-        if (!pages || !read_int(a[2], dev) || !read_float(a[3], scale) || !read_int(a[4], window) ||
-            !read_int(a[5], max_q) || !current_device(dev) || !(qt = plain(a[6], dev)) || !describe(qt, q) || q.ndim != 3 ||
-            !describe(plain(a[7], dev), table) || table.ndim != 2 || table.dtype != KVRT_INT32)
+        if (!h.read(a)) return kGeneral;
+        a += PoolHead::kArgs;
+        const int32_t dev = h.dev;
+        if (!read_float(a[0], scale) || !read_int(a[1], window) || !read_int(a[2], max_q) || !(qt = plain(a[3], dev)) ||
+            !describe(qt, q) || q.ndim != 3 || !describe(plain(a[4], dev), table) || table.ndim != 2 ||
+            table.dtype != KVRT_INT32)
             return kGeneral;
         const int64_t n = table.dims[0];
-        const int32_t *lengths = ints(a[8], dev, 1, n), *starts = ints(a[9], dev, 1, n + 1), *granted = nullptr;
-        if (!lengths || !starts || (a[10] != Py_None && !(granted = ints(a[10], dev, 1, n)))) return kGeneral;
+        const int32_t *lengths = ints(a[5], dev, 1, n), *starts = ints(a[6], dev, 1, n + 1), *granted = nullptr;
+        if (!lengths || !starts || (a[7] != Py_None && !(granted = ints(a[7], dev, 1, n)))) return kGeneral;
         if (max_q > q.dims[0]) max_q = (int32_t)q.dims[0];
         at::Tensor out;
-        if (a[11] == Py_None) {
+        if (a[8] == Py_None) {
             out = fresh(qt->sizes(), qt->scalar_type(), dev);
             if (!describe(&out, o)) return kGeneral;
-        } else if (!describe(plain(a[11], dev), o)) {
+        } else if (!describe(plain(a[8], dev), o)) {
             return kGeneral;
         }
-        const uint64_t size = block_api.attend_work(pages, n, table.dims[1], q.dims[0], q.dims[1], max_q);
+        const uint64_t size = block_api.attend_work(&h.pages, n, table.dims[1], q.dims[0], q.dims[1], max_q);
         at::Tensor work;
         if (size) work = fresh({(int64_t)size}, at::kByte, dev);
         const long rc = without_gil([&] {
-            return block_api.attend(pages, &q, &table, lengths, starts, granted, &o, scale, window, max_q,
-                                    size ? work.data_ptr() : nullptr, size, stream);
+            return block_api.attend(&h.pages, &q, &table, lengths, starts, granted, &o, scale, window, max_q,
+                                    size ? work.data_ptr() : nullptr, size, h.stream);
         });
         if (rc == KVRT_OK) {
             if (out.defined()) answer = THPVariable_Wrap(out);
-            else Py_INCREF(answer = a[11]);
+            else Py_INCREF(answer = a[8]);
         }
         return rc;
     });

@@ -206,7 +206,9 @@ class Block8Pool(_Status):
 
     ``k``, ``v``: codes [pages, kv_heads, block_size, head_dim], torch.int8 or
     torch.float8_e4m3fn; ``k_scale``, ``v_scale``: fp32 [pages, kv_heads]. A code
-    stands for code * scale; scales are read as within [2^-64, 2^32].
+    stands for code * scale; scales are read as within [2^-64, 2^32]. They are
+    ordinary tensors: each call uses (a captured one keeps) those the pool holds
+    when it is made, and others of the same shapes and types may be assigned.
     """
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
@@ -221,24 +223,33 @@ class Block8Pool(_Status):
                              f"{tuple(k.shape)}")
         if pages * heads * block > _I32_MAX:
             raise ValueError("a pool numbers its rows in 32 bits")
-        for t, name, want, dtype in ((k, "k", k.shape, k.dtype), (v, "v", k.shape, k.dtype),
-                                     (k_scale, "k_scale", (pages, heads), torch.float32),
-                                     (v_scale, "v_scale", (pages, heads), torch.float32)):
-            _same(t, name, self.device)
-            if tuple(t.shape) != tuple(want) or t.dtype != dtype or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(want)}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.kv_heads, self.block_size, self.head_dim = pages, heads, block, dim
+        self._dtype = k.dtype
         with _on(self.device):
             self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
-        c = L.KvrtBlock8()
-        c.k, c.v, c.k_scale, c.v_scale = k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
-        c.status = self._status.data_ptr()
-        c.dtype, c.pages, c.kv_heads, c.block, c.head_dim = _CODES[k.dtype], pages, heads, block, dim
-        self._c = c
-        self._ref = ctypes.byref(c)
-        self._at = ctypes.addressof(c)
         self._call = _calls()
+        self._sizes = self._c()  # what calls read beside the four public tensors
+        self._sizes_at = ctypes.addressof(self._sizes)
+
+    def _c(self) -> L.KvrtBlock8:
+        c = L.KvrtBlock8()
+        codes, scales = (self.pages, self.kv_heads, self.block_size, self.head_dim), (self.pages, self.kv_heads)
+        for name, want, dtype in (("k", codes, self._dtype), ("v", codes, self._dtype), ("k_scale", scales, torch.float32),
+                                  ("v_scale", scales, torch.float32)):
+            t = getattr(self, name)
+            _same(t, name, self.device)
+            if tuple(t.shape) != want or t.dtype != dtype or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor {want}")
+            setattr(c, name, t.data_ptr())
+        c.status = self._status.data_ptr()
+        c.dtype, c.pages, c.kv_heads, c.block, c.head_dim = _CODES[self._dtype], *codes
+        return c
+
+    def _head(self) -> tuple:
+        """What every native call begins with: sizes, stream, device and the pool's tensors."""
+        return (self._sizes_at, current_stream_handle(self.device), self.device.index, self.k, self.v, self.k_scale,
+                self.v_scale)
 
     @classmethod
     def zeros(cls, pages: int, kv_heads: int, head_dim: int, *, block_size: int = 16, dtype: str = "int8",
@@ -265,15 +276,16 @@ class Block8Pool(_Status):
         them are coded anew; rows behind them (rolled back) are dropped. A page
         takes one run of consecutive slots per call; a slot map that names a slot
         twice or enters a page twice leaves that page undefined."""
-        rc = self._call.block_append(self._at, current_stream_handle(self.device), self.device.index, k, v, slot_map)
+        rc = self._call.block_append(*self._head(), k, v, slot_map)
         if rc <= 0:
             return _check(rc, "kvrt_block8_append_async")
+        c = self._c()
         for t, name in ((k, "k"), (v, "v")):
             _same(t, name, self.device)
         _int32(slot_map, "slot_map", int(k.shape[0]), self.device)
         with _on(self.device):
             _check(self._lib.kvrt_block8_append_async(
-                self._ref, ctypes.byref(tensor_desc(k)), ctypes.byref(tensor_desc(v)), slot_map.data_ptr() or None,
+                ctypes.byref(c), ctypes.byref(tensor_desc(k)), ctypes.byref(tensor_desc(v)), slot_map.data_ptr() or None,
                 ctypes.c_void_p(current_stream_handle(self.device))), "kvrt_block8_append_async")
 
     def gather(self, table: torch.Tensor, lengths: torch.Tensor, lmax: int | None = None, *,
@@ -285,19 +297,19 @@ class Block8Pool(_Status):
         ``out``: (K, V) or (K, V, mask) destinations instead of new tensors (strided
         views with a contiguous last dimension); they then set Lmax and dtype."""
         if out is None and dtype in _FLOATS and mask_dtype in _MASKS:
-            got = self._call.block_gather_new(self._at, current_stream_handle(self.device), self.device.index, table,
-                                              lengths, start_pos, lmax, _FLOATS[dtype], _MASKS[mask_dtype])
+            got = self._call.block_gather_new(*self._head(), table, lengths, start_pos, lmax, _FLOATS[dtype],
+                                              _MASKS[mask_dtype])
             if type(got) is tuple:
                 return got
             if got < 0:
                 _check(got, "kvrt_block8_gather_async")
         elif out is not None and lmax is None:
-            rc = self._call.block_gather(self._at, current_stream_handle(self.device), self.device.index, table, lengths,
-                                         start_pos, out[0], out[1], out[2] if len(out) > 2 else None)
+            rc = self._call.block_gather(*self._head(), table, lengths, start_pos, out[0], out[1],
+                                         out[2] if len(out) > 2 else None)
             if rc <= 0:
                 _check(rc, "kvrt_block8_gather_async")
                 return out[0], out[1], out[2] if len(out) > 2 else None
-        td = self._table(table)
+        c, td = self._c(), self._table(table)
         n = int(table.shape[0])
         _int32(lengths, "lengths", n, self.device)
         if start_pos is not None:
@@ -322,7 +334,7 @@ class Block8Pool(_Status):
                     mask = torch.empty(shape[:1] + shape[2:3], dtype=mask_dtype, device=self.device)
             md = None if mask is None else ctypes.byref(tensor_desc(mask))
             _check(self._lib.kvrt_block8_gather_async(
-                self._ref, ctypes.byref(td), lengths.data_ptr(), None if start_pos is None else start_pos.data_ptr(),
+                ctypes.byref(c), ctypes.byref(td), lengths.data_ptr(), None if start_pos is None else start_pos.data_ptr(),
                 ctypes.byref(tensor_desc(out_k)), ctypes.byref(tensor_desc(out_v)), md,
                 ctypes.c_void_p(current_stream_handle(self.device))), "kvrt_block8_gather_async")
         return out_k, out_v, mask
@@ -339,13 +351,12 @@ class Block8Pool(_Status):
         request are left as they are (undefined in a new ``out``). ``max_q``: the
         most rows of one request (more raise ``BLOCK_BAD_INDEX``, the first
         ``max_q`` are computed)."""
-        got = self._call.block_attend(self._at, current_stream_handle(self.device), self.device.index, float(scale), window,
-                                      max_q, q, table, lengths, starts, granted, out)
+        got = self._call.block_attend(*self._head(), float(scale), window, max_q, q, table, lengths, starts, granted, out)
         if type(got) is not int:
             return got
         if got < 0:
             _check(got, "kvrt_block8_attend_async")
-        td = self._table(table)
+        c, td = self._c(), self._table(table)
         n = int(table.shape[0])
         _same(q, "q", self.device)
         _int32(lengths, "lengths", n, self.device)
@@ -360,11 +371,11 @@ class Block8Pool(_Status):
         with _on(self.device):
             if out is None:
                 out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-            size = self._lib.kvrt_block8_attend_work(self._ref, n, int(table.shape[1]), int(q.shape[0]), int(q.shape[1]),
+            size = self._lib.kvrt_block8_attend_work(ctypes.byref(c), n, int(table.shape[1]), int(q.shape[0]), int(q.shape[1]),
                                                      max_q)
             work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
             _check(self._lib.kvrt_block8_attend_async(
-                self._ref, ctypes.byref(tensor_desc(q)), ctypes.byref(td), lengths.data_ptr(), starts.data_ptr(),
+                ctypes.byref(c), ctypes.byref(tensor_desc(q)), ctypes.byref(td), lengths.data_ptr(), starts.data_ptr(),
                 None if granted is None else granted.data_ptr(), ctypes.byref(tensor_desc(out)), float(scale),
                 int(window), max_q, None if work is None else work.data_ptr(), size,
                 ctypes.c_void_p(current_stream_handle(self.device))), "kvrt_block8_attend_async")
