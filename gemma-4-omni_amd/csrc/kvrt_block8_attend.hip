@@ -555,11 +555,13 @@ hipError_t launch_block8_attend(const Block8AttendArgs &a, int dtype, int head_d
 // Zero at load and between launches. Calls on one stream run in order and share a
 // slice; a captured call has a slice of its own for good, since its graph may be
 // replayed beside anything else (a graph does not overlap itself). With the slices
-// used up, calls join in a second launch instead.
+// used up, calls join in a second launch instead, and so do calls on
+// hipStreamPerThread: that handle names another stream in each thread.
 constexpr int kSlices = 512;
 static __device__ uint32_t block8_counters[kSlices * kBlock8MaxWgs];
 
 uint32_t *block8_counter_slice(hipStream_t s) {
+    if (s == hipStreamPerThread) return nullptr;
     static std::mutex mu;
     static std::map<int, uint32_t *> base;
     static std::map<int, int> used;

@@ -730,7 +730,11 @@ int kvrt_block8_gather_async(const kvrt_block8 *pages, const kvrt_tensor *table,
  * rounded to fp16; scores, softmax and sums in fp32. Up to 16 query rows per KV
  * head ((Hq / kv_heads) * max_q) the keys of all requests are divided evenly
  * over the workgroups (a decode step). work: work_bytes >= kvrt_block8_attend_work device
- * bytes, 16-byte aligned; calls that may overlap need one each. Counterpart of
+ * bytes, 16-byte aligned; calls that may overlap need one each. Decode steps also
+ * count arrivals in words that the library keeps for each stream handle: a stream
+ * is idle when it is destroyed, or a new one of the same handle could run beside its
+ * last call. Without counters (hipStreamPerThread, whose handle all threads share) a
+ * second launch does their part, with the same result. Counterpart of
  * kvrt_attend_tensors_async and kvrt_attend_prefill_async. */
 int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, const kvrt_tensor *table,
                              const int32_t *lengths, const int32_t *starts, const int32_t *granted,

@@ -22,3 +22,46 @@ def _run(what: str) -> None:
 @pytest.mark.parametrize("what", ["first", "many"])
 def test_captured_calls_give_the_eager_bits(what):
     _run(what)
+
+
+def test_calls_on_every_threads_own_stream_keep_apart():
+    """hipStreamPerThread is one handle for a stream of each thread: calls of two threads
+    overlap on the GPU and give what they give alone."""
+    import ctypes
+    import threading
+
+    import torch
+
+    from kvrt import _lib as L
+    from kvrt.runtime import tensor_desc
+    from tests.block8_capture_child import SHAPES, served
+
+    lib, per_thread = L.load(), ctypes.c_void_p(2)
+    made = [served(SHAPES[0], seed) for seed in (1, 2)]
+    want = [pool.attend(*args, max_q=1) for pool, args in made]
+    torch.cuda.synchronize()
+    outs = [[torch.zeros_like(w) for _ in range(20)] for w in want]
+    works = []
+    for pool, (q, table, *_) in made:
+        size = lib.kvrt_block8_attend_work(pool._c(), *table.shape, q.shape[0], q.shape[1], 1)
+        works.append(torch.empty(size, dtype=torch.uint8, device="cuda"))
+    torch.cuda.synchronize()
+    codes = [[], []]
+
+    def run(i):
+        pool, (q, table, lengths, starts, scale) = made[i]
+        for out in outs[i]:  # one after the other on the thread's stream
+            codes[i].append(lib.kvrt_block8_attend_async(
+                pool._c(), tensor_desc(q), tensor_desc(table), lengths.data_ptr(), starts.data_ptr(), None, tensor_desc(out),
+                scale, 0, 1, works[i].data_ptr(), works[i].numel(), per_thread))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert codes[i] == [L.KVRT_OK] * 20
+        assert all(torch.equal(out, want[i]) for out in outs[i]), i
+        assert made[i][0].status() == 0
