@@ -731,10 +731,13 @@ int kvrt_block8_gather_async(const kvrt_block8 *pages, const kvrt_tensor *table,
  * head ((Hq / kv_heads) * max_q) the keys of all requests are divided evenly
  * over the workgroups (a decode step). work: work_bytes >= kvrt_block8_attend_work device
  * bytes, 16-byte aligned; calls that may overlap need one each. Decode steps also
- * count arrivals in words that the library keeps for each stream handle: a stream
- * is idle when it is destroyed, or a new one of the same handle could run beside its
- * last call. Without counters (hipStreamPerThread, whose handle all threads share) a
- * second launch does their part, with the same result. Counterpart of
+ * count arrivals in words that the library keeps, on each device for the first 64
+ * stream handles and the first 448 captures (each stream of a capture that makes
+ * such calls counts; a destroyed graph's words are not given to another). A stream is
+ * idle when it is destroyed, or a new one of the same handle could run beside its last
+ * call; calls that one capture records on one stream stay in their order. Calls past
+ * those numbers, and on hipStreamPerThread, whose handle all threads share, join in a
+ * second launch (2.4 to 6 us), with the same result. Counterpart of
  * kvrt_attend_tensors_async and kvrt_attend_prefill_async. */
 int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, const kvrt_tensor *table,
                              const int32_t *lengths, const int32_t *starts, const int32_t *granted,

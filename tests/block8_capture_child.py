@@ -1,8 +1,9 @@
 """Decode attention over 8-bit pages in a process of its own, for what depends on the
 calls a process made before: run by tests/test_gpu_block8_captures.py as
-``python block8_capture_child.py first|many``."""
+``python block8_capture_child.py first|many|layers``."""
 from __future__ import annotations
 
+import ctypes
 import sys
 from pathlib import Path
 
@@ -47,6 +48,25 @@ def capture(pool, args):
     with torch.cuda.graph(g):
         out = pool.attend(*args, max_q=1)
     return g, out
+
+
+def runtime():
+    return ctypes.CDLL(str(Path(torch.__file__).parent / "lib" / "libamdhip64.so"))
+
+
+def capture_id(stream):
+    status, id_ = ctypes.c_int(0), ctypes.c_ulonglong(0)
+    assert runtime().hipStreamGetCaptureInfo(ctypes.c_void_p(stream.cuda_stream), ctypes.byref(status), ctypes.byref(id_)) == 0
+    assert status.value == 1, "the stream is not being captured"
+    return id_.value
+
+
+def launches(g):
+    """Kernels of a graph captured with keep_graph."""
+    hip = runtime()
+    count = ctypes.c_size_t(0)
+    assert hip.hipGraphGetNodes(ctypes.c_void_p(g.raw_cuda_graph()), None, ctypes.byref(count)) == 0
+    return count.value
 
 
 def compare(name, g, out, pool, args):
@@ -95,6 +115,53 @@ def many() -> None:
         assert torch.equal(got, want), shape
 
 
+def layers() -> None:
+    """Captures of many layers: the calls of one capture share their counters, so each is
+    one launch, from the process's first capture on and however many calls there were;
+    also on two streams of one capture, whose calls overlap."""
+    (pool, args), side = served(SHAPES[1]), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs, ids = [], set()
+    for i in range(4):
+        g = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.stream(side):
+            g.capture_begin()
+            ids.add(capture_id(side))
+            outs = [pool.attend(*args, max_q=1) for _ in range(300)]
+            g.capture_end()
+        assert launches(g) == 300, (i, launches(g))
+        print("captured", i, flush=True)
+    assert len(ids) == 4, ids  # what tells captures on one stream apart
+    g.instantiate()
+    want = pool.attend(*args, max_q=1)
+    for _ in range(3):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for out in outs)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        pairs = []
+        for _ in range(20):
+            with torch.cuda.stream(side):
+                a = pool.attend(*args, max_q=1)
+            pairs.append((a, pool.attend(*args, max_q=1)))
+        main.wait_stream(side)
+    for _ in range(5):
+        for pair in pairs:
+            for out in pair:
+                out.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for pair in pairs for out in pair)
+    assert pool.status() == 0
+
+
 if __name__ == "__main__":
-    {"first": first, "many": many}[sys.argv[1]]()
+    {"first": first, "many": many, "layers": layers}[sys.argv[1]]()
     print("done", flush=True)

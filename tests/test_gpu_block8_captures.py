@@ -19,7 +19,7 @@ def _run(what: str) -> None:
     assert r.returncode == 0 and r.stdout.endswith("done\n"), (r.returncode, r.stdout[-2000:], r.stderr[-3000:])
 
 
-@pytest.mark.parametrize("what", ["first", "many"])
+@pytest.mark.parametrize("what", ["first", "many", "layers"])
 def test_captured_calls_give_the_eager_bits(what):
     _run(what)
 
