@@ -563,6 +563,7 @@ struct AttendPlan {
 static AttendPlan attend_plan(int kv_heads, int shift, int head_dim, int64_t n, int64_t width, int64_t rows, int64_t group,
                               int64_t max_q) {
     AttendPlan p{};
+    width = std::max<int64_t>(width, 1);  // a table without columns has rows to be zeroed
     p.chunk = group * max_q > 16;
     if (!p.chunk) {
         // as many workgroups as run at a time (their registers allow 4, 3, 2 and 1 per CU)
@@ -684,7 +685,8 @@ int kvrt_block8_gather_async(const kvrt_block8 *pages, const kvrt_tensor *table,
 uint64_t kvrt_block8_attend_work(const kvrt_block8 *pages, int64_t n, int64_t width, int64_t rows, int64_t hq,
                                  int32_t max_q) {
     Block8View v;
-    if (!view_of(pages, v) || n <= 0 || width <= 0 || rows <= 0 || hq <= 0 || hq % pages->kv_heads != 0 || max_q <= 0) return 0;
+    if (!view_of(pages, v) || n <= 0 || width < 0 || rows <= 0 || hq <= 0 || hq % pages->kv_heads != 0 || max_q <= 0)
+        return 0;
     const AttendPlan p = attend_plan(v.kv_heads, v.shift, pages->head_dim, n, width, rows, hq / v.kv_heads, max_q);
     return part_bytes(p.part_rows, pages->head_dim);
 }
@@ -709,8 +711,7 @@ int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, con
         (width > 0 && !table->data))
         return KVRT_EINVAL;
     a.group = (int)(hq / pages->kv_heads);
-    const AttendPlan plan = attend_plan(a.p.kv_heads, a.p.shift, pages->head_dim, n, std::max<int64_t>(width, 1), q->dims[0],
-                                        a.group, max_q);
+    const AttendPlan plan = attend_plan(a.p.kv_heads, a.p.shift, pages->head_dim, n, width, q->dims[0], a.group, max_q);
     const int64_t heads = n * pages->kv_heads;
     if (!plan.chunk && plan.most * heads >= (int64_t)1 << 31) return KVRT_EINVAL;  // units are numbered in 32 bits
     if (plan.chunk && plan.tiles > 65535) return KVRT_EINVAL;                      // row tiles are a grid dimension

@@ -226,3 +226,31 @@ def test_tables_hold_at_most_two_to_the_thirty_positions():
     o, q = _tensor(L, L.DT_BF16, (2, 2, 5, 128)), _tensor(L, L.DT_BF16, (2, 4, 128))
     assert lib.kvrt_block8_gather_async(p, wide, AT, None, o, o, None, None) == L.KVRT_EINVAL
     assert lib.kvrt_block8_attend_async(p, q, wide, AT, AT, None, q, 1.0, 0, 1, AT, 1 << 40, None) == L.KVRT_EINVAL
+
+
+WORKED = [(n, width, rows, hq, max_q, dim, block) for n in (1, 3, 70) for width in (0, 1, 9, 400) for rows in (1, 5, 900)
+          for hq, max_q in ((2, 1), (16, 2), (16, 5), (64, 300)) for dim, block in ((64, 16), (512, 128))]
+
+
+@pytest.mark.parametrize("dim,block", [(64, 16), (512, 128)])
+def test_attend_takes_the_workspace_it_asks_for(dim, block):
+    """Every size that attend_work answers is accepted (the launch itself then fails here),
+    and one byte less is refused; tables without columns among them."""
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is visible: the calls would launch on host memory")
+    L, lib = _lib()
+    p = _pages(L, head_dim=dim, block=block)
+    for n, width, rows, hq, max_q, *shape in WORKED:
+        if shape != [dim, block]:
+            continue
+        size = lib.kvrt_block8_attend_work(p, n, width, rows, hq, max_q)
+        table = _tensor(L, L.DT_INT32, (n, width), data=AT if width else None)
+        q = _tensor(L, L.DT_BF16, (rows, hq, dim))
+        call = lambda work, nbytes: lib.kvrt_block8_attend_async(p, q, table, AT, AT, None, q, 1.0, 0, max_q, work,  # noqa: E731
+                                                                 nbytes, None)
+        assert call(AT if size else None, size) == L.KVRT_EDEVICE, (n, width, rows, hq, max_q)
+        if size:
+            assert call(AT, size - 1) == L.KVRT_EINVAL
+    assert lib.kvrt_block8_attend_work(p, 2, -1, 2, 4, 1) == 0
