@@ -541,12 +541,16 @@ static bool disjoint(const kvrt_tensor *t) {
     return true;
 }
 
-// (2^30 positions: kernels add a step of keys, and subtract windows and row counts, in 32 bits)
+// Limits of a table, for the calls that build it and those that read it: requests are a
+// grid dimension; kernels add a step of keys, and subtract windows and row counts, in 32
+// bits.
+constexpr int64_t kTableRequests = 65535, kTablePositions = (int64_t)1 << 30;
+
 static bool table_ok(const kvrt_tensor *t, int shift, int64_t &n, int64_t &width) {
     if (!strided(t, KVRT_INT32, 4, 2, 4)) return false;
     n = t->dims[0];
     width = t->dims[1];
-    return n <= 65535 && width <= (int64_t)1 << 30 >> shift;
+    return n <= kTableRequests && width <= kTablePositions >> shift;
 }
 
 constexpr int64_t kMaxRows = (int64_t)1 << 30, kJoinBytes = 48 << 10;
@@ -597,10 +601,10 @@ extern "C" {
 int kvrt_block_tables_update_async(const kvrt_block_tables *t, const int32_t *lengths, const int32_t *new_rows,
                                    int64_t rows, int32_t *starts, int32_t *slot_map, int32_t *out_lengths,
                                    int32_t *granted, void *stream) {
-    if (!t || t->n < 1 || t->n > 65536 || t->max_pages < 1 || t->pool_pages < 1) return KVRT_EINVAL;
+    if (!t || t->n < 1 || t->n > kTableRequests || t->max_pages < 1 || t->pool_pages < 1) return KVRT_EINVAL;
     const int shift = block_shift(t->block);
     const int64_t limit = (int64_t)1 << 31;
-    if (shift < 0 || (int64_t)t->n * t->max_pages >= limit || (int64_t)t->max_pages * t->block >= limit ||
+    if (shift < 0 || (int64_t)t->n * t->max_pages >= limit || t->max_pages > kTablePositions >> shift ||
         (int64_t)t->pool_pages * t->block >= limit || rows < 0 || rows > kMaxRows)
         return KVRT_EINVAL;
     for (const void *p : {(const void *)t->table, (const void *)t->mapped, (const void *)t->free_pages,

@@ -137,12 +137,13 @@ class BlockTables(_Status):
                  device: torch.device | str | None = None) -> None:
         self._lib = L.load()
         self.n, self.max_pages, self.pool_pages, self.block_size = map(int, (n, max_pages, pool_pages, block_size))
-        if not 1 <= self.n <= 65536 or self.max_pages < 1 or self.pool_pages < 1:
-            raise ValueError("tables need 1 to 65536 requests and at least one page")
+        if not 1 <= self.n <= 65535 or self.max_pages < 1 or self.pool_pages < 1:
+            raise ValueError("tables need 1 to 65535 requests and at least one page")
         if self.block_size not in (16, 32, 64, 128):
             raise ValueError(f"block_size must be 16, 32, 64 or 128, got {block_size}")
-        if max(self.n * self.max_pages, self.max_pages * self.block_size, self.pool_pages * self.block_size) > _I32_MAX:
-            raise ValueError("tables number entries, positions and slots in 32 bits")
+        if max(self.n * self.max_pages, self.pool_pages * self.block_size) > _I32_MAX or \
+                self.max_pages * self.block_size > 2 ** 30:
+            raise ValueError("tables number entries and slots in 32 bits, and hold up to 2^30 positions a request")
         self.device = _device(device)
         make = dict(dtype=torch.int32, device=self.device)
         self.table = torch.full((self.n, self.max_pages), -1, **make)

@@ -655,8 +655,8 @@ typedef struct kvrt_block_tables {
     int32_t *free_count; /* [1]                                                            */
     int32_t *work;       /* [KVRT_BLOCK_TABLES_WORK(n)]: scratch of the calls              */
     int32_t *status;     /* device word, KVRT_BLOCK_* bits or'ed in                        */
-    int32_t n;           /* 1..65536                                                       */
-    int32_t max_pages;   /* n * max_pages and max_pages * block < 2^31                     */
+    int32_t n;           /* 1..65535                                                       */
+    int32_t max_pages;   /* n * max_pages < 2^31, max_pages * block <= 2^30                */
     int32_t pool_pages;  /* pool_pages * block < 2^31                                      */
     int32_t block;       /* tokens per page: 16, 32, 64 or 128                             */
 } kvrt_block_tables;

@@ -254,3 +254,37 @@ def test_attend_takes_the_workspace_it_asks_for(dim, block):
         if size:
             assert call(AT, size - 1) == L.KVRT_EINVAL
     assert lib.kvrt_block8_attend_work(p, 2, -1, 2, 4, 1) == 0
+
+
+def test_tables_that_update_takes_are_tables_that_attention_reads():
+    """One limit of requests (65535) and of positions (2^30) for all calls."""
+    import torch
+
+    from kvrt import BlockTables
+
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is visible: the calls would launch on host memory")
+    L, lib = _lib()
+
+    def update(n, max_pages, block):
+        t = L.KvrtBlockTables()
+        t.table = t.mapped = t.free_pages = t.free_count = t.work = t.status = AT
+        t.n, t.max_pages, t.pool_pages, t.block = n, max_pages, 8, block
+        return lib.kvrt_block_tables_update_async(t, AT, AT, 1, AT, AT, AT, AT, None)
+
+    def read(n, width, block):
+        p, table = _pages(L, block=block), _tensor(L, L.DT_INT32, (n, width))
+        o, q = _tensor(L, L.DT_BF16, (n, 2, 5, 128)), _tensor(L, L.DT_BF16, (2, 4, 128))
+        return (lib.kvrt_block8_gather_async(p, table, AT, None, o, o, None, None),
+                lib.kvrt_block8_attend_async(p, q, table, AT, AT, None, q, 1.0, 0, 1, AT, 1 << 40, None))
+
+    for block in (16, 128):
+        most = (1 << 30) // block
+        for n, width in ((1, most), (65535, 9)):
+            assert update(n, width, block) == L.KVRT_EDEVICE and read(n, width, block) == (L.KVRT_EDEVICE,) * 2
+            with pytest.raises(RuntimeError, match="GPU"):
+                BlockTables(n, width, 8, block_size=block)
+        for n, width in ((1, most + 1), (65536, 9), (65537, 9)):
+            assert update(n, width, block) == L.KVRT_EINVAL and read(n, width, block) == (L.KVRT_EINVAL,) * 2
+            with pytest.raises(ValueError, match="65535|positions"):
+                BlockTables(n, width, 8, block_size=block)
