@@ -366,7 +366,8 @@ class Block8Pool(_Status):
             _int32(granted, "granted", n, self.device)
         if q.dim() != 3:
             raise ValueError(f"q must be [T, Hq, {self.head_dim}], got {tuple(q.shape)}")
-        max_q = min(int(max_q), int(q.shape[0]))
+        # brought into 32 bits: a window past every key is none, negative numbers are refused
+        max_q, window = max(-1, min(int(max_q), int(q.shape[0]))), max(-1, min(int(window), _I32_MAX))
         if out is not None:
             _same(out, "out", self.device)
         with _on(self.device):
@@ -378,6 +379,6 @@ class Block8Pool(_Status):
             _check(self._lib.kvrt_block8_attend_async(
                 ctypes.byref(c), ctypes.byref(tensor_desc(q)), ctypes.byref(td), lengths.data_ptr(), starts.data_ptr(),
                 None if granted is None else granted.data_ptr(), ctypes.byref(tensor_desc(out)), float(scale),
-                int(window), max_q, None if work is None else work.data_ptr(), size,
+                window, max_q, None if work is None else work.data_ptr(), size,
                 ctypes.c_void_p(current_stream_handle(self.device))), "kvrt_block8_attend_async")
         return out

@@ -32,3 +32,27 @@ def test_a_table_without_columns_gives_zero_rows(hq, heads, dim, counts):
     assert pool.status() == R.BAD and (out[:rows] == 0).all()
     k, v, mask = pool.gather(table, _i32([0] * n), 3)
     assert (k == 0).all() and (v == 0).all() and not mask.any()
+
+
+@pytest.mark.parametrize("hq,count", [(2, 1), (4, 40)])
+def test_windows_and_row_counts_past_32_bits(hq, count):
+    """A window of any size past the keys is none; negative numbers are refused, also
+    where their lowest 32 bits are not."""
+    from kvrt import Block8Pool, KVRTError
+
+    gen = torch.Generator().manual_seed(2)
+    pool = Block8Pool.zeros(6, 2, 128)
+    x = randn_bf16(gen, (80, 2, 128)).cuda()
+    pool.append(x, x, _i32([*range(80)]))
+    q, table = randn_bf16(gen, (count, hq, 128)).cuda(), _i32([[0, 1, 2, 3, 4]])
+    call = lambda **kw: pool.attend(q, table, _i32([80]), _i32([0, count]), 0.1, **{"max_q": count, **kw})  # noqa: E731
+    want, short = call(), call(window=5)
+    assert not torch.equal(want, short)
+    for window in (2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 40 + 7, 2 ** 64 + 5):
+        assert torch.equal(call(window=window), want), window
+    assert torch.equal(call(max_q=2 ** 32 + count - 1), want) and torch.equal(call(max_q=2 ** 64), want)
+    for bad in (dict(window=-1), dict(window=-2 ** 32 + 5), dict(window=-2 ** 40), dict(max_q=-2 ** 32 + count),
+                dict(max_q=-2 ** 31)):
+        with pytest.raises(KVRTError):
+            call(**bad)
+    assert pool.status() == 0
