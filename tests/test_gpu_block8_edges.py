@@ -56,3 +56,27 @@ def test_windows_and_row_counts_past_32_bits(hq, count):
         with pytest.raises(KVRTError):
             call(**bad)
     assert pool.status() == 0
+
+
+@pytest.mark.parametrize("n", [64, 65, 700])
+@pytest.mark.parametrize("count", [1, 40])
+def test_bad_numbers_of_requests_without_rows_are_reported(n, count):
+    """Behind the last request with rows too, however many requests there are."""
+    from kvrt import Block8Pool
+
+    pool = Block8Pool.zeros(4, 1, 64)
+    x = randn_bf16(torch.Generator().manual_seed(3), (64, 1, 64)).cuda()
+    pool.append(x, x, _i32([*range(64)]))
+    table = torch.full((n, 4), -1, dtype=torch.int32)
+    table[1] = torch.arange(4)
+    lengths, starts = [0] * n, [0, 0] + [count] * (n - 1)
+    lengths[1] = 64
+    call = lambda lens: pool.attend(x[:count], table.cuda(), _i32(lens), _i32(starts), 0.1, max_q=count)  # noqa: E731
+    want = call(lengths)
+    assert pool.status() == 0
+    for i in (0, 2, n - 2, n - 1):
+        for bad in (65, -1):
+            lens = list(lengths)
+            lens[i] = bad
+            assert torch.equal(call(lens), want)
+            assert pool.status() == R.BAD, (i, bad)
