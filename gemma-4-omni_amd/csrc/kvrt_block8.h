@@ -62,11 +62,10 @@ struct Block8AttendArgs {
     int wgs;                               // workgroups the keys are divided over (each row tile)
     int join_most;                         // partials of a head that one workgroup may join (sets the division)
     int join_all;                          // divide so that no head has more
-    int join_here;                         // join_most with counters, 1 without: a second launch joins the others
     float scale_log2;                      // scale * log2(e)
     float *part_o;                         // partials of divided heads [tile][wg][2][16 rows][D]
     float2 *part_ml;                       // their (max, sum) [tile][wg][2][16]
-    uint32_t *counters;                    // arrivals [wg], zero between launches
+    uint32_t *counters;                    // arrivals [wg], zero between launches; none: a second launch joins
     // chunks (kvrt_block8_chunk.h): tiles of 32 * row_waves rows, at most `tiles` of them,
     // keys divided over `splits` workgroups; partials [tile][head][split][row][D]
     int row_waves, tiles, splits;

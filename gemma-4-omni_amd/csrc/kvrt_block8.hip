@@ -752,14 +752,13 @@ int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, con
     // more, all are; else a second launch joins the others. The division follows the
     // shape alone; without arrival counters the second launch joins every head.
     bool join = false;
-    a.join_most = a.join_here = 1;
+    a.join_most = 1;
     if (a.wgs > 1) {
         const int64_t rows = std::min<int64_t>(16, (int64_t)a.group * max_q);
         a.join_most = (int)std::min<int64_t>(32, kJoinBytes / (rows * pages->head_dim * 4));
         a.join_all = plan.most > a.join_most && heads * (a.join_most - 1) >= 512;
         a.counters = a.join_most > 1 ? block8_counter_slice(st) : nullptr;
-        a.join_here = a.counters ? a.join_most : 1;
-        join = plan.most > a.join_here && !(a.join_all && a.counters);
+        join = !a.counters || (plan.most > a.join_most && !a.join_all);
     }
     const hipError_t e = launch_block8_attend(a, pages->dtype, pages->head_dim, join, st);
     return e == hipSuccess ? KVRT_OK : KVRT_EDEVICE;

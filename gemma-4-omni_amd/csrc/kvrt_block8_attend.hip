@@ -399,7 +399,7 @@ __global__ __launch_bounds__(256) void block8_attend_kernel(Block8AttendArgs a) 
         const int parts = min(max(t_end - (t_begin - wave), 0), 4);
         const bool begins = ua == 0, ends = ub == units;
         const int w0 = seg / div.per, count = (seg + units - 1) / div.per - w0 + 1;  // workgroups of the head
-        const bool here = count <= a.join_here;                                       // joined in this launch
+        const bool here = a.counters && count <= a.join_most;                         // joined in this launch
         const int64_t slot0 = 0;
         for (int e = threadIdx.x; e < r.n * (D / 4); e += 256) {
             const int rr = e / (D / 4), d = 4 * (e % (D / 4));
@@ -493,7 +493,7 @@ __global__ __launch_bounds__(256) void block8_join_kernel(Block8AttendArgs a) {
     const Division div = divide(a, all, most);
     const int units = units_of(r), seg = before * a.p.kv_heads + head * units;
     const int w0 = seg / div.per, count = (seg + units - 1) / div.per - w0 + 1;
-    if (count <= a.join_here) return;
+    if (count == 1 || (a.counters && count <= a.join_most)) return;
     const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
     const int groups = count <= kFlat ? 1 : GROUPS;
     float M = kNegBig, sum = 0.f;

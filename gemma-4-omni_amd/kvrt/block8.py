@@ -247,11 +247,6 @@ class Block8Pool(_Status):
         c.dtype, c.pages, c.kv_heads, c.block, c.head_dim = _CODES[self._dtype], *codes
         return c
 
-    def _head(self) -> tuple:
-        """What every native call begins with: sizes, stream, device and the pool's tensors."""
-        return (self._sizes_at, current_stream_handle(self.device), self.device.index, self.k, self.v, self.k_scale,
-                self.v_scale)
-
     @classmethod
     def zeros(cls, pages: int, kv_heads: int, head_dim: int, *, block_size: int = 16, dtype: str = "int8",
               device: torch.device | str | None = None) -> "Block8Pool":
@@ -277,7 +272,8 @@ class Block8Pool(_Status):
         them are coded anew; rows behind them (rolled back) are dropped. A page
         takes one run of consecutive slots per call; a slot map that names a slot
         twice or enters a page twice leaves that page undefined."""
-        rc = self._call.block_append(*self._head(), k, v, slot_map)
+        rc = self._call.block_append(self._sizes_at, current_stream_handle(self.device), self.device.index, self.k, self.v,
+                                     self.k_scale, self.v_scale, k, v, slot_map)
         if rc <= 0:
             return _check(rc, "kvrt_block8_append_async")
         c = self._c()
@@ -298,14 +294,16 @@ class Block8Pool(_Status):
         ``out``: (K, V) or (K, V, mask) destinations instead of new tensors (strided
         views with a contiguous last dimension); they then set Lmax and dtype."""
         if out is None and dtype in _FLOATS and mask_dtype in _MASKS:
-            got = self._call.block_gather_new(*self._head(), table, lengths, start_pos, lmax, _FLOATS[dtype],
+            got = self._call.block_gather_new(self._sizes_at, current_stream_handle(self.device), self.device.index, self.k, self.v,
+                                              self.k_scale, self.v_scale, table, lengths, start_pos, lmax, _FLOATS[dtype],
                                               _MASKS[mask_dtype])
             if type(got) is tuple:
                 return got
             if got < 0:
                 _check(got, "kvrt_block8_gather_async")
         elif out is not None and lmax is None:
-            rc = self._call.block_gather(*self._head(), table, lengths, start_pos, out[0], out[1],
+            rc = self._call.block_gather(self._sizes_at, current_stream_handle(self.device), self.device.index, self.k, self.v,
+                                         self.k_scale, self.v_scale, table, lengths, start_pos, out[0], out[1],
                                          out[2] if len(out) > 2 else None)
             if rc <= 0:
                 _check(rc, "kvrt_block8_gather_async")
@@ -352,7 +350,9 @@ class Block8Pool(_Status):
         request are left as they are (undefined in a new ``out``). ``max_q``: the
         most rows of one request (more raise ``BLOCK_BAD_INDEX``, the first
         ``max_q`` are computed)."""
-        got = self._call.block_attend(*self._head(), float(scale), window, max_q, q, table, lengths, starts, granted, out)
+        got = self._call.block_attend(self._sizes_at, current_stream_handle(self.device), self.device.index, self.k, self.v,
+                                      self.k_scale, self.v_scale, float(scale), window, max_q, q, table, lengths, starts,
+                                      granted, out)
         if type(got) is not int:
             return got
         if got < 0:
