@@ -288,3 +288,19 @@ def test_tables_that_update_takes_are_tables_that_attention_reads():
             assert update(n, width, block) == L.KVRT_EINVAL and read(n, width, block) == (L.KVRT_EINVAL,) * 2
             with pytest.raises(ValueError, match="65535|positions"):
                 BlockTables(n, width, 8, block_size=block)
+
+
+def test_decode_divides_over_the_workgroups_that_run_at_a_time():
+    """A unit of work per place: waves a SIMD as the build reports them for the kernel
+    (a workgroup of four waves takes one on each), 256 CUs."""
+    L, lib = _lib()
+    report = L.LIB_PATH.parent / "kernel_resources.json"
+    if not report.exists():
+        pytest.skip("the build left no report")
+    built = json.loads(report.read_text())
+    for dim in (64, 128, 256, 512):
+        waves = [int(v["Occupancy"]) for k, v in built.items() if "block8_attend_kernel" in k and f"ELi{dim}E" in k]
+        assert len(waves) == 2  # int8, e4m3
+        p = _pages(L, head_dim=dim, kv_heads=8)
+        size = lib.kvrt_block8_attend_work(p, 64, 500, 64, 8, 1)
+        assert size == 256 * min(waves) * 2 * 16 * (4 * dim + 8), dim
