@@ -65,3 +65,53 @@ def test_calls_on_every_threads_own_stream_keep_apart():
         assert codes[i] == [L.KVRT_OK] * 20
         assert all(torch.equal(out, want[i]) for out in outs[i]), i
         assert made[i][0].status() == 0
+
+
+@pytest.mark.parametrize("name,hq,heads,dim", [("int8", 4, 2, 64), ("e4m3", 8, 1, 256), ("int8", 2, 1, 512)])
+def test_a_captured_chunk_step_follows_the_lengths(name, hq, heads, dim):
+    """Tables of so many rows that they take two launches, append, chunk attention and the
+    padded batch in one graph; chunks of other lengths at each replay, some refused."""
+    import torch
+
+    from kvrt import Block8Pool, BlockTables
+    from tests.helpers import randn_bf16
+
+    gen = torch.Generator().manual_seed(dim)
+    n, rows, block, pages = 3, 4400, 16, 330
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    k, v = (torch.zeros((rows, heads, dim), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q = torch.zeros((rows, hq, dim), dtype=torch.bfloat16, device="cuda")
+    keep, new = i32([0] * n), i32([0] * n)
+
+    def make():
+        return (BlockTables(n, 300, pages, block_size=block), Block8Pool.zeros(pages, heads, dim, block_size=block, dtype=name),
+                torch.full_like(q, 5.0))
+
+    def step(tables, pool, out):
+        plan = tables.update(keep, new, rows=rows)
+        pool.append(k, v, plan.slot_map)
+        pool.attend(q, tables.table, plan.lengths, plan.starts, dim ** -0.5, max_q=rows, granted=plan.granted, out=out)
+        return (*plan, *pool.gather(tables.table, plan.lengths, 500, dtype=torch.float32))
+
+    eager, graphed = make(), make()
+    step(*make())
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step(*graphed)
+    for lens, adds in (([0, 0, 0], [1400, 37, 1]), ([1400, 30, 1], [1, 2900, 33]), ([700, 0, 34], [4000, 100, 260]),
+                       ([701, 100, 290], [64, 65, 4200]), ([0, 3, 0], [0, 4000, 400])):
+        for t, x in ((keep, lens), (new, adds)):
+            t.copy_(i32(x))
+        for t in (k, v, q):
+            t.copy_(randn_bf16(gen, t.shape))
+        want = step(*eager)
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), lens
+        assert torch.equal(eager[2], graphed[2]), lens
+        assert eager[0].status() == graphed[0].status() and eager[1].status() == graphed[1].status()
+        for a, b in zip((eager[0].table, eager[0].free_count, eager[1].k.view(torch.int8), eager[1].v_scale),
+                        (graphed[0].table, graphed[0].free_count, graphed[1].k.view(torch.int8), graphed[1].v_scale)):
+            assert torch.equal(a, b), lens
