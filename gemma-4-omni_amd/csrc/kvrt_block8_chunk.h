@@ -15,10 +15,14 @@
 //
 // Bound by its vector and matrix instructions, which the two waves of a SIMD overlap only
 // in part: at D 128 over 5600 keys counters show vector issue on half of all cycles and
-// LDS on a quarter. Steps are therefore as long as LDS allows (fewer barriers), and nothing in a step waits for a load of its own. Measured: 4 requests of
-// 512 rows, 16 heads over 8, D 128: 46 us over 1400 keys, 151 us over 5600 (0.59 PFLOP/s);
-// 4 of 291, 8 heads over 1, D 256: 123 us over 4678 keys; one of 512, 16 heads over 2,
-// D 512: 126 us over 4096.
+// LDS on a quarter. Steps are therefore as long as LDS allows (fewer barriers), and nothing
+// in a step waits for a load of its own. That serves long contexts: looking pages up a
+// step ahead and a third staged step took the sliding chunk (four of 291 rows, window 512,
+// D 256) from 33 to 37 us and the talker's (512 rows over 1400 keys) from 44 to 46.
+// Measured, this kernel and the join of its splits: 4 requests of 512 rows, 16 heads over 8,
+// D 128: 46 us over 1400 keys, 155 us over 5600 (0.58 PFLOP/s); 4 of 291, 8 heads over 1,
+// D 256: 125 + 9 us over 4678 keys; one of 512, 16 heads over 2, D 512: 131 + 15 us over
+// 4096.
 //
 // Lane layouts (32x32x16): A[row l%32][k 8(l/32)+j], B[k 8(l/32)+j][col l%32],
 // D[row 8(i/4) + 4(l/32) + i%4][col l%32].
@@ -251,8 +255,8 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::NW) void block8_chunk_kernel(Bl
         ids = a.table[(int64_t)req * a.table_stride + (min(key, r.kend - 1) >> a.p.shift)];
     };
     // Codes of step s to registers (D 512: to LDS). Nothing here may read them: that would
-    // wait for the load in front of the step's work (one request, D 512, 4096 keys:
-    // 238 us instead of 136).
+    // wait for the load in front of the step's work (one request of 512 rows, D 512, 4096
+    // keys: 238 us for 136, when that was changed).
     auto fetch = [&](auto v_c, int s, int ids) __attribute__((always_inline)) {
         constexpr bool V = decltype(v_c)::value;
         const uint8_t *codes = V ? a.p.v : a.p.k;

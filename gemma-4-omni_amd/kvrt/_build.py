@@ -2,7 +2,8 @@
 
 The library is compiled from ``csrc/kvrt_kernels.hip`` (kernels),
 ``csrc/kvrt_prefill.hip`` and ``csrc/kvrt_prefill_wide.hip`` (chunked prefill),
-``csrc/kvrt_block8.hip`` and ``csrc/kvrt_block8_attend.hip`` (8-bit pages)
+``csrc/kvrt_block8.hip``, ``csrc/kvrt_block8_attend.hip`` and
+``csrc/kvrt_block8_chunk.hip`` (8-bit pages)
 and ``csrc/kvrt_runtime.hip`` (host runtime, C ABI in ``include/kvrt.h``);
 kvrt_pycall.so, the calls that read torch tensors directly, from
 ``csrc/kvrt_pycall.cpp`` with the host compiler. The build also compiles

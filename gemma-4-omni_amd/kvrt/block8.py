@@ -25,7 +25,8 @@ calls. The kernels are hand-written for gfx950 behind include/kvrt.h; there
 is no PyTorch or CPU path. Calls run on the current torch stream of the
 tensors' device. An object's calls belong on one stream at a time (``update``
 and ``append`` write its state); ``gather`` and ``attend`` only read a pool and
-may overlap, captured or not: each ``attend`` has a workspace of its own. The
+may overlap, captured or not: each ``attend`` has a workspace of its own. Pools
+have their tables' ``block_size``: page ids and slots do not carry it. The
 reference holds no paged or block-scaled KV.
 """
 from __future__ import annotations
@@ -349,7 +350,8 @@ class Block8Pool(_Status):
         only the last W of them. A row that sees no key becomes zeros; rows of no
         request are left as they are (undefined in a new ``out``). ``max_q``: the
         most rows of one request (more raise ``BLOCK_BAD_INDEX``, the first
-        ``max_q`` are computed)."""
+        ``max_q`` are computed). ``out`` shares no memory with ``q``. The same inputs
+        give the same bits, captured or not, whatever was called before."""
         got = self._call.block_attend(self._sizes_at, current_stream_handle(self.device), self.device.index, self.k, self.v,
                                       self.k_scale, self.v_scale, float(scale), window, max_q, q, table, lengths, starts,
                                       granted, out)

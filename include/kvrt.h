@@ -628,7 +628,8 @@ int kvrt_copy_rows_async(const kvrt_tensor *src, const kvrt_tensor *dst, int64_t
 /* ---- 8-bit pages with a scale per page and head ------------------------------- */
 /* Caller-owned pages of one layer. Codes are int8 in [-127, 127] or e4m3, and a
  * code stands for code * scale with one fp32 scale per (page, KV head). A scale
- * is read as within [2^-64, 2^32]. Every layer of a model has pages of its own;
+ * is read as within [2^-64, 2^32]. No append makes a NaN code; one that a caller puts
+ * into a row that some query of a request sees may reach its other queries. Every layer of a model has pages of its own;
  * one page table serves all of them. The calls below are context-free: they
  * run on the current device and the given stream, allocate nothing, return
  * KVRT_EINVAL (nothing enqueued) for arguments they do not take and
