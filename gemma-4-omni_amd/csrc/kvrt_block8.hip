@@ -554,6 +554,7 @@ static bool table_ok(const kvrt_tensor *t, int shift, int64_t &n, int64_t &width
 }
 
 constexpr int64_t kMaxRows = (int64_t)1 << 30, kJoinBytes = 48 << 10;
+constexpr int64_t kGridWgs = (1 << 24) - 1;  // workgroups of 256 threads whose threads 32 bits count
 
 // How a call's rows and keys are divided.
 struct AttendPlan {
@@ -640,6 +641,7 @@ int kvrt_block8_append_async(const kvrt_block8 *pages, const kvrt_tensor *k, con
         a.head[i] = x[i]->strides[1];
     }
     a.chunk = a.rows * 2 * pages->kv_heads <= 4096 ? 1 : 16;
+    if ((a.rows + a.chunk - 1) / a.chunk * 2 * pages->kv_heads > 4 * kGridWgs) return KVRT_EINVAL;
     const hipError_t e = launch_block8_append(a, pages->dtype, pages->head_dim, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? KVRT_OK : KVRT_EDEVICE;
 }
@@ -663,7 +665,7 @@ int kvrt_block8_gather_async(const kvrt_block8 *pages, const kvrt_tensor *table,
             return KVRT_EINVAL;
     }
     if (n == 0 || lmax == 0) return KVRT_OK;
-    if (lmax > kMaxRows || !disjoint(out_k) || !disjoint(out_v) || (mask && !disjoint(mask))) return KVRT_EINVAL;
+    if (lmax > kGridWgs * (4096 / pages->head_dim) || !disjoint(out_k) || !disjoint(out_v) || (mask && !disjoint(mask))) return KVRT_EINVAL;
     if (!aligned(lengths, 4) || (start_pos && !aligned(start_pos, 4)) || (width > 0 && !table->data))
         return KVRT_EINVAL;
     a.table = static_cast<const int32_t *>(table->data);

@@ -109,7 +109,8 @@ class _Status:
         """Wait for the current stream, then return and clear the reported bits:
         0, or ``BLOCK_BAD_INDEX`` (1: a page id, slot, length or row count out of
         range was skipped), ``BLOCK_NO_PAGES`` (2: a request was refused for want
-        of pages), ``BLOCK_NOT_FINITE`` (4: an appended value was not finite)."""
+        of pages), ``BLOCK_NOT_FINITE`` (4: an appended value was not finite). One that
+        a call on another stream raises meanwhile may be lost."""
         bits = int(self._status.item())
         if bits:
             self._status.zero_()

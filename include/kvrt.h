@@ -702,7 +702,8 @@ int kvrt_block_tables_update_async(const kvrt_block_tables *tables, const int32_
  * where s' > s, each code before the run becomes code * (s / s'), both rounded
  * to the nearest code (ties to even) and clamped to the largest. A page takes
  * one run per call: slots that put two runs into one page (or name one slot
- * twice) leave that page's rows undefined. Counterpart of kvrt_append_async's
+ * twice) leave that page's rows undefined. T * kv_heads <= 2^29 - 32 and T <= 2^30 (32
+ * bits count a launch's threads). Counterpart of kvrt_append_async's
  * in-kernel quantisation (one scale per token and head there). */
 int kvrt_block8_append_async(const kvrt_block8 *pages, const kvrt_tensor *k, const kvrt_tensor *v,
                              const int32_t *slot_map, void *hip_stream);
@@ -711,7 +712,8 @@ int kvrt_block8_append_async(const kvrt_block8 *pages, const kvrt_tensor *k, con
  * KVRT_BF16 or KVRT_FP32 (last dim contiguous, 16-byte aligned rows); row j of
  * request i is position start_pos[i] + j (start_pos device int32 [n], or NULL
  * for 0; a negative one is a bad index) while that lies below lengths[i],
- * zeros after. table: KVRT_INT32 [n, width], n <= 65535, width * block <= 2^30;
+ * zeros after; Lmax * head_dim <= 2^36 - 4096. table: KVRT_INT32 [n, width], n <= 65535,
+ * width * block <= 2^30;
  * mask [n, Lmax] as for
  * kvrt_gather_async, or NULL. Counterpart of kvrt_gather_async. */
 int kvrt_block8_gather_async(const kvrt_block8 *pages, const kvrt_tensor *table, const int32_t *lengths,

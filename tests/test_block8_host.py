@@ -304,3 +304,22 @@ def test_decode_divides_over_the_workgroups_that_run_at_a_time():
         p = _pages(L, head_dim=dim, kv_heads=8)
         size = lib.kvrt_block8_attend_work(p, 64, 500, 64, 8, 1)
         assert size == 256 * min(waves) * 2 * 16 * (4 * dim + 8), dim
+
+
+def test_launches_of_more_threads_than_32_bits_count_are_refused():
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is visible: the calls would launch on host memory")
+    L, lib = _lib()
+    for heads, most in ((1, (1 << 29) - 32), (8, (1 << 26) - 16)):  # a wave for 16 rows of each head of K and V
+        p = _pages(L, kv_heads=heads, head_dim=64)
+        for rows, want in ((most, L.KVRT_EDEVICE), (2 * most, L.KVRT_EINVAL)):
+            x = _tensor(L, L.DT_BF16, (rows, heads, 64))
+            assert lib.kvrt_block8_append_async(p, x, x, AT, None) == want, (heads, rows)
+    table = _tensor(L, L.DT_INT32, (1, 4))
+    for dim, rows in ((128, 32), (512, 8)):  # rows a workgroup of 256 threads
+        p, most = _pages(L, kv_heads=1, head_dim=dim), ((1 << 24) - 1) * rows
+        for lmax, want in ((most, L.KVRT_EDEVICE), (most + 1, L.KVRT_EINVAL)):
+            o = _tensor(L, L.DT_BF16, (1, 1, lmax, dim))
+            assert lib.kvrt_block8_gather_async(p, table, AT, None, o, o, None, None) == want, (dim, lmax)
