@@ -150,7 +150,8 @@ def prepare(case: dict, seed: int) -> dict:
             from kvrt import HeadRotation
 
             s["rotation"] = HeadRotation(d, s["inv_freq"], axes=_axis_of(c), adjacent=bool(c["adjacent"]),
-                                         norm=c["norm"], q_weight=s["qw"], k_weight=s["kw"], eps=EPS)
+                                         norm=c["norm"], eps=EPS,
+                                         **({} if c["norm"] == "none" else {"q_weight": s["qw"], "k_weight": s["kw"]}))
         return s
     lens = _lengths(c)
     s["lengths"] = torch.tensor(lens, device="cuda")
