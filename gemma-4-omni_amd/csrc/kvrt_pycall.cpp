@@ -550,12 +550,98 @@ PyObject *connect_blocks(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     Py_RETURN_NONE;
 }
 
+// ---- heads normed and rotated (kvrt/rotation.py) -------------------------------------
+
+decltype(&kvrt_rotate_heads_async) rotate_api;
+
+// Heads [n, H, Q, D] or packed [T, H, D] as kvrt_rotate_heads_async takes them.
+bool describe_heads(const at::Tensor *t, kvrt_tensor &d) {
+    if (!t || (t->dim() != 3 && t->dim() != 4) || !describe(t, d)) return false;
+    if (d.ndim == 3) {
+        d.ndim = 4;
+        d.dims[3] = d.dims[2], d.strides[3] = d.strides[2];
+        d.dims[2] = 1, d.strides[2] = 0;
+    }
+    return true;
+}
+
+// (rotation, stream, device, q, k, v, positions, out_q, out_k, out_v; each tensor may be None)
+// -> (q, k, v)
+PyObject *rotate_heads(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded_object(nargs, 10, [&](PyObject *&answer) -> long {
+        int32_t dev;
+        const auto *rot = static_cast<const kvrt_rotation *>(PyLong_AsVoidPtr(a[0]));
+        void *stream = PyLong_AsVoidPtr(a[1]);
+        if (!rot || !read_int(a[2], dev) || !current_device(dev)) return kGeneral;
+        kvrt_tensor in[3], to[3], pos;
+        at::Tensor fresh_out[3];
+        int64_t rank = 0;
+        for (int i = 0; i < 3; ++i) {
+            PyObject *const x = a[3 + i], *const o = a[7 + i];
+            if (x == Py_None) {
+                if (o != Py_None) return kGeneral;
+                continue;
+            }
+            const at::Tensor *t = plain(x, dev);
+            if (!describe_heads(t, in[i]) || (rank && rank != t->dim())) return kGeneral;
+            rank = t->dim();
+            if (o == Py_None) {
+                fresh_out[i] = fresh(t->sizes(), t->scalar_type(), dev);
+                if (!describe_heads(&fresh_out[i], to[i])) return kGeneral;
+            } else {
+                const at::Tensor *d = plain(o, dev);
+                if (!d || d->sizes() != t->sizes() || !describe_heads(d, to[i])) return kGeneral;
+            }
+        }
+        if (!rank) return kGeneral;
+        const bool turns = rot->n_freq > 0;
+        if (turns) {
+            const at::Tensor *p = plain(a[6], dev);
+            const int own = rank == 3 ? 1 : 2;  // dims of one axis' positions
+            if (!p || (p->dim() != own && p->dim() != own + 1) || !describe(p, pos)) return kGeneral;
+            const int lead = p->dim() == own ? 0 : 1;
+            kvrt_tensor x = pos;
+            x.ndim = 3;
+            x.dims[0] = lead ? pos.dims[0] : 1, x.strides[0] = lead ? pos.strides[0] : 0;
+            x.dims[1] = pos.dims[lead], x.strides[1] = pos.strides[lead];
+            x.dims[2] = own == 2 ? pos.dims[lead + 1] : 1, x.strides[2] = own == 2 ? pos.strides[lead + 1] : 0;
+            pos = x;
+        }
+        const auto at = [&](int i, kvrt_tensor *of) { return a[3 + i] == Py_None ? nullptr : of + i; };
+        const long rc = without_gil([&] {
+            return rotate_api(rot, at(0, in), at(1, in), at(2, in), turns ? &pos : nullptr, at(0, to), at(1, to), at(2, to),
+                              stream);
+        });
+        if (rc == KVRT_OK) {
+            PyObject *got[3];
+            for (int i = 0; i < 3; ++i) {
+                if (fresh_out[i].defined()) got[i] = THPVariable_Wrap(fresh_out[i]);
+                else Py_INCREF(got[i] = a[7 + i]);
+            }
+            answer = Py_BuildValue("(NNN)", got[0], got[1], got[2]);
+        }
+        return rc;
+    });
+}
+
+// (address of kvrt_rotate_heads_async): once, after loading
+PyObject *connect_rotate(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    void *p = nargs == 1 ? PyLong_AsVoidPtr(a[0]) : nullptr;
+    if (PyErr_Occurred()) return nullptr;
+    if (!p) {
+        PyErr_SetString(PyExc_TypeError, "connect_rotate takes one address");
+        return nullptr;
+    }
+    rotate_api = reinterpret_cast<decltype(rotate_api)>(p);
+    Py_RETURN_NONE;
+}
+
 #define KVRT_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {KVRT_METHOD(append_attend),   KVRT_METHOD(attend),        KVRT_METHOD(attend_talker),
                          KVRT_METHOD(write_positions), KVRT_METHOD(append_gather), KVRT_METHOD(attend_tensors),
                          KVRT_METHOD(connect),         KVRT_METHOD(block_update),  KVRT_METHOD(block_append),
                          KVRT_METHOD(block_gather),    KVRT_METHOD(block_gather_new), KVRT_METHOD(block_attend),
-                         KVRT_METHOD(connect_blocks),
+                         KVRT_METHOD(connect_blocks),  KVRT_METHOD(rotate_heads),  KVRT_METHOD(connect_rotate),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "kvrt_pycall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

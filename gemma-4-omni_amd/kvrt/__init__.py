@@ -9,11 +9,14 @@ behind the C ABI of include/kvrt.h (libkvrt.so, built in-tree).
   duplex_kernel/kv_cache.py and thinker_cache.py API over kvrt storage.
 * ``kvrt.block8`` — ``BlockTables`` / ``Block8Pool``: pages of 8-bit codes with one
   scale per page and head, tables and lengths on the GPU.
+* ``kvrt.rotation`` — ``HeadRotation``: query, key and value heads normed and rotated in
+  one pass, ahead of an append.
 * ``kvrt.talker`` — HF talker cache import and the Q1 position counter.
 """
 from .block8 import Block8Pool, BlockPlan, BlockTables
 from .cache import KVRTCache, KVRTCacheLayer, append_attend, attend, attend_padded, gather
+from .rotation import HeadRotation
 from .runtime import KVRTError, KVRuntime, LayerSpec, TalkerMask, attend_tensors, copy_rows
 
-__all__ = ["Block8Pool", "BlockPlan", "BlockTables", "KVRTCache", "KVRTCacheLayer", "KVRTError", "KVRuntime", "LayerSpec",
+__all__ = ["Block8Pool", "BlockPlan", "BlockTables", "HeadRotation", "KVRTCache", "KVRTCacheLayer", "KVRTError", "KVRuntime", "LayerSpec",
            "TalkerMask", "append_attend", "attend", "attend_padded", "attend_tensors", "copy_rows", "gather"]

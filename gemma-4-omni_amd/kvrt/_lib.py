@@ -8,7 +8,7 @@ from __future__ import annotations
 import ctypes
 import importlib.machinery
 import importlib.util
-from ctypes import POINTER, c_float, c_int32, c_int64, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_double, c_float, c_int32, c_int64, c_uint32, c_uint64, c_void_p
 
 from ._build import CALLS_PATH, LIB_PATH
 
@@ -55,6 +55,7 @@ CAP_SLOT_GENERATION = 1 << 11
 CAP_STREAM_CONFINED = 1 << 12
 CAP_ROLLBACK_POSITION = 1 << 13
 CAP_BLOCK8 = 1 << 14
+CAP_ROTATE_HEADS = 1 << 15
 
 # bits of the status word of 8-bit pages and their tables (kvrt.h KVRT_BLOCK_*)
 BLOCK_BAD_INDEX = 1
@@ -187,6 +188,23 @@ class KvrtBlockTables(ctypes.Structure):
     ]
 
 
+class KvrtRotation(ctypes.Structure):
+    _fields_ = [
+        ("turns", c_void_p),
+        ("axis", c_void_p),
+        ("q_weight", c_void_p),
+        ("k_weight", c_void_p),
+        ("head_dim", c_int32),
+        ("n_freq", c_int32),
+        ("adjacent", c_int32),
+        ("norm", c_int32),
+        ("n_axes", c_int32),
+        ("eps", c_float),
+        ("scaling", c_float),
+        ("reserved", c_int32),
+    ]
+
+
 # (name, restype, argtypes) of every symbol declared in include/kvrt.h.
 _T = POINTER(KvrtTensor)
 _I32P = POINTER(c_int32)
@@ -236,6 +254,8 @@ SIGNATURES = [
     ("kvrt_block8_attend_async", c_int32,
      [_B8, _T, _T, c_void_p, c_void_p, c_void_p, _T, c_float, c_int32, c_int32, c_void_p, c_uint64, c_void_p]),
     ("kvrt_block8_attend_work", c_uint64, [_B8, c_int64, c_int64, c_int64, c_int64, c_int32]),
+    ("kvrt_rotation_turns", c_int32, [POINTER(c_double), c_int32, POINTER(c_uint64)]),
+    ("kvrt_rotate_heads_async", c_int32, [POINTER(KvrtRotation), _T, _T, _T, _T, _T, _T, _T, c_void_p]),
     ("kvrt_session_state", c_int32, [c_void_p, c_int32, c_int32, _I32P]),
     ("kvrt_sync_lengths", c_int32, [c_void_p]),
     ("kvrt_get_counters", c_int32, [c_void_p, POINTER(KvrtCounters)]),

@@ -80,6 +80,7 @@ extern "C" {
 #define KVRT_CAP_STREAM_CONFINED (1ull << 12)
 #define KVRT_CAP_ROLLBACK_POSITION (1ull << 13) /* truncate checks expected_len; import refuses live slots */
 #define KVRT_CAP_BLOCK8 (1ull << 14) /* 8-bit pages with a scale per page and head, tables built on the GPU */
+#define KVRT_CAP_ROTATE_HEADS (1ull << 15) /* heads normed and rotated in one pass */
 
 /* ---- enums ------------------------------------------------------------- */
 enum kvrt_layout {
@@ -749,6 +750,55 @@ int kvrt_block8_attend_async(const kvrt_block8 *pages, const kvrt_tensor *q, con
 /* Bytes of kvrt_block8_attend_async's work for these arguments (0: none). */
 uint64_t kvrt_block8_attend_work(const kvrt_block8 *pages, int64_t n, int64_t width, int64_t rows, int64_t hq,
                                  int32_t max_q);
+
+/* ---- heads normed and rotated ------------------------------------------------- */
+/* What a layer does to its query, key and value heads before they are appended and
+ * attended: norms per head, then a rotation of query and key heads by their
+ * positions along one to four axes (time, height, width). Device tables are
+ * caller-owned and read when a call runs. */
+typedef struct kvrt_rotation {
+    const uint64_t *turns;  /* device [n_freq], from kvrt_rotation_turns                */
+    const uint8_t *axis;    /* device [n_freq], 8-byte aligned: the axis whose position
+                               turns pair f (>= n_axes: the last one's); NULL: axis 0
+                               (n_axes must be 1)                                       */
+    const float *q_weight;  /* device [head_dim], 16-byte aligned; NULL: ones           */
+    const float *k_weight;
+    int32_t head_dim;       /* 64, 128, 256 or 512                                      */
+    int32_t n_freq;         /* pairs that turn: a multiple of 8, 2 n_freq <= head_dim   */
+    int32_t adjacent;       /* pair f is dims (2f, 2f + 1); 0: dims (f, f + n_freq)     */
+    int32_t norm;           /* heads that are normed: 1 query | 2 key | 4 value         */
+    int32_t n_axes;         /* 1..4                                                     */
+    float eps;
+    float scaling;          /* of the cosines and sines                                 */
+    int32_t reserved;
+} kvrt_rotation;
+
+/* The table of n angular frequencies (radians a position, host): the fraction of
+ * inv_freq / 2 pi above whole turns in units of 2^-64. KVRT_EINVAL where one is not
+ * finite. */
+int kvrt_rotation_turns(const double *inv_freq, int32_t n, uint64_t *turns);
+
+/* q, k, v [n, heads, Q, head_dim] bf16 (each with its own number of heads; strided,
+ * last dim contiguous, rows 16-byte aligned; absent ones NULL with their out) to
+ * out_* of the same shapes:
+ *   y = x * weight / sqrt(mean(x^2) + eps)              where the kind is normed
+ *   (y_a, y_b) -> (y_a c - y_b s, y_b c + y_a s)        query and key heads, n_freq pairs
+ * with c, s = scaling * (cos, sin)(position * inv_freq), all in fp32, rounded to bf16
+ * once; value heads have no weight and do not turn. positions: device KVRT_INT32 or
+ * KVRT_INT64 [n_axes, n, Q], any strides, values within int32 (an int64's low word is
+ * taken); not read where n_freq is 0. An output may be its input itself, otherwise
+ * outputs share no memory with inputs or each other. fp32 sums of squares: |x| below
+ * 2^60. Context-free: runs on the current device and the given stream, allocates
+ * nothing, returns KVRT_EINVAL (nothing enqueued) for arguments it does not take and
+ * KVRT_EDEVICE when the launch fails.
+ * Replaces the listener's and talker's norm and rotation launches of each layer
+ * (kernel_rmsnorm_bf16 and kernel_rope_bf16,
+ * native/gemma4_listener_microbatch/gemma4_listener_kernels.cuh:145-500; the
+ * finalize_rmsnorm and rope_interleaved kernels of
+ * native/qwen_talker/qwen_talker_kernels.cu:13-205). */
+int kvrt_rotate_heads_async(const kvrt_rotation *rotation, const kvrt_tensor *q, const kvrt_tensor *k,
+                            const kvrt_tensor *v, const kvrt_tensor *positions, const kvrt_tensor *out_q,
+                            const kvrt_tensor *out_k, const kvrt_tensor *out_v, void *hip_stream);
 
 /* ---- state / diagnostics ----------------------------------------------------- */
 /* Host-authoritative length of (slot, layer). Replaces
