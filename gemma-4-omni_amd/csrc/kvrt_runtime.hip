@@ -20,6 +20,7 @@
 
 #include "kvrt_internal.h"
 #include "kvrt_range.h"
+#include "kvrt_shared.h"
 
 using namespace kvrt;
 
@@ -1119,6 +1120,36 @@ int tensor_call_launch(TensorCall &tc, float *ws, hipStream_t st, bool single) {
     return KVRT_OK;
 }
 
+// Limits of shared-prefix attention: positions of a prefix and a session together stay
+// below 2^31, and so do rows, and a launch's threads below 2^32 (two key ranges for each
+// of the fewest rows of a tile, 256 threads each).
+constexpr int kMaxSharedCapacity = 1 << 29;
+constexpr int64_t kMaxSharedRows = 1 << 22;
+
+// How a call's rows and keys are divided (SharedArgs), from the most keys that are seen
+// of the prefix and of an item's own rows.
+void shared_plan(SharedArgs &a, int D, int64_t pre_keys, int64_t own_keys) {
+    const int hkv = a.kv.kv_heads, tile = shared_tile(D);
+    const int64_t per_item = (int64_t)a.group * a.qn, rows = per_item * a.n_items;
+    a.own_tiles = (int)((per_item + tile - 1) / tile);
+    a.joined = a.prefix_slot >= 0 && (pre_keys == 0 || per_item >= 64);
+    a.pre_tiles = a.prefix_slot < 0 || a.joined ? 0 : (int)((rows + tile - 1) / tile);
+    const int64_t own = (own_keys + (a.joined ? pre_keys : 0) + kSharedKeys - 1) / kSharedKeys + 1;
+    const int64_t pre = a.pre_tiles ? (pre_keys + kSharedKeys - 1) / kSharedKeys : 0;
+    const int64_t target = D <= 128 ? 512 : 256;
+    const auto ranges = [&](int64_t tiles, int64_t per) { return std::max<int64_t>(1, (tiles + per - 1) / per); };
+    // the fewest tiles of a range, from 4 on, that give no more workgroups than that
+    int64_t per = 4;
+    for (int64_t high = std::max(own, pre); per < high;) {
+        const int64_t mid = (per + high) / 2;
+        if (hkv * (a.pre_tiles * ranges(pre, mid) + a.n_items * a.own_tiles * ranges(own, mid)) <= target) high = mid;
+        else per = mid + 1;
+    }
+    a.pre_splits = a.pre_tiles ? (int)std::min<int64_t>(ranges(pre, per), 32) : 0;
+    a.own_splits = (int)std::min<int64_t>(ranges(own, per), 32);
+    a.parts = a.pre_splits + a.own_splits;
+}
+
 }  // namespace
 
 // ===========================================================================
@@ -1130,7 +1161,7 @@ uint64_t kvrt_capabilities(void) {
     return KVRT_CAP_CONTIG | KVRT_CAP_RING | KVRT_CAP_PAGED | KVRT_CAP_INT8 | KVRT_CAP_FUSED_APPEND_ATTEND |
            KVRT_CAP_GATHER | KVRT_CAP_DEVICE_LENGTHS | KVRT_CAP_TENSOR_ATTEND | KVRT_CAP_PREFILL_MFMA |
            KVRT_CAP_TALKER_MASK | KVRT_CAP_PREFIX_ATTENTION | KVRT_CAP_SLOT_GENERATION | KVRT_CAP_STREAM_CONFINED |
-           KVRT_CAP_ROLLBACK_POSITION | KVRT_CAP_BLOCK8 | KVRT_CAP_ROTATE_HEADS;
+           KVRT_CAP_ROLLBACK_POSITION | KVRT_CAP_BLOCK8 | KVRT_CAP_ROTATE_HEADS | KVRT_CAP_SHARED_PREFIX;
 }
 
 const char *kvrt_strerror(int code) {
@@ -2252,6 +2283,102 @@ int kvrt_attend_prefill_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32
             keys += (uint64_t)(r.kend - r.kstart);
         }
     keys *= (uint64_t)hkv * (a.short_heads ? group / a.short_heads : 1);
+    c->counters.attended_keys += keys;
+    c->counters.attended_bytes += keys * (uint64_t)D * 2 * 2;
+    return KVRT_OK;
+}
+
+int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_t *slots, int32_t prefix_slot,
+                             const kvrt_tensor *q, const kvrt_tensor *out, float scale, float softcap,
+                             const float *slopes) {
+    int rc = begin(c);
+    if (rc) return rc;
+    if (!valid_layer(c, layer) || !distinct_slots(c, n, slots)) return KVRT_EINVAL;
+    const bool shared = prefix_slot != -1;
+    if (shared && !valid_slot(c, prefix_slot)) return KVRT_EINVAL;
+    for (int i = 0; i < n; ++i)
+        if (slots[i] == prefix_slot) return KVRT_EINVAL;
+    const kvrt_layer_spec &s = c->layers[layer].spec;
+    if (s.dtype != KVRT_BF16) return KVRT_EINVAL;
+    const int D = s.head_dim, hkv = s.kv_heads, cap = c->cfg.capacity;
+    if (cap > kMaxSharedCapacity) return KVRT_EINVAL;
+    if (!tensor_ok(q, KVRT_BF16, 4) || !tensor_ok(out, KVRT_BF16, 4) || !is_contiguous(q) || !is_contiguous(out))
+        return KVRT_EINVAL;
+    const int64_t hq = q->dims[1], qn = q->dims[2];
+    if (q->dims[0] != n || q->dims[3] != D || hq <= 0 || hq % hkv != 0 || qn <= 0 || qn > cap) return KVRT_EINVAL;
+    for (int i = 0; i < 4; ++i)
+        if (out->dims[i] != q->dims[i]) return KVRT_EINVAL;
+    // rows are numbered in 32 bits, as are a launch's threads
+    if (hq > INT32_MAX / qn || n * hq * qn > kMaxSharedRows) return KVRT_EINVAL;
+    if (!std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap) ||
+        reinterpret_cast<uintptr_t>(slopes) % 4 != 0)
+        return KVRT_EINVAL;
+    if (softcap > 0.f && !std::isfinite(scale / softcap)) return KVRT_EINVAL;
+    const int P = shared ? c->len_at(prefix_slot, layer) : 0;
+    const int window = s.window >= 2 * cap ? 0 : s.window;  // past every distance: none
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    const bool capturing = hipStreamIsCapturing(c->stream, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone;
+    int min_len = INT32_MAX;
+    int64_t own_keys = 0;  // most own keys that an item's rows see
+    for (int i = 0; i < n; ++i) {
+        const int L = c->len_at(slots[i], layer);
+        if (L < qn) return KVRT_ESTATE;
+        min_len = std::min(min_len, L);
+        const int oldest = window > 0 ? (int)std::max<int64_t>(0, L - qn - window + 1) : 0;
+        // (a captured call may find the whole window later)
+        if (s.layout == KVRT_LAYOUT_RING && ((capturing ? qn + window - 1 : L - oldest) > s.ring_rows ||
+                                             oldest < c->ring_floor(slots[i], layer)))
+            return KVRT_ESTATE;
+        if (s.layout == KVRT_LAYOUT_PAGED && oldest < c->first_live[slots[i]] * c->cfg.block_size) return KVRT_ESTATE;
+        own_keys = std::max<int64_t>(own_keys, L - oldest);
+    }
+    // the oldest key of the prefix that some row sees must still be stored
+    const int oldest = window > 0 ? (int)std::max<int64_t>(0, P + min_len - qn - window + 1) : 0;
+    const int pre_keys = std::max(0, P - oldest);
+    if (pre_keys > 0) {
+        if (s.layout == KVRT_LAYOUT_RING && (pre_keys > s.ring_rows || oldest < c->ring_floor(prefix_slot, layer)))
+            return KVRT_ESTATE;
+        if (s.layout == KVRT_LAYOUT_PAGED && oldest < c->first_live[prefix_slot] * c->cfg.block_size) return KVRT_ESTATE;
+    }
+    SharedArgs a{};
+    a.kv = make_view(c, layer);
+    a.len = make_len(c, layer);
+    a.q = static_cast<const uint16_t *>(q->data);
+    a.out = static_cast<uint16_t *>(out->data);
+    a.err = c->d_err;
+    a.pmask = launch_masks(c, n, slots);
+    if (!a.pmask && shared) a.pmask = launch_masks(c, 1, &prefix_slot);
+    a.slopes = slopes;
+    a.scale = scale * 1.4426950408889634f;
+    a.cap = softcap * 1.4426950408889634f;
+    a.inv_cap = softcap > 0.f ? scale / softcap : 0.f;
+    a.n_items = n;
+    a.group = (int)(hq / hkv);
+    a.qn = (int)qn;
+    a.window = window;
+    a.capacity = cap;
+    a.prefix_slot = prefix_slot;
+    for (int i = 0; i < n; ++i) a.slots[i] = slots[i];
+    shared_plan(a, D, pre_keys, own_keys);
+    const auto bytes = [&] {
+        const size_t rows = (size_t)n * hq * qn * a.parts;
+        return a.parts == 1 ? 0 : rows * D * 4 + rows * 8 + 256;
+    };
+    if (bytes() > c->ws_bytes) {
+        // a workspace that a capture cannot grow: one walk per row tile, which needs none
+        if (capturing) {
+            a.joined = shared;
+            a.pre_tiles = 0, a.pre_splits = 0, a.own_splits = 1, a.parts = 1;
+        } else if ((rc = ensure_workspace(c, bytes())) != KVRT_OK) {
+            return rc;
+        }
+    }
+    a.part_o = c->ws;
+    a.part_ml = reinterpret_cast<float2 *>(c->ws + (size_t)n * hq * qn * a.parts * D);
+    c->counters.launches += a.parts > 1 ? 2 : 1;
+    if (launch_shared(a, D, enq(c)) != hipSuccess) return poison(c);
+    const uint64_t keys = ((uint64_t)pre_keys * (a.joined ? n * a.own_tiles : a.pre_tiles) +
+                           (uint64_t)own_keys * n * a.own_tiles) * hkv;
     c->counters.attended_keys += keys;
     c->counters.attended_bytes += keys * (uint64_t)D * 2 * 2;
     return KVRT_OK;

@@ -1,0 +1,545 @@
+// kvrt_shared_kernel.h — attention of many sessions behind one shared prefix (gfx950).
+//
+// A session sees the prefix slot's P rows and then its own L: query row i of Q sits at
+// position P + L - Q + i, and the softmax runs over both. Scores are
+//   s = f(q . k * scale) + slope_h * (key - position),   f(x) = x or cap * tanh(x / cap)
+// in fp32, weights 2^(s log2 e - m) with a running max m, and the sum and the products
+// with V accumulate in fp32; weights enter P V as two bf16 terms (2^-17 relative: one
+// term's 2^-9 would show in the bf16 outputs of few-key rows).
+//
+// Why units: the prefix's keys are the same for every session, so a workgroup takes the
+// rows of up to kSharedTile rows of all sessions (query heads of one KV head) over a range
+// of them and reads each key once per tile of rows, where a decode per session reads it
+// once per session. A session's own keys go to workgroups of their own. Each unit leaves
+// (max, sum, output) of its rows, which a second launch joins by their maxima. Where a
+// session brings many rows (a chunk), its units take the prefix's keys and its own in one
+// walk (`joined`), and with one range per row nothing is left to join.
+//
+// A workgroup is four waves that stage 32-key tiles of K and V together by LDS DMA,
+// kStages of them in flight, one barrier per tile. With more than 16 rows (WIDE) a wave
+// has up to two blocks of 16 rows and all dims of their outputs; with up to 16 rows every
+// wave computes the scores of all of them, and a quarter of the dims: the scores' 2 D/32
+// matrix instructions are cheap beside the tile's bytes, and waves need neither exchange
+// nor join anything.
+//   S^T (16 keys x 16 rows) = K Q^T    D/32   v_mfma_f32_16x16x32_bf16, for two key halves
+//   O^T (16 dims x 16 rows) += V^T P^T  2      v_mfma_f32_16x16x32_bf16 per 16 dims
+// Lane layouts: A[row l%16][k 8(l/16)+j], B[k 8(l/16)+j][col l%16], D[row 4(l/16)+i][col
+// l%16]. The second product's inner index is free: k = 8(l/16)+j is key 16(j/4) + 4(l/16)
+// + j%4, the keys whose weights the lane holds, so weights go from one product's result
+// to the other's operand in their registers; V is read transposed (ds_read_b64_tr_b16).
+//
+// A staged tile is row-major, 16-byte chunks permuted within their row so that 16 lanes
+// that read one chunk of 16 rows (K), and 32 that read two chunks of 8 rows (V), find
+// every one of the 16 places of 16 bytes that the 64 banks hold once.
+#pragma once
+
+#include "kvrt_shared.h"
+#include "kvrt_wave.h"
+
+namespace kvrt {
+
+__device__ __forceinline__ f32x4_t mfma_bf16(uint4 a, uint4 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
+                                                   0, 0);
+}
+
+template <int D>
+struct SharedShape {
+    static constexpr int STAGES = D == 512 ? 2 : 3;
+    static constexpr int CHUNKS = D / 8;                  // 16-byte chunks of a row
+    static constexpr int BLK = kSharedKeys * D * 2;       // bytes of a staged K (or V) tile
+    static constexpr int IPW = D / 64;                    // DMA instructions per wave, tile and tensor
+    static constexpr int RPI = 512 / D;                   // rows per instruction (D 512: 1)
+    // chunk c of row r lies in place c ^ kx(r) (K), c ^ vx(r) (V) of its row
+    static __device__ __forceinline__ int kx(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
+    static __device__ __forceinline__ int vx(int r) { return D == 64 ? 2 * ((r >> 1) & 3) : 2 * (r & 7); }
+};
+
+// Words that nothing in the launch writes: uniform ones load as scalars.
+typedef const __attribute__((address_space(4))) int32_t *SharedInts;
+
+// One of the two runs of keys a unit walks: the prefix's or an item's own.
+struct Segment {
+    int slot;        // whose rows
+    int lo, last;    // keys [lo, last] that some row of the unit sees
+    int tile0, tiles;
+    int off;         // a row's position in this run of keys: its own position + off
+    int len;         // rows stored
+    int all_lo, all_hi;  // keys [all_lo, all_hi) that every row sees
+};
+
+__device__ __forceinline__ Segment segment_of(int slot, int len, int off, int minpos, int maxpos, int window) {
+    Segment s;
+    s.slot = slot;
+    s.off = off;
+    s.len = len;
+    const int end = max(min(len, off + maxpos + 1), 0);
+    s.lo = window > 0 ? min(max(off + minpos - window + 1, 0), end) : 0;
+    s.last = end - 1;
+    s.tile0 = s.lo / kSharedKeys;
+    s.tiles = end > s.lo ? (end + kSharedKeys - 1) / kSharedKeys - s.tile0 : 0;
+    s.all_lo = window > 0 ? off + maxpos - window + 1 : 0;
+    s.all_hi = min(off + minpos + 1, len);
+    return s;
+}
+
+// cap * tanh(y): by an exponential, below 1/4 (where that would cancel) by the series,
+// whose next term is 2^-21 of the value there.
+__device__ __forceinline__ float capped(float y, float cap) {
+    const float e = __builtin_amdgcn_exp2f(y * 2.8853900817779268f);  // e^(2y)
+    const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
+    const float y2 = y * y;
+    const float small = y * fmaf(y2, fmaf(y2, fmaf(y2, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+    return cap * (fabsf(y) < 0.25f ? small : big);
+}
+
+// A unit's work: tiles [x0, x1) of its list (the prefix's tiles, then its own), rows row0
+// .. row0 + nrows - 1 of the call's (item, query, head) order, KV head kvh.
+struct SharedUnit {
+    Segment pre, own;
+    int kvh, row0, nrows, x0, x1, part;
+    int lens;  // lane i: length of item i
+};
+
+template <int D, int LAYOUT, bool WIDE>
+__device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUnit &u, uint8_t *lds) {
+    using S = SharedShape<D>;
+    constexpr int RS = WIDE ? shared_tile(D) / 64 : 1;      // 16-row blocks per wave
+    constexpr int NB = WIDE ? D / 16 : D / 64;              // 16-dim blocks per wave
+    constexpr int NS = S::STAGES;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const int b0 = WIDE ? 0 : wave * NB;
+    const int nblocks = (u.nrows + 15) / 16;                // of the unit's rows
+    const int mine = WIDE ? max(0, min(RS, (nblocks - wave + 3) / 4)) : 1;  // this wave's: wave, wave + 4
+
+    // this lane's rows
+    const int per_item = a.group * a.qn;
+    int pos[RS];          // own position; -1 - P and below: a lane without a row sees nothing
+    float slope[RS];
+    uint4 qop[RS][D / 32];
+#pragma unroll
+    for (int s = 0; s < RS; ++s) {
+        const int r = 16 * (WIDE ? wave + 4 * s : 0) + col;
+        const bool valid = r < u.nrows;
+        const int f = u.row0 + (valid ? r : 0);
+        int item, rem, qr, hr;
+        udivmod_uniform(f, per_item, item, rem);
+        udivmod_uniform(rem, a.group, qr, hr);
+        const int len = __shfl(u.lens, item);
+        pos[s] = valid ? len - a.qn + qr : INT32_MIN / 2;
+        const int head = u.kvh * a.group + hr;
+        const uint16_t *qp = a.q + (((int64_t)item * (a.kv.kv_heads * a.group) + head) * a.qn + qr) * D + 8 * grp;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) qop[s][c] = *reinterpret_cast<const uint4 *>(qp + 32 * c);
+        slope[s] = a.slopes ? a.slopes[head] * 1.4426950408889634f : 0.f;
+    }
+    // masks of the two slots: length, and word `lane & 15`
+    int plen_p = 0, plen_o = 0;
+    uint32_t pw_p = ~0u, pw_o = ~0u;
+    if (a.pmask) {
+        if (u.pre.tiles > 0) load_prefix(a.pmask, u.pre.slot, lane, plen_p, pw_p);
+        if (u.own.tiles > 0) load_prefix(a.pmask, u.own.slot, lane, plen_o, pw_o);
+    }
+#pragma unroll
+    for (int s = 0; s < RS; ++s) {
+        asm volatile("" : "+v"(pos[s]), "+v"(slope[s]));
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)  // all loads of registers are done ahead of the first DMA
+            asm volatile("" : "+v"(qop[s][c].x), "+v"(qop[s][c].y), "+v"(qop[s][c].z), "+v"(qop[s][c].w));
+    }
+
+    float m[RS], l[RS];
+    f32x4_t o[RS][NB];
+#pragma unroll
+    for (int s = 0; s < RS; ++s) {
+        m[s] = kNegBig, l[s] = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) o[s][b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    }
+
+    // ---- staging: wave w fetches instructions w, w + 4, ... of a tile's K and V rows
+    bool bad = false;
+    const uint32_t lds_at = lds_addr(lds);
+    const auto *kg = static_cast<const uint16_t *>(a.kv.k), *vg = static_cast<const uint16_t *>(a.kv.v);
+    // PAGED, pages of 16 keys and more: the pages of the next tile's two 16-key halves
+    const bool scalar_pages = LAYOUT == KVRT_LAYOUT_PAGED && a.kv.block_shift >= 4;
+    int id0 = 0, id1 = 0;
+    auto where = [&](int x, int &key0) __attribute__((always_inline)) -> const Segment & {
+        const bool own = x >= u.pre.tiles;
+        const Segment &g = own ? u.own : u.pre;
+        key0 = (g.tile0 + (own ? x - u.pre.tiles : x)) * kSharedKeys;
+        return g;
+    };
+    auto load_ids = [&](int x) __attribute__((always_inline)) {
+        if constexpr (LAYOUT == KVRT_LAYOUT_PAGED) {
+            if (!scalar_pages) return;
+            int key0;
+            const Segment &g = where(x, key0);
+            const SharedInts table = (SharedInts)(uintptr_t)(a.kv.page_table + (int64_t)g.slot * a.kv.pt_stride);
+            id0 = table[min(max(key0, g.lo), g.last) >> a.kv.block_shift];
+            id1 = table[min(max(key0 + 16, g.lo), g.last) >> a.kv.block_shift];
+        }
+    };
+    auto stage = [&](int x, int buf) __attribute__((always_inline)) {
+        int key0;
+        const Segment &g = where(x, key0);
+        const int64_t head = LAYOUT == KVRT_LAYOUT_PAGED
+                                 ? 0
+                                 : (int64_t)g.slot * a.kv.slot_stride + (int64_t)u.kvh * a.kv.head_stride;
+        const int ring0 = LAYOUT == KVRT_LAYOUT_RING ? key0 % a.kv.rows : 0;
+#pragma unroll
+        for (int i = 0; i < S::IPW; ++i) {
+            const int ins = 4 * i + wave;
+            const int r = ins * S::RPI + lane / S::CHUNKS, c = lane % S::CHUNKS;
+            const int key = min(max(key0 + r, g.lo), g.last);  // rows nobody sees read one that somebody does
+            int64_t off;
+            if constexpr (LAYOUT == KVRT_LAYOUT_CONTIG) {
+                off = head + (int64_t)key * D;
+            } else if constexpr (LAYOUT == KVRT_LAYOUT_RING) {
+                int rr = ring0 + (key - key0);
+                if (a.kv.rows >= kSharedKeys) rr = rr >= a.kv.rows ? rr - a.kv.rows : rr;  // wraps once at most
+                else rr %= a.kv.rows;
+                off = head + (int64_t)rr * D;
+            } else {
+                const int page = scalar_pages ? (ins * S::RPI >= 16 ? id1 : id0)
+                                              : a.kv.page_table[(int64_t)g.slot * a.kv.pt_stride + (key >> a.kv.block_shift)];
+                off = page_row_offset(a.kv, page, u.kvh, key, D);
+                bad |= off < 0;
+                off = off < 0 ? 0 : off;
+            }
+            const uint32_t to = lds_at + (uint32_t)(buf * 2 * S::BLK + ins * 1024);
+            dma_load16_cached(kg + off + 8 * (c ^ S::kx(r)), to);
+            dma_load16_cached(vg + off + 8 * (c ^ S::vx(r)), to + S::BLK);
+        }
+    };
+
+    // ---- one tile
+    const int s16 = lane & 15, vrow = 4 * grp + (s16 >> 2);
+    auto compute = [&](int x, int buf) __attribute__((always_inline)) {
+        const uint8_t *kt = lds + buf * 2 * S::BLK, *vt = kt + S::BLK;
+        f32x4_t sc[RS][2];
+#pragma unroll
+        for (int s = 0; s < RS; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) sc[s][h] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = 16 * h + col;
+                const uint4 k = *reinterpret_cast<const uint4 *>(kt + r * 2 * D + 16 * ((4 * c + grp) ^ S::kx(r)));
+#pragma unroll
+                for (int s = 0; s < RS; ++s)
+                    if (s == 0 || s < mine) sc[s][h] = mfma_bf16(k, qop[s][c], sc[s][h]);
+            }
+        int key0;
+        const Segment &g = where(x, key0);
+        const bool own = x >= u.pre.tiles;
+        const int plen = own ? plen_o : plen_p;
+        const bool whole = key0 >= g.all_lo && key0 + kSharedKeys <= g.all_hi && key0 >= plen;
+        uint32_t word = ~0u;  // bit k: key0 + k passes the slot's mask
+        if (key0 < plen) word = (uint32_t)__builtin_amdgcn_readlane((int)(own ? pw_o : pw_p), (key0 >> 5) & (kPrefixWords - 1));
+        uint4 ph[RS], pl[RS];
+        float e[RS][8];
+#pragma unroll
+        for (int s = 0; s < RS; ++s) {
+            if (s > 0 && s >= mine) break;
+            const int at = pos[s] + g.off;
+            float t[8];
+            if (a.cap == 0.f) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] = sc[s][i / 4][i % 4] * a.scale;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] = capped(sc[s][i / 4][i % 4] * a.inv_cap, a.cap);
+            }
+            if (a.slopes) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        t[4 * h + i] = fmaf(slope[s], (float)(key0 + 16 * h + 4 * grp + i - at), t[4 * h + i]);
+            }
+            if (!whole) {
+                // bit k: key0 + k is seen by this row
+                const int hi = min(max(min(at, g.last) - key0 + 1, 0), 32);
+                const int lo = min(max(max(a.window > 0 ? at - a.window + 1 : 0, g.lo) - key0, 0), 32);
+                uint32_t vis = word & (hi >= 32 ? ~0u : (1u << hi) - 1u) & (lo >= 32 ? 0u : ~0u << lo);
+                vis >>= 4 * grp;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) t[4 * h + i] = (vis >> (16 * h + i)) & 1u ? t[4 * h + i] : -INFINITY;
+            }
+            float top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
+            top = pair<OpMax, 32>(pair<OpMax, 16>(top));
+            const float mn = top > m[s] + kRescaleSlack ? top : m[s];
+            if (__any(mn != m[s])) {
+                const float corr = __builtin_amdgcn_exp2f(m[s] - mn);
+                l[s] *= corr;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) o[s][b] *= corr;
+                m[s] = mn;
+            }
+            uint32_t hiw[4], low[4];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[s][i] = __builtin_amdgcn_exp2f(t[i] - m[s]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x0 = e[s][2 * i], x1 = e[s][2 * i + 1];
+                l[s] += x0 + x1;
+                hiw[i] = pack_bf16x2(x0, x1);
+                low[i] = pack_bf16x2(x0 - bf16_lo(hiw[i]), x1 - bf16_hi(hiw[i]));
+            }
+            ph[s] = make_uint4(hiw[0], hiw[1], hiw[2], hiw[3]);
+            pl[s] = make_uint4(low[0], low[1], low[2], low[3]);
+        }
+        // V^T of 16 dims: this lane's dim 16 b + col, keys 16 h + 4 grp + 0 .. 3
+        auto vop = [&](int b) __attribute__((always_inline)) {
+            uint2 v[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = 16 * h + vrow;
+                v[h] = lds_read_tr16(reinterpret_cast<const uint16_t *>(
+                    vt + r * 2 * D + 16 * ((2 * (b0 + b) + ((s16 & 3) >> 1)) ^ S::vx(r)) + 8 * (s16 & 1)));
+            }
+            return make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
+        };
+        bool plain = true;
+        if (!whole) {
+            // A row that some see and others do not may hold NaN or infinities, and 0 * NaN is
+            // not 0: such a tile's products are made one by one below
+            uint32_t odd = 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const uint4 v = vop(b);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    odd |= (w[i] & 0x7f80u) == 0x7f80u ? 1u : 0u;
+                    odd |= (w[i] & 0x7f800000u) == 0x7f800000u ? 1u : 0u;
+                }
+            }
+            plain = !__any(odd != 0);
+        }
+        if (plain) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const uint4 v = vop(b);
+#pragma unroll
+                for (int s = 0; s < RS; ++s)
+                    if (s == 0 || s < mine) {
+                        o[s][b] = mfma_bf16(v, ph[s], o[s][b]);
+                        o[s][b] = mfma_bf16(v, pl[s], o[s][b]);
+                    }
+            }
+        } else {
+#pragma clang loop unroll(disable)
+            for (int k = 0; k < kSharedKeys; ++k) {
+                const int at = 4 * (k >> 4) + (k & 3), from = 16 * ((k >> 2) & 3) + col;
+#pragma unroll
+                for (int s = 0; s < RS; ++s) {
+                    if (s > 0 && s >= mine) break;
+                    float p = e[s][0];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) p = at == i ? e[s][i] : p;
+                    p = __shfl(p, from);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const uint2 v = *reinterpret_cast<const uint2 *>(
+                            vt + k * 2 * D + 16 * ((2 * (b0 + b) + (grp >> 1)) ^ S::vx(k)) + 8 * (grp & 1));
+                        const float x[4] = {bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y)};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[s][b][i] = p == 0.f ? o[s][b][i] : fmaf(p, x[i], o[s][b][i]);
+                    }
+                }
+            }
+        }
+    };
+
+    const int n = u.x1 - u.x0;
+    constexpr int PER = 2 * S::IPW;  // a wave's DMAs of a tile
+    if (n > 0) {
+        wait_vmem<0>();  // queries, masks and lengths are in registers
+        load_ids(u.x0);
+#pragma unroll
+        for (int i = 0; i < NS - 1; ++i)
+            if (i < n) {
+                stage(u.x0 + i, i);
+                load_ids(u.x0 + min(i + 1, n - 1));
+            }
+        int buf = 0;
+        for (int i = 0; i < n; ++i) {
+            wait_vmem_steps<PER, NS - 2>(n - 1 - i);  // this wave's part of tile i has landed
+            __syncthreads();                          // every wave's has, and tile i - 1 is read
+            if (i + NS - 1 < n) {
+                stage(u.x0 + i + NS - 1, buf == 0 ? NS - 1 : buf - 1);
+                load_ids(u.x0 + min(i + NS, n - 1));
+            }
+            if (mine > 0) compute(u.x0 + i, buf);
+            buf = buf == NS - 1 ? 0 : buf + 1;
+        }
+    }
+    if (bad) a.err[0] = 1;
+#pragma unroll
+    for (int s = 0; s < RS; ++s) {
+        if (s >= mine) break;
+        const int r = 16 * (WIDE ? wave + 4 * s : 0) + col;
+        const float sum = pair<OpSum, 32>(pair<OpSum, 16>(l[s]));
+        if (r >= u.nrows) continue;
+        const int f = u.row0 + r;
+        if (a.parts == 1) {
+            int item, rem, qr, hr;
+            udivmod_uniform(f, per_item, item, rem);
+            udivmod_uniform(rem, a.group, qr, hr);
+            const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+            uint16_t *dst =
+                a.out + (((int64_t)item * (a.kv.kv_heads * a.group) + u.kvh * a.group + hr) * a.qn + qr) * D + 4 * grp;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                *reinterpret_cast<uint2 *>(dst + 16 * (b0 + b)) = make_uint2(
+                    pack_bf16x2(o[s][b][0] * inv, o[s][b][1] * inv), pack_bf16x2(o[s][b][2] * inv, o[s][b][3] * inv));
+        } else {
+            const int64_t at = ((int64_t)u.kvh * a.n_items * per_item + f) * a.parts + u.part;
+            float *dst = a.part_o + at * D + 4 * grp;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                *reinterpret_cast<float4 *>(dst + 16 * (b0 + b)) = make_float4(o[s][b][0], o[s][b][1], o[s][b][2], o[s][b][3]);
+            if (grp == 0 && b0 == 0) a.part_ml[at] = make_float2(m[s], sum);
+        }
+    }
+}
+
+template <int D, int LAYOUT>
+__global__ __launch_bounds__(256) void shared_attend_kernel(SharedArgs a) {
+    using S = SharedShape<D>;
+    constexpr int TILE = shared_tile(D);
+    __shared__ __align__(16) uint8_t lds[S::STAGES * 2 * S::BLK];
+    const int lane = threadIdx.x & 63;
+    const int hkv = a.kv.kv_heads, per_item = a.group * a.qn;
+    const int capacity = a.capacity;
+    const auto length = [&](int slot) __attribute__((always_inline)) {
+        return min(max(a.len.lens[(int64_t)slot * a.len.stride + a.len.offset], 0), capacity);
+    };
+    SharedUnit u;
+    u.lens = length(a.slots[min(lane, a.n_items - 1)]);
+    const int prefix = a.prefix_slot >= 0 ? __builtin_amdgcn_readfirstlane(length(a.prefix_slot)) : 0;
+    // KV heads are the least significant: workgroups of one head land on one XCD when
+    // there are eight, and share its L2
+    int at, splits;
+    udivmod_uniform(blockIdx.x, hkv, at, u.kvh);
+    const bool pre = at < a.pre_tiles * a.pre_splits;
+    int ks, tile, minpos, maxpos;
+    if (pre) {
+        splits = a.pre_splits;
+        udivmod_uniform(at, splits, tile, ks);
+        u.row0 = tile * TILE;
+        u.nrows = min(a.n_items * per_item - u.row0, TILE);
+        u.part = ks;
+        int lo = u.lens, hi = u.lens;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            lo = min(lo, __shfl_xor(lo, d));
+            hi = max(hi, __shfl_xor(hi, d));
+        }
+        minpos = __builtin_amdgcn_readfirstlane(lo) - a.qn;
+        maxpos = __builtin_amdgcn_readfirstlane(hi) - 1;
+        u.pre = segment_of(a.prefix_slot, prefix, prefix, minpos, maxpos, a.window);
+        u.own = segment_of(a.prefix_slot, 0, 0, 0, -1, 0);
+    } else {
+        int item, rem;
+        at -= a.pre_tiles * a.pre_splits;
+        splits = a.own_splits;
+        udivmod_uniform(at, splits * a.own_tiles, item, rem);
+        udivmod_uniform(rem, splits, tile, ks);
+        u.row0 = item * per_item + tile * TILE;
+        u.nrows = min(per_item - tile * TILE, TILE);
+        u.part = a.pre_splits + ks;
+        const int len = __builtin_amdgcn_readlane(u.lens, item);
+        int qf, ql, ignore;
+        udivmod_uniform(tile * TILE, a.group, qf, ignore);
+        udivmod_uniform(tile * TILE + u.nrows - 1, a.group, ql, ignore);
+        minpos = len - a.qn + qf;
+        maxpos = len - a.qn + ql;
+        u.own = segment_of(a.slots[item], len, 0, minpos, maxpos, a.window);
+        u.pre = segment_of(a.prefix_slot, a.joined ? prefix : 0, prefix, minpos, maxpos, a.window);
+    }
+    const int tiles = u.pre.tiles + u.own.tiles, per = (tiles + splits - 1) / splits;
+    u.x0 = min(ks * per, tiles);
+    u.x1 = min(u.x0 + per, tiles);
+    if (u.nrows > 16) shared_unit<D, LAYOUT, true>(a, u, lds);
+    else shared_unit<D, LAYOUT, false>(a, u, lds);
+}
+
+// Joins the partials of every row: a row's D / 4 threads walk its parts in order, kAhead
+// of them in flight.
+template <int D>
+__global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
+    constexpr int LANES = D / 4, ROWS = 256 / LANES, kAhead = 8;
+    const int per_item = a.group * a.qn;
+    const int64_t rows = (int64_t)a.n_items * per_item;
+    const int64_t at = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
+    if (at >= rows * a.kv.kv_heads) return;
+    const int kvh = (int)(at / rows), f = (int)(at - kvh * rows), d = 4 * (threadIdx.x % LANES);
+    float M = kNegBig, sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = 0; p0 < a.parts; p0 += kAhead) {
+        float2 ml[kAhead];
+        float4 x[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t p = at * a.parts + min(p0 + i, a.parts - 1);
+            ml[i] = a.part_ml[p];
+            x[i] = *reinterpret_cast<const float4 *>(a.part_o + p * D + d);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (p0 + i >= a.parts) ml[i] = make_float2(kNegBig, 0.f);
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) top = fmaxf(top, ml[i].x);
+        const float c = __builtin_amdgcn_exp2f(M - top);
+        sum *= c;
+        o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
+        M = top;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (ml[i].x == kNegBig && ml[i].y == 0.f) continue;  // it saw no key
+            const float w = __builtin_amdgcn_exp2f(ml[i].x - M);
+            sum = fmaf(ml[i].y, w, sum);
+            o = make_float4(fmaf(x[i].x, w, o.x), fmaf(x[i].y, w, o.y), fmaf(x[i].z, w, o.z), fmaf(x[i].w, w, o.w));
+        }
+    }
+    const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+    int item, rem, qr, hr;
+    udivmod_uniform(f, per_item, item, rem);
+    udivmod_uniform(rem, a.group, qr, hr);
+    uint16_t *dst = a.out + (((int64_t)item * (a.kv.kv_heads * a.group) + kvh * a.group + hr) * a.qn + qr) * D + d;
+    *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+}
+
+template <int D>
+static hipError_t launch_shared_dim(const SharedArgs &a, hipStream_t s) {
+    const int units = (a.pre_tiles * a.pre_splits + a.n_items * a.own_tiles * a.own_splits) * a.kv.kv_heads;
+    switch (a.kv.layout) {
+        case KVRT_LAYOUT_CONTIG:
+            hipLaunchKernelGGL((shared_attend_kernel<D, KVRT_LAYOUT_CONTIG>), dim3(units), dim3(256), 0, s, a);
+            break;
+        case KVRT_LAYOUT_RING:
+            hipLaunchKernelGGL((shared_attend_kernel<D, KVRT_LAYOUT_RING>), dim3(units), dim3(256), 0, s, a);
+            break;
+        case KVRT_LAYOUT_PAGED:
+            hipLaunchKernelGGL((shared_attend_kernel<D, KVRT_LAYOUT_PAGED>), dim3(units), dim3(256), 0, s, a);
+            break;
+        default: return hipErrorInvalidValue;
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.parts == 1) return e;
+    constexpr int ROWS = 1024 / D;
+    const int64_t rows = (int64_t)a.n_items * a.group * a.qn * a.kv.kv_heads;
+    hipLaunchKernelGGL((shared_join_kernel<D>), dim3((unsigned)((rows + ROWS - 1) / ROWS)), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace kvrt

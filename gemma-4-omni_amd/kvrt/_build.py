@@ -3,7 +3,8 @@
 The library is compiled from ``csrc/kvrt_kernels.hip`` (kernels),
 ``csrc/kvrt_prefill.hip`` and ``csrc/kvrt_prefill_wide.hip`` (chunked prefill),
 ``csrc/kvrt_block8.hip``, ``csrc/kvrt_block8_attend.hip`` and
-``csrc/kvrt_block8_chunk.hip`` (8-bit pages), ``csrc/kvrt_rotate.hip`` (heads normed and rotated)
+``csrc/kvrt_block8_chunk.hip`` (8-bit pages), ``csrc/kvrt_rotate.hip`` (heads normed and rotated),
+``csrc/kvrt_shared.hip`` and ``csrc/kvrt_shared_wide.hip`` (attention after a shared prefix)
 and ``csrc/kvrt_runtime.hip`` (host runtime, C ABI in ``include/kvrt.h``);
 kvrt_pycall.so, the calls that read torch tensors directly, from
 ``csrc/kvrt_pycall.cpp`` with the host compiler. The build also compiles
@@ -29,7 +30,8 @@ INCLUDE = PKG_DIR.parent.parent / "include"
 LIB_PATH = PKG_DIR / "libkvrt.so"
 CALLS_PATH = PKG_DIR / "kvrt_pycall.so"
 SOURCES = ("kvrt_kernels.hip", "kvrt_prefill.hip", "kvrt_prefill_wide.hip", "kvrt_prefill_short.hip", "kvrt_runtime.hip",
-           "kvrt_block8.hip", "kvrt_block8_attend.hip", "kvrt_block8_chunk.hip", "kvrt_rotate.hip")
+           "kvrt_block8.hip", "kvrt_block8_attend.hip", "kvrt_block8_chunk.hip", "kvrt_rotate.hip",
+           "kvrt_shared.hip", "kvrt_shared_wide.hip")
 
 AGPR_SOURCES = ("kvrt_prefill_wide.hip",)
 

@@ -56,6 +56,7 @@ CAP_STREAM_CONFINED = 1 << 12
 CAP_ROLLBACK_POSITION = 1 << 13
 CAP_BLOCK8 = 1 << 14
 CAP_ROTATE_HEADS = 1 << 15
+CAP_SHARED_PREFIX = 1 << 16
 
 # bits of the status word of 8-bit pages and their tables (kvrt.h KVRT_BLOCK_*)
 BLOCK_BAD_INDEX = 1
@@ -243,6 +244,8 @@ SIGNATURES = [
     ("kvrt_attend_prefill_async", c_int32, [c_void_p, c_int32, c_int32, _I32P, _T, _T, c_float]),
     ("kvrt_attend_talker_async", c_int32,
      [c_void_p, c_int32, c_int32, _I32P, _T, _T, c_float, POINTER(KvrtTalkerMask)]),
+    ("kvrt_attend_shared_async", c_int32,
+     [c_void_p, c_int32, c_int32, _I32P, c_int32, _T, _T, c_float, c_float, c_void_p]),
     ("kvrt_attend_tensors_async", c_int32, [_T, _T, _T, c_void_p, _T, _T, c_float, c_int32, c_void_p]),
     ("kvrt_attend_tensors_noalloc_async", c_int32, [_T, _T, _T, c_void_p, _T, _T, c_float, c_int32, c_void_p]),
     ("kvrt_tensors_status", c_int32, [c_void_p]),

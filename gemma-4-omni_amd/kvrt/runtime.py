@@ -557,6 +557,37 @@ class KVRuntime:
                "kvrt_attend_prefill_async")
         return out
 
+    def attend_shared(self, layer: int, q: torch.Tensor, slots: Sequence[int], scale: float, *,
+                      prefix_slot: int | None = None, softcap: float = 0.0, slopes: torch.Tensor | None = None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of q [n, Hq, Q, D] over the last Q positions of each slot, behind the
+        rows of ``prefix_slot`` that all of them share (None: no prefix).
+
+        A slot's rows follow the prefix's: its query row r sits at position P + L - Q + r,
+        P and L the two lengths, and the layer's window counts over both. The prefix is
+        read in place, once for all slots, where a clone per session would be read once
+        each. ``softcap`` c > 0 caps scores, c tanh(s / c); ``slopes`` (fp32 [Hq] on the
+        GPU) adds slopes[h] * (key - query position) to them. The prefix-attention masks
+        of the prefix slot and of the slots hold. bf16 layers, decode steps and chunks."""
+        require_cuda(q, "q")
+        if slopes is not None:
+            require_cuda(slopes, "slopes")
+            if slopes.dtype != torch.float32 or slopes.dim() != 1 or not slopes.is_contiguous() or \
+                    slopes.device != self.device or q.dim() != 4 or slopes.shape[0] != q.shape[1]:
+                raise ValueError(f"slopes must be a contiguous fp32 tensor of one slope per query head on {self.device}")
+        if prefix_slot is not None and int(prefix_slot) < 0:
+            raise ValueError(f"prefix_slot must be a slot or None, got {prefix_slot}")
+        q = q.contiguous()
+        out = torch.empty_like(q) if out is None else out
+        self._bind()
+        arr, n = self._slots(slots)
+        qd, od = tensor_desc(q), tensor_desc(out)
+        _check(self.lib.kvrt_attend_shared_async(self._ctx, layer, n, arr, -1 if prefix_slot is None else int(prefix_slot),
+                                                 ctypes.byref(qd), ctypes.byref(od), float(scale), float(softcap),
+                                                 None if slopes is None else slopes.data_ptr()),
+               "kvrt_attend_shared_async")
+        return out
+
     def attend_talker(self, layer: int, q: torch.Tensor, slots: Sequence[int], scale: float,
                       masks: Sequence["TalkerMask"], out: torch.Tensor | None = None) -> torch.Tensor:
         """Talker attention of q [n, Hq, Q, D] (Q = 2: prefix then audio query;

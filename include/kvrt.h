@@ -81,6 +81,7 @@ extern "C" {
 #define KVRT_CAP_ROLLBACK_POSITION (1ull << 13) /* truncate checks expected_len; import refuses live slots */
 #define KVRT_CAP_BLOCK8 (1ull << 14) /* 8-bit pages with a scale per page and head, tables built on the GPU */
 #define KVRT_CAP_ROTATE_HEADS (1ull << 15) /* heads normed and rotated in one pass */
+#define KVRT_CAP_SHARED_PREFIX (1ull << 16) /* attention after a shared prefix, capped and biased scores */
 
 /* ---- enums ------------------------------------------------------------- */
 enum kvrt_layout {
@@ -570,6 +571,31 @@ typedef struct kvrt_talker_mask {
 int kvrt_attend_talker_async(kvrt_ctx *ctx, int32_t layer, int32_t n, const int32_t *slots,
                              const kvrt_tensor *q, const kvrt_tensor *out, float scale,
                              const kvrt_talker_mask *masks);
+
+/* Attention of q [n, Hq, Q, D] (bf16 contiguous, out likewise) over the last Q
+ * positions of n slots of one layer behind a prefix that they share: slot i sees
+ * the P rows of prefix_slot (P its length), then its own L_i, so that its query
+ * row r sits at position P + L_i - Q + r. Nothing is copied: the prefix's rows are
+ * read once per 128 query rows (64 at head_dim 512) of the call. prefix_slot -1:
+ * no prefix. Scores are
+ *   s = f(q.k * scale) + slopes[h] * (key position - query position)
+ * with f(x) = softcap * tanh(x / softcap), or x where softcap is 0; slopes: DEVICE
+ * fp32 [Hq], NULL for no bias. Visibility as kvrt_attend_decode_async (causal, the
+ * layer's window over prefix and own rows together, the prefix-attention masks of
+ * prefix_slot and of the slots on their own rows); a row that sees no key becomes
+ * zeros, and rows that a query does not see do not reach it whatever they hold.
+ * Scores, softmax and sums in fp32, weights in two bf16 terms (2^-17 relative). Any
+ * 1 <= Q <= L_i, any Hq / kv_heads; bf16 layers of every layout; a capacity of at
+ * most 2^29; n * Hq * Q <= 2^22. prefix_slot is none of the slots; RING and PAGED
+ * layers still hold the oldest keys seen of both, a RING layer's rows those of Q +
+ * window - 1 positions (KVRT_ESTATE otherwise). A captured call replays on the
+ * lengths it then finds; one whose partials do not fit the context's workspace is
+ * captured in an undivided form (one eager call of the shape first sizes it).
+ * The reference copies the prefix into each session (duplex_kernel/kv_cache.py:41-67)
+ * and has no such call. */
+int kvrt_attend_shared_async(kvrt_ctx *ctx, int32_t layer, int32_t n, const int32_t *slots, int32_t prefix_slot,
+                             const kvrt_tensor *q, const kvrt_tensor *out, float scale, float softcap,
+                             const float *slopes);
 
 /* ---- context-free tensor kernels ------------------------------------------ */
 /* Decode attention over caller-owned HF-shaped K/V: k, v [n, kv_heads, Lmax, D]

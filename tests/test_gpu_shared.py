@@ -1,0 +1,338 @@
+"""Attention behind a shared prefix, with capped and biased scores, against the definition in
+64 bits (tests/shared_ref.py, which derives the tolerance)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from shared_ref import Sessions
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def _gen(seed: int) -> torch.Generator:
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _q(gen, n, hq, qn, d, by=1.0):
+    return (by * torch.randn(n, hq, qn, d, generator=gen, device="cuda")).to(BF16)
+
+
+DECODES = [
+    # lens, prefix, hq, hkv, d, layout, window, q
+    ([1], 1, 8, 1, 256, "contig", 0, 1),
+    ([1, 2, 3], 0, 16, 8, 128, "contig", 0, 1),
+    ([5, 1, 33], 31, 16, 8, 128, "contig", 0, 1),
+    ([40, 7, 64, 65], 97, 4, 4, 64, "contig", 0, 1),
+    ([130, 64, 200], 512, 16, 8, 128, "contig", 0, 2),
+    ([610, 500, 400, 333], 700, 16, 8, 128, "contig", 0, 1),
+    ([2, 400], 300, 8, 1, 256, "contig", 0, 2),
+    ([100, 31, 1, 64, 250], 333, 8, 1, 512, "contig", 0, 1),
+    ([90, 17], 65, 8, 1, 512, "contig", 0, 2),
+    ([33] * 17, 129, 12, 4, 128, "contig", 0, 1),
+    (list(range(1, 65)), 260, 16, 8, 128, "contig", 0, 1),
+    (list(range(70, 6, -1)), 100, 8, 1, 256, "contig", 0, 1),
+    (list(range(3, 43)), 77, 8, 1, 512, "contig", 0, 2),
+    ([300, 12, 90], 200, 16, 8, 128, "contig", 128, 1),
+    ([300, 12, 90], 200, 8, 1, 256, "ring", 128, 1),
+    ([20, 2, 700], 600, 16, 8, 64, "ring", 64, 2),
+    ([5, 6, 9], 40, 4, 2, 128, "ring", 7, 1),
+    ([5, 6, 9], 40, 4, 2, 128, "ring", 30, 2),
+    ([100, 1, 33, 256], 130, 16, 8, 128, "paged", 0, 1),
+    ([100, 2, 33, 256], 130, 8, 1, 512, "paged", 0, 2),
+    ([100, 2, 33, 256], 130, 8, 1, 256, "paged", 90, 1),
+    ([30, 31, 32], 15, 4, 2, 64, "paged", 0, 1),
+]
+
+
+@pytest.mark.parametrize("lens,prefix,hq,hkv,d,layout,window,qn", DECODES)
+@pytest.mark.parametrize("score", ["plain", "capped", "biased", "both"])
+def test_decode_steps(lens, prefix, hq, hkv, d, layout, window, qn, score):
+    gen = _gen(len(lens) + prefix + d)
+    s = Sessions(gen, lens, prefix, hkv=hkv, d=d, layout=layout, window=window, q=qn)
+    cap = 12.0 if score in ("capped", "both") else 0.0
+    slopes = torch.rand(hq, generator=gen, device="cuda") * 0.3 if score in ("biased", "both") else None
+    q = _q(gen, len(lens), hq, qn, d, 2.0 if cap else 1.0)
+    got = s.rt.attend_shared(0, q, range(s.n), d ** -0.5, prefix_slot=s.n, softcap=cap, slopes=slopes)
+    s.check(got, q, d ** -0.5, cap=cap, slopes=slopes)
+    got = s.rt.attend_shared(0, q, range(s.n), d ** -0.5, softcap=cap, slopes=slopes)
+    s.check(got, q, d ** -0.5, shared=False, cap=cap, slopes=slopes)
+    assert s.rt.health() == 0
+
+
+CHUNKS = [
+    ([3, 5], 9, 16, 8, 128, "contig", 0, 3),
+    ([40, 17, 100], 65, 16, 8, 128, "contig", 0, 17),
+    ([64], 300, 16, 8, 128, "contig", 0, 64),
+    ([200, 129], 31, 8, 4, 128, "contig", 0, 129),
+    ([50, 33], 100, 8, 1, 256, "contig", 0, 20),
+    ([70, 41], 100, 8, 1, 512, "contig", 0, 41),
+    ([300, 20], 90, 12, 4, 64, "contig", 0, 20),
+    ([260, 200], 333, 16, 8, 128, "contig", 100, 150),
+    ([260, 200], 64, 8, 1, 256, "ring", 100, 33),
+    ([75, 90], 200, 16, 8, 128, "paged", 0, 75),
+    ([75, 90], 200, 8, 1, 256, "paged", 60, 30),
+    ([600], 0, 16, 8, 128, "contig", 0, 600),
+]
+
+
+@pytest.mark.parametrize("lens,prefix,hq,hkv,d,layout,window,qn", CHUNKS)
+@pytest.mark.parametrize("score", ["plain", "both"])
+def test_chunks(lens, prefix, hq, hkv, d, layout, window, qn, score):
+    gen = _gen(len(lens) + prefix + d + qn)
+    s = Sessions(gen, lens, prefix, hkv=hkv, d=d, layout=layout, window=window, q=qn)
+    cap = 12.0 if score == "both" else 0.0
+    slopes = torch.rand(hq, generator=gen, device="cuda") * 0.3 if score == "both" else None
+    q = _q(gen, len(lens), hq, qn, d)
+    got = s.rt.attend_shared(0, q, range(s.n), d ** -0.5, prefix_slot=s.n, softcap=cap, slopes=slopes)
+    s.check(got, q, d ** -0.5, cap=cap, slopes=slopes)
+    assert s.rt.health() == 0
+
+
+@pytest.mark.parametrize("block", [1, 4, 16, 64])
+def test_pages_of_any_size(block):
+    gen = _gen(block)
+    s = Sessions(gen, [50, 3, 129], 70, hkv=2, d=128, layout="paged", block=block)
+    q = _q(gen, 3, 4, 1, 128)
+    s.check(s.rt.attend_shared(0, q, range(3), 0.1, prefix_slot=3), q, 0.1)
+    assert s.rt.health() == 0
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.25, 1.0, 30.0])
+@pytest.mark.parametrize("cap", [0.0, 1e-3, 5.0, 1e6])
+def test_scales_and_caps(scale, cap):
+    gen = _gen(3)
+    s = Sessions(gen, [70, 45], 130, hkv=2, d=64)
+    q = _q(gen, 2, 8, 1, 64)
+    s.check(s.rt.attend_shared(0, q, range(2), scale, prefix_slot=2, softcap=cap), q, scale, cap=cap)
+
+
+@pytest.mark.parametrize("lens,qn,hq", [([60, 45, 90], 1, 4), ([60, 45, 90], 40, 4), ([60, 64, 90], 2, 40)])
+def test_masks_of_the_prefix_and_of_the_sessions(lens, qn, hq):
+    gen = _gen(qn)
+    s = Sessions(gen, lens, 150, hkv=2, d=128)
+    masks = [torch.rand(20, generator=gen, device="cuda") < 0.5, None,
+             torch.zeros(90 - qn, dtype=torch.bool, device="cuda"), torch.rand(140, generator=gen, device="cuda") < 0.3]
+    for slot, m in enumerate(masks):
+        if m is not None:
+            s.rt.set_prefix_attention(slot, m)
+    q = _q(gen, 3, hq, qn, 128)
+    s.check(s.rt.attend_shared(0, q, range(3), 0.09, prefix_slot=3), q, 0.09, masks=masks)
+    # a canonical mask: only the first and last of 34 positions are seen; the hidden rows hold
+    # infinities and NaN
+    s.k[3][:, 1:33] = float("inf")
+    s.v[3][:, 1:33] = float("nan")
+    s.rt.set_prefix_attention(3, None)
+    s.load(3)
+    masks[3] = torch.zeros(34, dtype=torch.bool, device="cuda")
+    masks[3][0] = masks[3][33] = True
+    s.rt.set_prefix_attention(3, masks[3])
+    got = s.rt.attend_shared(0, q, range(3), 0.09, prefix_slot=3)
+    assert bool(got.isfinite().all())
+    s.check(got, q, 0.09, masks=masks)
+
+
+@pytest.mark.parametrize("qn,hq,hkv,d", [(2, 8, 1, 256), (2, 16, 8, 128), (50, 8, 4, 128), (40, 8, 1, 512), (40, 4, 1, 64)])
+def test_a_row_that_a_query_does_not_see_does_not_reach_it(qn, hq, hkv, d):
+    gen = _gen(d)
+    s = Sessions(gen, [qn + 30, qn + 1], 40, hkv=hkv, d=d, q=qn)
+    s.k[0][:, -1] = float("nan")            # seen by the last query only
+    s.v[0][:, -1, ::3] = float("inf")
+    s.v[1][:, -1] = float("nan")
+    s.v[1][:, -2, 1::2] = float("-inf")     # seen by the last two
+    for i in range(2):
+        s.load(i)
+    q = _q(gen, 2, hq, qn, d)
+    got = s.rt.attend_shared(0, q, range(2), d ** -0.5, prefix_slot=2)
+    assert bool(got[0, :, :-1].isfinite().all()) and bool(got[0, :, -1].isnan().all())
+    if qn > 2:
+        assert bool(got[1, :, :-2].isfinite().all())
+    assert bool(got[1, :, -1].isnan().all())
+    assert not bool(got[1, :, -2, 1::2].isfinite().any()) and bool(got[1, :, -2, ::2].isfinite().all())
+    q[:, 0] = float("nan")                  # a head's query reaches no other head
+    again = s.rt.attend_shared(0, q, range(2), d ** -0.5, prefix_slot=2)
+    assert bool(again[:, 0].isnan().all()) and torch.equal(again[:, 1:].nan_to_num(7.0), got[:, 1:].nan_to_num(7.0))
+
+
+def test_a_window_hides_the_prefix_of_some():
+    gen = _gen(11)
+    for layout in ("contig", "ring", "paged"):
+        s = Sessions(gen, [3, 50, 63, 64, 65, 200], 90, hkv=2, d=128, layout=layout, window=64)
+        s.v[6][:, :20] = float("nan")  # rows that no session sees any more
+        s.load(6)
+        q = _q(gen, 6, 4, 1, 128)
+        got = s.rt.attend_shared(0, q, range(6), 0.09, prefix_slot=6)
+        s.v[6][:, :20] = 0
+        s.check(got, q, 0.09)
+
+
+def test_same_as_a_clone_of_the_prefix():
+    """The answer of sessions that hold a copy of the prefix, to the two calls' errors."""
+    gen = _gen(12)
+    s = Sessions(gen, [40, 21], 100, hkv=8, d=128)
+    q = _q(gen, 2, 16, 1, 128)
+    got = s.rt.attend_shared(0, q, range(2), 0.09, prefix_slot=2)
+    from kvrt import KVRuntime, LayerSpec
+
+    rt = KVRuntime([LayerSpec(kv_heads=8, head_dim=128)], n_slots=2, capacity=200)
+    for i in range(2):
+        rt.import_(i, 0, torch.cat((s.k[2], s.k[i]), 1)[None], torch.cat((s.v[2], s.v[i]), 1)[None])
+    want = rt.attend(0, q, range(2), 0.09)
+    assert float((got.float() - want.float()).abs().max()) <= 2 ** -7 * float(want.float().abs().max())
+
+
+def test_shared_layers_read_their_source():
+    from kvrt import KVRuntime, LayerSpec
+
+    gen = _gen(13)
+    rt = KVRuntime([LayerSpec(kv_heads=2, head_dim=64), LayerSpec(kv_heads=2, head_dim=64, shared_src=0)], n_slots=3,
+                   capacity=64)
+    for slot, rows in enumerate((10, 20, 33)):
+        rt.import_(slot, 0, *(torch.randn(1, 2, rows, 64, generator=gen, device="cuda").to(BF16) for _ in range(2)))
+    q = _q(gen, 2, 4, 1, 64)
+    a, b = (rt.attend_shared(layer, q, [0, 1], 0.1, prefix_slot=2) for layer in (0, 1))
+    assert torch.equal(a, b)
+    swapped = rt.attend_shared(0, q.flip(0).contiguous(), [1, 0], 0.1, prefix_slot=2)
+    assert torch.equal(swapped.flip(0), a)
+
+
+@pytest.mark.parametrize("layout,window", [("contig", 0), ("ring", 48), ("paged", 0)])
+def test_a_captured_step_replays_as_lengths_grow(layout, window):
+    gen = _gen(14)
+    lens = [30, 5, 61]
+    s = Sessions(gen, lens, 75, hkv=2, d=128, layout=layout, window=window, spare=40)
+    q = _q(gen, 3, 8, 1, 128)
+    k, v = (torch.randn(3, 2, 1, 128, generator=gen, device="cuda").to(BF16) for _ in range(2))
+    if layout == "paged":
+        for i in range(3):
+            s.rt.reserve(i, 20)
+    s.rt.attend_shared(0, q, range(3), 0.09, prefix_slot=3)
+    torch.cuda.synchronize()
+    s.rt.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.rt.append(0, k, v, range(3))
+        got = s.rt.attend_shared(0, q, range(3), 0.09, prefix_slot=3)
+    s.rt.sync_lengths()
+    assert [s.rt.seq_length(i) for i in range(3)] == lens  # nothing ran yet
+    for step in range(6):
+        q.copy_(_q(gen, 3, 8, 1, 128))
+        k.copy_(torch.randn(3, 2, 1, 128, generator=gen, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for i in range(3):
+            s.k[i], s.v[i] = torch.cat((s.k[i], k[i]), 1), torch.cat((s.v[i], v[i]), 1)
+        s.check(got, q, 0.09)
+    assert s.rt.health() == 0
+
+
+def test_a_capture_without_workspace():
+    """A first call inside a capture, whose partials do not fit: the undivided form."""
+    gen = _gen(15)
+    s = Sessions(gen, [1200], 300, hkv=1, d=64)
+    q = _q(gen, 1, 32, 32, 64)
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    s.rt.synchronize()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        got = s.rt.attend_shared(0, q, range(1), 0.12, prefix_slot=1)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        s.check(got, q, 0.12)
+
+
+def test_rotated_appended_and_attended():
+    """A decode step and a chunk as a model makes them: heads normed and rotated at their
+    positions behind the prefix, rows appended, attention over prefix and rows."""
+    from kvrt import HeadRotation
+
+    gen = _gen(16)
+    n, hq, hkv, d, p = 3, 16, 8, 128, 50
+    lens = [20, 33, 7]
+    inv = 1e4 ** (-torch.arange(64, dtype=torch.float64) / 64)
+    qw, kw = (torch.rand(d, generator=gen, device="cuda") + 0.5 for _ in range(2))
+    rot = HeadRotation(d, inv, axes=[f % 3 for f in range(64)], q_weight=qw, k_weight=kw)
+    s = Sessions(gen, lens, p, hkv=hkv, d=d)
+    for qn in (1, 1, 2, 1):
+        x = torch.randn(n, qn, hq + 2 * hkv, d, generator=gen, device="cuda").to(BF16)
+        q, k, v = (t.transpose(1, 2) for t in x.split([hq, hkv, hkv], 2))
+        base = p + torch.tensor(s.lens, device="cuda")[:, None] + torch.arange(qn, device="cuda")
+        pos = torch.stack((base, base // 2, torch.zeros_like(base)))
+        rq, rk, _ = rot.apply(q, k, positions=pos)
+
+        def exact(t, weight):
+            y = t.double()
+            y = y / torch.sqrt(y.square().mean(-1, keepdim=True) + 1e-6) * weight.double()
+            angle = pos.double()[[f % 3 for f in range(64)]].permute(1, 2, 0)[:, None] * inv.cuda()
+            a, b = y[..., :64], y[..., 64:]
+            return torch.cat((a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()), -1)
+
+        for got, t, w in ((rq, q, qw), (rk, k, kw)):
+            want = exact(t, w)
+            pair = want.unflatten(-1, (2, 64)).norm(dim=-2).repeat(1, 1, 1, 2)
+            assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -17 * pair).all())
+        s.append(rk, v.contiguous())
+        got = s.rt.attend_shared(0, rq, range(n), d ** -0.5, prefix_slot=n, softcap=30.0)
+        s.check(got, rq, d ** -0.5, cap=30.0)
+    assert s.rt.health() == 0
+
+
+def test_refusals():
+    from kvrt import KVRTError, KVRuntime, LayerSpec
+
+    gen = _gen(17)
+    s = Sessions(gen, [20, 2], 30, hkv=2, d=64)
+    rt, q = s.rt, _q(gen, 2, 4, 1, 64)
+    ok = dict(prefix_slot=2)
+    good = rt.attend_shared(0, q, [0, 1], 0.1, **ok)
+    before = rt.counters()
+
+    def refused(code, layer=0, q=q, slots=(0, 1), scale=0.1, **kw):
+        with pytest.raises(KVRTError) as e:
+            rt.attend_shared(layer, q, slots, scale, **{**ok, **kw})
+        assert e.value.code == code
+
+    inf, nan = float("inf"), float("nan")
+    for kw in (dict(layer=1), dict(layer=-1), dict(slots=(0, 0)), dict(slots=(0, 3)), dict(slots=(0, 2)), dict(slots=(0,)),
+               dict(prefix_slot=3), dict(scale=nan), dict(scale=inf), dict(softcap=-1.0), dict(softcap=nan),
+               dict(softcap=inf), dict(scale=1e30, softcap=1e-30), dict(q=q[:1]), dict(q=q[:, :3].contiguous()),
+               dict(q=q[..., :32].contiguous()), dict(q=q.float()), dict(q=q[:, :, :0]),
+               dict(q=torch.zeros(2, 4, 60, 64, device="cuda", dtype=BF16)), dict(out=q[:, :2]), dict(out=q.float()),
+               dict(out=torch.zeros(2, 8, 1, 64, device="cuda", dtype=BF16)[:, ::2])):
+        refused(-1, **kw)
+    refused(-2, q=torch.zeros(2, 4, 3, 64, device="cuda", dtype=BF16))  # more queries than slot 1 has rows
+    for bad in (torch.ones(3, device="cuda"), torch.ones(4), torch.ones(4, device="cuda", dtype=BF16),
+                torch.ones(8, device="cuda")[::2], torch.ones(1, 4, device="cuda")):
+        with pytest.raises(ValueError):
+            rt.attend_shared(0, q, [0, 1], 0.1, prefix_slot=2, slopes=bad)
+    with pytest.raises(ValueError):
+        rt.attend_shared(0, q, [0, 1], 0.1, prefix_slot=-1)
+    with pytest.raises(ValueError):
+        rt.attend_shared(0, q.cpu(), [0, 1], 0.1)
+    assert rt.counters() == before
+    assert torch.equal(rt.attend_shared(0, q, [0, 1], 0.1, **ok), good)
+    int8 = KVRuntime([LayerSpec(kv_heads=2, head_dim=64, layout="paged", dtype="int8")], n_slots=2, capacity=32,
+                     pool_pages=8)
+    int8.append(0, *(torch.zeros(2, 2, 1, 64, device="cuda", dtype=BF16),) * 2, [0, 1])
+    with pytest.raises(KVRTError):
+        int8.attend_shared(0, q[:1], [0], 0.1, prefix_slot=1)
+    # rows that are gone: a ring's, after a rollback, and evicted pages of either slot
+    ring = Sessions(gen, [100], 100, hkv=2, d=64, layout="ring", window=32)
+    ring.rt.truncate(1, 0)
+    assert ring.rt.attend_shared(0, q[:1], [0], 0.1, prefix_slot=1).isfinite().all()
+    with pytest.raises(KVRTError):
+        ring.rt.attend_shared(0, torch.zeros(1, 4, 3, 64, device="cuda", dtype=BF16), [0], 0.1)
+    for slot in (0, 1):
+        paged = Sessions(gen, [40], 40, hkv=2, d=64, layout="paged", window=20)
+        paged.rt.evict(slot, 32)
+        if slot == 0:
+            with pytest.raises(KVRTError):
+                paged.rt.attend_shared(0, q[:1], [0], 0.1, prefix_slot=1)
+        else:  # the window no longer reaches the prefix
+            assert paged.rt.attend_shared(0, q[:1], [0], 0.1, prefix_slot=1).isfinite().all()
+            paged.rt.truncate(0, 3)
+            with pytest.raises(KVRTError):
+                paged.rt.attend_shared(0, q[:1], [0], 0.1, prefix_slot=1)
