@@ -1136,17 +1136,11 @@ void shared_plan(SharedArgs &a, int D, int64_t pre_keys, int64_t own_keys) {
     a.pre_tiles = a.prefix_slot < 0 || a.joined ? 0 : (int)((rows + tile - 1) / tile);
     const int64_t own = (own_keys + (a.joined ? pre_keys : 0) + kSharedKeys - 1) / kSharedKeys + 1;
     const int64_t pre = a.pre_tiles ? (pre_keys + kSharedKeys - 1) / kSharedKeys : 0;
-    const int64_t target = D <= 128 ? 512 : 256;
-    const auto ranges = [&](int64_t tiles, int64_t per) { return std::max<int64_t>(1, (tiles + per - 1) / per); };
-    // the fewest tiles of a range, from 4 on, that give no more workgroups than that
-    int64_t per = 4;
-    for (int64_t high = std::max(own, pre); per < high;) {
-        const int64_t mid = (per + high) / 2;
-        if (hkv * (a.pre_tiles * ranges(pre, mid) + a.n_items * a.own_tiles * ranges(own, mid)) <= target) high = mid;
-        else per = mid + 1;
-    }
-    a.pre_splits = a.pre_tiles ? (int)std::min<int64_t>(ranges(pre, per), 32) : 0;
-    a.own_splits = (int)std::min<int64_t>(ranges(own, per), 32);
+    static const int slots = env_int("KVRT_SH_SLOTS", 512), wp = env_int("KVRT_SH_WP", 20), wmin = env_int("KVRT_SH_MIN", 40);
+    const int64_t total = hkv * (a.pre_tiles * pre * wp + a.n_items * a.own_tiles * own * 10);
+    const int64_t most = std::max<int64_t>(wmin, (total + slots - 1) / slots);
+    a.pre_splits = a.pre_tiles ? (int)std::clamp<int64_t>((pre * wp + most - 1) / most, 1, 64) : 0;
+    a.own_splits = (int)std::clamp<int64_t>((own * 10 + most - 1) / most, 1, 64);
     a.parts = a.pre_splits + a.own_splits;
 }
 

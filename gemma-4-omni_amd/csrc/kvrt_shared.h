@@ -32,9 +32,9 @@ struct SharedArgs {
     int slots[kMaxItems];
 };
 
-// Rows of a tile: four waves of two 16-row blocks, one at head_dim 512, whose
-// accumulators and queries fill a wave's registers.
-constexpr int shared_tile(int head_dim) { return head_dim == 512 ? 64 : 128; }
+// Rows of a tile: four waves of two 16-row blocks, one from head_dim 256 on, where two
+// blocks' accumulators and queries would fill a wave's registers.
+constexpr int shared_tile(int head_dim) { return head_dim <= 128 ? 128 : 64; }
 constexpr int kSharedKeys = 32;  // keys of a staged tile
 
 hipError_t launch_shared(const SharedArgs &a, int head_dim, hipStream_t s);       // and the join of its partials

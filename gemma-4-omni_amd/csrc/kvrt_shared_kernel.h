@@ -28,9 +28,11 @@
 // + j%4, the keys whose weights the lane holds, so weights go from one product's result
 // to the other's operand in their registers; V is read transposed (ds_read_b64_tr_b16).
 //
-// A staged tile is row-major, 16-byte chunks permuted within their row so that 16 lanes
-// that read one chunk of 16 rows (K), and 32 that read two chunks of 8 rows (V), find
-// every one of the 16 places of 16 bytes that the 64 banks hold once.
+// A DMA instruction leaves 1 KiB: rows ins, ins + D/16, ... of the tile one after another.
+// Instructions lie 1 KiB and a padding apart, 16 bytes for K and 32 for V, so that 16 lanes
+// that read one 16-byte chunk of 16 rows (K), and 32 that read 32 bytes of 8 rows (V), find
+// each of the 64 banks once, and every operand's address is one register (at head_dim 64
+// and 128 two, by kx) and a constant.
 #pragma once
 
 #include "kvrt_shared.h"
@@ -38,25 +40,45 @@
 
 namespace kvrt {
 
+// LDS DMA of 16 bytes per lane from base + off (bytes), base uniform.
+__device__ __forceinline__ void shared_dma(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+}
+
 __device__ __forceinline__ f32x4_t mfma_bf16(uint4 a, uint4 b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
                                                    0, 0);
 }
 
+// The largest of three in one instruction (fmaxf of values that cross a branch takes another
+// for each of them, on account of signalling NaN). Assembly that reads a matrix
+// instruction's result needs its wait: settle() comes between.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ void settle(f32x4_t &a, f32x4_t &b) {
+    asm volatile("s_nop 15" : "+v"(a), "+v"(b));  // 16 states: more than an 8-pass instruction asks for
+}
+
 template <int D>
 struct SharedShape {
     static constexpr int STAGES = D == 512 ? 2 : 3;
-    static constexpr int CHUNKS = D / 8;                  // 16-byte chunks of a row
-    static constexpr int BLK = kSharedKeys * D * 2;       // bytes of a staged K (or V) tile
-    static constexpr int IPW = D / 64;                    // DMA instructions per wave, tile and tensor
-    static constexpr int RPI = 512 / D;                   // rows per instruction (D 512: 1)
-    // chunk c of row r lies in place c ^ kx(r) (K), c ^ vx(r) (V) of its row
-    static __device__ __forceinline__ int kx(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
-    static __device__ __forceinline__ int vx(int r) { return D == 64 ? 2 * ((r >> 1) & 3) : 2 * (r & 7); }
+    static constexpr int CHUNKS = D / 8;     // 16-byte chunks of a row
+    static constexpr int IPB = D / 16;       // DMA instructions of a K (or V) tile
+    static constexpr int IPW = IPB / 4;      // ... per wave
+    static constexpr int KP = 1024 + 16, VP = 1024 + 32;  // bytes between instructions
+    static constexpr int KBLK = IPB * KP, VBLK = IPB * VP, STAGE = KBLK + VBLK;
+    // chunk c of an instruction's row number `sub` of K lies in place c ^ kx(sub)
+    static __device__ __forceinline__ int kx(int sub) {
+        return D == 128 ? (sub & 1) << 3 : D == 64 ? ((sub >> 1) & 1) << 2 : 0;
+    }
 };
 
 // Words that nothing in the launch writes: uniform ones load as scalars.
 typedef const __attribute__((address_space(4))) int32_t *SharedInts;
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 
 // One of the two runs of keys a unit walks: the prefix's or an item's own.
 struct Segment {
@@ -101,18 +123,28 @@ struct SharedUnit {
     int lens;  // lane i: length of item i
 };
 
-template <int D, int LAYOUT, bool WIDE>
+// BLOCKS: 16-row blocks per wave, of the unit's blocks wave, wave + 4 (past its last one
+// they are computed and not stored: a branch would part the matrix instructions); 0: the
+// unit has one, which all waves share.
+template <int D, int LAYOUT, int BLOCKS>
 __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUnit &u, uint8_t *lds) {
     using S = SharedShape<D>;
-    constexpr int RS = WIDE ? shared_tile(D) / 64 : 1;      // 16-row blocks per wave
+    constexpr bool WIDE = BLOCKS > 0;
+    constexpr int RS = WIDE ? BLOCKS : 1;
     constexpr int NB = WIDE ? D / 16 : D / 64;              // 16-dim blocks per wave
     constexpr int NS = S::STAGES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
     const int b0 = WIDE ? 0 : wave * NB;
     const int nblocks = (u.nrows + 15) / 16;                // of the unit's rows
-    const int mine = WIDE ? max(0, min(RS, (nblocks - wave + 3) / 4)) : 1;  // this wave's: wave, wave + 4
+    const bool some = !WIDE || wave < nblocks;              // this wave has rows
 
+    // A negative scale is moved into q's sign bits (exact), so that the largest score has the
+    // largest product; a zero scale stays above 0, so that a masked score (-INFINITY) keeps
+    // its weight of 0. Scores that are capped or biased are made one by one, in log2 units.
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+    const bool made = a.cap != 0.f || a.slopes;
+    const float unit = made ? 1.f : fmaxf(fabsf(a.scale), 1e-37f);
     // this lane's rows
     const int per_item = a.group * a.qn;
     int pos[RS];          // own position; -1 - P and below: a lane without a row sees nothing
@@ -145,8 +177,11 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
     for (int s = 0; s < RS; ++s) {
         asm volatile("" : "+v"(pos[s]), "+v"(slope[s]));
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c)  // all loads of registers are done ahead of the first DMA
-            asm volatile("" : "+v"(qop[s][c].x), "+v"(qop[s][c].y), "+v"(qop[s][c].z), "+v"(qop[s][c].w));
+        for (int c = 0; c < D / 32; ++c) {
+            uint4 &x = qop[s][c];
+            x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+            asm volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w));  // loaded ahead of the first DMA
+        }
     }
 
     float m[RS], l[RS];
@@ -188,36 +223,56 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
                                  ? 0
                                  : (int64_t)g.slot * a.kv.slot_stride + (int64_t)u.kvh * a.kv.head_stride;
         const int ring0 = LAYOUT == KVRT_LAYOUT_RING ? key0 % a.kv.rows : 0;
+        const int sub = lane / S::CHUNKS, c = lane % S::CHUNKS;
 #pragma unroll
         for (int i = 0; i < S::IPW; ++i) {
-            const int ins = 4 * i + wave;
-            const int r = ins * S::RPI + lane / S::CHUNKS, c = lane % S::CHUNKS;
+            const int ins = 4 * i + wave, r = ins + S::IPB * sub;
             const int key = min(max(key0 + r, g.lo), g.last);  // rows nobody sees read one that somebody does
+            const uint32_t to = lds_at + (uint32_t)(buf * S::STAGE), kto = to + ins * S::KP, vto = to + S::KBLK + ins * S::VP;
             int64_t off;
             if constexpr (LAYOUT == KVRT_LAYOUT_CONTIG) {
-                off = head + (int64_t)key * D;
+                const int64_t base = head + (int64_t)key0 * D;
+                const uint32_t at = (uint32_t)(key - key0) * (2 * D);
+                shared_dma(kg + base, at + 16 * (c ^ S::kx(sub)), kto);
+                shared_dma(vg + base, at + 16 * c, vto);
+                continue;
             } else if constexpr (LAYOUT == KVRT_LAYOUT_RING) {
                 int rr = ring0 + (key - key0);
                 if (a.kv.rows >= kSharedKeys) rr = rr >= a.kv.rows ? rr - a.kv.rows : rr;  // wraps once at most
                 else rr %= a.kv.rows;
                 off = head + (int64_t)rr * D;
             } else {
-                const int page = scalar_pages ? (ins * S::RPI >= 16 ? id1 : id0)
+                const int page = scalar_pages ? (r >= 16 ? id1 : id0)
                                               : a.kv.page_table[(int64_t)g.slot * a.kv.pt_stride + (key >> a.kv.block_shift)];
                 off = page_row_offset(a.kv, page, u.kvh, key, D);
                 bad |= off < 0;
                 off = off < 0 ? 0 : off;
             }
-            const uint32_t to = lds_at + (uint32_t)(buf * 2 * S::BLK + ins * 1024);
-            dma_load16_cached(kg + off + 8 * (c ^ S::kx(r)), to);
-            dma_load16_cached(vg + off + 8 * (c ^ S::vx(r)), to + S::BLK);
+            dma_load16_cached(kg + off + 8 * (c ^ S::kx(sub)), kto);
+            dma_load16_cached(vg + off + 8 * c, vto);
         }
     };
 
     // ---- one tile
+    // K: key row col (and + 16), chunk 4 c + grp; V: key row 4 grp + s16 / 4 (and + 16), dims
+    // 4 (s16 % 4) .. + 3 of a block
     const int s16 = lane & 15, vrow = 4 * grp + (s16 >> 2);
-    auto compute = [&](int x, int buf) __attribute__((always_inline)) {
-        const uint8_t *kt = lds + buf * 2 * S::BLK, *vt = kt + S::BLK;
+    constexpr int H = 16 / S::IPB * 2 * D;  // bytes from row r to r + 16 (D 512: 16 instructions)
+    const int kadr = (col % S::IPB) * S::KP + (col / S::IPB) * 2 * D + 16 * grp, kx = 16 * S::kx(col / S::IPB);
+    const int vadr = (vrow % S::IPB) * S::VP + (vrow / S::IPB) * 2 * D + 8 * (s16 & 3) + 32 * b0;
+    uint4 ph[RS], pl[RS];  // a tile's weights, high and low terms
+    // V^T of 16 dims: this lane's dim 16 b + col, keys 16 h + 4 grp + 0 .. 3
+    auto vop = [&](const uint8_t *vt, int b) __attribute__((always_inline)) {
+        uint2 v[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            v[h] = lds_read_tr16(reinterpret_cast<const uint16_t *>(vt + vadr + 32 * b + h * (D == 512 ? 16 * S::VP : H)));
+        return make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
+    };
+    // The weights of tile x. True where some query does not see all of it and its V holds NaN
+    // or infinities: 0 * NaN is not 0, so that its products are made one by one (add_odd).
+    auto weigh = [&](int x, int buf) __attribute__((always_inline)) {
+        const uint8_t *kt = lds + buf * S::STAGE, *vt = kt + S::KBLK;
         f32x4_t sc[RS][2];
 #pragma unroll
         for (int s = 0; s < RS; ++s)
@@ -227,12 +282,11 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
         for (int c = 0; c < D / 32; ++c)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int r = 16 * h + col;
-                const uint4 k = *reinterpret_cast<const uint4 *>(kt + r * 2 * D + 16 * ((4 * c + grp) ^ S::kx(r)));
+                const uint4 k = *reinterpret_cast<const uint4 *>(kt + kadr + ((64 * c) ^ kx) + h * (D == 512 ? 16 * S::KP : H));
 #pragma unroll
-                for (int s = 0; s < RS; ++s)
-                    if (s == 0 || s < mine) sc[s][h] = mfma_bf16(k, qop[s][c], sc[s][h]);
+                for (int s = 0; s < RS; ++s) sc[s][h] = mfma_bf16(k, qop[s][c], sc[s][h]);
             }
+        __builtin_amdgcn_sched_barrier(0);
         int key0;
         const Segment &g = where(x, key0);
         const bool own = x >= u.pre.tiles;
@@ -240,26 +294,24 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
         const bool whole = key0 >= g.all_lo && key0 + kSharedKeys <= g.all_hi && key0 >= plen;
         uint32_t word = ~0u;  // bit k: key0 + k passes the slot's mask
         if (key0 < plen) word = (uint32_t)__builtin_amdgcn_readlane((int)(own ? pw_o : pw_p), (key0 >> 5) & (kPrefixWords - 1));
-        uint4 ph[RS], pl[RS];
-        float e[RS][8];
 #pragma unroll
         for (int s = 0; s < RS; ++s) {
-            if (s > 0 && s >= mine) break;
             const int at = pos[s] + g.off;
+            settle(sc[s][0], sc[s][1]);
             float t[8];
-            if (a.cap == 0.f) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] = sc[s][i / 4][i % 4] * a.scale;
-            } else {
+            for (int i = 0; i < 8; ++i) t[i] = sc[s][i / 4][i % 4];
+            if (made) {
+                const float by = a.cap != 0.f ? fabsf(a.inv_cap) : fabsf(a.scale);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] = capped(sc[s][i / 4][i % 4] * a.inv_cap, a.cap);
-            }
-            if (a.slopes) {
+                for (int i = 0; i < 8; ++i) t[i] *= by;
+                if (a.cap != 0.f) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                    for (int i = 0; i < 8; ++i) t[i] = capped(t[i], a.cap);
+                }
+                const float far = (float)(key0 + 4 * grp - at);  // below 2^24 in earnest, and rounded beyond
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        t[4 * h + i] = fmaf(slope[s], (float)(key0 + 16 * h + 4 * grp + i - at), t[4 * h + i]);
+                for (int i = 0; i < 8; ++i) t[i] = fmaf(slope[s], far + (float)(16 * (i / 4) + i % 4), t[i]);
             }
             if (!whole) {
                 // bit k: key0 + k is seen by this row
@@ -272,8 +324,8 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
 #pragma unroll
                     for (int i = 0; i < 4; ++i) t[4 * h + i] = (vis >> (16 * h + i)) & 1u ? t[4 * h + i] : -INFINITY;
             }
-            float top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
-            top = pair<OpMax, 32>(pair<OpMax, 16>(top));
+            float top = max3(max3(max3(t[0], t[1], t[2]), t[3], t[4]), max3(t[5], t[6], t[7]), t[7]);
+            top = pair<OpMax, 32>(pair<OpMax, 16>(top * unit));
             const float mn = top > m[s] + kRescaleSlack ? top : m[s];
             if (__any(mn != m[s])) {
                 const float corr = __builtin_amdgcn_exp2f(m[s] - mn);
@@ -284,10 +336,9 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
             }
             uint32_t hiw[4], low[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[s][i] = __builtin_amdgcn_exp2f(t[i] - m[s]);
-#pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float x0 = e[s][2 * i], x1 = e[s][2 * i + 1];
+                const float x0 = __builtin_amdgcn_exp2f(fmaf(t[2 * i], unit, -m[s]));
+                const float x1 = __builtin_amdgcn_exp2f(fmaf(t[2 * i + 1], unit, -m[s]));
                 l[s] += x0 + x1;
                 hiw[i] = pack_bf16x2(x0, x1);
                 low[i] = pack_bf16x2(x0 - bf16_lo(hiw[i]), x1 - bf16_hi(hiw[i]));
@@ -295,64 +346,48 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
             ph[s] = make_uint4(hiw[0], hiw[1], hiw[2], hiw[3]);
             pl[s] = make_uint4(low[0], low[1], low[2], low[3]);
         }
-        // V^T of 16 dims: this lane's dim 16 b + col, keys 16 h + 4 grp + 0 .. 3
-        auto vop = [&](int b) __attribute__((always_inline)) {
-            uint2 v[2];
+        if (whole) return false;
+        u16x2_t most = {0, 0};
+#pragma clang loop unroll_count(2)
+        for (int b = 0; b < NB; ++b) {
+            const uint4 v = vop(vt, b);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = 16 * h + vrow;
-                v[h] = lds_read_tr16(reinterpret_cast<const uint16_t *>(
-                    vt + r * 2 * D + 16 * ((2 * (b0 + b) + ((s16 & 3) >> 1)) ^ S::vx(r)) + 8 * (s16 & 1)));
-            }
-            return make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
-        };
-        bool plain = true;
-        if (!whole) {
-            // A row that some see and others do not may hold NaN or infinities, and 0 * NaN is
-            // not 0: such a tile's products are made one by one below
-            uint32_t odd = 0;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const uint4 v = vop(b);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    odd |= (w[i] & 0x7f80u) == 0x7f80u ? 1u : 0u;
-                    odd |= (w[i] & 0x7f800000u) == 0x7f800000u ? 1u : 0u;
-                }
-            }
-            plain = !__any(odd != 0);
+            for (int i = 0; i < 4; ++i)
+                most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, w[i] & 0x7fff7fffu));
         }
-        if (plain) {
+        return __any(most[0] >= 0x7f80 || most[1] >= 0x7f80) != 0;
+    };
+    auto add = [&](int buf) __attribute__((always_inline)) {
+        const uint8_t *vt = lds + buf * S::STAGE + S::KBLK;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const uint4 v = vop(b);
+        for (int b = 0; b < NB; ++b) {
+            const uint4 v = vop(vt, b);
 #pragma unroll
-                for (int s = 0; s < RS; ++s)
-                    if (s == 0 || s < mine) {
-                        o[s][b] = mfma_bf16(v, ph[s], o[s][b]);
-                        o[s][b] = mfma_bf16(v, pl[s], o[s][b]);
-                    }
-            }
-        } else {
+            for (int s = 0; s < RS; ++s) o[s][b] = mfma_bf16(v, ph[s], o[s][b]);
+#pragma unroll
+            for (int s = 0; s < RS; ++s) o[s][b] = mfma_bf16(v, pl[s], o[s][b]);
+        }
+    };
+    auto add_odd = [&](int buf) __attribute__((always_inline)) {
+        const uint8_t *vt = lds + buf * S::STAGE + S::KBLK;
 #pragma clang loop unroll(disable)
-            for (int k = 0; k < kSharedKeys; ++k) {
-                const int at = 4 * (k >> 4) + (k & 3), from = 16 * ((k >> 2) & 3) + col;
+        for (int k = 0; k < kSharedKeys; ++k) {
+            const int at = 2 * (k >> 4) + ((k >> 1) & 1), from = 16 * ((k >> 2) & 3) + col;
 #pragma unroll
-                for (int s = 0; s < RS; ++s) {
-                    if (s > 0 && s >= mine) break;
-                    float p = e[s][0];
+            for (int s = 0; s < RS; ++s) {
+                const uint4 hs = ph[s], ls = pl[s];
+                const uint32_t hw = at < 2 ? (at == 0 ? hs.x : hs.y) : at == 2 ? hs.z : hs.w;
+                const uint32_t lw = at < 2 ? (at == 0 ? ls.x : ls.y) : at == 2 ? ls.z : ls.w;
+                const float p = __shfl(k & 1 ? bf16_hi(hw) + bf16_hi(lw) : bf16_lo(hw) + bf16_lo(lw), from);
 #pragma unroll
-                    for (int i = 1; i < 8; ++i) p = at == i ? e[s][i] : p;
-                    p = __shfl(p, from);
+                for (int b = 0; b < NB; ++b) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(
+                        vt + (k % S::IPB) * S::VP + (k / S::IPB) * 2 * D + 32 * (b0 + b) + 8 * grp);
+                    const float x[4] = {bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y)};
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const uint2 v = *reinterpret_cast<const uint2 *>(
-                            vt + k * 2 * D + 16 * ((2 * (b0 + b) + (grp >> 1)) ^ S::vx(k)) + 8 * (grp & 1));
-                        const float x[4] = {bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y)};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[s][b][i] = p == 0.f ? o[s][b][i] : fmaf(p, x[i], o[s][b][i]);
-                    }
+                    for (int i = 0; i < 4; ++i) o[s][b][i] = p == 0.f ? o[s][b][i] : fmaf(p, x[i], o[s][b][i]);
+                    __builtin_amdgcn_sched_barrier(0);  // (one block's values at a time: registers)
                 }
             }
         }
@@ -369,22 +404,32 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
                 stage(u.x0 + i, i);
                 load_ids(u.x0 + min(i + 1, n - 1));
             }
-        int buf = 0;
-        for (int i = 0; i < n; ++i) {
-            wait_vmem_steps<PER, NS - 2>(n - 1 - i);  // this wave's part of tile i has landed
-            __syncthreads();                          // every wave's has, and tile i - 1 is read
-            if (i + NS - 1 < n) {
-                stage(u.x0 + i + NS - 1, buf == 0 ? NS - 1 : buf - 1);
-                load_ids(u.x0 + min(i + NS, n - 1));
+        // (add_odd stands outside the loop that all other tiles stay in: beside it in one loop,
+        // the accumulators were copied at every tile)
+        for (int i = 0, buf = 0;; ++i) {
+            bool odd = false;
+            for (; i < n; ++i) {
+                wait_vmem_steps<PER, NS - 2>(n - 1 - i);  // this wave's part of tile i has landed
+                __syncthreads();                          // every wave's has, and tile i - 1 is read
+                if (i + NS - 1 < n) {
+                    stage(u.x0 + i + NS - 1, buf == 0 ? NS - 1 : buf - 1);
+                    load_ids(u.x0 + min(i + NS, n - 1));
+                }
+                if (some) {
+                    odd = weigh(u.x0 + i, buf);
+                    if (odd) break;
+                    add(buf);
+                }
+                buf = buf == NS - 1 ? 0 : buf + 1;
             }
-            if (mine > 0) compute(u.x0 + i, buf);
+            if (!odd) break;
+            add_odd(buf);
             buf = buf == NS - 1 ? 0 : buf + 1;
         }
     }
     if (bad) a.err[0] = 1;
 #pragma unroll
     for (int s = 0; s < RS; ++s) {
-        if (s >= mine) break;
         const int r = 16 * (WIDE ? wave + 4 * s : 0) + col;
         const float sum = pair<OpSum, 32>(pair<OpSum, 16>(l[s]));
         if (r >= u.nrows) continue;
@@ -412,10 +457,10 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
 }
 
 template <int D, int LAYOUT>
-__global__ __launch_bounds__(256) void shared_attend_kernel(SharedArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void shared_attend_kernel(SharedArgs a) {
     using S = SharedShape<D>;
     constexpr int TILE = shared_tile(D);
-    __shared__ __align__(16) uint8_t lds[S::STAGES * 2 * S::BLK];
+    __shared__ __align__(16) uint8_t lds[S::STAGES * S::STAGE];
     const int lane = threadIdx.x & 63;
     const int hkv = a.kv.kv_heads, per_item = a.group * a.qn;
     const int capacity = a.capacity;
@@ -468,8 +513,9 @@ __global__ __launch_bounds__(256) void shared_attend_kernel(SharedArgs a) {
     const int tiles = u.pre.tiles + u.own.tiles, per = (tiles + splits - 1) / splits;
     u.x0 = min(ks * per, tiles);
     u.x1 = min(u.x0 + per, tiles);
-    if (u.nrows > 16) shared_unit<D, LAYOUT, true>(a, u, lds);
-    else shared_unit<D, LAYOUT, false>(a, u, lds);
+    if (u.nrows <= 16) shared_unit<D, LAYOUT, 0>(a, u, lds);
+    else if (TILE == 64 || u.nrows <= 64) shared_unit<D, LAYOUT, 1>(a, u, lds);
+    else shared_unit<D, LAYOUT, TILE / 64>(a, u, lds);
 }
 
 // Joins the partials of every row: a row's D / 4 threads walk its parts in order, kAhead

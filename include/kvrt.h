@@ -576,7 +576,7 @@ int kvrt_attend_talker_async(kvrt_ctx *ctx, int32_t layer, int32_t n, const int3
  * positions of n slots of one layer behind a prefix that they share: slot i sees
  * the P rows of prefix_slot (P its length), then its own L_i, so that its query
  * row r sits at position P + L_i - Q + r. Nothing is copied: the prefix's rows are
- * read once per 128 query rows (64 at head_dim 512) of the call. prefix_slot -1:
+ * read once per 128 query rows (64 from head_dim 256 on) of the call. prefix_slot -1:
  * no prefix. Scores are
  *   s = f(q.k * scale) + slopes[h] * (key position - query position)
  * with f(x) = softcap * tanh(x / softcap), or x where softcap is 0; slopes: DEVICE
