@@ -1126,21 +1126,69 @@ int tensor_call_launch(TensorCall &tc, float *ws, hipStream_t st, bool single) {
 constexpr int kMaxSharedCapacity = 1 << 29;
 constexpr int64_t kMaxSharedRows = 1 << 22;
 
-// How a call's rows and keys are divided (SharedArgs), from the most keys that are seen
-// of the prefix and of an item's own rows.
-void shared_plan(SharedArgs &a, int D, int64_t pre_keys, int64_t own_keys) {
-    const int hkv = a.kv.kv_heads, tile = shared_tile(D);
+// How a call's rows and keys are divided (SharedArgs): pre_keys of the prefix are seen, and
+// own[i] of item i's rows. The shortest time of a simple model is taken: a launch lasts as
+// long as its longest unit, and at least as its units' work shared by 256 CUs; a unit takes
+// kTile us a key tile (measured with a workgroup per CU; two that share one overlap in part)
+// and kUnit of its own; partials are joined by a second launch.
+//   us a tile, head_dim 64 / 128 / 256 / 512: up to 16 rows 0.6, 0.8, 1.2, 1.8; up to 64 rows
+//   0.8, 1.1, 1.9, 2.5; up to 128 rows 1.0, 1.5
+void shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own) {
+    const int hkv = a.kv.kv_heads, tile = shared_tile(D), dim = D == 64 ? 0 : D == 128 ? 1 : D == 256 ? 2 : 3;
     const int64_t per_item = (int64_t)a.group * a.qn, rows = per_item * a.n_items;
+    const auto tiles_of = [](int64_t keys) { return (keys + kSharedKeys - 1) / kSharedKeys + (keys % kSharedKeys > 1 ? 1 : 0); };
+    const auto cost = [&](int64_t r) {
+        static const double us[3][4] = {{0.6, 0.8, 1.2, 1.8}, {0.8, 1.1, 1.9, 2.5}, {1.0, 1.5, 1.9, 2.5}};
+        return us[r <= 16 ? 0 : r <= 64 ? 1 : 2][dim];
+    };
+    constexpr double kUnit = 1.5, kJoin = 4.5, kJoinBytes = 3e6;  // us, us, bytes a us
     a.own_tiles = (int)((per_item + tile - 1) / tile);
     a.joined = a.prefix_slot >= 0 && (pre_keys == 0 || per_item >= 64);
     a.pre_tiles = a.prefix_slot < 0 || a.joined ? 0 : (int)((rows + tile - 1) / tile);
-    const int64_t own = (own_keys + (a.joined ? pre_keys : 0) + kSharedKeys - 1) / kSharedKeys + 1;
-    const int64_t pre = a.pre_tiles ? (pre_keys + kSharedKeys - 1) / kSharedKeys : 0;
-    static const int slots = env_int("KVRT_SH_SLOTS", 512), wp = env_int("KVRT_SH_WP", 20), wmin = env_int("KVRT_SH_MIN", 40);
-    const int64_t total = hkv * (a.pre_tiles * pre * wp + a.n_items * a.own_tiles * own * 10);
-    const int64_t most = std::max<int64_t>(wmin, (total + slots - 1) / slots);
-    a.pre_splits = a.pre_tiles ? (int)std::clamp<int64_t>((pre * wp + most - 1) / most, 1, 64) : 0;
-    a.own_splits = (int)std::clamp<int64_t>((own * 10 + most - 1) / most, 1, 64);
+    const int64_t pre = tiles_of(pre_keys);
+    int64_t items[kMaxItems], most = 1;
+    for (int i = 0; i < a.n_items; ++i) {
+        items[i] = std::max<int64_t>(1, tiles_of(own[i]) + (a.joined ? pre : 0));
+        most = std::max(most, items[i]);
+    }
+    const double cp = cost(std::min<int64_t>(rows, tile)), co = cost(std::min<int64_t>(per_item, tile));
+    const double share = 1.0 / 256 * (D <= 128 ? 0.7 : 1.0);
+    const bool ragged = !a.joined && a.own_tiles == 1;
+    // ranges of an item of t tiles: even ones, or of `per` tiles where items differ
+    const auto ranges = [](int64_t t, int64_t per) { return std::max<int64_t>(1, (t + per - 1) / per); };
+    double best = 1e30;
+    int64_t best_pre = 1, best_per = most;
+    for (int64_t per = 1;; per = std::min(most, per + 1 + per / 4)) {
+        const int64_t splits = ranges(most, per);
+        if (splits <= 32) {
+            double work = 0, units = 0;
+            for (int i = 0; i < a.n_items; ++i) {
+                const double u = (double)(ragged ? ranges(items[i], per) : splits);
+                units += u * a.own_tiles;
+                work += (items[i] * co + u * kUnit) * a.own_tiles;
+            }
+            for (int64_t pp = 1;; pp = std::min(pre, pp + 1 + pp / 4)) {
+                const int64_t ps = a.pre_tiles ? ranges(pre, pp) : 0;
+                if (ps <= 64) {
+                    const double all = hkv * (work + a.pre_tiles * (pre * cp + ps * kUnit)) * share;
+                    const double longest = std::max((double)std::min(per, most) * co, a.pre_tiles ? pp * cp : 0.0) + kUnit;
+                    const int64_t parts = splits + ps;
+                    double t = std::max(all, longest);
+                    if (parts > 1) t += kJoin + (double)rows * hkv * parts * D * 8 / kJoinBytes;
+                    if (t < best) best = t, best_pre = ps, best_per = per;
+                }
+                if (!a.pre_tiles || pp >= pre) break;
+            }
+        }
+        if (per >= most) break;
+    }
+    a.pre_splits = (int)best_pre;
+    a.own_splits = (int)ranges(most, best_per);
+    a.own_per = a.own_wgs = 0;
+    if (ragged && a.own_splits > 1) {
+        a.own_per = (int)best_per;
+        for (int i = 0; i < a.n_items; ++i) a.own_wgs += (int)ranges(items[i], best_per);
+    }
     a.parts = a.pre_splits + a.own_splits;
 }
 
@@ -2313,7 +2361,7 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     const bool capturing = hipStreamIsCapturing(c->stream, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone;
     int min_len = INT32_MAX;
-    int64_t own_keys = 0;  // most own keys that an item's rows see
+    int64_t own_keys[kMaxItems], all_own = 0;  // own keys that each item's rows see
     for (int i = 0; i < n; ++i) {
         const int L = c->len_at(slots[i], layer);
         if (L < qn) return KVRT_ESTATE;
@@ -2324,7 +2372,8 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
                                              oldest < c->ring_floor(slots[i], layer)))
             return KVRT_ESTATE;
         if (s.layout == KVRT_LAYOUT_PAGED && oldest < c->first_live[slots[i]] * c->cfg.block_size) return KVRT_ESTATE;
-        own_keys = std::max<int64_t>(own_keys, L - oldest);
+        own_keys[i] = L - oldest;
+        all_own += own_keys[i];
     }
     // the oldest key of the prefix that some row sees must still be stored
     const int oldest = window > 0 ? (int)std::max<int64_t>(0, P + min_len - qn - window + 1) : 0;
@@ -2362,7 +2411,7 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
         // a workspace that a capture cannot grow: one walk per row tile, which needs none
         if (capturing) {
             a.joined = shared;
-            a.pre_tiles = 0, a.pre_splits = 0, a.own_splits = 1, a.parts = 1;
+            a.pre_tiles = 0, a.pre_splits = 0, a.own_per = 0, a.own_splits = 1, a.parts = 1;
         } else if ((rc = ensure_workspace(c, bytes())) != KVRT_OK) {
             return rc;
         }
@@ -2372,7 +2421,7 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
     c->counters.launches += a.parts > 1 ? 2 : 1;
     if (launch_shared(a, D, enq(c)) != hipSuccess) return poison(c);
     const uint64_t keys = ((uint64_t)pre_keys * (a.joined ? n * a.own_tiles : a.pre_tiles) +
-                           (uint64_t)own_keys * n * a.own_tiles) * hkv;
+                           (uint64_t)all_own * a.own_tiles) * hkv;
     c->counters.attended_keys += keys;
     c->counters.attended_bytes += keys * (uint64_t)D * 2 * 2;
     return KVRT_OK;

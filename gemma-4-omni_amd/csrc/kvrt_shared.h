@@ -27,7 +27,10 @@ struct SharedArgs {
     // kSharedTile<D> rows, keys in pre_splits ranges (pre_tiles 0: none); then those of
     // each item, its rows in own_tiles tiles, keys in own_splits ranges: its own keys, with
     // `joined` those of the prefix before them.
+    // own_per > 0 (items of one tile): an item's keys go to ranges of that many key tiles,
+    // own_splits at most, all items' to own_wgs units for each KV head.
     int pre_tiles, pre_splits, own_tiles, own_splits, joined;
+    int own_per, own_wgs;
     int parts;                // partials of a row; 1: units write the answer
     int slots[kMaxItems];
 };

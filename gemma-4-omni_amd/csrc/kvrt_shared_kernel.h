@@ -495,9 +495,50 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void shared_at
     } else {
         int item, rem;
         at -= a.pre_tiles * a.pre_splits;
-        splits = a.own_splits;
-        udivmod_uniform(at, splits * a.own_tiles, item, rem);
-        udivmod_uniform(rem, splits, tile, ks);
+        if (a.own_per > 0) {
+            // sessions of unequal length: each takes a range of own_per tiles after another
+            const int t = lane < a.n_items ? segment_of(0, u.lens, 0, u.lens - a.qn, u.lens - 1, a.window).tiles : 0;
+            int per = a.own_per, sum, most;
+            for (bool again = true;; again = false) {
+                sum = lane < a.n_items ? max(1, (t + per - 1) / per) : 0;
+                most = sum;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const int y = __shfl_up(sum, d);
+                    if (lane >= d) sum += y;
+                    most = max(most, __shfl_xor(most, d));
+                }
+                if (!again || (__builtin_amdgcn_readlane(sum, 63) <= a.own_wgs && most <= a.own_splits)) break;
+                // (more of them than the launch and its partials were made for: a replay on longer
+                // sessions) n sessions take at most total / per + n ranges
+                int all = t, top = t;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    all += __shfl_xor(all, d);
+                    top = max(top, __shfl_xor(top, d));
+                }
+                const int spare = a.own_wgs - a.n_items;
+                per = max((top + a.own_splits - 1) / a.own_splits, spare > 0 ? (all + spare - 1) / spare : top);
+                per = __builtin_amdgcn_readfirstlane(max(per, 1));
+            }
+            const uint64_t past = __ballot(sum > at);
+            if (past == 0) return;
+            item = __builtin_ctzll(past);
+            const int first = item == 0 ? 0 : __builtin_amdgcn_readlane(sum, item - 1);
+            splits = __builtin_amdgcn_readlane(sum, item) - first;
+            ks = at - first;
+            tile = 0;
+            if (ks == splits - 1) {  // parts that this session does not have
+                const int none = a.own_splits - splits;
+                for (int i = threadIdx.x; i < none * per_item; i += 256)
+                    a.part_ml[((int64_t)u.kvh * a.n_items * per_item + item * per_item + i / none) * a.parts + a.pre_splits +
+                              splits + i % none] = make_float2(kNegBig, 0.f);
+            }
+        } else {
+            splits = a.own_splits;
+            udivmod_uniform(at, splits * a.own_tiles, item, rem);
+            udivmod_uniform(rem, splits, tile, ks);
+        }
         u.row0 = item * per_item + tile * TILE;
         u.nrows = min(per_item - tile * TILE, TILE);
         u.part = a.pre_splits + ks;
@@ -518,30 +559,23 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void shared_at
     else shared_unit<D, LAYOUT, TILE / 64>(a, u, lds);
 }
 
-// Joins the partials of every row: a row's D / 4 threads walk its parts in order, kAhead
-// of them in flight.
-template <int D>
+// Joins the partials of every row. A row's parts are dealt to GROUPS groups of D / 4
+// threads, so that few rows of many parts take one or two round trips of loads (kAhead
+// parts a thread at a time), and the groups' sums are added in group order.
+template <int D, int GROUPS>
 __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
-    constexpr int LANES = D / 4, ROWS = 256 / LANES, kAhead = 8;
-    const int per_item = a.group * a.qn;
+    constexpr int LANES = D / 4, ROWS = 256 / (LANES * GROUPS), kAhead = 8;
+    __shared__ float4 so[GROUPS > 1 ? 256 : 1];
+    __shared__ float2 sml[GROUPS > 1 ? 256 : 1];
+    const int per_item = a.group * a.qn, lane = threadIdx.x % LANES, group = threadIdx.x / LANES % GROUPS;
     const int64_t rows = (int64_t)a.n_items * per_item;
-    const int64_t at = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
-    if (at >= rows * a.kv.kv_heads) return;
-    const int kvh = (int)(at / rows), f = (int)(at - kvh * rows), d = 4 * (threadIdx.x % LANES);
+    const int64_t at = (int64_t)blockIdx.x * ROWS + threadIdx.x / (LANES * GROUPS);
+    const bool live = at < rows * a.kv.kv_heads;
+    const int kvh = live ? (int)(at / rows) : 0, f = live ? (int)(at - kvh * rows) : 0, d = 4 * lane;
+    const int n = live ? a.parts : 0;
     float M = kNegBig, sum = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = 0; p0 < a.parts; p0 += kAhead) {
-        float2 ml[kAhead];
-        float4 x[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int64_t p = at * a.parts + min(p0 + i, a.parts - 1);
-            ml[i] = a.part_ml[p];
-            x[i] = *reinterpret_cast<const float4 *>(a.part_o + p * D + d);
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-            if (p0 + i >= a.parts) ml[i] = make_float2(kNegBig, 0.f);
+    const auto take = [&](const float2(&ml)[kAhead], const float4(&x)[kAhead]) __attribute__((always_inline)) {
         float top = M;
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) top = fmaxf(top, ml[i].x);
@@ -556,7 +590,38 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
             sum = fmaf(ml[i].y, w, sum);
             o = make_float4(fmaf(x[i].x, w, o.x), fmaf(x[i].y, w, o.y), fmaf(x[i].z, w, o.z), fmaf(x[i].w, w, o.w));
         }
+    };
+    float2 ml[kAhead];
+    float4 x[kAhead];
+    for (int p0 = group; p0 < n; p0 += kAhead * GROUPS) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t p = at * n + min(p0 + i * GROUPS, n - 1);
+            ml[i] = a.part_ml[p];
+            x[i] = *reinterpret_cast<const float4 *>(a.part_o + p * D + d);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (p0 + i * GROUPS >= n) ml[i] = make_float2(kNegBig, 0.f);
+        take(ml, x);
     }
+    if constexpr (GROUPS > 1) {
+        so[threadIdx.x] = o;
+        sml[threadIdx.x] = make_float2(M, sum);
+        __syncthreads();
+        if (group != 0) return;
+#pragma unroll
+        for (int g0 = 1; g0 < GROUPS; g0 += kAhead) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int g = threadIdx.x + min(g0 + i, GROUPS - 1) * LANES;
+                ml[i] = g0 + i < GROUPS ? sml[g] : make_float2(kNegBig, 0.f);
+                x[i] = so[g];
+            }
+            take(ml, x);
+        }
+    }
+    if (!live) return;
     const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
     int item, rem, qr, hr;
     udivmod_uniform(f, per_item, item, rem);
@@ -565,9 +630,20 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
     *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
 }
 
+template <int D, int GROUPS>
+static hipError_t launch_shared_join(const SharedArgs &a, hipStream_t s) {
+    if constexpr (GROUPS > 1)  // as many groups as leave each a batch of eight parts
+        if (a.parts <= 8 * (GROUPS / 2)) return launch_shared_join<D, GROUPS / 2>(a, s);
+    constexpr int ROWS = 1024 / (D * GROUPS);
+    const int64_t rows = (int64_t)a.n_items * a.group * a.qn * a.kv.kv_heads;
+    hipLaunchKernelGGL((shared_join_kernel<D, GROUPS>), dim3((unsigned)((rows + ROWS - 1) / ROWS)), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
 template <int D>
 static hipError_t launch_shared_dim(const SharedArgs &a, hipStream_t s) {
-    const int units = (a.pre_tiles * a.pre_splits + a.n_items * a.own_tiles * a.own_splits) * a.kv.kv_heads;
+    const int units = (a.pre_tiles * a.pre_splits +
+                       (a.own_per > 0 ? a.own_wgs : a.n_items * a.own_tiles * a.own_splits)) * a.kv.kv_heads;
     switch (a.kv.layout) {
         case KVRT_LAYOUT_CONTIG:
             hipLaunchKernelGGL((shared_attend_kernel<D, KVRT_LAYOUT_CONTIG>), dim3(units), dim3(256), 0, s, a);
@@ -582,10 +658,7 @@ static hipError_t launch_shared_dim(const SharedArgs &a, hipStream_t s) {
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.parts == 1) return e;
-    constexpr int ROWS = 1024 / D;
-    const int64_t rows = (int64_t)a.n_items * a.group * a.qn * a.kv.kv_heads;
-    hipLaunchKernelGGL((shared_join_kernel<D>), dim3((unsigned)((rows + ROWS - 1) / ROWS)), dim3(256), 0, s, a);
-    return hipGetLastError();
+    return launch_shared_join<D, (D == 512 ? 2 : D == 256 ? 4 : 8)>(a, s);
 }
 
 }  // namespace kvrt
