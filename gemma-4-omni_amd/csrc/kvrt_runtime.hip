@@ -1153,6 +1153,7 @@ void shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own) {
     }
     const double cp = cost(std::min<int64_t>(rows, tile)), co = cost(std::min<int64_t>(per_item, tile));
     const double share = 1.0 / 256 * (D <= 128 ? 0.7 : 1.0);
+    const double slots = 256.0 * (D == 64 ? 3 : D == 128 ? 2 : 1);
     const bool ragged = !a.joined && a.own_tiles == 1;
     // ranges of an item of t tiles: even ones, or of `per` tiles where items differ
     const auto ranges = [](int64_t t, int64_t per) { return std::max<int64_t>(1, (t + per - 1) / per); };
@@ -1173,7 +1174,8 @@ void shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own) {
                     const double all = hkv * (work + a.pre_tiles * (pre * cp + ps * kUnit)) * share;
                     const double longest = std::max((double)std::min(per, most) * co, a.pre_tiles ? pp * cp : 0.0) + kUnit;
                     const int64_t parts = splits + ps;
-                    double t = std::max(all, longest);
+                    // units that do not run at a time leave a last round part empty
+                    double t = units * hkv + a.pre_tiles * ps * hkv > slots ? all + longest / 2 : std::max(all, longest);
                     if (parts > 1) t += kJoin + (double)rows * hkv * parts * D * 8 / kJoinBytes;
                     if (t < best) best = t, best_pre = ps, best_per = per;
                 }

@@ -62,6 +62,25 @@ __device__ __forceinline__ void settle(f32x4_t &a, f32x4_t &b) {
     asm volatile("s_nop 15" : "+v"(a), "+v"(b));  // 16 states: more than an 8-pass instruction asks for
 }
 
+// x of the lanes before and this one, combined: lane 63 has all of them. Steps within 16
+// lanes and then over them are register moves (DPP); shuffles through LDS take ten times
+// their latency ahead of a workgroup's first load.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or(int none, int x) {
+    return __builtin_amdgcn_update_dpp(none, x, CTRL, ROWS, 0xF, false);
+}
+template <class Op>
+__device__ __forceinline__ int wave_scan(int x, int none, Op op) {
+    x = op(x, dpp_or<0x111, 0xF>(none, x));  // from 1, 2, 4, 8 lanes below in the row of 16
+    x = op(x, dpp_or<0x112, 0xF>(none, x));
+    x = op(x, dpp_or<0x114, 0xF>(none, x));
+    x = op(x, dpp_or<0x118, 0xF>(none, x));
+    x = op(x, dpp_or<0x142, 0xA>(none, x));  // lane 15 to row 1, 47 to row 3
+    x = op(x, dpp_or<0x143, 0xC>(none, x));  // lane 31 to rows 2 and 3
+    return x;
+}
+__device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(x, 63); }
+
 template <int D>
 struct SharedShape {
     static constexpr int STAGES = D == 512 ? 2 : 3;
@@ -76,8 +95,6 @@ struct SharedShape {
     }
 };
 
-// Words that nothing in the launch writes: uniform ones load as scalars.
-typedef const __attribute__((address_space(4))) int32_t *SharedInts;
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 
 // One of the two runs of keys a unit walks: the prefix's or an item's own.
@@ -197,24 +214,14 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
     bool bad = false;
     const uint32_t lds_at = lds_addr(lds);
     const auto *kg = static_cast<const uint16_t *>(a.kv.k), *vg = static_cast<const uint16_t *>(a.kv.v);
-    // PAGED, pages of 16 keys and more: the pages of the next tile's two 16-key halves
-    const bool scalar_pages = LAYOUT == KVRT_LAYOUT_PAGED && a.kv.block_shift >= 4;
-    int id0 = 0, id1 = 0;
+    // PAGED: entry `lane` past win_page of the table of slot win_slot, loaded again where a tile
+    // leaves it (64 pages: every 32 tiles at 16 keys a page)
+    int window = -1, win_slot = -1, win_page = 0;
     auto where = [&](int x, int &key0) __attribute__((always_inline)) -> const Segment & {
         const bool own = x >= u.pre.tiles;
         const Segment &g = own ? u.own : u.pre;
         key0 = (g.tile0 + (own ? x - u.pre.tiles : x)) * kSharedKeys;
         return g;
-    };
-    auto load_ids = [&](int x) __attribute__((always_inline)) {
-        if constexpr (LAYOUT == KVRT_LAYOUT_PAGED) {
-            if (!scalar_pages) return;
-            int key0;
-            const Segment &g = where(x, key0);
-            const SharedInts table = (SharedInts)(uintptr_t)(a.kv.page_table + (int64_t)g.slot * a.kv.pt_stride);
-            id0 = table[min(max(key0, g.lo), g.last) >> a.kv.block_shift];
-            id1 = table[min(max(key0 + 16, g.lo), g.last) >> a.kv.block_shift];
-        }
     };
     auto stage = [&](int x, int buf) __attribute__((always_inline)) {
         int key0;
@@ -224,6 +231,20 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
                                  : (int64_t)g.slot * a.kv.slot_stride + (int64_t)u.kvh * a.kv.head_stride;
         const int ring0 = LAYOUT == KVRT_LAYOUT_RING ? key0 % a.kv.rows : 0;
         const int sub = lane / S::CHUNKS, c = lane % S::CHUNKS;
+        int page0 = 0, page1 = 0;  // of the tile's two halves, where pages hold 16 keys and more
+        if constexpr (LAYOUT == KVRT_LAYOUT_PAGED) {
+            const int p0 = min(max(key0, g.lo), g.last) >> a.kv.block_shift;
+            const int p1 = min(max(key0 + 16, g.lo), g.last) >> a.kv.block_shift;
+            const int end = min(key0 + kSharedKeys - 1, g.last) >> a.kv.block_shift;
+            if (g.slot != win_slot || end - win_page >= 64) {
+                win_slot = g.slot, win_page = p0;
+                window = load_page_window(a.kv, win_slot, win_page, lane);
+            }
+            if constexpr (D < 512) {  // (head_dim 512 has no scalar registers left)
+                page0 = __builtin_amdgcn_readlane(window, p0 - win_page);
+                page1 = __builtin_amdgcn_readlane(window, p1 - win_page);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < S::IPW; ++i) {
             const int ins = 4 * i + wave, r = ins + S::IPB * sub;
@@ -242,8 +263,8 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
                 else rr %= a.kv.rows;
                 off = head + (int64_t)rr * D;
             } else {
-                const int page = scalar_pages ? (r >= 16 ? id1 : id0)
-                                              : a.kv.page_table[(int64_t)g.slot * a.kv.pt_stride + (key >> a.kv.block_shift)];
+                int page = r >= 16 ? page1 : page0;
+                if (D == 512 || a.kv.block_shift < 4) page = __shfl(window, (key >> a.kv.block_shift) - win_page);
                 off = page_row_offset(a.kv, page, u.kvh, key, D);
                 bad |= off < 0;
                 off = off < 0 ? 0 : off;
@@ -397,13 +418,9 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
     constexpr int PER = 2 * S::IPW;  // a wave's DMAs of a tile
     if (n > 0) {
         wait_vmem<0>();  // queries, masks and lengths are in registers
-        load_ids(u.x0);
 #pragma unroll
         for (int i = 0; i < NS - 1; ++i)
-            if (i < n) {
-                stage(u.x0 + i, i);
-                load_ids(u.x0 + min(i + 1, n - 1));
-            }
+            if (i < n) stage(u.x0 + i, i);
         // (add_odd stands outside the loop that all other tiles stay in: beside it in one loop,
         // the accumulators were copied at every tile)
         for (int i = 0, buf = 0;; ++i) {
@@ -411,10 +428,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
             for (; i < n; ++i) {
                 wait_vmem_steps<PER, NS - 2>(n - 1 - i);  // this wave's part of tile i has landed
                 __syncthreads();                          // every wave's has, and tile i - 1 is read
-                if (i + NS - 1 < n) {
-                    stage(u.x0 + i + NS - 1, buf == 0 ? NS - 1 : buf - 1);
-                    load_ids(u.x0 + min(i + NS, n - 1));
-                }
+                if (i + NS - 1 < n) stage(u.x0 + i + NS - 1, buf == 0 ? NS - 1 : buf - 1);
                 if (some) {
                     odd = weigh(u.x0 + i, buf);
                     if (odd) break;
@@ -482,14 +496,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void shared_at
         u.row0 = tile * TILE;
         u.nrows = min(a.n_items * per_item - u.row0, TILE);
         u.part = ks;
-        int lo = u.lens, hi = u.lens;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            lo = min(lo, __shfl_xor(lo, d));
-            hi = max(hi, __shfl_xor(hi, d));
-        }
-        minpos = __builtin_amdgcn_readfirstlane(lo) - a.qn;
-        maxpos = __builtin_amdgcn_readfirstlane(hi) - 1;
+        // (lanes past the items hold the last one's length)
+        minpos = wave_total(wave_scan(u.lens, INT32_MAX, [](int x, int y) { return min(x, y); })) - a.qn;
+        maxpos = wave_total(wave_scan(u.lens, INT32_MIN, [](int x, int y) { return max(x, y); })) - 1;
         u.pre = segment_of(a.prefix_slot, prefix, prefix, minpos, maxpos, a.window);
         u.own = segment_of(a.prefix_slot, 0, 0, 0, -1, 0);
     } else {
@@ -498,28 +507,18 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void shared_at
         if (a.own_per > 0) {
             // sessions of unequal length: each takes a range of own_per tiles after another
             const int t = lane < a.n_items ? segment_of(0, u.lens, 0, u.lens - a.qn, u.lens - 1, a.window).tiles : 0;
-            int per = a.own_per, sum, most;
-            for (bool again = true;; again = false) {
-                sum = lane < a.n_items ? max(1, (t + per - 1) / per) : 0;
-                most = sum;
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const int y = __shfl_up(sum, d);
-                    if (lane >= d) sum += y;
-                    most = max(most, __shfl_xor(most, d));
-                }
-                if (!again || (__builtin_amdgcn_readlane(sum, 63) <= a.own_wgs && most <= a.own_splits)) break;
-                // (more of them than the launch and its partials were made for: a replay on longer
-                // sessions) n sessions take at most total / per + n ranges
-                int all = t, top = t;
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    all += __shfl_xor(all, d);
-                    top = max(top, __shfl_xor(top, d));
-                }
-                const int spare = a.own_wgs - a.n_items;
-                per = max((top + a.own_splits - 1) / a.own_splits, spare > 0 ? (all + spare - 1) / spare : top);
-                per = __builtin_amdgcn_readfirstlane(max(per, 1));
+            const auto add = [](int x, int y) { return x + y; };
+            int per = a.own_per;
+            int mine = lane < a.n_items ? max(1, (t + per - 1) / per) : 0;
+            int sum = wave_scan(mine, 0, add);
+            if (wave_total(sum) > a.own_wgs || __any(mine > a.own_splits)) {
+                // more of them than the launch and its partials were made for (a replay on longer
+                // sessions): n sessions take at most total / per + n ranges
+                const int all = wave_total(wave_scan(t, 0, add)), spare = a.own_wgs - a.n_items;
+                const int top = wave_total(wave_scan(t, 0, [](int x, int y) { return max(x, y); }));
+                per = max(max((top + a.own_splits - 1) / a.own_splits, spare > 0 ? (all + spare - 1) / spare : top), 1);
+                mine = lane < a.n_items ? max(1, (t + per - 1) / per) : 0;
+                sum = wave_scan(mine, 0, add);
             }
             const uint64_t past = __ballot(sum > at);
             if (past == 0) return;
