@@ -36,6 +36,7 @@ struct Api {
     decltype(&kvrt_write_positions_async) write;
     decltype(&kvrt_append_gather_async) gather;
     decltype(&kvrt_attend_tensors_async) tensors;
+    decltype(&kvrt_attend_shared_async) shared;
 } api;
 
 PyObject *talker_mask_type;
@@ -191,6 +192,24 @@ PyObject *attend(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     });
 }
 
+// (ctx, stream, layer, slots, scale, q, out, prefix slot or -1, softcap, slopes or None)
+PyObject *attend_shared(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return guarded(nargs, 10, [&]() -> long {
+        Head h;
+        float scale, cap;
+        int32_t prefix;
+        kvrt_tensor q, o, slopes;
+        const bool biased = a[9] != Py_None;
+        if (!h.read(a) || !read_float(a[4], scale) || !read_tensor(a[5], true, q) || !read_tensor(a[6], false, o) ||
+            !read_int(a[7], prefix) || !read_float(a[8], cap) || (biased && !read_tensor(a[9], true, slopes)) || !h.bind())
+            return kGeneral;
+        return without_gil([&] {
+            return api.shared(h.ctx, h.layer, h.n, h.slots, prefix, &q, &o, scale, cap,
+                              biased ? static_cast<const float *>(slopes.data) : nullptr);
+        });
+    });
+}
+
 // (ctx, stream, layer, slots, scale, q, out, masks)
 PyObject *attend_talker(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     return guarded(nargs, 8, [&]() -> long {
@@ -286,6 +305,18 @@ PyObject *connect(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     api.write = reinterpret_cast<decltype(api.write)>(p[4]);
     api.gather = reinterpret_cast<decltype(api.gather)>(p[5]);
     api.tensors = reinterpret_cast<decltype(api.tensors)>(p[6]);
+    Py_RETURN_NONE;
+}
+
+// (address of kvrt_attend_shared_async): once, after connect
+PyObject *connect_shared(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    void *p = nargs == 1 ? PyLong_AsVoidPtr(a[0]) : nullptr;
+    if (PyErr_Occurred()) return nullptr;
+    if (!p) {
+        PyErr_SetString(PyExc_TypeError, "connect_shared takes one address");
+        return nullptr;
+    }
+    api.shared = reinterpret_cast<decltype(api.shared)>(p);
     Py_RETURN_NONE;
 }
 
@@ -642,6 +673,7 @@ PyMethodDef methods[] = {KVRT_METHOD(append_attend),   KVRT_METHOD(attend),     
                          KVRT_METHOD(connect),         KVRT_METHOD(block_update),  KVRT_METHOD(block_append),
                          KVRT_METHOD(block_gather),    KVRT_METHOD(block_gather_new), KVRT_METHOD(block_attend),
                          KVRT_METHOD(connect_blocks),  KVRT_METHOD(rotate_heads),  KVRT_METHOD(connect_rotate),
+                         KVRT_METHOD(attend_shared),   KVRT_METHOD(connect_shared),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "kvrt_pycall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -110,6 +110,7 @@ def calls():
                lib.kvrt_attend_talker_async, lib.kvrt_write_positions_async, lib.kvrt_append_gather_async,
                lib.kvrt_attend_tensors_async)
         mod.connect(TalkerMask, *(ctypes.cast(f, ctypes.c_void_p).value for f in fns))
+        mod.connect_shared(ctypes.cast(lib.kvrt_attend_shared_async, ctypes.c_void_p).value)
         _calls = mod
     return _calls
 
@@ -577,12 +578,19 @@ class KVRuntime:
                 raise ValueError(f"slopes must be a contiguous fp32 tensor of one slope per query head on {self.device}")
         if prefix_slot is not None and int(prefix_slot) < 0:
             raise ValueError(f"prefix_slot must be a slot or None, got {prefix_slot}")
+        prefix = -1 if prefix_slot is None else int(prefix_slot)
+        slots = slots if type(slots) in (list, tuple) else tuple(slots)
+        o = torch.empty_like(q) if out is None else out
+        rc = self._call.attend_shared(*self._bound(), layer, slots, float(scale), q, o, prefix, float(softcap), slopes)
+        if rc <= 0:
+            _check(rc, "kvrt_attend_shared_async")
+            return o
         q = q.contiguous()
         out = torch.empty_like(q) if out is None else out
         self._bind()
         arr, n = self._slots(slots)
         qd, od = tensor_desc(q), tensor_desc(out)
-        _check(self.lib.kvrt_attend_shared_async(self._ctx, layer, n, arr, -1 if prefix_slot is None else int(prefix_slot),
+        _check(self.lib.kvrt_attend_shared_async(self._ctx, layer, n, arr, prefix,
                                                  ctypes.byref(qd), ctypes.byref(od), float(scale), float(softcap),
                                                  None if slopes is None else slopes.data_ptr()),
                "kvrt_attend_shared_async")
