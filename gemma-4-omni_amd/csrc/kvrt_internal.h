@@ -309,6 +309,15 @@ struct PrefillArgs {
     int32_t slots[kMaxItems];
 };
 
+// The same behind a prefix that the items share (kvrt_attend_shared_async, chunks): item i
+// sees the rows of prefix_slot, then its own. No masks.
+struct SharedChunkArgs : PrefillArgs {
+    int32_t prefix_slot;      // -1: none
+    int32_t capacity;         // lengths are taken as at most this
+    float cap, inv_cap;       // softcap * log2(e) (0: none), scale / softcap
+    const float *slopes;      // [Hq] bias by distance, or null
+};
+
 // Edits lens[idx[i]] = val[i]. With check set (a rollback), all of them or
 // none: only when every lens[idx[i]] still holds expect[i], the value the
 // host validated against; otherwise err[0] is raised and nothing changes.
@@ -399,6 +408,10 @@ hipError_t launch_decode_talker(const TalkerArgs &a, int head_dim, int rows_per_
 hipError_t launch_prefill(const PrefillArgs &a, int head_dim, hipStream_t s);
 hipError_t launch_prefill_wide(const PrefillArgs &a, int head_dim, hipStream_t s);  // head_dim 256, 512
 hipError_t launch_prefill_short(const PrefillArgs &a, int head_dim, hipStream_t s);  // head_dim 64, 128, few keys
+// The merge of a key-split prefill's partials.
+hipError_t launch_prefill_merge(const PrefillArgs &a, int head_dim, hipStream_t s);
+hipError_t launch_shared_chunk(const SharedChunkArgs &a, int head_dim, hipStream_t s);
+hipError_t launch_shared_chunk_wide(const SharedChunkArgs &a, int head_dim, hipStream_t s);  // head_dim 256, 512
 constexpr int kPfKeys = 32;  // keys per staged block of the prefill kernel
 hipError_t launch_set_lens(const SetLenArgs &a, hipStream_t s);
 hipError_t launch_set_pages(int32_t *pt, int n, const int32_t *idx, const int32_t *val,

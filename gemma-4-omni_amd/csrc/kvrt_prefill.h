@@ -154,14 +154,90 @@ struct PrefillShape {
     static_assert(IPB % RW == 0, "a block's DMAs split evenly over its row waves");
 };
 
-template <int D, int LAYOUT, int RW, int KS, int NS>
-__global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
-    using P = PrefillShape<D, RW, KS, NS>;
-    constexpr int KBLK = P::KBLK, VBLK = P::VBLK, IPB = P::IPB, IPW = P::IPW;
+__device__ __forceinline__ int shared_slot(const PrefillArgs &) { return 0; }
+__device__ __forceinline__ int shared_slot(const SharedChunkArgs &a) { return max(a.prefix_slot, 0); }
+
+// One row of a SHARED tile, by one wave without matrix instructions, so that rows of K and V
+// that it does not see do not touch it whatever they hold: keys over lanes for the scores,
+// dims over lanes for the values. It runs where a tile meets NaN or infinities among rows
+// that some of its queries do not see.
+template <int D, int LAYOUT>
+__device__ __forceinline__ void shared_row(const SharedChunkArgs &a, int item, int kvh, int row, int L, int P, int own0,
+                                           int kstart, int kend, int nks, int ks, int lane) {
+    constexpr int E = D / 64;  // dims per lane
+    int qr, hr;
+    udivmod_uniform(row, a.group, qr, hr);
+    const int hq = a.kv.kv_heads * a.group, head = kvh * a.group + hr, slot = a.slots[item];
+    const int pq = L - a.qn + qr, gap = own0 - P;
+    const int64_t orow = ((int64_t)item * hq + head) * a.qn + qr;
+    const uint16_t *q = a.q + orow * D;
+    const auto *kg = static_cast<const uint16_t *>(a.kv.k), *vg = static_cast<const uint16_t *>(a.kv.v);
+    const float slope = a.slopes ? a.slopes[head] * 1.4426950408889634f : 0.f;
+    // element offset of key k's row, -1 where this row does not see it (or its page is unmapped)
+    const auto at = [&](int k) __attribute__((always_inline)) -> int64_t {
+        const bool own = k >= own0;
+        const int pos = own ? pq : pq - gap;
+        if (k >= kend || k > pos || (!own && k >= P) || (a.window > 0 && k <= pos - a.window)) return -1;
+        return row_offset<LAYOUT>(a.kv, own ? slot : shared_slot(a), kvh, own ? k - own0 : k, D);
+    };
+    const auto score = [&](int k, int64_t off) __attribute__((always_inline)) {
+        if (off < 0) return -INFINITY;
+        float x = 0.f;
+#pragma clang loop unroll(disable)
+        for (int d = 0; d < D; ++d) x = fmaf(bf16_to_f32(q[d]), bf16_to_f32(kg[off + d]), x);
+        if (a.cap != 0.f) {
+            float one[1] = {x};
+            cap_scores<1>(one, a.inv_cap, a.cap);
+            x = one[0];
+        } else {
+            x *= a.scale_log2;
+        }
+        return fmaf(slope, (float)(k - (k >= own0 ? pq : pq - gap)), x);
+    };
+    float m = kNegBig, l = 0.f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int k0 = kstart; k0 < kend; k0 += 64) {
+        const int64_t off = at(k0 + lane);
+        const float t = score(k0 + lane, off);
+        const float top = fmaxf(m, group_max<64>(t)), c = __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        const float p = off < 0 ? 0.f : __builtin_amdgcn_exp2f(t - m);
+        l = fmaf(l, c, group_sum<64>(p));
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= c;
+        for (int j = 0; j < min(64, kend - k0); ++j) {
+            const float pj = __shfl(p, j);
+            const int64_t oj = __shfl(off, j);
+            if (oj < 0) continue;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(pj, bf16_to_f32(vg[oj + E * lane + e]), acc[e]);
+        }
+    }
+    if (nks == 1) {
+        const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) a.out[orow * D + E * lane + e] = f32_to_bf16(acc[e] * inv);
+    } else {
+        const int64_t pi = orow * nks + ks;
+#pragma unroll
+        for (int e = 0; e < E; ++e) a.part_o[pi * D + E * lane + e] = acc[e];
+        if (lane == 0) a.part_ml[pi] = make_float2(m, l);
+    }
+}
+
+// SHARED: behind a prefix that the items share, with scores capped and biased
+// (SharedChunkArgs). Keys are numbered as staged: the prefix's P rows from 0, the item's own
+// from own0 = P rounded up to whole blocks, so that a block's rows are of one slot.
+template <int D, int LAYOUT, int RW, int KS, int NS, bool SHARED = false>
+__global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_t<SHARED, SharedChunkArgs, PrefillArgs> a) {
+    using P_ = PrefillShape<D, RW, KS, NS>;
+    constexpr int KBLK = P_::KBLK, VBLK = P_::VBLK, IPB = P_::IPB, IPW = P_::IPW;
     constexpr int NB = D / 32;  // 32-dim blocks of the output
     __shared__ __align__(16) uint8_t sk[NS * KS * KBLK];
     __shared__ __align__(16) uint8_t sv[NS * KS * VBLK];
     __shared__ float2 sml[KS > 1 ? KS * RW * 32 : 1];  // (m, l) of the parts' rows
+    __shared__ int again;                              // SHARED: the tile is to be computed again
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int part = wave / RW, rw = wave % RW;
@@ -176,7 +252,16 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
     const int qb = gridDim.z - 1 - blockIdx.z;
     const int g = a.group, hq = a.kv.kv_heads * g;
     const int slot = a.slots[item];
-    const int L = __builtin_amdgcn_readfirstlane(a.len.lens[(int64_t)slot * a.len.stride + a.len.offset]);
+    int L = __builtin_amdgcn_readfirstlane(a.len.lens[(int64_t)slot * a.len.stride + a.len.offset]);
+    int P = 0, own0 = 0, gap = 0;  // SHARED: rows of the prefix, number of the item's first key, numbers between
+    if constexpr (SHARED) {
+        if (a.prefix_slot >= 0)
+            P = __builtin_amdgcn_readfirstlane(a.len.lens[(int64_t)a.prefix_slot * a.len.stride + a.len.offset]);
+        P = min(max(P, 0), a.capacity);
+        own0 = (P + kPfKeys - 1) / kPfKeys * kPfKeys;
+        gap = own0 - P;
+        L = own0 + min(max(L, 0), a.capacity);
+    }
     int plen;  // prefix-attention mask of the slot
     uint32_t pw;
     load_prefix(a.pmask, slot, lane, plen, pw);
@@ -207,14 +292,24 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
     const int pq = base_pos + qr;
     // the workgroup's keys: from its first query's window to its last query;
     // with a key split, range ks of them in whole blocks
-    const KeyRange range = prefill_range(base_pos, qf, ql, a.window, nks, ks, kPfKeys);
+    const KeyRange range = SHARED ? shared_range(base_pos, qf, ql, a.window, nks, ks, kPfKeys, P, own0)
+                                  : prefill_range(base_pos, qf, ql, a.window, nks, ks, kPfKeys);
     const int kstart = range.kstart, kend = range.kend;
     const int wkend = base_pos + wql + 1;  // the same for this wave's rows
-    const int wkstart = a.window > 0 ? max(0, base_pos + wqf - a.window + 1) : 0;
+    const int wkstart = SHARED ? shared_first_key(base_pos + wqf, a.window, P, own0)
+                        : a.window > 0 ? max(0, base_pos + wqf - a.window + 1) : 0;
     const int ngroups = (kend - kstart + kPfKeys * KS - 1) / (kPfKeys * KS);  // <= 0: no keys, nothing is fetched
     // keys this lane's row sees: [klo, khi] (none if the lane has no row)
     const int khi = qvalid ? min(kend - 1, pq) : -1;
     const int klo = a.window > 0 ? pq - a.window + 1 : 0;
+    // SHARED: scores that are capped or biased are made one by one, in log2 units
+    bool made = false;
+    float slope = 0.f;
+    if constexpr (SHARED) {
+        made = a.cap != 0.f || a.slopes;
+        if (a.slopes) slope = a.slopes[kvh * g + hr] * 1.4426950408889634f;
+        asm volatile("" : "+v"(slope));  // loaded ahead of the first DMA
+    }
 
     float m = kNegBig, l = 0.f;  // running max (both halves alike) and this lane's partial sum
     f32x16_t o[NB];
@@ -233,6 +328,9 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
     const int64_t head_base = LAYOUT == KVRT_LAYOUT_PAGED
                                   ? 0
                                   : (int64_t)slot * a.kv.slot_stride + (int64_t)kvh * a.kv.head_stride;
+    const int64_t pre_base = !SHARED || LAYOUT == KVRT_LAYOUT_PAGED
+                                 ? 0
+                                 : (int64_t)shared_slot(a) * a.kv.slot_stride + (int64_t)kvh * a.kv.head_stride;
     const uint32_t sk_a = lds_addr(sk), sv_a = lds_addr(sv);
     const int lrow = IPB * (lane / (D / 8)) + rw;  // this lane's row of its wave's first instruction
     const uint32_t vchunk = lane % (D / 8) * 16, kchunk = vchunk ^ (uint32_t)(16 * pf_kx<D>(lane / (D / 8)));
@@ -250,6 +348,12 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
     // PAGED: the entries of the pages from the block at key t on; loaded a group
     // ahead, so that no DMA waits for them
     auto load_pages = [&](int t) __attribute__((always_inline)) {
+        if constexpr (SHARED) {
+            const int t0 = min(t, kend - 1);
+            const bool own = t0 >= own0;
+            return load_page_window(a.kv, own ? slot : shared_slot(a), (own ? t0 - own0 : min(t0, P - 1)) >> a.kv.block_shift,
+                                    lane);
+        }
         return load_page_window(a.kv, slot, min(t, kend - 1) >> a.kv.block_shift, lane);
     };
     int pages = 0;  // of the block at kt
@@ -258,6 +362,18 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
     auto next_fetch = [&]() __attribute__((always_inline)) {
         const int t0 = min(kt, kend - 1);
         Fetch f;
+        if constexpr (SHARED) {
+            const bool own = t0 >= own0;
+            const int key = own ? t0 - own0 : min(t0, P - 1);  // in its slot
+            f.off = own ? head_base : pre_base;
+            if constexpr (LAYOUT == KVRT_LAYOUT_CONTIG) f.off += (int64_t)key * D;
+            f.r0 = LAYOUT == KVRT_LAYOUT_RING ? key % a.kv.rows : key;
+            f.last = own ? kend - 1 - t0 : min(kend, P) - 1 - key;
+            f.pages = pages;
+            kt += kPfKeys * KS;
+            if constexpr (LAYOUT == KVRT_LAYOUT_PAGED) pages = load_pages(kt);
+            return f;
+        }
         f.off = head_base;
         f.r0 = t0;
         f.last = kend - 1 - t0;
@@ -308,7 +424,7 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
     // A negative scale is moved into q's sign bits (exact, below), so that the
     // largest score always has the largest product; a zero scale stays above 0,
     // so that a masked score (-INFINITY) keeps its weight of 0.
-    const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);
+    const float scale = made ? 1.f : fmaxf(fabsf(a.scale_log2), 1e-37f);
     const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
 
     // ---- operands: A of S^T is key row col, chunk 2c + half; A of V^T is dims
@@ -403,9 +519,38 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
     // keys every row of the wave sees: blocks inside take no per-key test
     const int vis_hi = min(kend, base_pos + wqf + 1);
     const int vis_lo = max(plen, a.window > 0 ? base_pos + wql - a.window + 1 : 0);
-    // Masks the scores of keys t0 .. t0 + 31 (-INFINITY).
+    // Makes capped and biased scores of the products with keys t0 .. t0 + 31.
+    auto make = [&](int t0) __attribute__((always_inline)) {
+        if constexpr (SHARED) {
+            if (!made) return;
+            if (a.cap != 0.f) {
+                cap_scores<16>(s, fabsf(a.inv_cap), a.cap);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] *= fabsf(a.scale_log2);
+            }
+            if (a.slopes) {
+                const float far = (float)(t0 + 4 * half - (t0 < own0 ? pq - gap : pq));
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = fmaf(slope, far + (float)(8 * (i >> 2) + (i & 3)), s[i]);
+            }
+        }
+    };
+    // Masks the scores of keys t0 .. t0 + 31 (-INFINITY); SHARED: whether there was one to mask.
     auto mask = [&](int t0) __attribute__((always_inline)) {
-        if (t0 >= vis_lo && t0 + kPfKeys <= vis_hi) return;
+        if constexpr (SHARED) {
+            const bool pre = t0 < own0;
+            const int sh = pre ? gap : 0, end = pre ? min(kend, P) : kend;
+            if (t0 >= vis_lo - sh && t0 + kPfKeys <= min(end, vis_hi - sh)) return false;
+            const int hi = min(end - 1, qvalid ? pq - sh : -1), lo = a.window > 0 ? klo - sh : 0;
+            const int nhi = min(max(hi - t0 + 1, 0), 32), nlo = min(max(lo - t0, 0), 32);
+            uint32_t vis = (nhi >= 32 ? 0xffffffffu : (1u << nhi) - 1u) & (nlo >= 32 ? 0u : 0xffffffffu << nlo);
+            vis >>= 4 * half;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = (vis >> (8 * (i >> 2) + (i & 3))) & 1u ? s[i] : -INFINITY;
+            return true;
+        }
+        if (t0 >= vis_lo && t0 + kPfKeys <= vis_hi) return false;
         // bit k: key t0 + k is visible to this lane's row
         const int nhi = min(max(khi - t0 + 1, 0), 32), nlo = min(max(klo - t0, 0), 32);
         uint32_t vis = (nhi >= 32 ? 0xffffffffu : (1u << nhi) - 1u) & (nlo >= 32 ? 0u : 0xffffffffu << nlo);
@@ -419,6 +564,27 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
         vis >>= 4 * half;  // this half's keys: bit 8 (i / 4) + i % 4
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = (vis >> (8 * (i >> 2) + (i & 3))) & 1u ? s[i] : -INFINITY;
+        return true;
+    };
+    // SHARED: a block that some rows do not see whole, whose V holds NaN or infinities (0 * NaN
+    // is not 0): the tile is then computed again, row by row.
+    bool partly = false;  // the block whose P V is next
+    uint32_t odd = 0;
+    auto look = [&](int vblk) __attribute__((always_inline)) {
+        if constexpr (SHARED) {
+            if (!partly) return;
+            typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+            u16x2_t most = {0, 0};
+#pragma clang loop unroll_count(4)
+            for (int i = 0; i < IPB; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(&sv[vblk * VBLK + i * kPfVPitch + 16 * lane]);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, w[e] & 0x7fff7fffu));
+            }
+            odd |= most[0] >= 0x7f80 || most[1] >= 0x7f80 ? 1u : 0u;
+        }
     };
     // The softmax of s in NSOFT steps. The running max moves only where a
     // block's max exceeds it by kRescaleSlack; corr rescales what has been
@@ -517,7 +683,8 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
         __syncthreads();
         if (jlo == 0 && jhi > 0) {
             score_steps(part, 0, std::true_type{});
-            mask(key0(0));
+            make(key0(0));
+            partly = mask(key0(0));
             StaticFor<0, NSOFT>::run(soft_step);
             take_p();
         }
@@ -532,9 +699,11 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
             cur = it;
             const bool do_s = it + 1 >= jlo && it + 1 < jhi, do_v = it >= jlo && it < jhi;
             const int kblk = ((it + 1) % NS) * KS + part, vblk = (it % NS) * KS + part;
+            if (do_v) look(vblk);
             if (do_s) {
                 score_steps(kblk, vblk, std::false_type{});
-                mask(key0(it + 1));
+                make(key0(it + 1));
+                partly = mask(key0(it + 1));
             } else {
                 if (it + 1 < ngroups) StaticFor<0, NK>::run(dma_at);
 #pragma unroll
@@ -558,6 +727,17 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) keep_acc<D>(o[b]);
     if (bad) a.err[0] = 1;
+    if constexpr (SHARED) {
+        if (threadIdx.x == 0) again = 0;
+        __syncthreads();  // (and every wave is done with the buffers)
+        if (odd) again = 1;
+        __syncthreads();
+        if (again) {
+            for (int row = wg0 + wave; row < min(R, wg0 + RW * 32); row += P_::NW)
+                shared_row<D, LAYOUT>(a, item, kvh, row, L, P, own0, kstart, kend, nks, ks, lane);
+            return;
+        }
+    }
     l = pair<OpSum, 32>(l);
 
     // this lane's row again (from here on: keeping it over the loop would cost
@@ -621,7 +801,7 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
         // store a share of the dims, in part order. The buffers take BS
         // 32-dim blocks of all waves at a time.
         constexpr int BS = NS * D / (32 * RW) < NB ? NS * D / (32 * RW) : NB;
-        static_assert(BS >= 1 && NB % BS == 0 && BS * P::NW * 2048 <= NS * KS * KBLK, "blocks fit the buffers");
+        static_assert(BS >= 1 && NB % BS == 0 && BS * P_::NW * 2048 <= NS * KS * KBLK, "blocks fit the buffers");
         if (ehalf == 0) sml[wave * 32 + col] = make_float2(m, l);
         __syncthreads();  // also: every wave is done with the buffers
         float M = kNegBig, Lsum = 0.f;
@@ -635,7 +815,7 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
         float w = __builtin_amdgcn_exp2f(m - M);
         if (nks == 1) w *= Lsum > 0.f ? 1.0f / Lsum : 0.f;
         // [wave][block][group i][lane], the waves' first halves in sk, the second in sv
-        constexpr int WHALF = P::NW / 2;
+        constexpr int WHALF = P_::NW / 2;
         auto xo = [&](int wv) __attribute__((always_inline)) {
             return reinterpret_cast<float4 *>(wv < WHALF ? sk : sv) + (wv % WHALF) * BS * 256 + lane;
         };
@@ -679,16 +859,16 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(PrefillArgs a) {
     }
 }
 
-template <int D, int RW, int KS, int NS, int LAYOUT>
-static hipError_t launch_prefill_layout(const PrefillArgs &a, hipStream_t s) {
+template <int D, int RW, int KS, int NS, int LAYOUT, class Args>
+static hipError_t launch_prefill_layout(const Args &a, hipStream_t s) {
     const int64_t rows = (int64_t)a.group * a.qn;
     const dim3 grid(a.n_ksplit * a.kv.kv_heads, a.n_items, (unsigned)((rows + 32 * RW - 1) / (32 * RW)));
-    hipLaunchKernelGGL((prefill_kernel<D, LAYOUT, RW, KS, NS>), grid, dim3(64 * RW * KS), 0, s, a);
+    hipLaunchKernelGGL((prefill_kernel<D, LAYOUT, RW, KS, NS, std::is_same_v<Args, SharedChunkArgs>>), grid, dim3(64 * RW * KS), 0, s, a);
     return hipGetLastError();
 }
 
-template <int D, int RW, int KS, int NS>
-static hipError_t launch_prefill_shape(const PrefillArgs &a, hipStream_t s) {
+template <int D, int RW, int KS, int NS, class Args>
+static hipError_t launch_prefill_shape(const Args &a, hipStream_t s) {
     switch (a.kv.layout) {
         case KVRT_LAYOUT_CONTIG: return launch_prefill_layout<D, RW, KS, NS, KVRT_LAYOUT_CONTIG>(a, s);
         case KVRT_LAYOUT_RING: return launch_prefill_layout<D, RW, KS, NS, KVRT_LAYOUT_RING>(a, s);

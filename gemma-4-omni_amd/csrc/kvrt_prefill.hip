@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a, int D
 }
 
 // The key-split merge: (item, q head, query) rows x D / 4 threads.
-static hipError_t launch_prefill_merge(const PrefillArgs &a, int head_dim, hipStream_t s) {
+hipError_t launch_prefill_merge(const PrefillArgs &a, int head_dim, hipStream_t s) {
     if (head_dim < 4 || (head_dim & (head_dim - 1)) != 0) return hipErrorInvalidValue;
     int dshift = 0;
     while ((1 << dshift) < head_dim / 4) ++dshift;

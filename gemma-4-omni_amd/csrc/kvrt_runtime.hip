@@ -1120,11 +1120,124 @@ int tensor_call_launch(TensorCall &tc, float *ws, hipStream_t st, bool single) {
     return KVRT_OK;
 }
 
+// Shape of a chunk's launch (PrefillArgs): n items of qn queries, `group` heads per KV head,
+// any 16 of which see at most block_keys keys. plain: the 16-query kernel may take it.
+int prefill_shape(kvrt_ctx *c, PrefillArgs &a, const kvrt_layer_spec &s, int64_t qn, int64_t block_keys, bool plain) {
+    const int D = s.head_dim, hkv = s.kv_heads, n = a.n_items, group = a.group;
+    const int64_t hq = (int64_t)group * hkv;
+    // Shape of the launch: row_waves 32-row blocks x key_parts per workgroup and
+    // key ranges per row block. A chunk's time is the chain of key blocks one
+    // wave walks (about 1.1 us a block at head_dim 256, 2 us at 512, 0.5 us
+    // below), so the smaller the grid, the more waves share a row block's keys,
+    // first inside a workgroup (combined through LDS), then over workgroups
+    // (partials in the workspace and a merge launch, ~6 us).
+    static const int ksplit_env = env_int("KVRT_PF_KSPLIT", 0);
+    const int64_t rows = (int64_t)group * qn;
+    const auto wgs = [&](int w) { return (rows + 32 * w - 1) / (32 * w) * hkv * n; };  // workgroups of w row blocks
+    int rw = 4, parts = 1;
+    // least keys of a key range, and least keys that a split has to take off a
+    // workgroup's walk to be worth its merge (head_dim 512: one row block's
+    // accumulators fill the AGPRs and two staged groups the LDS: no parts)
+    int min_keys = 96, split_keys = 120;
+    if (D == 256) {
+        // a workgroup's 137 KB of LDS leave one per CU: past two rounds of
+        // them (without a window their lengths differ and the rounds overlap)
+        // four row blocks per workgroup and no parts are faster (window 512, 3
+        // streams x Q 1200: 44.6 -> 32.7 us; 4 x Q 600: 23.8 against 29.6 us);
+        // so are they where two parts would not have a block each
+        if (block_keys > 64 && wgs(2) <= (s.window > 0 ? 384 : 512)) rw = 2, parts = 2;
+        min_keys = 80, split_keys = 400;
+    } else if (D <= 128 && s.layout == KVRT_LAYOUT_PAGED) {
+        // A row's address costs a lane more than its DMA: two row blocks share
+        // the fetching, and a split pays with half the keys. Few keys take no
+        // more parts than they have blocks (Hq 16 x Q 12 over 12: 4.6 us, two
+        // parts 5.5, four 5.7; Q 40 over 60: 6.4, four parts 7.2; over 220:
+        // 11.1, two parts 11.2).
+        if (block_keys <= 32) rw = 4, parts = 1;
+        else if (wgs(2) < 256) rw = 2, parts = block_keys <= 160 ? 2 : 4;
+        else if (wgs(4) < 512) rw = 2, parts = 2;
+        min_keys = 180, split_keys = 250;
+    } else if (D <= 128) {
+        // Few keys: 16-query tiles (kvrt_prefill_short.hip), whose chain per
+        // tile is half as long. 16-query tiles against the shape chosen below,
+        // us (graph replays, warm rows):
+        // up to one round of row blocks, D 128: Q 64 over 64 4.2 and 5.3, over
+        // 164 5.8 and 6.9; Q 40 over 300 7.4 and 7.7, over 400 9.3 and 8.3
+        // (more than one 16-query workgroup per CU: 8 heads of their own, 2 x
+        // Q 300 over 300, 8.1 and 7.8).
+        // Three or four heads of a group fill a workgroup's eight waves and the
+        // line lies lower: 3 heads x Q 40 over 150 6.6 and 7.1, over 200 7.4
+        // and 7.0; 4 heads over 40 4.9 and 5.2, over 100 5.9 and 5.7.
+        // D 64: Q 40 over 150 4.4 and 5.3, over 220 5.0 and 5.2.
+        // In a second round (4 x Q 200): over 300 8.7 and 9.5, over 550 11.9 and
+        // 12.5; D 64 over 400 7.3 and 8.1.
+        // Beyond, while the 16-query grid is at most four workgroups per CU: 16
+        // x Q 100 over 160 10.7 and 10.9, over 320 14.5 and 14.1; past that (32
+        // x Q 100 over 100) 15.0 and 11.1.
+        int heads = 1;  // q heads of a workgroup
+        for (int h = 2; h <= std::min(group, 4); ++h)
+            if (group % h == 0) heads = h;
+        const int64_t blocks = wgs(1), wgs16 = (qn + 15) / 16 * hkv * (group / heads) * n;
+        int short_keys = 0;
+        if (D == 128 && blocks <= 256) short_keys = heads == 3 ? 160 : heads > 3 ? 64 : wgs16 <= 256 ? 320 : 208;
+        else if (D == 128 && blocks <= 512) short_keys = heads <= 2 ? 576 : 320;
+        else if (D == 128) short_keys = wgs16 <= 1024 ? 224 : 0;
+        else if (blocks <= 256) short_keys = heads <= 3 ? 160 : 64;
+        else if (blocks <= 512 && heads <= 2) short_keys = 416;
+        if (plain && block_keys <= short_keys && ksplit_env < 2) {
+            a.short_heads = heads;
+            // two query blocks on the same tiles from two workgroups per CU on
+            const bool pair = wgs16 >= 512;
+            rw = pair ? 2 : 1;
+            parts = pair && heads > 2 ? 1 : 2;
+        } else if (blocks <= (D == 64 ? 512 : 256)) {
+            // four parts while one round of workgroups (at D 64 two per CU)
+            // takes the grid (Hq 16, one stream x Q 512: 8.8 us, two parts
+            // 10.9; D 64 x Q 450, 2 streams, 7.6 and 8.6)
+            rw = 1, parts = 4;
+        } else if (D == 128 && wgs(2) < 256) {
+            // (3 streams x Q 274 over 947: 16.9 us, two parts 17.4)
+            rw = 2, parts = 4;
+        } else if (wgs(4) < 512) {
+            // two parts up to two rounds of four row blocks (4 x Q 512: 15.4
+            // us, four parts 20.4), none beyond (4 x Q 1400: 98.7 us, two
+            // parts 102.6)
+            rw = 2, parts = 2;
+        }
+        min_keys = 160, split_keys = 500;
+    }
+    a.row_waves = rw;
+    a.key_parts = parts;
+    // Key ranges: as many as keep the grid within one round of 256 workgroups
+    // (Q 291 at head_dim 512 over 2339 keys, 4 streams: 156 us unsplit, 99 / 87 /
+    // 121 us with 2 / 3 / 4 ranges). Not inside a capture that would need a
+    // larger workspace. KVRT_PF_KSPLIT=1 turns it off, n >= 2 forces n ranges.
+    a.n_ksplit = 1;
+    const int64_t want = ksplit_env > 0 ? ksplit_env : std::min<int64_t>(256 / wgs(rw), block_keys / min_keys);
+    const int nks = (int)std::min<int64_t>(want, 16);
+    if (nks > 1 && !a.short_heads && (ksplit_env > 0 || block_keys * (nks - 1) / nks >= split_keys)) {
+        const size_t po = ((size_t)n * hq * qn * nks * D + 63) / 64 * 64;
+        const size_t bytes = po * 4 + (size_t)n * hq * qn * nks * 8 + 256;
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        const bool capturing = hipStreamIsCapturing(c->stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
+        if (bytes <= c->ws_bytes || (!capturing && ensure_workspace(c, bytes) == KVRT_OK)) {
+            a.n_ksplit = nks;
+            a.part_o = c->ws;
+            a.part_ml = reinterpret_cast<float2 *>(c->ws + po);
+        }
+        if (c->poisoned) return KVRT_EDEVICE;
+    }
+    return KVRT_OK;
+}
+
 // Limits of shared-prefix attention: positions of a prefix and a session together stay
 // below 2^31, and so do rows, and a launch's threads below 2^32 (two key ranges for each
 // of the fewest rows of a tile, 256 threads each).
 constexpr int kMaxSharedCapacity = 1 << 29;
 constexpr int64_t kMaxSharedRows = 1 << 22;
+// Rows of an item and KV head from which its workgroups read the prefix for themselves: its
+// tile is as good as full without other items' rows.
+constexpr int64_t kJoinRows = 64;
 
 // How a call's rows and keys are divided (SharedArgs): pre_keys of the prefix are seen, and
 // own[i] of item i's rows. The shortest time of a simple model is taken: a launch lasts as
@@ -1143,7 +1256,7 @@ void shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own) {
     };
     constexpr double kUnit = 1.5, kJoin = 4.5, kJoinBytes = 3e6;  // us, us, bytes a us
     a.own_tiles = (int)((per_item + tile - 1) / tile);
-    a.joined = a.prefix_slot >= 0 && (pre_keys == 0 || per_item >= 64);
+    a.joined = a.prefix_slot >= 0 && (pre_keys == 0 || per_item >= kJoinRows);
     a.pre_tiles = a.prefix_slot < 0 || a.joined ? 0 : (int)((rows + tile - 1) / tile);
     const int64_t pre = tiles_of(pre_keys);
     int64_t items[kMaxItems], most = 1;
@@ -2209,115 +2322,15 @@ int kvrt_attend_prefill_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32
     a.group = group;
     a.qn = (int)qn;
     a.window = s.window;
-    // Shape of the launch: row_waves 32-row blocks x key_parts per workgroup and
-    // key ranges per row block. A chunk's time is the chain of key blocks one
-    // wave walks (about 1.1 us a block at head_dim 256, 2 us at 512, 0.5 us
-    // below), so the smaller the grid, the more waves share a row block's keys,
-    // first inside a workgroup (combined through LDS), then over workgroups
-    // (partials in the workspace and a merge launch, ~6 us).
-    static const int ksplit_env = env_int("KVRT_PF_KSPLIT", 0);
-    const int64_t rows = (int64_t)group * qn;
-    const auto wgs = [&](int w) { return (rows + 32 * w - 1) / (32 * w) * hkv * n; };  // workgroups of w row blocks
-    int rw = 4, parts = 1;
-    // least keys of a key range, and least keys that a split has to take off a
-    // workgroup's walk to be worth its merge (head_dim 512: one row block's
-    // accumulators fill the AGPRs and two staged groups the LDS: no parts)
-    int min_keys = 96, split_keys = 120;
-    if (D == 256) {
-        // a workgroup's 137 KB of LDS leave one per CU: past two rounds of
-        // them (without a window their lengths differ and the rounds overlap)
-        // four row blocks per workgroup and no parts are faster (window 512, 3
-        // streams x Q 1200: 44.6 -> 32.7 us; 4 x Q 600: 23.8 against 29.6 us);
-        // so are they where two parts would not have a block each
-        if (block_keys > 64 && wgs(2) <= (s.window > 0 ? 384 : 512)) rw = 2, parts = 2;
-        min_keys = 80, split_keys = 400;
-    } else if (D <= 128 && s.layout == KVRT_LAYOUT_PAGED) {
-        // A row's address costs a lane more than its DMA: two row blocks share
-        // the fetching, and a split pays with half the keys. Few keys take no
-        // more parts than they have blocks (Hq 16 x Q 12 over 12: 4.6 us, two
-        // parts 5.5, four 5.7; Q 40 over 60: 6.4, four parts 7.2; over 220:
-        // 11.1, two parts 11.2).
-        if (block_keys <= 32) rw = 4, parts = 1;
-        else if (wgs(2) < 256) rw = 2, parts = block_keys <= 160 ? 2 : 4;
-        else if (wgs(4) < 512) rw = 2, parts = 2;
-        min_keys = 180, split_keys = 250;
-    } else if (D <= 128) {
-        // Few keys: 16-query tiles (kvrt_prefill_short.hip), whose chain per
-        // tile is half as long. 16-query tiles against the shape chosen below,
-        // us (graph replays, warm rows):
-        // up to one round of row blocks, D 128: Q 64 over 64 4.2 and 5.3, over
-        // 164 5.8 and 6.9; Q 40 over 300 7.4 and 7.7, over 400 9.3 and 8.3
-        // (more than one 16-query workgroup per CU: 8 heads of their own, 2 x
-        // Q 300 over 300, 8.1 and 7.8).
-        // Three or four heads of a group fill a workgroup's eight waves and the
-        // line lies lower: 3 heads x Q 40 over 150 6.6 and 7.1, over 200 7.4
-        // and 7.0; 4 heads over 40 4.9 and 5.2, over 100 5.9 and 5.7.
-        // D 64: Q 40 over 150 4.4 and 5.3, over 220 5.0 and 5.2.
-        // In a second round (4 x Q 200): over 300 8.7 and 9.5, over 550 11.9 and
-        // 12.5; D 64 over 400 7.3 and 8.1.
-        // Beyond, while the 16-query grid is at most four workgroups per CU: 16
-        // x Q 100 over 160 10.7 and 10.9, over 320 14.5 and 14.1; past that (32
-        // x Q 100 over 100) 15.0 and 11.1.
-        int heads = 1;  // q heads of a workgroup
-        for (int h = 2; h <= std::min(group, 4); ++h)
-            if (group % h == 0) heads = h;
-        const int64_t blocks = wgs(1), wgs16 = (qn + 15) / 16 * hkv * (group / heads) * n;
-        int short_keys = 0;
-        if (D == 128 && blocks <= 256) short_keys = heads == 3 ? 160 : heads > 3 ? 64 : wgs16 <= 256 ? 320 : 208;
-        else if (D == 128 && blocks <= 512) short_keys = heads <= 2 ? 576 : 320;
-        else if (D == 128) short_keys = wgs16 <= 1024 ? 224 : 0;
-        else if (blocks <= 256) short_keys = heads <= 3 ? 160 : 64;
-        else if (blocks <= 512 && heads <= 2) short_keys = 416;
-        if (block_keys <= short_keys && ksplit_env < 2) {
-            a.short_heads = heads;
-            // two query blocks on the same tiles from two workgroups per CU on
-            const bool pair = wgs16 >= 512;
-            rw = pair ? 2 : 1;
-            parts = pair && heads > 2 ? 1 : 2;
-        } else if (blocks <= (D == 64 ? 512 : 256)) {
-            // four parts while one round of workgroups (at D 64 two per CU)
-            // takes the grid (Hq 16, one stream x Q 512: 8.8 us, two parts
-            // 10.9; D 64 x Q 450, 2 streams, 7.6 and 8.6)
-            rw = 1, parts = 4;
-        } else if (D == 128 && wgs(2) < 256) {
-            // (3 streams x Q 274 over 947: 16.9 us, two parts 17.4)
-            rw = 2, parts = 4;
-        } else if (wgs(4) < 512) {
-            // two parts up to two rounds of four row blocks (4 x Q 512: 15.4
-            // us, four parts 20.4), none beyond (4 x Q 1400: 98.7 us, two
-            // parts 102.6)
-            rw = 2, parts = 2;
-        }
-        min_keys = 160, split_keys = 500;
-    }
-    a.row_waves = rw;
-    a.key_parts = parts;
-    // Key ranges: as many as keep the grid within one round of 256 workgroups
-    // (Q 291 at head_dim 512 over 2339 keys, 4 streams: 156 us unsplit, 99 / 87 /
-    // 121 us with 2 / 3 / 4 ranges). Not inside a capture that would need a
-    // larger workspace. KVRT_PF_KSPLIT=1 turns it off, n >= 2 forces n ranges.
-    a.n_ksplit = 1;
-    const int64_t want = ksplit_env > 0 ? ksplit_env : std::min<int64_t>(256 / wgs(rw), block_keys / min_keys);
-    const int nks = (int)std::min<int64_t>(want, 16);
-    if (nks > 1 && !a.short_heads && (ksplit_env > 0 || block_keys * (nks - 1) / nks >= split_keys)) {
-        const size_t po = ((size_t)n * hq * qn * nks * D + 63) / 64 * 64;
-        const size_t bytes = po * 4 + (size_t)n * hq * qn * nks * 8 + 256;
-        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-        const bool capturing = hipStreamIsCapturing(c->stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
-        if (bytes <= c->ws_bytes || (!capturing && ensure_workspace(c, bytes) == KVRT_OK)) {
-            a.n_ksplit = nks;
-            a.part_o = c->ws;
-            a.part_ml = reinterpret_cast<float2 *>(c->ws + po);
-        }
-        if (c->poisoned) return KVRT_EDEVICE;
-    }
+    rc = prefill_shape(c, a, s, qn, block_keys, true);
+    if (rc != KVRT_OK) return rc;
     a.pmask = launch_masks(c, n, slots);
     a.scale_log2 = scale * 1.4426950408889634f;
     for (int i = 0; i < n; ++i) a.slots[i] = slots[i];
     c->counters.launches += a.n_ksplit > 1 ? 2 : 1;
     if (launch_prefill(a, D, enq(c)) != hipSuccess) return poison(c);
-    // keys its workgroups read: those of 32 rw rows, or of rw 16-query blocks by short_heads heads
-    const int64_t wg_rows = a.short_heads ? 16 * rw : 32 * rw, per_query = a.short_heads ? 1 : group;
+    // keys its workgroups read: those of 32 row_waves rows, or of row_waves 16-query blocks by short_heads heads
+    const int64_t wg_rows = (a.short_heads ? 16 : 32) * a.row_waves, per_query = a.short_heads ? 1 : group;
     uint64_t keys = 0;
     for (int i = 0; i < n; ++i)
         for (int64_t r0 = 0; r0 < qn * per_query; r0 += wg_rows) {
@@ -2354,6 +2367,7 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
         if (out->dims[i] != q->dims[i]) return KVRT_EINVAL;
     // rows are numbered in 32 bits, as are a launch's threads
     if (hq > INT32_MAX / qn || n * hq * qn > kMaxSharedRows) return KVRT_EINVAL;
+    const int64_t per_item = hq / hkv * qn;
     if (!std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap) ||
         reinterpret_cast<uintptr_t>(slopes) % 4 != 0)
         return KVRT_EINVAL;
@@ -2404,6 +2418,39 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
     a.capacity = cap;
     a.prefix_slot = prefix_slot;
     for (int i = 0; i < n; ++i) a.slots[i] = slots[i];
+    if (!a.pmask && per_item > 16 && (!shared || per_item >= kJoinRows) &&
+        !(s.layout == KVRT_LAYOUT_RING && s.ring_rows < kPfKeys)) {
+        // many rows of each item: the prefill's tiles
+        SharedChunkArgs p{};
+        p.kv = a.kv;
+        p.len = a.len;
+        p.q = a.q;
+        p.out = a.out;
+        p.err = a.err;
+        p.n_items = n;
+        p.group = a.group;
+        p.qn = a.qn;
+        p.window = window;
+        p.scale_log2 = a.scale;
+        p.prefix_slot = prefix_slot;
+        p.capacity = cap;
+        p.cap = a.cap;
+        p.inv_cap = a.inv_cap;
+        p.slopes = slopes;
+        for (int i = 0; i < n; ++i) p.slots[i] = slots[i];
+        int64_t keys = 0;  // most keys that any 16 queries see
+        for (int i = 0; i < n; ++i) keys = std::max<int64_t>(keys, own_keys[i]);
+        keys += pre_keys;
+        if (window > 0) keys = std::min<int64_t>(keys, window + 15);
+        rc = prefill_shape(c, p, s, qn, keys, false);
+        if (rc != KVRT_OK) return rc;
+        c->counters.launches += p.n_ksplit > 1 ? 2 : 1;
+        if (launch_shared_chunk(p, D, enq(c)) != hipSuccess) return poison(c);
+        const uint64_t read = ((uint64_t)pre_keys * n + all_own) * ((per_item + 32 * p.row_waves - 1) / (32 * p.row_waves)) * hkv;
+        c->counters.attended_keys += read;
+        c->counters.attended_bytes += read * (uint64_t)D * 2 * 2;
+        return KVRT_OK;
+    }
     shared_plan(a, D, pre_keys, own_keys);
     const auto bytes = [&] {
         const size_t rows = (size_t)n * hq * qn * a.parts;

@@ -122,16 +122,6 @@ __device__ __forceinline__ Segment segment_of(int slot, int len, int off, int mi
     return s;
 }
 
-// cap * tanh(y): by an exponential, below 1/4 (where that would cancel) by the series,
-// whose next term is 2^-21 of the value there.
-__device__ __forceinline__ float capped(float y, float cap) {
-    const float e = __builtin_amdgcn_exp2f(y * 2.8853900817779268f);  // e^(2y)
-    const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
-    const float y2 = y * y;
-    const float small = y * fmaf(y2, fmaf(y2, fmaf(y2, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
-    return cap * (fabsf(y) < 0.25f ? small : big);
-}
-
 // A unit's work: tiles [x0, x1) of its list (the prefix's tiles, then its own), rows row0
 // .. row0 + nrows - 1 of the call's (item, query, head) order, KV head kvh.
 struct SharedUnit {
@@ -323,16 +313,17 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
 #pragma unroll
             for (int i = 0; i < 8; ++i) t[i] = sc[s][i / 4][i % 4];
             if (made) {
-                const float by = a.cap != 0.f ? fabsf(a.inv_cap) : fabsf(a.scale);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] *= by;
                 if (a.cap != 0.f) {
+                    cap_scores<8>(t, fabsf(a.inv_cap), a.cap);
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) t[i] = capped(t[i], a.cap);
+                    for (int i = 0; i < 8; ++i) t[i] *= fabsf(a.scale);
                 }
-                const float far = (float)(key0 + 4 * grp - at);  // below 2^24 in earnest, and rounded beyond
+                if (a.slopes) {
+                    const float far = (float)(key0 + 4 * grp - at);  // below 2^24 in earnest, and rounded beyond
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t[i] = fmaf(slope[s], far + (float)(16 * (i / 4) + i % 4), t[i]);
+                    for (int i = 0; i < 8; ++i) t[i] = fmaf(slope[s], far + (float)(16 * (i / 4) + i % 4), t[i]);
+                }
             }
             if (!whole) {
                 // bit k: key0 + k is seen by this row

@@ -159,6 +159,31 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
+// cap * tanh(y) of N scores' products x, y = by * x, cap in log2 units: cap - 2 cap / (e^2y + 1).
+// Near 0 that cancels: it is off by up to cap * 2^-22 (2^-24 of e, times 1/2, 2^-23 of the
+// reciprocal, the roundings). Up to kSmallCap that is 2^-16 of a weight, a 128th of the answer's
+// rounding; above, scores below cap / 4 take the series, whose next term is 2^-21 of the
+// value there. (The series costs as much again: a chunk of 2 x 291 queries, 8 heads of 128
+// over 2000 keys, capped: 33.5 us with it for every cap, without KVAR.)
+constexpr float kSmallCap = 64.f * 1.4426950408889634f;
+template <int N, class T>
+__device__ __forceinline__ void cap_scores(T &x, float by, float cap) {
+    if (cap <= kSmallCap) {
+        const float by2 = by * 2.8853900817779268f;  // 2 log2(e)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            x[i] = fmaf(-2.f * cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x[i] * by2) + 1.f), cap);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float y = x[i] * by, y2 = y * y;
+        const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * 2.8853900817779268f) + 1.f);
+        const float small = y * fmaf(y2, fmaf(y2, fmaf(y2, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+        x[i] = cap * (fabsf(y) < 0.25f ? small : big);
+    }
+}
+
 // gfx950 LDS transpose read: in each group of 16 lanes, lane s gives the
 // address of 4 consecutive bf16; lane t = 4a + e receives element e of the
 // chunks of lanes a, a + 4, a + 8, a + 12.

@@ -4,7 +4,8 @@ The library is compiled from ``csrc/kvrt_kernels.hip`` (kernels),
 ``csrc/kvrt_prefill.hip`` and ``csrc/kvrt_prefill_wide.hip`` (chunked prefill),
 ``csrc/kvrt_block8.hip``, ``csrc/kvrt_block8_attend.hip`` and
 ``csrc/kvrt_block8_chunk.hip`` (8-bit pages), ``csrc/kvrt_rotate.hip`` (heads normed and rotated),
-``csrc/kvrt_shared.hip`` and ``csrc/kvrt_shared_wide.hip`` (attention after a shared prefix)
+``csrc/kvrt_shared.hip``, ``csrc/kvrt_shared_wide.hip``, ``csrc/kvrt_shared_chunk.hip`` and
+``csrc/kvrt_shared_chunk_wide.hip`` (attention after a shared prefix)
 and ``csrc/kvrt_runtime.hip`` (host runtime, C ABI in ``include/kvrt.h``);
 kvrt_pycall.so, the calls that read torch tensors directly, from
 ``csrc/kvrt_pycall.cpp`` with the host compiler. The build also compiles
@@ -31,9 +32,9 @@ LIB_PATH = PKG_DIR / "libkvrt.so"
 CALLS_PATH = PKG_DIR / "kvrt_pycall.so"
 SOURCES = ("kvrt_kernels.hip", "kvrt_prefill.hip", "kvrt_prefill_wide.hip", "kvrt_prefill_short.hip", "kvrt_runtime.hip",
            "kvrt_block8.hip", "kvrt_block8_attend.hip", "kvrt_block8_chunk.hip", "kvrt_rotate.hip",
-           "kvrt_shared.hip", "kvrt_shared_wide.hip")
+           "kvrt_shared.hip", "kvrt_shared_wide.hip", "kvrt_shared_chunk.hip", "kvrt_shared_chunk_wide.hip")
 
-AGPR_SOURCES = ("kvrt_prefill_wide.hip",)
+AGPR_SOURCES = ("kvrt_prefill_wide.hip", "kvrt_shared_chunk_wide.hip")
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -43,7 +44,7 @@ HIPCC_FLAGS = [
     # Packed FP32 VALU forms are kept out of every code object.
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-fhip-fp32-correctly-rounded-divide-sqrt",
-    # (all sources but the wide prefill's:) MFMA accumulators live in ordinary VGPRs. With the default AGPR form the
+    # (all sources but those of wide chunks:) MFMA accumulators live in ordinary VGPRs. With the default AGPR form the
     # prefill tile loop copied its output accumulators between the two
     # register files every tile (72 v_accvgpr moves per 32-key tile at D 128);
     # the VGPR form drops them and raises occupancy of several decode and

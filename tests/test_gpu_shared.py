@@ -74,6 +74,15 @@ CHUNKS = [
     ([75, 90], 200, 16, 8, 128, "paged", 0, 75),
     ([75, 90], 200, 8, 1, 256, "paged", 60, 30),
     ([600], 0, 16, 8, 128, "contig", 0, 600),
+    ([20, 33], 0, 8, 1, 256, "contig", 0, 3),
+    ([900], 701, 8, 4, 128, "contig", 0, 40),
+    ([45, 300], 1000, 8, 1, 512, "contig", 0, 45),
+    ([333], 1400, 8, 1, 256, "ring", 700, 60),
+    ([1203, 64], 515, 8, 2, 64, "paged", 0, 64),
+    ([400, 390, 64], 64, 16, 4, 128, "paged", 0, 33),
+    ([64, 65], 1, 8, 1, 256, "contig", 0, 64),
+    ([100, 90], 33, 8, 2, 128, "contig", 10, 90),
+    ([700] * 9, 130, 16, 8, 128, "contig", 0, 300),
 ]
 
 
@@ -133,10 +142,13 @@ def test_masks_of_the_prefix_and_of_the_sessions(lens, qn, hq):
     s.check(got, q, 0.09, masks=masks)
 
 
-@pytest.mark.parametrize("qn,hq,hkv,d", [(2, 8, 1, 256), (2, 16, 8, 128), (50, 8, 4, 128), (40, 8, 1, 512), (40, 4, 1, 64)])
-def test_a_row_that_a_query_does_not_see_does_not_reach_it(qn, hq, hkv, d):
+@pytest.mark.parametrize("qn,hq,hkv,d,layout,more", [
+    (2, 8, 1, 256, "contig", 0), (2, 16, 8, 128, "paged", 0), (50, 8, 4, 128, "contig", 0), (40, 8, 1, 512, "paged", 0),
+    (40, 4, 1, 64, "contig", 0), (40, 8, 1, 512, "contig", 1000), (90, 4, 4, 128, "contig", 900),
+    (70, 8, 1, 256, "contig", 1000), (34, 2, 1, 64, "paged", 1100), (9, 8, 2, 128, "contig", 0)])
+def test_a_row_that_a_query_does_not_see_does_not_reach_it(qn, hq, hkv, d, layout, more):
     gen = _gen(d)
-    s = Sessions(gen, [qn + 30, qn + 1], 40, hkv=hkv, d=d, q=qn)
+    s = Sessions(gen, [qn + 30, qn + 1], 40 + more, hkv=hkv, d=d, q=qn, layout=layout)
     s.k[0][:, -1] = float("nan")            # seen by the last query only
     s.v[0][:, -1, ::3] = float("inf")
     s.v[1][:, -1] = float("nan")
@@ -146,6 +158,7 @@ def test_a_row_that_a_query_does_not_see_does_not_reach_it(qn, hq, hkv, d):
     q = _q(gen, 2, hq, qn, d)
     got = s.rt.attend_shared(0, q, range(2), d ** -0.5, prefix_slot=2)
     assert bool(got[0, :, :-1].isfinite().all()) and bool(got[0, :, -1].isnan().all())
+    s.check(got, q, d ** -0.5)
     if qn > 2:
         assert bool(got[1, :, :-2].isfinite().all())
     assert bool(got[1, :, -1].isnan().all())
@@ -336,3 +349,53 @@ def test_refusals():
             paged.rt.truncate(0, 3)
             with pytest.raises(KVRTError):
                 paged.rt.attend_shared(0, q[:1], [0], 0.1, prefix_slot=1)
+
+
+@pytest.mark.parametrize("cap", [0.5, 63.0, 65.0, 2e4])
+@pytest.mark.parametrize("qn,hq,d,layout", [(1, 8, 128, "contig"), (70, 4, 64, "paged"), (40, 8, 256, "contig")])
+def test_chunks_capped_on_both_sides_of_the_series(cap, qn, hq, d, layout):
+    gen = _gen(int(cap) + qn)
+    s = Sessions(gen, [qn + 200, qn], 410, hkv=2, d=d, q=qn, layout=layout)
+    q = _q(gen, 2, hq, qn, d)
+    slopes = torch.linspace(-0.02, 0.05, hq, device="cuda")
+    for scale in (0.3, -2.0, 1e-4):
+        s.check(s.rt.attend_shared(0, q, range(2), scale, prefix_slot=2, softcap=cap, slopes=slopes), q, scale, cap=cap,
+                slopes=slopes)
+
+
+@pytest.mark.parametrize("layout,window", [("contig", 0), ("ring", 900), ("paged", 0)])
+def test_a_captured_chunk_replays_as_lengths_grow(layout, window):
+    """Key ranges of a chunk are the device's own: sized for the lengths that the capture
+    knew, right for those of each replay, between other calls that use the workspace."""
+    gen = _gen(17)
+    lens = [40, 33]
+    s = Sessions(gen, lens, 700, hkv=1, d=256, layout=layout, window=window, spare=200, q=40,
+                 ring=1000 if layout == "ring" else None)
+    q = _q(gen, 2, 8, 40, 256)
+    k, v = (torch.randn(2, 1, 30, 256, generator=gen, device="cuda").to(BF16) for _ in range(2))
+    if layout == "paged":
+        for i in range(2):
+            s.rt.reserve(i, 160)
+    other = _q(gen, 2, 8, 1, 256)
+    s.check(s.rt.attend_shared(0, q[:, :, :33].contiguous(), range(2), 0.06, prefix_slot=2), q[:, :, :33], 0.06)
+    s.check(s.rt.attend_shared(0, other, range(2), 0.06, prefix_slot=2), other, 0.06)
+    torch.cuda.synchronize()
+    s.rt.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for j in range(30):  # (rows are appended at most two at a time)
+            s.rt.append(0, k[:, :, j:j + 1].contiguous(), v[:, :, j:j + 1].contiguous(), range(2))
+        got = s.rt.attend_shared(0, q, range(2), 0.06, prefix_slot=2, softcap=30.0)
+    for step in range(4):
+        q.copy_(_q(gen, 2, 8, 40, 256))
+        graph.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            s.k[i], s.v[i] = torch.cat((s.k[i], k[i]), 1), torch.cat((s.v[i], v[i]), 1)
+        s.check(got, q, 0.06, cap=30.0)
+        s.rt.synchronize()  # (the capture bound another stream)
+        s.rt.sync_lengths()
+        eager = s.rt.attend_shared(0, other, range(2), 0.06, prefix_slot=2)
+        s.check(eager, other, 0.06)
+        s.rt.synchronize()
+    assert s.rt.health() == 0
