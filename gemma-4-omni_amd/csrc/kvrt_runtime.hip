@@ -1122,9 +1122,8 @@ int tensor_call_launch(TensorCall &tc, float *ws, hipStream_t st, bool single) {
 
 // Shape of a chunk's launch (PrefillArgs): n items of qn queries, `group` heads per KV head,
 // any 16 of which see at most block_keys keys. plain: the 16-query kernel may take it.
-int prefill_shape(kvrt_ctx *c, PrefillArgs &a, const kvrt_layer_spec &s, int64_t qn, int64_t block_keys, bool plain) {
+void prefill_shape(PrefillArgs &a, const kvrt_layer_spec &s, int64_t qn, int64_t block_keys, bool plain) {
     const int D = s.head_dim, hkv = s.kv_heads, n = a.n_items, group = a.group;
-    const int64_t hq = (int64_t)group * hkv;
     // Shape of the launch: row_waves 32-row blocks x key_parts per workgroup and
     // key ranges per row block. A chunk's time is the chain of key blocks one
     // wave walks (about 1.1 us a block at head_dim 256, 2 us at 512, 0.5 us
@@ -1210,24 +1209,28 @@ int prefill_shape(kvrt_ctx *c, PrefillArgs &a, const kvrt_layer_spec &s, int64_t
     a.key_parts = parts;
     // Key ranges: as many as keep the grid within one round of 256 workgroups
     // (Q 291 at head_dim 512 over 2339 keys, 4 streams: 156 us unsplit, 99 / 87 /
-    // 121 us with 2 / 3 / 4 ranges). Not inside a capture that would need a
-    // larger workspace. KVRT_PF_KSPLIT=1 turns it off, n >= 2 forces n ranges.
+    // 121 us with 2 / 3 / 4 ranges). KVRT_PF_KSPLIT=1 turns it off, n >= 2 forces n ranges.
     a.n_ksplit = 1;
     const int64_t want = ksplit_env > 0 ? ksplit_env : std::min<int64_t>(256 / wgs(rw), block_keys / min_keys);
     const int nks = (int)std::min<int64_t>(want, 16);
-    if (nks > 1 && !a.short_heads && (ksplit_env > 0 || block_keys * (nks - 1) / nks >= split_keys)) {
-        const size_t po = ((size_t)n * hq * qn * nks * D + 63) / 64 * 64;
-        const size_t bytes = po * 4 + (size_t)n * hq * qn * nks * 8 + 256;
-        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-        const bool capturing = hipStreamIsCapturing(c->stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
-        if (bytes <= c->ws_bytes || (!capturing && ensure_workspace(c, bytes) == KVRT_OK)) {
-            a.n_ksplit = nks;
-            a.part_o = c->ws;
-            a.part_ml = reinterpret_cast<float2 *>(c->ws + po);
-        }
-        if (c->poisoned) return KVRT_EDEVICE;
+    if (nks > 1 && !a.short_heads && (ksplit_env > 0 || block_keys * (nks - 1) / nks >= split_keys)) a.n_ksplit = nks;
+}
+
+// The workspace of a.n_ksplit key ranges; inside a capture that would need a larger one, one
+// range.
+int prefill_partials(kvrt_ctx *c, PrefillArgs &a, const kvrt_layer_spec &s) {
+    if (a.n_ksplit == 1) return KVRT_OK;
+    const size_t parts = (size_t)a.n_items * a.group * s.kv_heads * a.qn * a.n_ksplit;
+    const size_t po = (parts * s.head_dim + 63) / 64 * 64, bytes = po * 4 + parts * 8 + 256;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    const bool capturing = hipStreamIsCapturing(c->stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
+    if (bytes <= c->ws_bytes || (!capturing && ensure_workspace(c, bytes) == KVRT_OK)) {
+        a.part_o = c->ws;
+        a.part_ml = reinterpret_cast<float2 *>(c->ws + po);
+    } else {
+        a.n_ksplit = 1;
     }
-    return KVRT_OK;
+    return c->poisoned ? KVRT_EDEVICE : KVRT_OK;
 }
 
 // Limits of shared-prefix attention: positions of a prefix and a session together stay
@@ -1235,28 +1238,31 @@ int prefill_shape(kvrt_ctx *c, PrefillArgs &a, const kvrt_layer_spec &s, int64_t
 // of the fewest rows of a tile, 256 threads each).
 constexpr int kMaxSharedCapacity = 1 << 29;
 constexpr int64_t kMaxSharedRows = 1 << 22;
-// Rows of an item and KV head from which its workgroups read the prefix for themselves: its
-// tile is as good as full without other items' rows.
-constexpr int64_t kJoinRows = 64;
+constexpr int kMaxSharedParts = 128;  // key ranges of an item, and of the prefix
 
 // How a call's rows and keys are divided (SharedArgs): pre_keys of the prefix are seen, and
-// own[i] of item i's rows. The shortest time of a simple model is taken: a launch lasts as
-// long as its longest unit, and at least as its units' work shared by 256 CUs; a unit takes
-// kTile us a key tile (measured with a workgroup per CU; two that share one overlap in part)
-// and kUnit of its own; partials are joined by a second launch.
-//   us a tile, head_dim 64 / 128 / 256 / 512: up to 16 rows 0.6, 0.8, 1.2, 1.8; up to 64 rows
-//   0.8, 1.1, 1.9, 2.5; up to 128 rows 1.0, 1.5
-void shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own) {
+// own[i] of item i's rows. joined: each item's workgroups read the prefix too, as the head of
+// its own keys. The shortest time of a simple model is taken, and returned, us: a launch lasts
+// as long as its longest unit, and at least as its units' work shared by 256 CUs (two and more
+// on one overlap in part: kShare); a unit takes some us a key tile and kUnit of its own;
+// partials are joined by a second launch. The constants are fitted to 1152 measured calls
+// (1 to 16 items of 1 to 512 rows, 512 to 33768 keys), which they meet with 4 to 9 % (rms).
+double shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own, bool joined) {
     const int hkv = a.kv.kv_heads, tile = shared_tile(D), dim = D == 64 ? 0 : D == 128 ? 1 : D == 256 ? 2 : 3;
     const int64_t per_item = (int64_t)a.group * a.qn, rows = per_item * a.n_items;
     const auto tiles_of = [](int64_t keys) { return (keys + kSharedKeys - 1) / kSharedKeys + (keys % kSharedKeys > 1 ? 1 : 0); };
     const auto cost = [&](int64_t r) {
-        static const double us[3][4] = {{0.6, 0.8, 1.2, 1.8}, {0.8, 1.1, 1.9, 2.5}, {1.0, 1.5, 1.9, 2.5}};
+        // up to 16 rows, up to 64, up to 128 (head_dim 64 and 128)
+        static const double us[3][4] = {{0.75, 0.8, 1.0, 1.9}, {0.8, 1.0, 1.2, 2.4}, {1.2, 1.5}};
         return us[r <= 16 ? 0 : r <= 64 ? 1 : 2][dim];
     };
-    constexpr double kUnit = 1.5, kJoin = 4.5, kJoinBytes = 3e6;  // us, us, bytes a us
+    // (by head_dim 64, 128, 256, 512; a launch alone is 1.5 us)
+    static const double kUnits[4] = {1.1, 4.3, 4.2, 7.1}, kJoins[4] = {3.8, 1.1, 1.4, 0.1}, kShares[4] = {0.6, 0.6, 0.87, 0.89};
+    static const double kParts[4] = {0.02, 0.01, 0.03, 0.06};  // us a part of a row
+    constexpr double kLaunch = 1.5, kJoinBytes = 3.2e6;  // us, bytes a us
+    const double kUnit = kUnits[dim], kBytes = D == 512 ? 4.6e6 : 5.2e6;
     a.own_tiles = (int)((per_item + tile - 1) / tile);
-    a.joined = a.prefix_slot >= 0 && (pre_keys == 0 || per_item >= kJoinRows);
+    a.joined = joined;
     a.pre_tiles = a.prefix_slot < 0 || a.joined ? 0 : (int)((rows + tile - 1) / tile);
     const int64_t pre = tiles_of(pre_keys);
     int64_t items[kMaxItems], most = 1;
@@ -1265,8 +1271,10 @@ void shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own) {
         most = std::max(most, items[i]);
     }
     const double cp = cost(std::min<int64_t>(rows, tile)), co = cost(std::min<int64_t>(per_item, tile));
-    const double share = 1.0 / 256 * (D <= 128 ? 0.7 : 1.0);
-    const double slots = 256.0 * (D == 64 ? 3 : D == 128 ? 2 : 1);
+    const double share = kShares[dim] / 256;
+    int64_t all_own = 0;
+    for (int i = 0; i < a.n_items; ++i) all_own += own[i];
+    const double floor = (double)(all_own + pre_keys) * hkv * D * 4 / kBytes;
     const bool ragged = !a.joined && a.own_tiles == 1;
     // ranges of an item of t tiles: even ones, or of `per` tiles where items differ
     const auto ranges = [](int64_t t, int64_t per) { return std::max<int64_t>(1, (t + per - 1) / per); };
@@ -1274,7 +1282,7 @@ void shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own) {
     int64_t best_pre = 1, best_per = most;
     for (int64_t per = 1;; per = std::min(most, per + 1 + per / 4)) {
         const int64_t splits = ranges(most, per);
-        if (splits <= 32) {
+        if (splits <= kMaxSharedParts) {
             double work = 0, units = 0;
             for (int i = 0; i < a.n_items; ++i) {
                 const double u = (double)(ragged ? ranges(items[i], per) : splits);
@@ -1283,13 +1291,15 @@ void shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own) {
             }
             for (int64_t pp = 1;; pp = std::min(pre, pp + 1 + pp / 4)) {
                 const int64_t ps = a.pre_tiles ? ranges(pre, pp) : 0;
-                if (ps <= 64) {
-                    const double all = hkv * (work + a.pre_tiles * (pre * cp + ps * kUnit)) * share;
+                if (ps <= kMaxSharedParts) {
+                    double all = hkv * (work + a.pre_tiles * (pre * cp + ps * kUnit)) * share;
+                    const double c = (units + a.pre_tiles * ps) * hkv / 256;  // units on a CU, whole ones
+                    if (c > 1) all *= std::ceil(c) / c;
                     const double longest = std::max((double)std::min(per, most) * co, a.pre_tiles ? pp * cp : 0.0) + kUnit;
                     const int64_t parts = splits + ps;
-                    // units that do not run at a time leave a last round part empty
-                    double t = units * hkv + a.pre_tiles * ps * hkv > slots ? all + longest / 2 : std::max(all, longest);
-                    if (parts > 1) t += kJoin + (double)rows * hkv * parts * D * 8 / kJoinBytes;
+                    double t = std::max(all, longest);
+                    t = std::max(t, floor) + kLaunch;
+                    if (parts > 1) t += kJoins[dim] + kParts[dim] * parts + (double)rows * hkv * parts * D * 8 / kJoinBytes;
                     if (t < best) best = t, best_pre = ps, best_per = per;
                 }
                 if (!a.pre_tiles || pp >= pre) break;
@@ -1305,6 +1315,25 @@ void shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own) {
         for (int i = 0; i < a.n_items; ++i) a.own_wgs += (int)ranges(items[i], best_per);
     }
     a.parts = a.pre_splits + a.own_splits;
+    return best;
+}
+
+// The time of a call on the prefill's tiles, its shape chosen, us: the chain of 32-key blocks
+// that a wave walks, in rounds of 256 workgroups, or `all` keys of all items read once, and
+// the launches (fitted to the same calls: 8 %).
+double chunk_time(const SharedChunkArgs &a, int D, int64_t keys, int64_t all) {
+    const int rw = a.row_waves, hkv = a.kv.kv_heads;
+    const double block = D == 64    ? (rw == 1 ? 0.82 : rw == 2 ? (a.key_parts == 4 ? 0.9 : 0.55) : 0.5)
+                         : D == 128 ? (rw == 1 ? 1.2 : rw == 2 ? (a.key_parts == 4 ? 1.5 : 0.95) : 0.75)
+                         : D == 256 ? (rw == 2 ? 1.35 : 1.2)
+                                    : 2.0;
+    const int64_t rows = (int64_t)a.group * a.qn, range = 32 * a.n_ksplit * a.key_parts;
+    const double wgs = (double)((rows + 32 * rw - 1) / (32 * rw)) * hkv * a.n_items * a.n_ksplit;
+    const double rounds = wgs <= 256 ? 1.0 : wgs / 256 * (D == 64 ? 0.75 : 1.0);
+    double t = std::max((double)((keys + range - 1) / range) * block * rounds, (double)all * hkv * D * 4 / (D <= 128 ? 4.2e6 : 5.4e6));
+    t += D == 64 ? 4.5 : D == 128 ? 5.2 : D == 256 ? 7.5 : 8.5;
+    if (a.n_ksplit > 1) t += 2.9 + (double)rows * a.n_items * hkv * a.n_ksplit * D * 8 / 3.6e6;
+    return t;
 }
 
 }  // namespace
@@ -2322,7 +2351,8 @@ int kvrt_attend_prefill_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32
     a.group = group;
     a.qn = (int)qn;
     a.window = s.window;
-    rc = prefill_shape(c, a, s, qn, block_keys, true);
+    prefill_shape(a, s, qn, block_keys, true);
+    rc = prefill_partials(c, a, s);
     if (rc != KVRT_OK) return rc;
     a.pmask = launch_masks(c, n, slots);
     a.scale_log2 = scale * 1.4426950408889634f;
@@ -2418,9 +2448,20 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
     a.capacity = cap;
     a.prefix_slot = prefix_slot;
     for (int i = 0; i < n; ++i) a.slots[i] = slots[i];
-    if (!a.pmask && per_item > 16 && (!shared || per_item >= kJoinRows) &&
-        !(s.layout == KVRT_LAYOUT_RING && s.ring_rows < kPfKeys)) {
-        // many rows of each item: the prefill's tiles
+    // the prefix's keys once for the rows of all items, or for each item with its own keys
+    // (also where no row sees the prefix now: a replay may find it otherwise)
+    double time = shared_plan(a, D, pre_keys, own_keys, shared);
+    if (shared && pre_keys > 0) {
+        SharedArgs apart = a;
+        const double t = shared_plan(apart, D, pre_keys, own_keys, false);
+        if (t < time) a = apart, time = t;
+    }
+    // Or, without masks, on the prefill's tiles: 32 rows a wave, as chunks have them. us a call,
+    // joined / apart / on the prefill's tiles, prefix 4096 and 100 rows each, by rows of an
+    // item and KV head: 16 items, 8 KV heads of 128: 1 row 48 / 12 / 28, 16 49 / 27 / 29, 64
+    // 61 / 54 / 43, 256 142 / 192 / 112; 4 items, one KV head of 512: 1 row 16 / 18 / 27, 128
+    // 38 / 35 / 41, 512 65 / 74 / 57.
+    if (!a.pmask && !(s.layout == KVRT_LAYOUT_RING && s.ring_rows < kPfKeys)) {
         SharedChunkArgs p{};
         p.kv = a.kv;
         p.len = a.len;
@@ -2442,16 +2483,19 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
         for (int i = 0; i < n; ++i) keys = std::max<int64_t>(keys, own_keys[i]);
         keys += pre_keys;
         if (window > 0) keys = std::min<int64_t>(keys, window + 15);
-        rc = prefill_shape(c, p, s, qn, keys, false);
-        if (rc != KVRT_OK) return rc;
-        c->counters.launches += p.n_ksplit > 1 ? 2 : 1;
-        if (launch_shared_chunk(p, D, enq(c)) != hipSuccess) return poison(c);
-        const uint64_t read = ((uint64_t)pre_keys * n + all_own) * ((per_item + 32 * p.row_waves - 1) / (32 * p.row_waves)) * hkv;
-        c->counters.attended_keys += read;
-        c->counters.attended_bytes += read * (uint64_t)D * 2 * 2;
-        return KVRT_OK;
+        prefill_shape(p, s, qn, keys, false);
+        if (chunk_time(p, D, keys, all_own + pre_keys) < time) {
+            rc = prefill_partials(c, p, s);
+            if (rc != KVRT_OK) return rc;
+            c->counters.launches += p.n_ksplit > 1 ? 2 : 1;
+            if (launch_shared_chunk(p, D, enq(c)) != hipSuccess) return poison(c);
+            const uint64_t tiles = (per_item + 32 * p.row_waves - 1) / (32 * p.row_waves);
+            const uint64_t read = ((uint64_t)pre_keys * n + all_own) * tiles * hkv;
+            c->counters.attended_keys += read;
+            c->counters.attended_bytes += read * (uint64_t)D * 2 * 2;
+            return KVRT_OK;
+        }
     }
-    shared_plan(a, D, pre_keys, own_keys);
     const auto bytes = [&] {
         const size_t rows = (size_t)n * hq * qn * a.parts;
         return a.parts == 1 ? 0 : rows * D * 4 + rows * 8 + 256;
