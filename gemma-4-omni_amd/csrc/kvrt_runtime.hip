@@ -1120,119 +1120,6 @@ int tensor_call_launch(TensorCall &tc, float *ws, hipStream_t st, bool single) {
     return KVRT_OK;
 }
 
-// Shape of a chunk's launch (PrefillArgs): n items of qn queries, `group` heads per KV head,
-// any 16 of which see at most block_keys keys. plain: the 16-query kernel may take it.
-void prefill_shape(PrefillArgs &a, const kvrt_layer_spec &s, int64_t qn, int64_t block_keys, bool plain) {
-    const int D = s.head_dim, hkv = s.kv_heads, n = a.n_items, group = a.group;
-    // Shape of the launch: row_waves 32-row blocks x key_parts per workgroup and
-    // key ranges per row block. A chunk's time is the chain of key blocks one
-    // wave walks (about 1.1 us a block at head_dim 256, 2 us at 512, 0.5 us
-    // below), so the smaller the grid, the more waves share a row block's keys,
-    // first inside a workgroup (combined through LDS), then over workgroups
-    // (partials in the workspace and a merge launch, ~6 us).
-    static const int ksplit_env = env_int("KVRT_PF_KSPLIT", 0);
-    const int64_t rows = (int64_t)group * qn;
-    const auto wgs = [&](int w) { return (rows + 32 * w - 1) / (32 * w) * hkv * n; };  // workgroups of w row blocks
-    int rw = 4, parts = 1;
-    // least keys of a key range, and least keys that a split has to take off a
-    // workgroup's walk to be worth its merge (head_dim 512: one row block's
-    // accumulators fill the AGPRs and two staged groups the LDS: no parts)
-    int min_keys = 96, split_keys = 120;
-    if (D == 256) {
-        // a workgroup's 137 KB of LDS leave one per CU: past two rounds of
-        // them (without a window their lengths differ and the rounds overlap)
-        // four row blocks per workgroup and no parts are faster (window 512, 3
-        // streams x Q 1200: 44.6 -> 32.7 us; 4 x Q 600: 23.8 against 29.6 us);
-        // so are they where two parts would not have a block each
-        if (block_keys > 64 && wgs(2) <= (s.window > 0 ? 384 : 512)) rw = 2, parts = 2;
-        min_keys = 80, split_keys = 400;
-    } else if (D <= 128 && s.layout == KVRT_LAYOUT_PAGED) {
-        // A row's address costs a lane more than its DMA: two row blocks share
-        // the fetching, and a split pays with half the keys. Few keys take no
-        // more parts than they have blocks (Hq 16 x Q 12 over 12: 4.6 us, two
-        // parts 5.5, four 5.7; Q 40 over 60: 6.4, four parts 7.2; over 220:
-        // 11.1, two parts 11.2).
-        if (block_keys <= 32) rw = 4, parts = 1;
-        else if (wgs(2) < 256) rw = 2, parts = block_keys <= 160 ? 2 : 4;
-        else if (wgs(4) < 512) rw = 2, parts = 2;
-        min_keys = 180, split_keys = 250;
-    } else if (D <= 128) {
-        // Few keys: 16-query tiles (kvrt_prefill_short.hip), whose chain per
-        // tile is half as long. 16-query tiles against the shape chosen below,
-        // us (graph replays, warm rows):
-        // up to one round of row blocks, D 128: Q 64 over 64 4.2 and 5.3, over
-        // 164 5.8 and 6.9; Q 40 over 300 7.4 and 7.7, over 400 9.3 and 8.3
-        // (more than one 16-query workgroup per CU: 8 heads of their own, 2 x
-        // Q 300 over 300, 8.1 and 7.8).
-        // Three or four heads of a group fill a workgroup's eight waves and the
-        // line lies lower: 3 heads x Q 40 over 150 6.6 and 7.1, over 200 7.4
-        // and 7.0; 4 heads over 40 4.9 and 5.2, over 100 5.9 and 5.7.
-        // D 64: Q 40 over 150 4.4 and 5.3, over 220 5.0 and 5.2.
-        // In a second round (4 x Q 200): over 300 8.7 and 9.5, over 550 11.9 and
-        // 12.5; D 64 over 400 7.3 and 8.1.
-        // Beyond, while the 16-query grid is at most four workgroups per CU: 16
-        // x Q 100 over 160 10.7 and 10.9, over 320 14.5 and 14.1; past that (32
-        // x Q 100 over 100) 15.0 and 11.1.
-        int heads = 1;  // q heads of a workgroup
-        for (int h = 2; h <= std::min(group, 4); ++h)
-            if (group % h == 0) heads = h;
-        const int64_t blocks = wgs(1), wgs16 = (qn + 15) / 16 * hkv * (group / heads) * n;
-        int short_keys = 0;
-        if (D == 128 && blocks <= 256) short_keys = heads == 3 ? 160 : heads > 3 ? 64 : wgs16 <= 256 ? 320 : 208;
-        else if (D == 128 && blocks <= 512) short_keys = heads <= 2 ? 576 : 320;
-        else if (D == 128) short_keys = wgs16 <= 1024 ? 224 : 0;
-        else if (blocks <= 256) short_keys = heads <= 3 ? 160 : 64;
-        else if (blocks <= 512 && heads <= 2) short_keys = 416;
-        if (plain && block_keys <= short_keys && ksplit_env < 2) {
-            a.short_heads = heads;
-            // two query blocks on the same tiles from two workgroups per CU on
-            const bool pair = wgs16 >= 512;
-            rw = pair ? 2 : 1;
-            parts = pair && heads > 2 ? 1 : 2;
-        } else if (blocks <= (D == 64 ? 512 : 256)) {
-            // four parts while one round of workgroups (at D 64 two per CU)
-            // takes the grid (Hq 16, one stream x Q 512: 8.8 us, two parts
-            // 10.9; D 64 x Q 450, 2 streams, 7.6 and 8.6)
-            rw = 1, parts = 4;
-        } else if (D == 128 && wgs(2) < 256) {
-            // (3 streams x Q 274 over 947: 16.9 us, two parts 17.4)
-            rw = 2, parts = 4;
-        } else if (wgs(4) < 512) {
-            // two parts up to two rounds of four row blocks (4 x Q 512: 15.4
-            // us, four parts 20.4), none beyond (4 x Q 1400: 98.7 us, two
-            // parts 102.6)
-            rw = 2, parts = 2;
-        }
-        min_keys = 160, split_keys = 500;
-    }
-    a.row_waves = rw;
-    a.key_parts = parts;
-    // Key ranges: as many as keep the grid within one round of 256 workgroups
-    // (Q 291 at head_dim 512 over 2339 keys, 4 streams: 156 us unsplit, 99 / 87 /
-    // 121 us with 2 / 3 / 4 ranges). KVRT_PF_KSPLIT=1 turns it off, n >= 2 forces n ranges.
-    a.n_ksplit = 1;
-    const int64_t want = ksplit_env > 0 ? ksplit_env : std::min<int64_t>(256 / wgs(rw), block_keys / min_keys);
-    const int nks = (int)std::min<int64_t>(want, 16);
-    if (nks > 1 && !a.short_heads && (ksplit_env > 0 || block_keys * (nks - 1) / nks >= split_keys)) a.n_ksplit = nks;
-}
-
-// The workspace of a.n_ksplit key ranges; inside a capture that would need a larger one, one
-// range.
-int prefill_partials(kvrt_ctx *c, PrefillArgs &a, const kvrt_layer_spec &s) {
-    if (a.n_ksplit == 1) return KVRT_OK;
-    const size_t parts = (size_t)a.n_items * a.group * s.kv_heads * a.qn * a.n_ksplit;
-    const size_t po = (parts * s.head_dim + 63) / 64 * 64, bytes = po * 4 + parts * 8 + 256;
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    const bool capturing = hipStreamIsCapturing(c->stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
-    if (bytes <= c->ws_bytes || (!capturing && ensure_workspace(c, bytes) == KVRT_OK)) {
-        a.part_o = c->ws;
-        a.part_ml = reinterpret_cast<float2 *>(c->ws + po);
-    } else {
-        a.n_ksplit = 1;
-    }
-    return c->poisoned ? KVRT_EDEVICE : KVRT_OK;
-}
-
 // Limits of shared-prefix attention: positions of a prefix and a session together stay
 // below 2^31, and so do rows, and a launch's threads below 2^32 (two key ranges for each
 // of the fewest rows of a tile, 256 threads each).
@@ -1318,22 +1205,44 @@ double shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own, b
     return best;
 }
 
-// The time of a call on the prefill's tiles, its shape chosen, us: the chain of 32-key blocks
-// that a wave walks, in rounds of 256 workgroups, or `all` keys of all items read once, and
-// the launches (fitted to the same calls: 8 %).
-double chunk_time(const SharedChunkArgs &a, int D, int64_t keys, int64_t all) {
-    const int rw = a.row_waves, hkv = a.kv.kv_heads;
-    const double block = D == 64    ? (rw == 1 ? 0.82 : rw == 2 ? (a.key_parts == 4 ? 0.9 : 0.55) : 0.5)
-                         : D == 128 ? (rw == 1 ? 1.2 : rw == 2 ? (a.key_parts == 4 ? 1.5 : 0.95) : 0.75)
-                         : D == 256 ? (rw == 2 ? 1.35 : 1.2)
-                                    : 2.0;
-    const int64_t rows = (int64_t)a.group * a.qn, range = 32 * a.n_ksplit * a.key_parts;
-    const double wgs = (double)((rows + 32 * rw - 1) / (32 * rw)) * hkv * a.n_items * a.n_ksplit;
-    const double rounds = wgs <= 256 ? 1.0 : wgs / 256 * (D == 64 ? 0.75 : 1.0);
-    double t = std::max((double)((keys + range - 1) / range) * block * rounds, (double)all * hkv * D * 4 / (D <= 128 ? 4.2e6 : 5.4e6));
-    t += D == 64 ? 4.5 : D == 128 ? 5.2 : D == 256 ? 7.5 : 8.5;
-    if (a.n_ksplit > 1) t += 2.9 + (double)rows * a.n_items * hkv * a.n_ksplit * D * 8 / 3.6e6;
-    return t;
+// The shape of a call on the prefill's tiles (PrefillArgs: row blocks and key parts of a
+// workgroup, key ranges), for items whose rows see `keys` keys at most, `all` together, and its
+// time, us: the chain of 32-key blocks that a wave walks, in rounds of 256 workgroups that
+// overlap where LDS holds more than one to a CU, and the merge of ranges. Fitted to 5000 calls
+// (1 to 8 items of 16 to 2200 rows, 300 to 20000 keys, every shape, 1 to 32 ranges), which the
+// times meet with 4 to 8 % (rms); the shape taken is 1.5 % slower than the best on average, the
+// prefill's rule for shorter chunks 10 %.
+double chunk_shape(SharedChunkArgs &a, int D, int64_t keys, int64_t all) {
+    struct Shape {
+        int rw, parts;
+        double block, paged, more;  // us a block, the same for PAGED, ... times workgroups on a CU
+        double base, merge, bytes;  // us, us, bytes a us of the partials
+    };
+    static const Shape kShapes[4][4] = {
+        {{4, 1, 0.67, 0.85, 0.62, 5.7, 2.3, 3.1e6}, {2, 2, 0.67, 1.05, 0.65, 6.3, 2.2, 2.7e6},
+         {2, 4, 0.96, 1.34, 1.0, 6.9, 1.9, 1.6e6}, {1, 4, 0.74, 0, 0.76, 6.0, 2.1, 1.9e6}},
+        {{4, 1, 0.78, 1.07, 0.73, 7.2, 2.0, 3.6e6}, {2, 2, 0.82, 1.46, 0.75, 7.5, 1.9, 3.0e6},
+         {2, 4, 1.25, 1.94, 1.0, 8.5, 1.6, 2.0e6}, {1, 4, 1.05, 0, 1.0, 7.2, 1.3, 1.6e6}},
+        {{4, 1, 1.19, 1.83, 1.0, 9.0, 2.2, 3.9e6}, {2, 2, 1.25, 2.5, 1.0, 11.1, 1.1, 2.9e6}},
+        {{4, 1, 2.0, 3.26, 1.0, 15.0, 1.0, 4.4e6}},
+    };
+    const int hkv = a.kv.kv_heads, dim = D == 64 ? 0 : D == 128 ? 1 : D == 256 ? 2 : 3;
+    const bool paged = a.kv.layout == KVRT_LAYOUT_PAGED;
+    const int64_t rows = (int64_t)a.group * a.qn, blocks = (keys + kPfKeys - 1) / kPfKeys;
+    const double read = (double)all * hkv * D * 4 / 5.2e6;
+    double best = 1e30;
+    for (const Shape &s : kShapes[dim]) {
+        const int64_t tiles = s.rw ? (rows + 32 * s.rw - 1) / (32 * s.rw) : 0;
+        if (s.rw == 0 || (paged && s.paged == 0) || tiles > 65535) continue;  // (a grid's third dimension)
+        for (int64_t nks = 1; nks == 1 || (nks <= 32 && nks * 2 <= blocks); nks += 1 + nks / 4) {
+            const int64_t chain = ((blocks + nks - 1) / nks + s.parts - 1) / s.parts;
+            const int64_t round = (tiles * hkv * a.n_items * nks + 255) / 256;
+            double t = std::max(chain * (paged ? s.paged : s.block) * std::max(1.0, round * s.more), read) + s.base;
+            if (nks > 1) t += s.merge + (double)rows * a.n_items * hkv * nks * D * 8 / s.bytes;
+            if (t < best) best = t, a.row_waves = s.rw, a.key_parts = s.parts, a.n_ksplit = (int)nks;
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -2351,16 +2260,115 @@ int kvrt_attend_prefill_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32
     a.group = group;
     a.qn = (int)qn;
     a.window = s.window;
-    prefill_shape(a, s, qn, block_keys, true);
-    rc = prefill_partials(c, a, s);
-    if (rc != KVRT_OK) return rc;
+    // Shape of the launch: row_waves 32-row blocks x key_parts per workgroup and
+    // key ranges per row block. A chunk's time is the chain of key blocks one
+    // wave walks (about 1.1 us a block at head_dim 256, 2 us at 512, 0.5 us
+    // below), so the smaller the grid, the more waves share a row block's keys,
+    // first inside a workgroup (combined through LDS), then over workgroups
+    // (partials in the workspace and a merge launch, ~6 us).
+    static const int ksplit_env = env_int("KVRT_PF_KSPLIT", 0);
+    const int64_t rows = (int64_t)group * qn;
+    const auto wgs = [&](int w) { return (rows + 32 * w - 1) / (32 * w) * hkv * n; };  // workgroups of w row blocks
+    int rw = 4, parts = 1;
+    // least keys of a key range, and least keys that a split has to take off a
+    // workgroup's walk to be worth its merge (head_dim 512: one row block's
+    // accumulators fill the AGPRs and two staged groups the LDS: no parts)
+    int min_keys = 96, split_keys = 120;
+    if (D == 256) {
+        // a workgroup's 137 KB of LDS leave one per CU: past two rounds of
+        // them (without a window their lengths differ and the rounds overlap)
+        // four row blocks per workgroup and no parts are faster (window 512, 3
+        // streams x Q 1200: 44.6 -> 32.7 us; 4 x Q 600: 23.8 against 29.6 us);
+        // so are they where two parts would not have a block each
+        if (block_keys > 64 && wgs(2) <= (s.window > 0 ? 384 : 512)) rw = 2, parts = 2;
+        min_keys = 80, split_keys = 400;
+    } else if (D <= 128 && s.layout == KVRT_LAYOUT_PAGED) {
+        // A row's address costs a lane more than its DMA: two row blocks share
+        // the fetching, and a split pays with half the keys. Few keys take no
+        // more parts than they have blocks (Hq 16 x Q 12 over 12: 4.6 us, two
+        // parts 5.5, four 5.7; Q 40 over 60: 6.4, four parts 7.2; over 220:
+        // 11.1, two parts 11.2).
+        if (block_keys <= 32) rw = 4, parts = 1;
+        else if (wgs(2) < 256) rw = 2, parts = block_keys <= 160 ? 2 : 4;
+        else if (wgs(4) < 512) rw = 2, parts = 2;
+        min_keys = 180, split_keys = 250;
+    } else if (D <= 128) {
+        // Few keys: 16-query tiles (kvrt_prefill_short.hip), whose chain per
+        // tile is half as long. 16-query tiles against the shape chosen below,
+        // us (graph replays, warm rows):
+        // up to one round of row blocks, D 128: Q 64 over 64 4.2 and 5.3, over
+        // 164 5.8 and 6.9; Q 40 over 300 7.4 and 7.7, over 400 9.3 and 8.3
+        // (more than one 16-query workgroup per CU: 8 heads of their own, 2 x
+        // Q 300 over 300, 8.1 and 7.8).
+        // Three or four heads of a group fill a workgroup's eight waves and the
+        // line lies lower: 3 heads x Q 40 over 150 6.6 and 7.1, over 200 7.4
+        // and 7.0; 4 heads over 40 4.9 and 5.2, over 100 5.9 and 5.7.
+        // D 64: Q 40 over 150 4.4 and 5.3, over 220 5.0 and 5.2.
+        // In a second round (4 x Q 200): over 300 8.7 and 9.5, over 550 11.9 and
+        // 12.5; D 64 over 400 7.3 and 8.1.
+        // Beyond, while the 16-query grid is at most four workgroups per CU: 16
+        // x Q 100 over 160 10.7 and 10.9, over 320 14.5 and 14.1; past that (32
+        // x Q 100 over 100) 15.0 and 11.1.
+        int heads = 1;  // q heads of a workgroup
+        for (int h = 2; h <= std::min(group, 4); ++h)
+            if (group % h == 0) heads = h;
+        const int64_t blocks = wgs(1), wgs16 = (qn + 15) / 16 * hkv * (group / heads) * n;
+        int short_keys = 0;
+        if (D == 128 && blocks <= 256) short_keys = heads == 3 ? 160 : heads > 3 ? 64 : wgs16 <= 256 ? 320 : 208;
+        else if (D == 128 && blocks <= 512) short_keys = heads <= 2 ? 576 : 320;
+        else if (D == 128) short_keys = wgs16 <= 1024 ? 224 : 0;
+        else if (blocks <= 256) short_keys = heads <= 3 ? 160 : 64;
+        else if (blocks <= 512 && heads <= 2) short_keys = 416;
+        if (block_keys <= short_keys && ksplit_env < 2) {
+            a.short_heads = heads;
+            // two query blocks on the same tiles from two workgroups per CU on
+            const bool pair = wgs16 >= 512;
+            rw = pair ? 2 : 1;
+            parts = pair && heads > 2 ? 1 : 2;
+        } else if (blocks <= (D == 64 ? 512 : 256)) {
+            // four parts while one round of workgroups (at D 64 two per CU)
+            // takes the grid (Hq 16, one stream x Q 512: 8.8 us, two parts
+            // 10.9; D 64 x Q 450, 2 streams, 7.6 and 8.6)
+            rw = 1, parts = 4;
+        } else if (D == 128 && wgs(2) < 256) {
+            // (3 streams x Q 274 over 947: 16.9 us, two parts 17.4)
+            rw = 2, parts = 4;
+        } else if (wgs(4) < 512) {
+            // two parts up to two rounds of four row blocks (4 x Q 512: 15.4
+            // us, four parts 20.4), none beyond (4 x Q 1400: 98.7 us, two
+            // parts 102.6)
+            rw = 2, parts = 2;
+        }
+        min_keys = 160, split_keys = 500;
+    }
+    a.row_waves = rw;
+    a.key_parts = parts;
+    // Key ranges: as many as keep the grid within one round of 256 workgroups
+    // (Q 291 at head_dim 512 over 2339 keys, 4 streams: 156 us unsplit, 99 / 87 /
+    // 121 us with 2 / 3 / 4 ranges). Not inside a capture that would need a
+    // larger workspace. KVRT_PF_KSPLIT=1 turns it off, n >= 2 forces n ranges.
+    a.n_ksplit = 1;
+    const int64_t want = ksplit_env > 0 ? ksplit_env : std::min<int64_t>(256 / wgs(rw), block_keys / min_keys);
+    const int nks = (int)std::min<int64_t>(want, 16);
+    if (nks > 1 && !a.short_heads && (ksplit_env > 0 || block_keys * (nks - 1) / nks >= split_keys)) {
+        const size_t po = ((size_t)n * hq * qn * nks * D + 63) / 64 * 64;
+        const size_t bytes = po * 4 + (size_t)n * hq * qn * nks * 8 + 256;
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        const bool capturing = hipStreamIsCapturing(c->stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
+        if (bytes <= c->ws_bytes || (!capturing && ensure_workspace(c, bytes) == KVRT_OK)) {
+            a.n_ksplit = nks;
+            a.part_o = c->ws;
+            a.part_ml = reinterpret_cast<float2 *>(c->ws + po);
+        }
+        if (c->poisoned) return KVRT_EDEVICE;
+    }
     a.pmask = launch_masks(c, n, slots);
     a.scale_log2 = scale * 1.4426950408889634f;
     for (int i = 0; i < n; ++i) a.slots[i] = slots[i];
     c->counters.launches += a.n_ksplit > 1 ? 2 : 1;
     if (launch_prefill(a, D, enq(c)) != hipSuccess) return poison(c);
-    // keys its workgroups read: those of 32 row_waves rows, or of row_waves 16-query blocks by short_heads heads
-    const int64_t wg_rows = (a.short_heads ? 16 : 32) * a.row_waves, per_query = a.short_heads ? 1 : group;
+    // keys its workgroups read: those of 32 rw rows, or of rw 16-query blocks by short_heads heads
+    const int64_t wg_rows = a.short_heads ? 16 * rw : 32 * rw, per_query = a.short_heads ? 1 : group;
     uint64_t keys = 0;
     for (int i = 0; i < n; ++i)
         for (int64_t r0 = 0; r0 < qn * per_query; r0 += wg_rows) {
@@ -2479,14 +2487,19 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
         p.inv_cap = a.inv_cap;
         p.slopes = slopes;
         for (int i = 0; i < n; ++i) p.slots[i] = slots[i];
-        int64_t keys = 0;  // most keys that any 16 queries see
+        int64_t keys = 0;  // most keys that the rows of a tile see
         for (int i = 0; i < n; ++i) keys = std::max<int64_t>(keys, own_keys[i]);
         keys += pre_keys;
         if (window > 0) keys = std::min<int64_t>(keys, window + 15);
-        prefill_shape(p, s, qn, keys, false);
-        if (chunk_time(p, D, keys, all_own + pre_keys) < time) {
-            rc = prefill_partials(c, p, s);
-            if (rc != KVRT_OK) return rc;
+        if (chunk_shape(p, D, keys, all_own + pre_keys) < time) {
+            const size_t parts = (size_t)n * hq * qn * p.n_ksplit, po = (parts * D + 63) / 64 * 64;
+            const size_t bytes = p.n_ksplit == 1 ? 0 : po * 4 + parts * 8 + 256;
+            if (bytes > c->ws_bytes) {
+                if (capturing) p.n_ksplit = 1;  // (a workspace that a capture cannot grow)
+                else if ((rc = ensure_workspace(c, bytes)) != KVRT_OK) return rc;
+            }
+            p.part_o = c->ws;
+            p.part_ml = reinterpret_cast<float2 *>(c->ws + po);
             c->counters.launches += p.n_ksplit > 1 ? 2 : 1;
             if (launch_shared_chunk(p, D, enq(c)) != hipSuccess) return poison(c);
             const uint64_t tiles = (per_item + 32 * p.row_waves - 1) / (32 * p.row_waves);
