@@ -1126,6 +1126,7 @@ int tensor_call_launch(TensorCall &tc, float *ws, hipStream_t st, bool single) {
 constexpr int kMaxSharedCapacity = 1 << 29;
 constexpr int64_t kMaxSharedRows = 1 << 22;
 constexpr int kMaxSharedParts = 128;  // key ranges of an item, and of the prefix
+constexpr double kMaxSharedUnits = 1 << 23;  // workgroups
 
 // How a call's rows and keys are divided (SharedArgs): pre_keys of the prefix are seen, and
 // own[i] of item i's rows. joined: each item's workgroups read the prefix too, as the head of
@@ -1161,7 +1162,8 @@ double shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own, b
     const double share = kShares[dim] / 256;
     int64_t all_own = 0;
     for (int i = 0; i < a.n_items; ++i) all_own += own[i];
-    const double floor = (double)(all_own + pre_keys) * hkv * D * 4 / kBytes;
+    // (the 64-row tiles of one item that head_dim 256 and 512 have do not meet in the L2)
+    const double floor = (double)(all_own * (D >= 256 ? a.own_tiles : 1) + pre_keys) * hkv * D * 4 / kBytes;
     const bool ragged = !a.joined && a.own_tiles == 1;
     // ranges of an item of t tiles: even ones, or of `per` tiles where items differ
     const auto ranges = [](int64_t t, int64_t per) { return std::max<int64_t>(1, (t + per - 1) / per); };
@@ -1178,9 +1180,9 @@ double shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own, b
             }
             for (int64_t pp = 1;; pp = std::min(pre, pp + 1 + pp / 4)) {
                 const int64_t ps = a.pre_tiles ? ranges(pre, pp) : 0;
-                if (ps <= kMaxSharedParts) {
+                const double c = (units + a.pre_tiles * ps) * hkv / 256;  // units on a CU, whole ones
+                if (ps <= kMaxSharedParts && (c <= kMaxSharedUnits / 256 || splits + ps <= 2)) {
                     double all = hkv * (work + a.pre_tiles * (pre * cp + ps * kUnit)) * share;
-                    const double c = (units + a.pre_tiles * ps) * hkv / 256;  // units on a CU, whole ones
                     if (c > 1) all *= std::ceil(c) / c;
                     const double longest = std::max((double)std::min(per, most) * co, a.pre_tiles ? pp * cp : 0.0) + kUnit;
                     const int64_t parts = splits + ps;
@@ -1237,7 +1239,9 @@ double chunk_shape(SharedChunkArgs &a, int D, int64_t keys, int64_t all) {
         for (int64_t nks = 1; nks == 1 || (nks <= 32 && nks * 2 <= blocks); nks += 1 + nks / 4) {
             const int64_t chain = ((blocks + nks - 1) / nks + s.parts - 1) / s.parts;
             const int64_t round = (tiles * hkv * a.n_items * nks + 255) / 256;
-            double t = std::max(chain * (paged ? s.paged : s.block) * std::max(1.0, round * s.more), read) + s.base;
+            const double walk = chain * (paged ? s.paged : s.block) * std::max(1.0, round * s.more);
+            // (up to head_dim 128 they overlap in part)
+            double t = std::max(walk, read) + (D <= 128 ? 0.2 : 0.0) * std::min(walk, read) + s.base;
             if (nks > 1) t += s.merge + (double)rows * a.n_items * hkv * nks * D * 8 / s.bytes;
             if (t < best) best = t, a.row_waves = s.rw, a.key_parts = s.parts, a.n_ksplit = (int)nks;
         }
