@@ -7,20 +7,21 @@
 // with V accumulate in fp32; weights enter P V as two bf16 terms (2^-17 relative: one
 // term's 2^-9 would show in the bf16 outputs of few-key rows).
 //
-// Why units: the prefix's keys are the same for every session, so a workgroup takes the
-// rows of up to kSharedTile rows of all sessions (query heads of one KV head) over a range
-// of them and reads each key once per tile of rows, where a decode per session reads it
-// once per session. A session's own keys go to workgroups of their own. Each unit leaves
-// (max, sum, output) of its rows, which a second launch joins by their maxima. Where a
-// session brings many rows (a chunk), its units take the prefix's keys and its own in one
-// walk (`joined`), and with one range per row nothing is left to join.
+// Why units: the prefix's keys are the same for every session, so a workgroup takes up to
+// shared_tile(D) rows of all sessions (query heads of one KV head) over a range of them and
+// reads each key once per tile of rows, where a decode per session reads it once per session.
+// A session's own keys go to workgroups of their own. Each unit leaves (max, sum, output) of
+// its rows, which a second launch joins by their maxima. Where a session's rows nearly fill a
+// tile, or one launch is all that a short call is worth, its units take the prefix's keys and
+// its own in one walk (`joined`); the host weighs the two (shared_plan). Chunks without masks
+// have the prefill's 32-row tiles instead (kvrt_shared_chunk.hip).
 //
-// A workgroup is four waves that stage 32-key tiles of K and V together by LDS DMA,
-// kStages of them in flight, one barrier per tile. With more than 16 rows (WIDE) a wave
-// has up to two blocks of 16 rows and all dims of their outputs; with up to 16 rows every
-// wave computes the scores of all of them, and a quarter of the dims: the scores' 2 D/32
-// matrix instructions are cheap beside the tile's bytes, and waves need neither exchange
-// nor join anything.
+// A workgroup is four waves that stage 32-key tiles of K and V together by LDS DMA, STAGES of
+// them in flight (three; two at head_dim 512, where four took as long), one barrier per tile.
+// With more than 16 rows (WIDE) a wave has up to two blocks of 16 rows and all dims of their
+// outputs; with up to 16 rows every wave computes the scores of all of them, and a quarter of
+// the dims: the scores' 2 D/32 matrix instructions are cheap beside the tile's bytes, and
+// waves need neither exchange nor join anything.
 //   S^T (16 keys x 16 rows) = K Q^T    D/32   v_mfma_f32_16x16x32_bf16, for two key halves
 //   O^T (16 dims x 16 rows) += V^T P^T  2      v_mfma_f32_16x16x32_bf16 per 16 dims
 // Lane layouts: A[row l%16][k 8(l/16)+j], B[k 8(l/16)+j][col l%16], D[row 4(l/16)+i][col
@@ -33,6 +34,13 @@
 // that read one 16-byte chunk of 16 rows (K), and 32 that read 32 bytes of 8 rows (V), find
 // each of the 64 banks once, and every operand's address is one register (at head_dim 64
 // and 128 two, by kx) and a constant.
+//
+// What bounds it: with many sessions or keys the bytes (64 sessions, one row each, 8 KV heads
+// of 128, behind 4096 rows: 245 MB in 53 us, 4.6 TB/s, and 4.7 us of joins; 16 paged ones
+// behind 1024: 119 MB in 27 us, 4.4 TB/s; a copy of 1 GiB 5.1). With few, the chain of a
+// unit: launch, lengths, first bytes, 0.8 us a tile of 16 rows at head_dim 128 (2.4 of 64 rows
+// at 512, where a tile's reads from LDS last as long), and the join's launch (four sessions
+// behind 2048 rows: 7.1 + 3.6 us).
 #pragma once
 
 #include "kvrt_shared.h"
@@ -179,16 +187,6 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
     if (a.pmask) {
         if (u.pre.tiles > 0) load_prefix(a.pmask, u.pre.slot, lane, plen_p, pw_p);
         if (u.own.tiles > 0) load_prefix(a.pmask, u.own.slot, lane, plen_o, pw_o);
-    }
-#pragma unroll
-    for (int s = 0; s < RS; ++s) {
-        asm volatile("" : "+v"(pos[s]), "+v"(slope[s]));
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-            uint4 &x = qop[s][c];
-            x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
-            asm volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w));  // loaded ahead of the first DMA
-        }
     }
 
     float m[RS], l[RS];
@@ -408,10 +406,21 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
     const int n = u.x1 - u.x0;
     constexpr int PER = 2 * S::IPW;  // a wave's DMAs of a tile
     if (n > 0) {
-        wait_vmem<0>();  // queries, masks and lengths are in registers
 #pragma unroll
         for (int i = 0; i < NS - 1; ++i)
             if (i < n) stage(u.x0 + i, i);
+        // The queries travel beside the first tiles' bytes and are waited for here (a decode
+        // step of 16 windowed sessions 7.5 -> 7.1 us, 16 paged ones 28.9 -> 27.2).
+#pragma unroll
+        for (int s = 0; s < RS; ++s) {
+            asm volatile("" : "+v"(pos[s]), "+v"(slope[s]));
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                uint4 &x = qop[s][c];
+                x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+                asm volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w));
+            }
+        }
         // (add_odd stands outside the loop that all other tiles stay in: beside it in one loop,
         // the accumulators were copied at every tile)
         for (int i = 0, buf = 0;; ++i) {

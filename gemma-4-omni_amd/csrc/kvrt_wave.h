@@ -161,10 +161,10 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 // cap * tanh(y) of N scores' products x, y = by * x, cap in log2 units: cap - 2 cap / (e^2y + 1).
 // Near 0 that cancels: it is off by up to cap * 2^-22 (2^-24 of e, times 1/2, 2^-23 of the
-// reciprocal, the roundings). Up to kSmallCap that is 2^-16 of a weight, a 128th of the answer's
+// reciprocal, the roundings). Up to kSmallCap that is 2^-16 of a weight, a 256th of the answer's
 // rounding; above, scores below cap / 4 take the series, whose next term is 2^-21 of the
-// value there. (The series costs as much again: a chunk of 2 x 291 queries, 8 heads of 128
-// over 2000 keys, capped: 33.5 us with it for every cap, without KVAR.)
+// value there. (2 x 291 queries, 8 heads of 128 over 2000 keys, one shape of tiles: 33.5 us with
+// the series for every cap, 30.0 without; 23 without a cap.)
 constexpr float kSmallCap = 64.f * 1.4426950408889634f;
 template <int N, class T>
 __device__ __forceinline__ void cap_scores(T &x, float by, float cap) {
