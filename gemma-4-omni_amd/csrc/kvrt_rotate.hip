@@ -155,11 +155,22 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
         widen(x[u][0], y);
         widen(x[u][1], y + 8);
         if (normed) {
-            float sum = 0.f;
+            const auto mean = [&](float eps) __attribute__((always_inline)) {
+                float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sum = fmaf(y[i], y[i], sum);
-            sum = group_sum<LANES>(sum);
-            const float inv = __builtin_amdgcn_rsqf(fmaf(sum, 1.0f / D, a.eps));  // within 1 ulp
+                for (int i = 0; i < 16; ++i) sum = fmaf(y[i], y[i], sum);
+                return fmaf(group_sum<LANES>(sum), 1.0f / D, eps);
+            };
+            float m = mean(a.eps);
+            // where squares leave fp32's range, x and eps are taken by a power of two (exact, and
+            // the quotient the same)
+            const float by = m < 0x1p-100f ? 0x1p100f : m > 0x1p100f ? 0x1p-70f : 1.f;
+            if (__any(by != 1.f)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[i] *= by;
+                m = mean(a.eps * by * by);
+            }
+            const float inv = __builtin_amdgcn_rsqf(m);  // within 1 ulp
 #pragma unroll
             for (int i = 0; i < 16; ++i) y[i] *= inv * w[i];
         }

@@ -571,6 +571,9 @@ class KVRuntime:
         GPU) adds slopes[h] * (key - query position) to them. The prefix-attention masks
         of the prefix slot and of the slots hold. bf16 layers, decode steps and chunks."""
         require_cuda(q, "q")
+        for t, name in ((q, "q"), (out, "out")):
+            if t is not None and t.device != self.device:
+                raise ValueError(f"{name} must be on {self.device}, got {t.device}")
         if slopes is not None:
             require_cuda(slopes, "slopes")
             if slopes.dtype != torch.float32 or slopes.dim() != 1 or not slopes.is_contiguous() or \

@@ -251,3 +251,27 @@ def test_refusals():
     with pytest.raises(KVRTError):  # destination rows that coincide
         rot.apply(q, positions=pos, out=(torch.zeros(2, 1, 3, 128, device="cuda", dtype=BF16).expand(2, 4, 3, 128), None, None))
     assert math.isfinite(float(rot.apply(q, positions=pos)[0].float().sum()))
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-38, 1e-6, 1e30])
+@pytest.mark.parametrize("d", [64, 512])
+def test_magnitudes_whose_squares_leave_fp32(eps, d):
+    """Rows of 1e-39 to 3e38 side by side in a wave: the norm's squares would underflow or
+    overflow, its quotient does not."""
+    from kvrt import HeadRotation
+
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    sizes = torch.tensor([1e-39, 1e-30, 1e-22, 1e-19, 3e-18, 1e-15, 1e-6, 1.0, 1e9, 1e15, 2e18, 1e19, 1e25, 2e37],
+                         dtype=torch.float64, device="cuda")
+    x = torch.randn(2, 14, 9, d, generator=gen, device="cuda", dtype=torch.float64).clamp(-4, 4) * sizes[:, None, None]
+    x = x.to(BF16)
+    x[0, 3, 2] = 0 if eps else 1
+    freq = _freqs(d // 2)
+    w = torch.rand(d, generator=gen, device="cuda") + 0.5
+    rot = HeadRotation(d, freq, q_weight=w, eps=eps)
+    pos = _positions(gen, 1, 2, 9, 5000)
+    got = rot.apply(x, positions=pos)[0]
+    f32 = torch.tensor(eps, dtype=torch.float32).item()
+    want, tol = _reference(x, "q", (freq, [0] * (d // 2), False, "qk", w, f32, 1.0), pos)
+    # answers below fp32's normal numbers round to a step of bf16's smallest, 2^-133
+    assert bool(((got.double() - want).abs() <= tol + 2.0 ** -133).all())

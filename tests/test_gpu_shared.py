@@ -399,3 +399,16 @@ def test_a_captured_chunk_replays_as_lengths_grow(layout, window):
         s.check(eager, other, 0.06)
         s.rt.synchronize()
     assert s.rt.health() == 0
+
+
+def test_answers_go_to_memory_of_the_same_gpu():
+    s = Sessions(_gen(18), [9], 5, hkv=1, d=64)
+    q = _q(s.gen, 1, 2, 1, 64)
+    with pytest.raises(ValueError):
+        s.rt.attend_shared(0, q, [0], 0.1, prefix_slot=1, out=torch.zeros(1, 2, 1, 64, dtype=BF16))
+    out = torch.full((2, 2, 1, 64), 7.0, device="cuda", dtype=BF16)
+    got = s.rt.attend_shared(0, q, [0], 0.1, prefix_slot=1, out=out[:1])
+    s.check(got, q, 0.1)
+    assert bool((out[1] == 7).all())
+    again = q.clone()
+    assert torch.equal(s.rt.attend_shared(0, again, [0], 0.1, prefix_slot=1, out=again), got) and torch.equal(again, got)
