@@ -341,7 +341,9 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
         int64_t off;   // elements: CONTIG the block's first row, RING the head's, PAGED 0
         int r0, last;  // first row (RING) or key (PAGED); last row of the block inside the range
         int pages;     // PAGED: entry of the block's page `lane` (a block spans at most 32)
+        int first;     // SHARED, PAGED: row of the range's first key (pages ahead of it may be gone)
     };
+    const int kfirst = SHARED ? shared_first_key(base_pos + qf, a.window, P, own0) : kstart;
     int kt = kstart + part * kPfKeys, krow = 0;  // first key of the block, its row in the ring
     int rlast = 0;                               // ... of the range's last key
     if constexpr (LAYOUT == KVRT_LAYOUT_RING) krow = kt % a.kv.rows, rlast = (kend - 1) % a.kv.rows;
@@ -369,6 +371,7 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
             if constexpr (LAYOUT == KVRT_LAYOUT_CONTIG) f.off += (int64_t)key * D;
             f.r0 = LAYOUT == KVRT_LAYOUT_RING ? key % a.kv.rows : key;
             f.last = own ? kend - 1 - t0 : min(kend, P) - 1 - key;
+            f.first = max(0, kfirst - t0);
             f.pages = pages;
             kt += kPfKeys * KS;
             if constexpr (LAYOUT == KVRT_LAYOUT_PAGED) pages = load_pages(kt);
@@ -401,7 +404,7 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
             rr = rr >= a.kv.rows ? rr - a.kv.rows : rr;
             dma_load16_cached(base + (int64_t)rr * D + chunk / 2, dst);
         } else {
-            const int key = f.r0 + r;
+            const int key = f.r0 + (SHARED ? max(r, f.first) : r);
             const int page = __shfl(f.pages, (key >> a.kv.block_shift) - (f.r0 >> a.kv.block_shift));
             int64_t off = page_row_offset(a.kv, page, kvh, key, D);
             bad |= off < 0;

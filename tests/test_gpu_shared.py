@@ -412,3 +412,101 @@ def test_answers_go_to_memory_of_the_same_gpu():
     assert bool((out[1] == 7).all())
     again = q.clone()
     assert torch.equal(s.rt.attend_shared(0, again, [0], 0.1, prefix_slot=1, out=again), got) and torch.equal(again, got)
+
+
+@pytest.mark.parametrize("layout", ["contig", "paged"])
+@pytest.mark.parametrize("hkv,d,n", [(8, 128, 5), (1, 512, 3), (2, 64, 1)])
+def test_a_captured_step_replays_on_sessions_many_times_as_long(layout, hkv, d, n):
+    """A launch's ranges are made for the lengths at its capture: longer sessions take longer
+    ranges, and ones of unequal growth each their share."""
+    gen = _gen(d)
+    s = Sessions(gen, [33] * n, 300, hkv=hkv, d=d, layout=layout, spare=4000)
+    q = _q(gen, n, 2 * hkv, 1, d)
+    if layout == "paged":
+        for i in range(n):
+            s.rt.reserve(i, 3900)
+    s.check(s.rt.attend_shared(0, q, range(n), 0.1, prefix_slot=n), q, 0.1)
+    s.rt.synchronize()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = s.rt.attend_shared(0, q, range(n), 0.1, prefix_slot=n)
+    for step, lens in enumerate(([700] * n, [3800, 40, 900, 2000, 1][:n], [1] * n, [5, 3900, 17, 33, 64][:n])):
+        s.rt.synchronize()
+        s.rt.sync_lengths()
+        for i, rows in enumerate(lens):
+            s.rt.truncate(i, 0)
+            s.k[i], s.v[i] = (torch.randn(hkv, rows, d, generator=gen, device="cuda").to(BF16) for _ in range(2))
+            s.rt.import_(i, 0, s.k[i][None], s.v[i][None])
+        s.lens = list(lens)
+        s.rt.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        s.check(got, q, 0.1)
+    assert s.rt.health() == 0
+
+
+def test_two_captured_calls_and_a_larger_one_between_them():
+    """Captured calls of one runtime keep the workspace that they were captured with."""
+    gen = _gen(20)
+    s = Sessions(gen, [500, 420, 60], 900, hkv=2, d=128, spare=100)
+    a, b, c = (_q(gen, 3, 16, qn, 128) for qn in (1, 40, 60))
+    small = _q(gen, 1, 16, 1, 128)
+    s.rt.attend_shared(0, a, range(3), 0.1, prefix_slot=3)
+    s.rt.synchronize()
+    graphs, outs = [], []
+    for q in (a, b):
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(s.rt.attend_shared(0, q, range(3), 0.1, prefix_slot=3, softcap=20.0))
+        s.rt.synchronize()
+        graphs.append(g)
+    for step in range(3):
+        for x in (a, b):
+            x.copy_(_q(gen, 3, 16, x.shape[2], 128))
+        graphs[step % 2].replay()
+        graphs[1 - step % 2].replay()
+        torch.cuda.synchronize()
+        s.check(outs[0], a, 0.1, cap=20.0)
+        s.check(outs[1], b, 0.1, cap=20.0)
+        eager = s.rt.attend_shared(0, c, range(3), 0.1, prefix_slot=3)
+        s.check(eager, c, 0.1)
+        s.rt.synchronize()
+
+
+def test_rows_behind_the_items_stay_as_they_were():
+    gen = _gen(21)
+    for qn, d, hkv in ((1, 128, 2), (30, 64, 1), (70, 256, 1), (3, 512, 1)):
+        s = Sessions(gen, [80, 130], 200, hkv=hkv, d=d)
+        q = _q(gen, 2, 4 * hkv, qn, d)
+        room = torch.full((4, 4 * hkv, qn, d), 3.0, device="cuda", dtype=BF16)
+        s.check(s.rt.attend_shared(0, q, range(2), 0.1, prefix_slot=2, out=room[1:3]), q, 0.1)
+        assert bool((room[0] == 3).all()) and bool((room[3] == 3).all())
+
+
+@pytest.mark.parametrize("hq,d", [(16, 64), (64, 64), (64, 128), (64, 256), (64, 512)])
+@pytest.mark.parametrize("imported", [False, True])
+@pytest.mark.parametrize("qn,prefix,evict_prefix", [(30, 0, 0), (30, 50, 0), (30, 300, 0), (300, 620, 496)])
+def test_chunks_over_evicted_pages(qn, prefix, evict_prefix, imported, hq, d):
+    """Pages ahead of the window are gone, also those that share a 32-key tile with its start."""
+    from kvrt import KVRuntime
+
+    window = 500
+    s = Sessions(_gen(qn), [679, 679], prefix, hkv=1, d=d, layout="paged", window=window, q=qn)
+    q = _q(s.gen, 2, hq, qn, d)
+    oldest = 679 - qn - window + 1
+    for i in range(2):
+        if oldest >= 16:
+            s.rt.evict(i, oldest // 16 * 16)
+    if evict_prefix:
+        s.rt.evict(2, evict_prefix)
+    kept = [oldest // 16 * 16 if oldest >= 16 else 0] * 2 + [evict_prefix]
+    if imported:  # sessions that never had those pages
+        s.rt = KVRuntime(s.rt.layers, n_slots=3, capacity=700, max_q=2, block_size=16, pool_pages=150, pool_seed=3)
+        for i, first in enumerate(kept):
+            s.rt.import_(i, 0, s.k[i][None].contiguous(), s.v[i][None].contiguous(), first_pos=first)
+    got = s.rt.attend_shared(0, q, range(2), 0.1, prefix_slot=2)
+    torch.cuda.synchronize()
+    assert s.rt.health() == 0
+    s.check(got, q, 0.1)

@@ -40,6 +40,9 @@ int main() {
                                         const int key = own ? t0 - own0 : std::min(t0, P - 1);
                                         const int last = own ? r.kend - 1 - t0 : std::min(r.kend, P) - 1 - key;
                                         const int rows = own ? len : P;
+                                        // (rows from the first key on, which one of the queries sees)
+                                        const int first = std::max(0, shared_first_key(base + qf, window, P, own0) - t0);
+                                        if (first > last) return std::printf("first %d > %d\n", first, last), 1;
                                         if (key < 0 || last < 0 || key + std::min(last, block - 1) >= rows)
                                             return std::printf("rows %d + %d of %d (P %d len %d Q %d kt %d)\n", key, last, rows, P, len, Q, kt), 1;
                                     }
