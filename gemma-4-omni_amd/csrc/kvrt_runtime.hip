@@ -2410,7 +2410,8 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
     // rows are numbered in 32 bits, as are a launch's threads
     if (hq > INT32_MAX / qn || n * hq * qn > kMaxSharedRows) return KVRT_EINVAL;
     const int64_t per_item = hq / hkv * qn;
-    if (!std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap) ||
+    constexpr float kLog2e = 1.4426950408889634f;
+    if (!std::isfinite(scale * kLog2e) || !(softcap >= 0.f) || !std::isfinite(softcap * kLog2e) ||
         reinterpret_cast<uintptr_t>(slopes) % 4 != 0)
         return KVRT_EINVAL;
     if (softcap > 0.f && !std::isfinite(scale / softcap)) return KVRT_EINVAL;
@@ -2450,8 +2451,8 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
     a.pmask = launch_masks(c, n, slots);
     if (!a.pmask && shared) a.pmask = launch_masks(c, 1, &prefix_slot);
     a.slopes = slopes;
-    a.scale = scale * 1.4426950408889634f;
-    a.cap = softcap * 1.4426950408889634f;
+    a.scale = scale * kLog2e;
+    a.cap = softcap * kLog2e;
     a.inv_cap = softcap > 0.f ? scale / softcap : 0.f;
     a.n_items = n;
     a.group = (int)(hq / hkv);

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from shared_ref import Sessions
+from shared_ref import Sessions, attend
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -510,3 +510,59 @@ def test_chunks_over_evicted_pages(qn, prefix, evict_prefix, imported, hq, d):
     torch.cuda.synchronize()
     assert s.rt.health() == 0
     s.check(got, q, 0.1)
+
+
+def test_refusals_of_scales_past_fp32_in_log2_units():
+    from kvrt import KVRTError
+
+    s = Sessions(_gen(22), [9], 5, hkv=1, d=64)
+    q = _q(s.gen, 1, 2, 1, 64)
+    for kw in (dict(scale=3e38), dict(scale=-3e38), dict(scale=0.1, softcap=3e38)):
+        with pytest.raises(KVRTError) as e:
+            s.rt.attend_shared(0, q, [0], prefix_slot=1, **kw)
+        assert e.value.code == -1
+    s.check(s.rt.attend_shared(0, q, [0], 0.1, prefix_slot=1, softcap=2e38), q, 0.1)
+    for none in ([], ()):
+        with pytest.raises(KVRTError):
+            s.rt.attend_shared(0, q[:0], none, 0.1, prefix_slot=1)
+
+
+@pytest.mark.parametrize("hq,hkv", [(6, 2), (5, 1), (21, 3), (11, 11)])
+@pytest.mark.parametrize("qn,d,layout,window", [(1, 64, "paged", 0), (2, 256, "contig", 0), (33, 128, "paged", 50),
+                                                (130, 64, "contig", 0), (47, 512, "ring", 90)])
+def test_groups_of_odd_numbers_of_heads(hq, hkv, qn, d, layout, window):
+    gen = _gen(hq * qn)
+    s = Sessions(gen, [qn + 5, 171, qn], 97, hkv=hkv, d=d, layout=layout, window=window, q=qn)
+    q = _q(gen, 3, hq, qn, d)
+    slopes = torch.linspace(-0.03, 0.04, hq, device="cuda")
+    s.check(s.rt.attend_shared(0, q, range(3), 0.11, prefix_slot=3), q, 0.11)
+    s.check(s.rt.attend_shared(0, q, range(3), 0.11, prefix_slot=3, softcap=9.0, slopes=slopes), q, 0.11, cap=9.0,
+            slopes=slopes)
+
+
+@pytest.mark.parametrize("layout", ["contig", "paged"])
+def test_rows_past_32_bits_of_bytes_and_elements(layout):
+    """A prefix of 8.5 million rows of 1 KiB, whose end lies 8.7 GB behind its slot's start, and
+    sessions in slots behind it."""
+    from kvrt import KVRuntime, LayerSpec
+
+    gen = _gen(23)
+    rows, window, d = 8_500_000, 70, 512
+    rt = KVRuntime([LayerSpec(kv_heads=1, head_dim=d, layout=layout, window=window)], n_slots=3, capacity=rows + 20,
+                   block_size=64, pool_pages=rows // 64 + 20 if layout == "paged" else 0, pool_seed=5)
+    k, v = (torch.zeros(1, 1, rows, d, device="cuda", dtype=BF16) for _ in range(2))
+    for t in (k, v):
+        t[:, :, -200:] = torch.randn(200, d, generator=gen, device="cuda")
+    rt.import_(0, 0, k, v)
+    own = [[torch.randn(1, n, d, generator=gen, device="cuda").to(BF16) for _ in range(2)] for n in (33, 61)]
+    for i, (a, b) in enumerate(own):
+        rt.import_(i + 1, 0, a[None], b[None])
+    for hq, qn in ((4, 1), (32, 33)):
+        q = _q(gen, 2, hq, qn, d)
+        got = rt.attend_shared(0, q, [1, 2], 0.05, prefix_slot=0)
+        for i, (a, b) in enumerate(own):
+            keys, values = torch.cat((k[0][:, -200:], a), 1), torch.cat((v[0][:, -200:], b), 1)
+            n = keys.shape[1]
+            want, tol = attend(q[i], keys, values, list(range(n - qn, n)), 0.05, window=window)
+            assert bool(((got[i].double() - want).abs() <= tol).all())
+    assert rt.health() == 0
