@@ -575,9 +575,9 @@ int kvrt_attend_talker_async(kvrt_ctx *ctx, int32_t layer, int32_t n, const int3
 /* Attention of q [n, Hq, Q, D] (bf16 contiguous, out likewise) over the last Q
  * positions of n slots of one layer behind a prefix that they share: slot i sees
  * the P rows of prefix_slot (P its length), then its own L_i, so that its query
- * row r sits at position P + L_i - Q + r. Nothing is copied: the prefix's rows are
- * read once per 128 query rows (64 from head_dim 256 on) of the call. prefix_slot -1:
- * no prefix. Scores are
+ * row r sits at position P + L_i - Q + r. Nothing is copied: with few rows a slot the
+ * prefix's rows are read once per 128 query rows (64 from head_dim 256 on) of the call,
+ * with more once for each slot's tile of rows. prefix_slot -1: no prefix. Scores are
  *   s = f(q.k * scale) + slopes[h] * (key position - query position)
  * with f(x) = softcap * tanh(x / softcap), or x where softcap is 0; slopes: DEVICE
  * fp32 [Hq], NULL for no bias. Visibility as kvrt_attend_decode_async (causal, the
@@ -586,7 +586,8 @@ int kvrt_attend_talker_async(kvrt_ctx *ctx, int32_t layer, int32_t n, const int3
  * zeros, and rows that a query does not see do not reach it whatever they hold.
  * Scores, softmax and sums in fp32, weights in two bf16 terms (2^-17 relative). Any
  * 1 <= Q <= L_i, any Hq / kv_heads; bf16 layers of every layout; a capacity of at
- * most 2^29; n * Hq * Q <= 2^22. prefix_slot is none of the slots; RING and PAGED
+ * most 2^29; n * Hq * Q <= 2^22; scale and softcap finite in log2 units (times
+ * log2 e), as is their quotient. prefix_slot is none of the slots; RING and PAGED
  * layers still hold the oldest keys seen of both, a RING layer's rows those of Q +
  * window - 1 positions (KVRT_ESTATE otherwise). A captured call replays on the
  * lengths it then finds; one whose partials do not fit the context's workspace is
