@@ -566,3 +566,30 @@ def test_rows_past_32_bits_of_bytes_and_elements(layout):
             want, tol = attend(q[i], keys, values, list(range(n - qn, n)), 0.05, window=window)
             assert bool(((got[i].double() - want).abs() <= tol).all())
     assert rt.health() == 0
+
+
+@pytest.mark.parametrize("block", [1, 8, 128])
+@pytest.mark.parametrize("d,window", [(64, 0), (128, 333), (512, 90)])
+def test_chunks_on_pages_of_any_size(block, d, window):
+    gen = _gen(block + d)
+    s = Sessions(gen, [611, 45], 270, hkv=1, d=d, layout="paged", block=block, window=window, q=45)
+    q = _q(gen, 2, 32, 45, d)
+    s.check(s.rt.attend_shared(0, q, range(2), 0.08, prefix_slot=2), q, 0.08)
+    assert s.rt.health() == 0
+
+
+def test_calls_on_another_stream():
+    gen = _gen(24)
+    s = Sessions(gen, [200, 31], 400, hkv=2, d=128)
+    for qn in (1, 30):
+        q = _q(gen, 2, 8, qn, 128)
+        here = s.rt.attend_shared(0, q, range(2), 0.1, prefix_slot=2)
+        s.check(here, q, 0.1)
+        s.rt.synchronize()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            there = s.rt.attend_shared(0, q, range(2), 0.1, prefix_slot=2)
+            s.rt.synchronize()
+        torch.cuda.synchronize()
+        assert torch.equal(here, there)
