@@ -341,7 +341,10 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
         int64_t off;   // elements: CONTIG the block's first row, RING the head's, PAGED 0
         int r0, last;  // first row (RING) or key (PAGED); last row of the block inside the range
         int pages;     // PAGED: entry of the block's page `lane` (a block spans at most 32)
-        int first;     // SHARED, PAGED: row of the range's first key (pages ahead of it may be gone)
+        // SHARED, PAGED: row of the range's first key (pages ahead of it may be gone), first row
+        // of the page of this lane's rows, and (head_dim 512, where an instruction is one row) of
+        // the last 16 rows'
+        int first, row0, row1;
     };
     const int kfirst = SHARED ? shared_first_key(base_pos + qf, a.window, P, own0) : kstart;
     int kt = kstart + part * kPfKeys, krow = 0;  // first key of the block, its row in the ring
@@ -371,8 +374,21 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
             if constexpr (LAYOUT == KVRT_LAYOUT_CONTIG) f.off += (int64_t)key * D;
             f.r0 = LAYOUT == KVRT_LAYOUT_RING ? key % a.kv.rows : key;
             f.last = own ? kend - 1 - t0 : min(kend, P) - 1 - key;
-            f.first = max(0, kfirst - t0);
-            f.pages = pages;
+            if constexpr (LAYOUT == KVRT_LAYOUT_PAGED) {
+                // A block starts at a multiple of 32 in its slot (or has one row to read, a last
+                // one again) and a page holds 16 rows or more: the halves of a block lie in one
+                // page each, and a row's place is an addition (4 x 512 queries behind 1400 rows,
+                // head_dim 128: KVA us, 99 with every row's page looked up; 4 x 291, head_dim
+                // 512: KVB and 123).
+                f.first = max(0, kfirst - t0);
+                const int lo = page_row(a.kv, __builtin_amdgcn_readlane(pages, 0), kvh, 0);
+                const int hi = page_row(a.kv, __builtin_amdgcn_readlane(pages, a.kv.block_shift == 4 ? 1 : 0), kvh, 0);
+                const bool upper = f.last >= 16;  // else no row is read from there
+                bad |= (f.first < 16 && lo < 0) || (upper && hi < 0);
+                f.row0 = max(f.first >= 16 ? hi : lo, 0);
+                f.row1 = max(upper ? hi : lo, 0);
+                if constexpr (IPB <= 16) f.row0 = lrow >= 16 ? f.row1 : f.row0;
+            }
             kt += kPfKeys * KS;
             if constexpr (LAYOUT == KVRT_LAYOUT_PAGED) pages = load_pages(kt);
             return f;
@@ -403,8 +419,12 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
             int rr = f.r0 + r;  // rows of a block wrap at most once
             rr = rr >= a.kv.rows ? rr - a.kv.rows : rr;
             dma_load16_cached(base + (int64_t)rr * D + chunk / 2, dst);
+        } else if constexpr (SHARED) {
+            const int at = max(r, f.first);
+            const int row = (IPB <= 16 || at < 16 ? f.row0 : f.row1) + ((f.r0 + at) & (a.kv.rows - 1));
+            dma_load16_cached(base + (int64_t)row * D + chunk / 2, dst);
         } else {
-            const int key = f.r0 + (SHARED ? max(r, f.first) : r);
+            const int key = f.r0 + r;
             const int page = __shfl(f.pages, (key >> a.kv.block_shift) - (f.r0 >> a.kv.block_shift));
             int64_t off = page_row_offset(a.kv, page, kvh, key, D);
             bad |= off < 0;

@@ -2474,7 +2474,10 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
     // item and KV head: 16 items, 8 KV heads of 128: 1 row 48 / 12 / 28, 16 49 / 27 / 29, 64
     // 61 / 54 / 43, 256 142 / 192 / 112; 4 items, one KV head of 512: 1 row 16 / 18 / 27, 128
     // 38 / 35 / 41, 512 65 / 74 / 57.
-    if (!a.pmask && !(s.layout == KVRT_LAYOUT_RING && s.ring_rows < kPfKeys)) {
+    // (A ring holds a block of 32 keys; pages of 8 rows and fewer are the first kernel's, whose
+    // 86 us for 4 x 512 queries behind 1400 rows are 99 where every row's page is looked up.)
+    if (!a.pmask && !(s.layout == KVRT_LAYOUT_RING && s.ring_rows < kPfKeys) &&
+        !(s.layout == KVRT_LAYOUT_PAGED && c->cfg.block_size < 16)) {
         SharedChunkArgs p{};
         p.kv = a.kv;
         p.len = a.len;

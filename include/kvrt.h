@@ -786,8 +786,8 @@ uint64_t kvrt_block8_attend_work(const kvrt_block8 *pages, int64_t n, int64_t wi
 typedef struct kvrt_rotation {
     const uint64_t *turns;  /* device [n_freq], from kvrt_rotation_turns                */
     const uint8_t *axis;    /* device [n_freq], 8-byte aligned: the axis whose position
-                               turns pair f (>= n_axes: the last one's); NULL: axis 0
-                               (n_axes must be 1)                                       */
+                               turns pair f, below n_axes (a larger value takes one of
+                               the axes given); NULL: axis 0 (n_axes must be 1)         */
     const float *q_weight;  /* device [head_dim], 16-byte aligned; NULL: ones           */
     const float *k_weight;
     int32_t head_dim;       /* 64, 128, 256 or 512                                      */
@@ -814,8 +814,7 @@ int kvrt_rotation_turns(const double *inv_freq, int32_t n, uint64_t *turns);
  * once; value heads have no weight and do not turn. positions: device KVRT_INT32 or
  * KVRT_INT64 [n_axes, n, Q], any strides, values within int32 (an int64's low word is
  * taken); not read where n_freq is 0. An output may be its input itself, otherwise
- * outputs share no memory with inputs or each other. fp32 sums of squares: |x| below
- * 2^60. Context-free: runs on the current device and the given stream, allocates
+ * outputs share no memory with inputs or each other. Context-free: runs on the current device and the given stream, allocates
  * nothing, returns KVRT_EINVAL (nothing enqueued) for arguments it does not take and
  * KVRT_EDEVICE when the launch fails.
  * Replaces the listener's and talker's norm and rotation launches of each layer
