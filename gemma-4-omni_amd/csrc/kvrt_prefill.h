@@ -341,10 +341,11 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
         int64_t off;   // elements: CONTIG the block's first row, RING the head's, PAGED 0
         int r0, last;  // first row (RING) or key (PAGED); last row of the block inside the range
         int pages;     // PAGED: entry of the block's page `lane` (a block spans at most 32)
-        // SHARED, PAGED: row of the range's first key (pages ahead of it may be gone), first row
-        // of the page of this lane's rows, and (head_dim 512, where an instruction is one row) of
-        // the last 16 rows'
-        int first, row0, row1;
+        // SHARED, PAGED: row of the range's first key (pages ahead of it may be gone); where row 0
+        // of the block would lie if all were in the page of its first half (of this lane's rows),
+        // and of its second (head_dim 512, where an instruction is one row): elements
+        int first;
+        int64_t at0, at1;
     };
     const int kfirst = SHARED ? shared_first_key(base_pos + qf, a.window, P, own0) : kstart;
     int kt = kstart + part * kPfKeys, krow = 0;  // first key of the block, its row in the ring
@@ -385,9 +386,11 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
                 const int hi = page_row(a.kv, __builtin_amdgcn_readlane(pages, a.kv.block_shift == 4 ? 1 : 0), kvh, 0);
                 const bool upper = f.last >= 16;  // else no row is read from there
                 bad |= (f.first < 16 && lo < 0) || (upper && hi < 0);
-                f.row0 = max(f.first >= 16 ? hi : lo, 0);
-                f.row1 = max(upper ? hi : lo, 0);
-                if constexpr (IPB <= 16) f.row0 = lrow >= 16 ? f.row1 : f.row0;
+                const int in = key & (a.kv.rows - 1);
+                const int row0 = max(lo, 0) + in, row1 = a.kv.block_shift == 4 ? max(hi, 0) + in - 16 : row0;
+                f.at0 = (int64_t)(f.first >= 16 ? row1 : row0) * D;
+                f.at1 = (int64_t)(upper ? row1 : row0) * D;
+                if constexpr (IPB <= 16) f.at0 = lrow >= 16 ? f.at1 : f.at0;
             }
             kt += kPfKeys * KS;
             if constexpr (LAYOUT == KVRT_LAYOUT_PAGED) pages = load_pages(kt);
@@ -420,9 +423,12 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
             rr = rr >= a.kv.rows ? rr - a.kv.rows : rr;
             dma_load16_cached(base + (int64_t)rr * D + chunk / 2, dst);
         } else if constexpr (SHARED) {
-            const int at = max(r, f.first);
-            const int row = (IPB <= 16 || at < 16 ? f.row0 : f.row1) + ((f.r0 + at) & (a.kv.rows - 1));
-            dma_load16_cached(base + (int64_t)row * D + chunk / 2, dst);
+            if constexpr (IPB <= 16) {
+                dma_load16_cached(base + f.at0 + (uint32_t)(max(r, f.first) * D + chunk / 2), dst);
+            } else {
+                const int at = max(min(rw + i * RW, f.last), f.first);
+                dma_load16_at(base + (at < 16 ? f.at0 : f.at1) + at * D, chunk, dst);
+            }
         } else {
             const int key = f.r0 + r;
             const int page = __shfl(f.pages, (key >> a.kv.block_shift) - (f.r0 >> a.kv.block_shift));
