@@ -1221,12 +1221,12 @@ double chunk_shape(SharedChunkArgs &a, int D, int64_t keys, int64_t all) {
         double base, merge, bytes;  // us, us, bytes a us of the partials
     };
     static const Shape kShapes[4][4] = {
-        {{4, 1, 0.67, 0.85, 0.62, 5.7, 2.3, 3.1e6}, {2, 2, 0.67, 1.05, 0.65, 6.3, 2.2, 2.7e6},
-         {2, 4, 0.96, 1.34, 1.0, 6.9, 1.9, 1.6e6}, {1, 4, 0.74, 0, 0.76, 6.0, 2.1, 1.9e6}},
-        {{4, 1, 0.78, 1.07, 0.73, 7.2, 2.0, 3.6e6}, {2, 2, 0.82, 1.46, 0.75, 7.5, 1.9, 3.0e6},
-         {2, 4, 1.25, 1.94, 1.0, 8.5, 1.6, 2.0e6}, {1, 4, 1.05, 0, 1.0, 7.2, 1.3, 1.6e6}},
-        {{4, 1, 1.19, 1.83, 1.0, 9.0, 2.2, 3.9e6}, {2, 2, 1.25, 2.5, 1.0, 11.1, 1.1, 2.9e6}},
-        {{4, 1, 2.0, 3.26, 1.0, 15.0, 1.0, 4.4e6}},
+        {{4, 1, 0.67, 0.85, 0.62, 5.7, 2.3, 3.1e6}, {2, 2, 0.67, 0.9, 0.65, 6.3, 2.2, 2.7e6},
+         {2, 4, 0.96, 1.2, 1.0, 6.9, 1.9, 1.6e6}, {1, 4, 0.74, 0, 0.76, 6.0, 2.1, 1.9e6}},
+        {{4, 1, 0.78, 1.0, 0.73, 7.2, 2.0, 3.6e6}, {2, 2, 0.82, 1.08, 0.75, 7.5, 1.9, 3.0e6},
+         {2, 4, 1.25, 1.55, 1.0, 8.5, 1.6, 2.0e6}, {1, 4, 1.05, 0, 1.0, 7.2, 1.3, 1.6e6}},
+        {{4, 1, 1.19, 1.42, 1.0, 9.0, 2.2, 3.9e6}, {2, 2, 1.25, 1.55, 1.0, 11.1, 1.1, 2.9e6}},
+        {{4, 1, 2.0, 2.25, 1.0, 15.0, 1.0, 4.4e6}},
     };
     const int hkv = a.kv.kv_heads, dim = D == 64 ? 0 : D == 128 ? 1 : D == 256 ? 2 : 3;
     const bool paged = a.kv.layout == KVRT_LAYOUT_PAGED;
