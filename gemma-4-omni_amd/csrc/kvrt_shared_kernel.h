@@ -17,7 +17,8 @@
 // have the prefill's 32-row tiles instead (kvrt_shared_chunk.hip).
 //
 // A workgroup is four waves that stage 32-key tiles of K and V together by LDS DMA, STAGES of
-// them in flight (three; two at head_dim 512, where four took as long), one barrier per tile.
+// them in flight (three, four at head_dim 256 and six at 128 took as long; two at 512, which
+// fill the LDS), one barrier per tile.
 // With more than 16 rows (WIDE) a wave has up to two blocks of 16 rows and all dims of their
 // outputs; with up to 16 rows every wave computes the scores of all of them, and a quarter of
 // the dims: the scores' 2 D/32 matrix instructions are cheap beside the tile's bytes, and
