@@ -212,7 +212,8 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
         key0 = (g.tile0 + (own ? x - u.pre.tiles : x)) * kSharedKeys;
         return g;
     };
-    auto stage = [&](int x, int buf) __attribute__((always_inline)) {
+    auto stage = [&](auto of_k, auto of_v, int x, int buf) __attribute__((always_inline)) {
+        constexpr bool OF_K = decltype(of_k)::value, OF_V = decltype(of_v)::value;
         int key0;
         const Segment &g = where(x, key0);
         const int64_t head = LAYOUT == KVRT_LAYOUT_PAGED
@@ -243,8 +244,8 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
             if constexpr (LAYOUT == KVRT_LAYOUT_CONTIG) {
                 const int64_t base = head + (int64_t)key0 * D;
                 const uint32_t at = (uint32_t)(key - key0) * (2 * D);
-                shared_dma(kg + base, at + 16 * (c ^ S::kx(sub)), kto);
-                shared_dma(vg + base, at + 16 * c, vto);
+                if constexpr (OF_K) shared_dma(kg + base, at + 16 * (c ^ S::kx(sub)), kto);
+                if constexpr (OF_V) shared_dma(vg + base, at + 16 * c, vto);
                 continue;
             } else if constexpr (LAYOUT == KVRT_LAYOUT_RING) {
                 int rr = ring0 + (key - key0);
@@ -258,8 +259,8 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
                 bad |= off < 0;
                 off = off < 0 ? 0 : off;
             }
-            dma_load16_cached(kg + off + 8 * (c ^ S::kx(sub)), kto);
-            dma_load16_cached(vg + off + 8 * c, vto);
+            if constexpr (OF_K) dma_load16_cached(kg + off + 8 * (c ^ S::kx(sub)), kto);
+            if constexpr (OF_V) dma_load16_cached(vg + off + 8 * c, vto);
         }
     };
 
@@ -279,10 +280,9 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
             v[h] = lds_read_tr16(reinterpret_cast<const uint16_t *>(vt + vadr + 32 * b + h * (D == 512 ? 16 * S::VP : H)));
         return make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
     };
-    // The weights of tile x. True where some query does not see all of it and its V holds NaN
-    // or infinities: 0 * NaN is not 0, so that its products are made one by one (add_odd).
+    // The weights of tile x; whether all queries see all of it.
     auto weigh = [&](int x, int buf) __attribute__((always_inline)) {
-        const uint8_t *kt = lds + buf * S::STAGE, *vt = kt + S::KBLK;
+        const uint8_t *kt = lds + buf * S::STAGE;
         f32x4_t sc[RS][2];
 #pragma unroll
         for (int s = 0; s < RS; ++s)
@@ -357,7 +357,12 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
             ph[s] = make_uint4(hiw[0], hiw[1], hiw[2], hiw[3]);
             pl[s] = make_uint4(low[0], low[1], low[2], low[3]);
         }
-        if (whole) return false;
+        return whole;
+    };
+    // Whether V of a tile that some query does not see whole holds NaN or infinities: 0 * NaN is
+    // not 0, so that its products are made one by one (add_odd).
+    auto look = [&](int buf) __attribute__((always_inline)) {
+        const uint8_t *vt = lds + buf * S::STAGE + S::KBLK;
         u16x2_t most = {0, 0};
 #pragma clang loop unroll_count(2)
         for (int b = 0; b < NB; ++b) {
@@ -406,10 +411,23 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
 
     const int n = u.x1 - u.x0;
     constexpr int PER = 2 * S::IPW;  // a wave's DMAs of a tile
+    // With two stages (head_dim 512) K and V travel apart: a tile's K from when the last but
+    // one's was read, its V half a tile later, so that both have a tile and a half under way (4
+    // sessions of 8192 rows, 8 KV heads: 114 -> 107 us; 8 behind 8192 29.9 -> 27.3). On pages,
+    // where every row's page would be looked up twice, together (116 us; apart 140).
+    constexpr bool APART = NS == 2 && LAYOUT != KVRT_LAYOUT_PAGED;
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
     if (n > 0) {
+        if constexpr (APART) {
+            stage(yes, no, u.x0, 0);
+            stage(no, yes, u.x0, 0);
+            if (n > 1) stage(yes, no, u.x0 + 1, 1);
+        } else {
 #pragma unroll
-        for (int i = 0; i < NS - 1; ++i)
-            if (i < n) stage(u.x0 + i, i);
+            for (int i = 0; i < NS - 1; ++i)
+                if (i < n) stage(yes, yes, u.x0 + i, i);
+        }
         // The queries travel beside the first tiles' bytes and are waited for here (a decode
         // step of 16 windowed sessions 7.5 -> 7.1 us, 16 paged ones 28.9 -> 27.2).
 #pragma unroll
@@ -427,11 +445,26 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
         for (int i = 0, buf = 0;; ++i) {
             bool odd = false;
             for (; i < n; ++i) {
-                wait_vmem_steps<PER, NS - 2>(n - 1 - i);  // this wave's part of tile i has landed
-                __syncthreads();                          // every wave's has, and tile i - 1 is read
-                if (i + NS - 1 < n) stage(u.x0 + i + NS - 1, buf == 0 ? NS - 1 : buf - 1);
+                const bool more = i + 1 < n;
+                bool whole = true;
+                if constexpr (APART) {
+                    if (more) wait_vmem<PER>();  // V of tile i and K of the next may be under way
+                    else wait_vmem<PER / 2>();
+                    __syncthreads();             // every wave's K of tile i has landed, V of tile i - 1 is read
+                    if (more) stage(no, yes, u.x0 + i + 1, buf ^ 1);
+                    if (some) whole = weigh(u.x0 + i, buf);
+                    if (more) wait_vmem<PER>();  // K and V of the next
+                    else wait_vmem<0>();
+                    __syncthreads();             // every wave's V of tile i has landed, its K is read
+                    if (i + 2 < n) stage(yes, no, u.x0 + i + 2, buf);
+                } else {
+                    wait_vmem_steps<PER, NS - 2>(n - 1 - i);  // this wave's part of tile i has landed
+                    __syncthreads();                          // every wave's has, and tile i - 1 is read
+                    if (i + NS - 1 < n) stage(yes, yes, u.x0 + i + NS - 1, buf == 0 ? NS - 1 : buf - 1);
+                    if (some) whole = weigh(u.x0 + i, buf);
+                }
                 if (some) {
-                    odd = weigh(u.x0 + i, buf);
+                    odd = !whole && look(buf);
                     if (odd) break;
                     add(buf);
                 }
