@@ -230,7 +230,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
                 win_slot = g.slot, win_page = p0;
                 window = load_page_window(a.kv, win_slot, win_page, lane);
             }
-            if constexpr (D < 512) {  // (head_dim 512 has no scalar registers left)
+            if constexpr (D < 512) {  // (at 512 a shuffle a row is as fast)
                 page0 = __builtin_amdgcn_readlane(window, p0 - win_page);
                 page1 = __builtin_amdgcn_readlane(window, p1 - win_page);
             }
