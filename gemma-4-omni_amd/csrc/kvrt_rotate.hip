@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "kvrt.h"
 #include "kvrt_device.h"
@@ -42,6 +43,14 @@ constexpr int kMaxAxes = 4;
 // thousand 4.5 and 4.9, 197 thousand 5.6 and 5.3, 1 million 18.1 and 13.0; the other dims
 // cross at the same place.
 constexpr int64_t kOneHeadLanes = 160 * 1024;
+// Calls past that store around the L2, whose 32 MB would be written back after the last lane
+// has ended, and calls of more than this many lanes (32 bytes each, in and out) load around it
+// too, so that what was read does not push the answers out of the last cache. us a call, and
+// of it and a reader of its query heads, head_dim 128, 16 + 8 heads, by MB of answers:
+//   plain 8.4 6.4 / 11.0, 25 12.2 / 18.4, 101 46.1 / 65.9, 403 162 / 246
+//   stores around 5.7 / 10.2, 10.7 / 18.4, 43.0 / 67.2, 154 / 254
+//   stores and loads 5.8 / 10.4, 10.2 / 19.0, 43.1 / 64.9, 149 / 238
+constexpr int64_t kLargeLanes = 1024 * 1024;
 
 struct RotateArgs {
     const uint16_t *src[kKinds];
@@ -63,14 +72,13 @@ struct RotateArgs {
     float eps, scaling;
 };
 
-__device__ __forceinline__ void widen(uint4 x, float *f) {
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void widen(u32x4_t x, float *f) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[2 * i] = bf16_lo(w[i]), f[2 * i + 1] = bf16_hi(w[i]);
+    for (int i = 0; i < 4; ++i) f[2 * i] = bf16_lo(x[i]), f[2 * i + 1] = bf16_hi(x[i]);
 }
-__device__ __forceinline__ uint4 narrow(const float *f) {
-    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                      pack_bf16x2(f[6], f[7]));
+__device__ __forceinline__ u32x4_t narrow(const float *f) {
+    return (u32x4_t){pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
 }
 
 // Position p on axis `axis` of a token.
@@ -81,7 +89,7 @@ __device__ __forceinline__ int position(const RotateArgs &a, int axis, int item,
 
 }  // namespace
 
-template <int D, int PER, bool ADJACENT>
+template <int D, int PER, bool ADJACENT, bool LARGE>
 __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
     constexpr int LANES = D / 16;
     const uint32_t group = (blockIdx.x * 256u + threadIdx.x) / LANES;
@@ -107,12 +115,18 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
     const int64_t s_head = pick(a.s_head), d_head = pick(a.d_head);
     const uint16_t *src = pick(a.src) + item * pick(a.s_item) + row * pick(a.s_row) + h0 * s_head;
     uint16_t *dst = pick(a.dst) + item * pick(a.d_item) + row * pick(a.d_row) + h0 * d_head;
-    uint4 x[PER][2];
+    u32x4_t x[PER][2];
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
         const uint16_t *p = src + min(u, heads - 1 - h0) * s_head;  // past the last head: the last once more
-        x[u][0] = *reinterpret_cast<const uint4 *>(p + lo);
-        x[u][1] = *reinterpret_cast<const uint4 *>(p + hi);
+        const auto *one = reinterpret_cast<const u32x4_t *>(p + lo), *two = reinterpret_cast<const u32x4_t *>(p + hi);
+        if constexpr (LARGE) {
+            x[u][0] = __builtin_nontemporal_load(one);
+            x[u][1] = __builtin_nontemporal_load(two);
+        } else {
+            x[u][0] = *one;
+            x[u][1] = *two;
+        }
     }
     const bool normed = (a.norm >> (is_q ? 0 : is_k ? 1 : 2)) & 1;
     const float *weight = is_q ? a.weight[0] : is_k ? a.weight[1] : nullptr;
@@ -182,8 +196,14 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
             two = fmaf(two, c[i], t * s[i]);
         }
         if (h0 + u < heads) {
-            *reinterpret_cast<uint4 *>(dst + u * d_head + lo) = narrow(y);
-            *reinterpret_cast<uint4 *>(dst + u * d_head + hi) = narrow(y + 8);
+            auto *one = reinterpret_cast<u32x4_t *>(dst + u * d_head + lo), *two = reinterpret_cast<u32x4_t *>(dst + u * d_head + hi);
+            if constexpr (PER > 1) {
+                __builtin_nontemporal_store(narrow(y), one);
+                __builtin_nontemporal_store(narrow(y + 8), two);
+            } else {
+                *one = narrow(y);
+                *two = narrow(y + 8);
+            }
         }
     }
 }
@@ -191,18 +211,20 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
 namespace {
 
 template <int D>
-hipError_t launch_rotate(RotateArgs &a, int64_t tokens, int per, bool adjacent, hipStream_t s) {
+hipError_t launch_rotate(RotateArgs &a, int64_t tokens, int per, bool large, bool adjacent, hipStream_t s) {
     int all = 0;
     for (int i = 0; i < kKinds; ++i) all += a.chunks[i] = (a.heads[i] + per - 1) / per;
     a.groups = (uint32_t)(tokens * all);
     const dim3 grid((unsigned)((tokens * all * (D / 16) + 255) / 256));
-    if (per == 1) {
-        if (adjacent) hipLaunchKernelGGL((rotate_kernel<D, 1, true>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((rotate_kernel<D, 1, false>), grid, dim3(256), 0, s, a);
-    } else {
-        if (adjacent) hipLaunchKernelGGL((rotate_kernel<D, 4, true>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((rotate_kernel<D, 4, false>), grid, dim3(256), 0, s, a);
-    }
+    const auto launch = [&](auto per_c, auto large_c) {
+        constexpr int PER = decltype(per_c)::value;
+        constexpr bool LARGE = decltype(large_c)::value;
+        if (adjacent) hipLaunchKernelGGL((rotate_kernel<D, PER, true, LARGE>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((rotate_kernel<D, PER, false, LARGE>), grid, dim3(256), 0, s, a);
+    };
+    if (per == 1) launch(std::integral_constant<int, 1>{}, std::false_type{});
+    else if (!large) launch(std::integral_constant<int, 4>{}, std::false_type{});
+    else launch(std::integral_constant<int, 4>{}, std::true_type{});
     return hipGetLastError();
 }
 
@@ -304,14 +326,16 @@ int kvrt_rotate_heads_async(const kvrt_rotation *rot, const kvrt_tensor *q, cons
     a.scaling = rot->scaling;
     const int64_t tokens = n * rows;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const int per = tokens * heads * (D / 16) <= kOneHeadLanes ? 1 : 4;
+    const int64_t lanes = tokens * heads * (D / 16);
+    const int per = lanes <= kOneHeadLanes ? 1 : 4;
+    const bool large = lanes > kLargeLanes;
     const bool adj = rot->adjacent != 0;
     hipError_t e;
     switch (D) {
-        case 64: e = launch_rotate<64>(a, tokens, per, adj, s); break;
-        case 128: e = launch_rotate<128>(a, tokens, per, adj, s); break;
-        case 256: e = launch_rotate<256>(a, tokens, per, adj, s); break;
-        default: e = launch_rotate<512>(a, tokens, per, adj, s); break;
+        case 64: e = launch_rotate<64>(a, tokens, per, large, adj, s); break;
+        case 128: e = launch_rotate<128>(a, tokens, per, large, adj, s); break;
+        case 256: e = launch_rotate<256>(a, tokens, per, large, adj, s); break;
+        default: e = launch_rotate<512>(a, tokens, per, large, adj, s); break;
     }
     return e == hipSuccess ? KVRT_OK : KVRT_EDEVICE;
 }

@@ -275,3 +275,27 @@ def test_magnitudes_whose_squares_leave_fp32(eps, d):
     want, tol = _reference(x, "q", (freq, [0] * (d // 2), False, "qk", w, f32, 1.0), pos)
     # answers below fp32's normal numbers round to a step of bf16's smallest, 2^-133
     assert bool(((got.double() - want).abs() <= tol + 2.0 ** -133).all())
+
+
+@pytest.mark.parametrize("d,hq,hkv,tokens,adjacent", [(128, 7, 2, 2400, False), (512, 5, 1, 1000, True),
+                                                      (64, 9, 3, 23000, True), (256, 13, 5, 3700, False)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_long_prompts_of_any_number_of_heads(d, hq, hkv, tokens, adjacent, in_place):
+    """Heads in groups of four with one to three left over, from views of a projection, in
+    calls of up to a million lanes and of more."""
+    from kvrt import HeadRotation
+
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    x = torch.randn(1, tokens, hq + 2 * hkv, d, generator=gen, device="cuda").to(BF16)
+    q, k, v = (t.transpose(1, 2) for t in x.split([hq, hkv, hkv], 2))
+    freq = _freqs(d // 2)
+    w = torch.rand(d, generator=gen, device="cuda") + 0.5
+    rot = HeadRotation(d, freq, adjacent=adjacent, norm="qkv", q_weight=w, k_weight=w.flip(0))
+    pos = _positions(gen, 1, 1, tokens, 100000)
+    before = x.clone()
+    got = rot.apply(q, k, v, positions=pos, out=(q, k, v) if in_place else None)
+    eps = torch.tensor(1e-6, dtype=torch.float32).item()
+    for kind, g, src, weight in zip("qkv", got, before.split([hq, hkv, hkv], 2), (w, w.flip(0), None)):
+        _check(g, src.transpose(1, 2), kind, (freq, [0] * (d // 2), adjacent, "qkv", weight, eps, 1.0), pos)
+    if not in_place:
+        assert torch.equal(x, before)
