@@ -2461,6 +2461,7 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
     a.capacity = cap;
     a.prefix_slot = prefix_slot;
     for (int i = 0; i < n; ++i) a.slots[i] = slots[i];
+    a.large = (all_own + pre_keys) * hkv * D * 4 > (int64_t)128 << 20;
     // the prefix's keys once for the rows of all items, or for each item with its own keys
     // (also where no row sees the prefix now: a replay may find it otherwise)
     double time = shared_plan(a, D, pre_keys, own_keys, shared);

@@ -32,6 +32,7 @@ struct SharedArgs {
     int pre_tiles, pre_splits, own_tiles, own_splits, joined;
     int own_per, own_wgs;
     int parts;                // partials of a row; 1: units write the answer
+    int large;                // the rows of K and V seen are more than half the last cache
     int slots[kMaxItems];
 };
 

@@ -49,9 +49,17 @@
 
 namespace kvrt {
 
-// LDS DMA of 16 bytes per lane from base + off (bytes), base uniform.
+// LDS DMA of 16 bytes per lane from base + off (bytes), base uniform; ONCE: of rows that are
+// not read again.
+template <bool ONCE>
 __device__ __forceinline__ void shared_dma(const void *base, uint32_t off, uint32_t lds) {
-    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+    if constexpr (ONCE) asm volatile("global_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+    else asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+}
+template <bool ONCE>
+__device__ __forceinline__ void shared_dma(const void *at, uint32_t lds) {
+    if constexpr (ONCE) dma_load16(at, lds);
+    else dma_load16_cached(at, lds);
 }
 
 __device__ __forceinline__ f32x4_t mfma_bf16(uint4 a, uint4 b, f32x4_t c) {
@@ -136,6 +144,7 @@ __device__ __forceinline__ Segment segment_of(int slot, int len, int off, int mi
 struct SharedUnit {
     Segment pre, own;
     int kvh, row0, nrows, x0, x1, part;
+    bool once;  // no other unit reads its rows
     int lens;  // lane i: length of item i
 };
 
@@ -212,8 +221,8 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
         key0 = (g.tile0 + (own ? x - u.pre.tiles : x)) * kSharedKeys;
         return g;
     };
-    auto stage = [&](auto of_k, auto of_v, int x, int buf) __attribute__((always_inline)) {
-        constexpr bool OF_K = decltype(of_k)::value, OF_V = decltype(of_v)::value;
+    auto stage_as = [&](auto once_c, auto of_k, auto of_v, int x, int buf) __attribute__((always_inline)) {
+        constexpr bool ONCE = decltype(once_c)::value, OF_K = decltype(of_k)::value, OF_V = decltype(of_v)::value;
         int key0;
         const Segment &g = where(x, key0);
         const int64_t head = LAYOUT == KVRT_LAYOUT_PAGED
@@ -244,8 +253,8 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
             if constexpr (LAYOUT == KVRT_LAYOUT_CONTIG) {
                 const int64_t base = head + (int64_t)key0 * D;
                 const uint32_t at = (uint32_t)(key - key0) * (2 * D);
-                if constexpr (OF_K) shared_dma(kg + base, at + 16 * (c ^ S::kx(sub)), kto);
-                if constexpr (OF_V) shared_dma(vg + base, at + 16 * c, vto);
+                if constexpr (OF_K) shared_dma<ONCE>(kg + base, at + 16 * (c ^ S::kx(sub)), kto);
+                if constexpr (OF_V) shared_dma<ONCE>(vg + base, at + 16 * c, vto);
                 continue;
             } else if constexpr (LAYOUT == KVRT_LAYOUT_RING) {
                 int rr = ring0 + (key - key0);
@@ -259,9 +268,14 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
                 bad |= off < 0;
                 off = off < 0 ? 0 : off;
             }
-            if constexpr (OF_K) dma_load16_cached(kg + off + 8 * (c ^ S::kx(sub)), kto);
-            if constexpr (OF_V) dma_load16_cached(vg + off + 8 * c, vto);
+            if constexpr (OF_K) shared_dma<ONCE>(kg + off + 8 * (c ^ S::kx(sub)), kto);
+            if constexpr (OF_V) shared_dma<ONCE>(vg + off + 8 * c, vto);
         }
+    };
+
+    auto stage = [&](auto of_k, auto of_v, int x, int buf) __attribute__((always_inline)) {
+        if (LAYOUT != KVRT_LAYOUT_PAGED && u.once) stage_as(std::true_type{}, of_k, of_v, x, buf);
+        else stage_as(std::false_type{}, of_k, of_v, x, buf);
     };
 
     // ---- one tile
@@ -584,6 +598,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void shared_at
         u.own = segment_of(a.slots[item], len, 0, minpos, maxpos, a.window);
         u.pre = segment_of(a.prefix_slot, a.joined ? prefix : 0, prefix, minpos, maxpos, a.window);
     }
+    // In calls that outgrow the last cache, rows that one unit reads pass the caches by (64
+    // sessions behind 4096 rows 55.9 -> 52.3 us a call, 4 of 8192 at head_dim 512 106 -> 97). In
+    // smaller ones the next call finds them there (8 of 8 rows behind 8192 at 512 27.7 us, 29.2
+    // past the caches), as other units find what several read (16 behind 4096 28 and 32).
+    u.once = LAYOUT != KVRT_LAYOUT_PAGED && a.large && (pre ? a.pre_tiles == 1 : a.own_tiles == 1 && !a.joined);
     const int tiles = u.pre.tiles + u.own.tiles, per = (tiles + splits - 1) / splits;
     u.x0 = min(ks * per, tiles);
     u.x1 = min(u.x0 + per, tiles);

@@ -593,3 +593,19 @@ def test_calls_on_another_stream():
             s.rt.synchronize()
         torch.cuda.synchronize()
         assert torch.equal(here, there)
+
+
+@pytest.mark.parametrize("d,lens,prefix,layout,window", [(128, [9000, 8000, 7], 20000, "contig", 0),
+                                                         (512, [3000, 2500, 1], 5000, "contig", 0),
+                                                         (64, [20000, 40000, 33], 17000, "ring", 50000)])
+def test_calls_that_outgrow_the_caches(d, lens, prefix, layout, window):
+    gen = _gen(25)
+    s = Sessions(gen, lens, prefix, hkv=8, d=d, layout=layout, window=window)
+    for qn, masked in ((1, False), (1, True)):
+        q = _q(gen, 3, 16, qn, d)
+        masks = None
+        if masked:
+            masks = [None, None, None, torch.rand(500, generator=gen, device="cuda") < 0.5]
+            s.rt.set_prefix_attention(3, masks[3])
+        s.check(s.rt.attend_shared(0, q, range(3), 0.1, prefix_slot=3), q, 0.1, masks=masks)
+    assert s.rt.health() == 0
