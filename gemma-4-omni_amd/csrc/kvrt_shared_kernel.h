@@ -37,8 +37,8 @@
 // and 128 two, by kx) and a constant.
 //
 // What bounds it: with many sessions or keys the bytes (64 sessions, one row each, 8 KV heads
-// of 128, behind 4096 rows: 245 MB in 53 us, 4.6 TB/s, and 4.7 us of joins; 16 paged ones
-// behind 1024: 119 MB in 27 us, 4.4 TB/s; a copy of 1 GiB 5.1). With few, the chain of a
+// of 128, behind 4096 rows: 245 MB in 48.6 us, 5.0 TB/s, and 4.6 us of joins; 16 paged ones
+// behind 1024: 119 MB in 28 us, 4.2 TB/s; a copy of 1 GiB 5.1). With few, the chain of a
 // unit: launch, lengths, first bytes, 0.8 us a tile of 16 rows at head_dim 128 (2.4 of 64 rows
 // at 512, where a tile's reads from LDS last as long), and the join's launch (four sessions
 // behind 2048 rows: 7.1 + 3.6 us).
@@ -599,7 +599,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void shared_at
         u.pre = segment_of(a.prefix_slot, a.joined ? prefix : 0, prefix, minpos, maxpos, a.window);
     }
     // In calls that outgrow the last cache, rows that one unit reads pass the caches by (64
-    // sessions behind 4096 rows 55.9 -> 52.3 us a call, 4 of 8192 at head_dim 512 106 -> 97). In
+    // sessions behind 4096 rows 55.9 -> 52.0 us a call, 4 of 8192 at head_dim 512 106 -> 97). In
     // smaller ones the next call finds them there (8 of 8 rows behind 8192 at 512 27.7 us, 29.2
     // past the caches), as other units find what several read (16 behind 4096 28 and 32).
     u.once = LAYOUT != KVRT_LAYOUT_PAGED && a.large && (pre ? a.pre_tiles == 1 : a.own_tiles == 1 && !a.joined);
