@@ -6,8 +6,8 @@
 // the prefix first, so that the only new work of a block is whose slot it lies in, and, where
 // asked for, the scores' cap and bias. A block that some rows see in part is looked through
 // for NaN and infinities in V once, on its way to the product.
-// Measured: 4 x 512 queries of 16 heads of 128 behind 1400 rows and 577 to 700 of their own 57
-// us, 520 TFLOP/s with P counted once (the tiles of kvrt_shared_kernel.h 75 and a join of 11;
+// Measured: 4 x 512 queries of 16 heads of 128 behind 1400 rows and 577 to 700 of their own 55
+// us, 545 TFLOP/s with P counted once (the tiles of kvrt_shared_kernel.h 75 and a join of 11;
 // the same chunk over prefixes cloned into each session 54); 2 x 291 capped ones over 2000 22
 // and a merge of 4.6. Bound by matrix and vector instructions that in part follow each other.
 #include "kvrt_prefill.h"
