@@ -111,6 +111,35 @@ __device__ __forceinline__ void scale_accs(f32x16_t (&o)[D / 32], float c) {
     }
 }
 
+// none += 0 * o for every accumulator: NaN where one is no number. At head_dim 512 as above.
+template <int D>
+__device__ __forceinline__ void add_zeros(f32x16_t (&o)[D / 32], float &none) {
+    if constexpr (D < 512) {
+        float x[4] = {};  // (one sum alone is a chain of as many instructions)
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i & 3] = fmaf(o[b][i], 0.f, x[i & 3]);
+        none += (x[0] + x[1]) + (x[2] + x[3]);
+    } else {
+        float t, t2, more = 0.f;
+        asm volatile(
+            "s_nop 15\n\t"
+            ".set kvrt_i, 0\n\t"
+            ".rept 128\n\t"
+            "v_accvgpr_read_b32 %16, a[kvrt_i]\n\t"
+            "v_accvgpr_read_b32 %17, a[kvrt_i + 1]\n\t"
+            "v_fma_f32 %18, %16, 0, %18\n\t"
+            "v_fma_f32 %19, %17, 0, %19\n\t"
+            ".set kvrt_i, kvrt_i + 2\n\t"
+            ".endr"
+            : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]), "+a"(o[6]), "+a"(o[7]),
+              "+a"(o[8]), "+a"(o[9]), "+a"(o[10]), "+a"(o[11]), "+a"(o[12]), "+a"(o[13]), "+a"(o[14]), "+a"(o[15]),
+              "=&v"(t), "=&v"(t2), "+v"(none), "+v"(more));
+        none += more;
+    }
+}
+
 // LDS DMA of 16 bytes per lane from base + off (bytes): the tile's address is
 // uniform and a lane's offset fixed, so a DMA costs no 64-bit lane arithmetic.
 __device__ __forceinline__ void dma_load16_at(const void *base, uint32_t off, uint32_t lds) {
@@ -159,8 +188,7 @@ __device__ __forceinline__ int shared_slot(const SharedChunkArgs &a) { return ma
 
 // One row of a SHARED tile, by one wave without matrix instructions, so that rows of K and V
 // that it does not see do not touch it whatever they hold: keys over lanes for the scores,
-// dims over lanes for the values. It runs where a tile meets NaN or infinities among rows
-// that some of its queries do not see.
+// dims over lanes for the values. It runs where the matrix products met NaN or infinities in V.
 template <int D, int LAYOUT>
 __device__ __forceinline__ void shared_row(const SharedChunkArgs &a, int item, int kvh, int row, int L, int P, int own0,
                                            int kstart, int kend, int nks, int ks, int lane) {
@@ -181,10 +209,7 @@ __device__ __forceinline__ void shared_row(const SharedChunkArgs &a, int item, i
         return row_offset<LAYOUT>(a.kv, own ? slot : shared_slot(a), kvh, own ? k - own0 : k, D);
     };
     const auto score = [&](int k, int64_t off) __attribute__((always_inline)) {
-        if (off < 0) return -INFINITY;
-        float x = 0.f;
-#pragma clang loop unroll(disable)
-        for (int d = 0; d < D; ++d) x = fmaf(bf16_to_f32(q[d]), bf16_to_f32(kg[off + d]), x);
+        float x = dot_rows(q, kg + (off < 0 ? 0 : off), D);
         if (a.cap != 0.f) {
             float one[1] = {x};
             cap_scores<1>(one, a.inv_cap, a.cap);
@@ -192,7 +217,7 @@ __device__ __forceinline__ void shared_row(const SharedChunkArgs &a, int item, i
         } else {
             x *= a.scale_log2;
         }
-        return fmaf(slope, (float)(k - (k >= own0 ? pq : pq - gap)), x);
+        return off < 0 ? -INFINITY : fmaf(slope, (float)(k - (k >= own0 ? pq : pq - gap)), x);
     };
     float m = kNegBig, l = 0.f, acc[E];
 #pragma unroll
@@ -204,14 +229,26 @@ __device__ __forceinline__ void shared_row(const SharedChunkArgs &a, int item, i
         m = top;
         const float p = off < 0 ? 0.f : __builtin_amdgcn_exp2f(t - m);
         l = fmaf(l, c, group_sum<64>(p));
+        const uint64_t some = __ballot(off >= 0);
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] *= c;
-        for (int j = 0; j < min(64, kend - k0); ++j) {
-            const float pj = __shfl(p, j);
-            const int64_t oj = __shfl(off, j);
-            if (oj < 0) continue;
+#pragma clang loop unroll(disable)
+        for (int j = 0; j < 64; j += 4) {
+            // four keys' values under way at a time
+            uint16_t v[4][E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(pj, bf16_to_f32(vg[oj + E * lane + e]), acc[e]);
+            for (int i = 0; i < 4; ++i) {
+                const int64_t oj = __shfl(off, j + i);
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[i][e] = vg[(oj < 0 ? 0 : oj) + E * lane + e];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float pj = __shfl(p, j + i);
+                if (!(some >> (j + i) & 1u)) continue;
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = fmaf(pj, bf16_to_f32(v[i][e]), acc[e]);
+            }
         }
     }
     if (nks == 1) {
@@ -565,21 +602,21 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
             }
         }
     };
-    // Masks the scores of keys t0 .. t0 + 31 (-INFINITY); SHARED: whether there was one to mask.
+    // Masks the scores of keys t0 .. t0 + 31 (-INFINITY).
     auto mask = [&](int t0) __attribute__((always_inline)) {
         if constexpr (SHARED) {
             const bool pre = t0 < own0;
             const int sh = pre ? gap : 0, end = pre ? min(kend, P) : kend;
-            if (t0 >= vis_lo - sh && t0 + kPfKeys <= min(end, vis_hi - sh)) return false;
+            if (t0 >= vis_lo - sh && t0 + kPfKeys <= min(end, vis_hi - sh)) return;
             const int hi = min(end - 1, qvalid ? pq - sh : -1), lo = a.window > 0 ? klo - sh : 0;
             const int nhi = min(max(hi - t0 + 1, 0), 32), nlo = min(max(lo - t0, 0), 32);
             uint32_t vis = (nhi >= 32 ? 0xffffffffu : (1u << nhi) - 1u) & (nlo >= 32 ? 0u : 0xffffffffu << nlo);
             vis >>= 4 * half;
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = (vis >> (8 * (i >> 2) + (i & 3))) & 1u ? s[i] : -INFINITY;
-            return true;
+            return;
         }
-        if (t0 >= vis_lo && t0 + kPfKeys <= vis_hi) return false;
+        if (t0 >= vis_lo && t0 + kPfKeys <= vis_hi) return;
         // bit k: key t0 + k is visible to this lane's row
         const int nhi = min(max(khi - t0 + 1, 0), 32), nlo = min(max(klo - t0, 0), 32);
         uint32_t vis = (nhi >= 32 ? 0xffffffffu : (1u << nhi) - 1u) & (nlo >= 32 ? 0u : 0xffffffffu << nlo);
@@ -593,27 +630,6 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
         vis >>= 4 * half;  // this half's keys: bit 8 (i / 4) + i % 4
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = (vis >> (8 * (i >> 2) + (i & 3))) & 1u ? s[i] : -INFINITY;
-        return true;
-    };
-    // SHARED: a block that some rows do not see whole, whose V holds NaN or infinities (0 * NaN
-    // is not 0): the tile is then computed again, row by row.
-    bool partly = false;  // the block whose P V is next
-    uint32_t odd = 0;
-    auto look = [&](int vblk) __attribute__((always_inline)) {
-        if constexpr (SHARED) {
-            if (!partly) return;
-            typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
-            u16x2_t most = {0, 0};
-#pragma clang loop unroll_count(4)
-            for (int i = 0; i < IPB; ++i) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(&sv[vblk * VBLK + i * kPfVPitch + 16 * lane]);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, w[e] & 0x7fff7fffu));
-            }
-            odd |= most[0] >= 0x7f80 || most[1] >= 0x7f80 ? 1u : 0u;
-        }
     };
     // The softmax of s in NSOFT steps. The running max moves only where a
     // block's max exceeds it by kRescaleSlack; corr rescales what has been
@@ -713,7 +729,7 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
         if (jlo == 0 && jhi > 0) {
             score_steps(part, 0, std::true_type{});
             make(key0(0));
-            partly = mask(key0(0));
+            mask(key0(0));
             StaticFor<0, NSOFT>::run(soft_step);
             take_p();
         }
@@ -728,11 +744,10 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
             cur = it;
             const bool do_s = it + 1 >= jlo && it + 1 < jhi, do_v = it >= jlo && it < jhi;
             const int kblk = ((it + 1) % NS) * KS + part, vblk = (it % NS) * KS + part;
-            if (do_v) look(vblk);
             if (do_s) {
                 score_steps(kblk, vblk, std::false_type{});
                 make(key0(it + 1));
-                partly = mask(key0(it + 1));
+                mask(key0(it + 1));
             } else {
                 if (it + 1 < ngroups) StaticFor<0, NK>::run(dma_at);
 #pragma unroll
@@ -757,6 +772,13 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
     for (int b = 0; b < NB; ++b) keep_acc<D>(o[b]);
     if (bad) a.err[0] = 1;
     if constexpr (SHARED) {
+        // NaN or an infinity in V gives NaN in a row that does not see it (0 * NaN), and in one that
+        // does where the low term of its weight is 0 or below (inf * 0, inf - inf), which the row
+        // path makes an infinity. Rows whose scores are not numbers are NaN as they are.
+        float none = 0.f;
+        add_zeros<D>(o, none);
+        const float sum = pair<OpSum, 32>(l);
+        const bool odd = qvalid && none != none && sum == sum;
         if (threadIdx.x == 0) again = 0;
         __syncthreads();  // (and every wave is done with the buffers)
         if (odd) again = 1;

@@ -4,8 +4,8 @@
 // The prefill's tiles as they are: 32 rows of (query, head) a wave on 32x32 matrix
 // instructions, online softmax, P in two bf16 terms. Keys are numbered in whole blocks of 32,
 // the prefix first, so that the only new work of a block is whose slot it lies in, and, where
-// asked for, the scores' cap and bias. A block that some rows see in part is looked through
-// for NaN and infinities in V once, on its way to the product.
+// asked for, the scores' cap and bias. A tile that ends with NaN in a row whose scores are
+// numbers met NaN or infinities in V, and is computed again row by row.
 // Measured: 4 x 512 queries of 16 heads of 128 behind 1400 rows and 577 to 700 of their own 55
 // us, 545 TFLOP/s with P counted once (the tiles of kvrt_shared_kernel.h 75 and a join of 11;
 // the same chunk over prefixes cloned into each session 54); 2 x 291 capped ones over 2000 22

@@ -148,6 +148,76 @@ struct SharedUnit {
     int lens;  // lane i: length of item i
 };
 
+// Outputs dim0 .. dim0 + DIMS - 1 of row f of a unit by one wave, each key's weight one fp32
+// number, 2^(score - m); those that are not numbers are stored. Keys over lanes and halves of the
+// dims over halves of the wave for the scores; dims over lanes for the values. The arguments are
+// read again here, so that the loop over the tiles holds no registers for a row that may never
+// come.
+template <int D, int LAYOUT, int DIMS>
+__device__ __forceinline__ void row_again(const SharedUnit &u, int f, int dim0, float m, float sum, int lane) {
+    constexpr int E = (DIMS + 63) / 64;  // dims per lane
+    uint64_t args = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+    asm volatile("" : "+s"(args));
+    const auto &a = *reinterpret_cast<const SharedArgs __attribute__((address_space(4))) *>(args);
+    const int per_item = a.group * a.qn;
+    int item, rem, qr, hr;
+    udivmod_uniform(f, per_item, item, rem);
+    udivmod_uniform(rem, a.group, qr, hr);
+    const int head = u.kvh * a.group + hr;
+    const int len = min(max(a.len.lens[(int64_t)a.slots[item] * a.len.stride + a.len.offset], 0), a.capacity);
+    const int pos = len - a.qn + qr;
+    KVView kv;
+    kv.k = a.kv.k, kv.v = a.kv.v, kv.page_table = a.kv.page_table;
+    kv.slot_stride = a.kv.slot_stride, kv.head_stride = a.kv.head_stride, kv.row_stride = a.kv.row_stride;
+    kv.kv_heads = a.kv.kv_heads, kv.rows = a.kv.rows, kv.pt_stride = a.kv.pt_stride;
+    kv.block_shift = a.kv.block_shift, kv.pool_pages = a.kv.pool_pages;
+    const int64_t row = ((int64_t)item * (a.kv.kv_heads * a.group) + head) * a.qn + qr;
+    const auto *kg = static_cast<const uint16_t *>(a.kv.k), *vg = static_cast<const uint16_t *>(a.kv.v);
+    const int half = D / 2 * (lane >> 5);
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma clang loop unroll(disable)
+    for (int x = u.x0; x < u.x1; ++x) {
+        const bool own = x >= u.pre.tiles;
+        const int tile = own ? u.own.tile0 + x - u.pre.tiles : u.pre.tile0 + x;
+        const int slot = own ? u.own.slot : u.pre.slot, at = pos + (own ? u.own.off : u.pre.off);
+        const int lo = own ? u.own.lo : u.pre.lo, last = own ? u.own.last : u.pre.last;
+        const int key = tile * kSharedKeys + (lane & 31);
+        bool seen = key >= lo && key <= min(at, last) && (a.window == 0 || key > at - a.window);
+        if (a.pmask && key < a.pmask[slot].len) seen &= (a.pmask[slot].bits[(key >> 5) & (kPrefixWords - 1)] >> (key & 31) & 1u) != 0;
+        const int64_t off = seen ? row_offset<LAYOUT>(kv, slot, u.kvh, key, D) : -1;  // (-1: its page is not mapped)
+        float t = pair<OpSum, 32>(dot_rows(a.q + row * D + half, kg + (off < 0 ? 0 : off) + half, D / 2));
+        if (a.cap != 0.f) {
+            float one[1] = {t};
+            cap_scores<1>(one, a.inv_cap, a.cap);
+            t = one[0];
+        } else {
+            t *= a.scale;
+        }
+        if (a.slopes) t = fmaf(a.slopes[head] * 1.4426950408889634f, (float)(key - at), t);
+        const float p = off < 0 ? 0.f : __builtin_amdgcn_exp2f(t - m);
+        const uint32_t some = (uint32_t)__ballot(off >= 0);
+#pragma clang loop unroll(disable)
+        for (int j = 0; j < kSharedKeys; ++j) {
+            const float w = __shfl(p, j);
+            const uint16_t *v = vg + __shfl(off, j) + dim0;
+            if (!(some >> j & 1u)) continue;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (64 * e + lane < DIMS) acc[e] = fmaf(w, bf16_to_f32(v[64 * e + lane]), acc[e]);
+        }
+    }
+    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int d = 64 * e + lane;
+        if (d >= DIMS || acc[e] - acc[e] == 0.f) continue;
+        if (a.parts == 1) a.out[row * D + dim0 + d] = f32_to_bf16(acc[e] * inv);
+        else a.part_o[(((int64_t)u.kvh * a.n_items * per_item + f) * a.parts + u.part) * D + dim0 + d] = acc[e];
+    }
+}
+
 // BLOCKS: 16-row blocks per wave, of the unit's blocks wave, wave + 4 (past its last one
 // they are computed and not stored: a branch would part the matrix instructions); 0: the
 // unit has one, which all waves share.
@@ -215,16 +285,20 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
     // PAGED: entry `lane` past win_page of the table of slot win_slot, loaded again where a tile
     // leaves it (64 pages: every 32 tiles at 16 keys a page)
     int window = -1, win_slot = -1, win_page = 0;
-    auto where = [&](int x, int &key0) __attribute__((always_inline)) -> const Segment & {
+    auto where = [&](int x, int &key0) __attribute__((always_inline)) {
         const bool own = x >= u.pre.tiles;
-        const Segment &g = own ? u.own : u.pre;
-        key0 = (g.tile0 + (own ? x - u.pre.tiles : x)) * kSharedKeys;
+        const auto pick = [&](int pre, int its) __attribute__((always_inline)) { return own ? its : pre; };
+        Segment g;
+        g.slot = pick(u.pre.slot, u.own.slot), g.lo = pick(u.pre.lo, u.own.lo), g.last = pick(u.pre.last, u.own.last);
+        g.off = pick(u.pre.off, u.own.off), g.all_lo = pick(u.pre.all_lo, u.own.all_lo);
+        g.all_hi = pick(u.pre.all_hi, u.own.all_hi);
+        key0 = ((own ? u.own.tile0 - u.pre.tiles : u.pre.tile0) + x) * kSharedKeys;
         return g;
     };
     auto stage_as = [&](auto once_c, auto of_k, auto of_v, int x, int buf) __attribute__((always_inline)) {
         constexpr bool ONCE = decltype(once_c)::value, OF_K = decltype(of_k)::value, OF_V = decltype(of_v)::value;
         int key0;
-        const Segment &g = where(x, key0);
+        const Segment g = where(x, key0);
         const int64_t head = LAYOUT == KVRT_LAYOUT_PAGED
                                  ? 0
                                  : (int64_t)g.slot * a.kv.slot_stride + (int64_t)u.kvh * a.kv.head_stride;
@@ -312,7 +386,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
             }
         __builtin_amdgcn_sched_barrier(0);
         int key0;
-        const Segment &g = where(x, key0);
+        const Segment g = where(x, key0);
         const bool own = x >= u.pre.tiles;
         const int plen = own ? plen_o : plen_p;
         const bool whole = key0 >= g.all_lo && key0 + kSharedKeys <= g.all_hi && key0 >= plen;
@@ -494,6 +568,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
     for (int s = 0; s < RS; ++s) {
         const int r = 16 * (WIDE ? wave + 4 * s : 0) + col;
         const float sum = pair<OpSum, 32>(pair<OpSum, 16>(l[s]));
+        l[s] = sum;
         if (r >= u.nrows) continue;
         const int f = u.row0 + r;
         if (a.parts == 1) {
@@ -514,6 +589,28 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
             for (int b = 0; b < NB; ++b)
                 *reinterpret_cast<float4 *>(dst + 16 * (b0 + b)) = make_float4(o[s][b][0], o[s][b][1], o[s][b][2], o[s][b][3]);
             if (grp == 0 && b0 == 0) a.part_ml[at] = make_float2(m[s], sum);
+        }
+    }
+    // A seen infinity times a weight's two terms is NaN where the low one is 0 or below (inf * 0,
+    // inf - inf), and the infinity by definition. Outputs that are not numbers, of rows whose
+    // scores are, are added up again with whole weights and stored over.
+#pragma unroll
+    for (int s = 0; s < RS; ++s) {
+        float none[4] = {};  // one NaN where an output is no number
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) none[i] = fmaf(o[s][b][i], 0.f, none[i]);
+        none[0] += none[1] + (none[2] + none[3]);
+        const uint64_t odd = __ballot(none[0] != none[0] && l[s] == l[s]);
+        if (__builtin_expect_with_probability(odd == 0, 1, 0.9999)) continue;
+        const int row0 = 16 * (WIDE ? wave + 4 * s : 0);
+        uint32_t left = (uint32_t)(odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xffffu;  // rows of the block
+        left &= u.nrows - row0 >= 16 ? 0xffffu : (1u << max(u.nrows - row0, 0)) - 1u;
+        wait_vmem<0>();  // the rows' first answers are stored
+        for (; left != 0; left &= left - 1) {
+            const int c = __builtin_ctz(left);
+            row_again<D, LAYOUT, 16 * NB>(u, u.row0 + row0 + c, 16 * b0, __shfl(m[s], c), __shfl(l[s], c), lane);
         }
     }
 }

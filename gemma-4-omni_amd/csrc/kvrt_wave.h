@@ -184,6 +184,23 @@ __device__ __forceinline__ void cap_scores(T &x, float by, float cap) {
     }
 }
 
+// Sum of n elements of q times k (16-byte aligned rows, n a multiple of 32), for rows that are
+// made without matrix instructions.
+__device__ __forceinline__ float dot_rows(const uint16_t *q, const uint16_t *k, int n) {
+    float x = 0.f;
+#pragma clang loop unroll_count(4)
+    for (int d = 0; d < n; d += 8) {
+        const uint4 a = *reinterpret_cast<const uint4 *>(q + d), b = *reinterpret_cast<const uint4 *>(k + d);
+        const uint32_t u[4] = {a.x, a.y, a.z, a.w}, w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x = fmaf(bf16_lo(u[e]), bf16_lo(w[e]), x);
+            x = fmaf(bf16_hi(u[e]), bf16_hi(w[e]), x);
+        }
+    }
+    return x;
+}
+
 // gfx950 LDS transpose read: in each group of 16 lanes, lane s gives the
 // address of 4 consecutive bf16; lane t = 4a + e receives element e of the
 // chunks of lanes a, a + 4, a + 8, a + 12.

@@ -569,7 +569,9 @@ class KVRuntime:
         read in place, once for all slots, where a clone per session would be read once
         each. ``softcap`` c > 0 caps scores, c tanh(s / c); ``slopes`` (fp32 [Hq] on the
         GPU) adds slopes[h] * (key - query position) to them. The prefix-attention masks
-        of the prefix slot and of the slots hold. bf16 layers, decode steps and chunks."""
+        of the prefix slot and of the slots hold. bf16 layers, decode steps and chunks.
+        NaN and infinities in rows that a query does not see do not reach it; an infinity
+        in V that it sees stays one."""
         require_cuda(q, "q")
         for t, name in ((q, "q"), (out, "out")):
             if t is not None and t.device != self.device:

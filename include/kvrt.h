@@ -584,6 +584,8 @@ int kvrt_attend_talker_async(kvrt_ctx *ctx, int32_t layer, int32_t n, const int3
  * layer's window over prefix and own rows together, the prefix-attention masks of
  * prefix_slot and of the slots on their own rows); a row that sees no key becomes
  * zeros, and rows that a query does not see do not reach it whatever they hold.
+ * An infinity in V that a query sees gives that infinity, or NaN beside one of the
+ * other sign (one whose weight is below fp32's range may also be missed).
  * Scores, softmax and sums in fp32, weights in two bf16 terms (2^-17 relative). Any
  * 1 <= Q <= L_i, any Hq / kv_heads; bf16 layers of every layout; a capacity of at
  * most 2^29; n * Hq * Q <= 2^22; scale and softcap finite in log2 units (times
