@@ -20,7 +20,7 @@
 
 #include "kvrt_internal.h"
 #include "kvrt_range.h"
-#include "kvrt_shared.h"
+#include "kvrt_shared_plan.h"
 
 using namespace kvrt;
 
@@ -422,25 +422,31 @@ size_t workspace_bound(const kvrt_ctx *c) {
     return best;
 }
 
-int ensure_workspace(kvrt_ctx *c, size_t bytes) {
-    if (bytes <= c->ws_bytes) return KVRT_OK;
-    // Never allocate inside a stream capture (the bound sized at create
-    // covers every call, so this only triggers if the tuning changed).
+// Grows the workspace to `bytes` or more; false, with nothing changed, in a stream capture or short
+// of memory. What it replaces is kept until the context goes (a captured graph may still use
+// it), so that it at least doubles: all of those together stay below the live one.
+bool grow_workspace(kvrt_ctx *c, size_t bytes) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(c->stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone)
-        return KVRT_ESTATE;
-    if (c->ws) {
-        c->retired_ws.push_back(c->ws);  // a captured graph may still use it
-        c->ws = nullptr;
-        c->ws_bytes = 0;
+    if (hipStreamIsCapturing(c->stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone) return false;
+    for (size_t want : {std::max({bytes, 2 * c->ws_bytes, (size_t)1 << 20}), bytes}) {
+        float *ws = nullptr;
+        if (hipMalloc(&ws, want) == hipSuccess) {
+            if (c->ws) c->retired_ws.push_back(c->ws);
+            c->ws = ws;
+            c->ws_bytes = want;
+            return true;
+        }
+        (void)hipGetLastError();  // (it would be the next launch's)
     }
-    size_t want = std::max(bytes, (size_t)1 << 20);
-    if (hipMalloc(&c->ws, want) != hipSuccess) {
-        c->ws = nullptr;
-        return poison(c);
-    }
-    c->ws_bytes = want;
-    return KVRT_OK;
+    return false;
+}
+
+// For calls that have no form without it. The bound sized at create covers the decodes, so that
+// this grows it only if their tuning changed.
+int ensure_workspace(kvrt_ctx *c, size_t bytes) {
+    if (bytes <= c->ws_bytes || grow_workspace(c, bytes)) return KVRT_OK;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(c->stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone ? KVRT_ESTATE : poison(c);
 }
 
 int visible_keys(const kvrt_layer_spec &s, int len, int q) {
@@ -1125,129 +1131,9 @@ int tensor_call_launch(TensorCall &tc, float *ws, hipStream_t st, bool single) {
 // of the fewest rows of a tile, 256 threads each).
 constexpr int kMaxSharedCapacity = 1 << 29;
 constexpr int64_t kMaxSharedRows = 1 << 22;
-constexpr int kMaxSharedParts = 128;  // key ranges of an item, and of the prefix
-constexpr double kMaxSharedUnits = 1 << 23;  // workgroups
-
-// How a call's rows and keys are divided (SharedArgs): pre_keys of the prefix are seen, and
-// own[i] of item i's rows. joined: each item's workgroups read the prefix too, as the head of
-// its own keys. The shortest time of a simple model is taken, and returned, us: a launch lasts
-// as long as its longest unit, and at least as its units' work shared by 256 CUs (two and more
-// on one overlap in part: kShare); a unit takes some us a key tile and kUnit of its own;
-// partials are joined by a second launch. The constants are fitted to 1152 measured calls
-// (1 to 16 items of 1 to 512 rows, 512 to 33768 keys), which they meet with 4 to 9 % (rms).
-double shared_plan(SharedArgs &a, int D, int64_t pre_keys, const int64_t *own, bool joined) {
-    const int hkv = a.kv.kv_heads, tile = shared_tile(D), dim = D == 64 ? 0 : D == 128 ? 1 : D == 256 ? 2 : 3;
-    const int64_t per_item = (int64_t)a.group * a.qn, rows = per_item * a.n_items;
-    const auto tiles_of = [](int64_t keys) { return (keys + kSharedKeys - 1) / kSharedKeys + (keys % kSharedKeys > 1 ? 1 : 0); };
-    const auto cost = [&](int64_t r) {
-        // up to 16 rows, up to 64, up to 128 (head_dim 64 and 128)
-        static const double us[3][4] = {{0.75, 0.8, 1.0, 1.9}, {0.8, 1.0, 1.2, 2.4}, {1.2, 1.5}};
-        return us[r <= 16 ? 0 : r <= 64 ? 1 : 2][dim];
-    };
-    // (by head_dim 64, 128, 256, 512; a launch alone is 1.5 us)
-    static const double kUnits[4] = {1.1, 4.3, 4.2, 7.1}, kJoins[4] = {3.8, 1.1, 1.4, 0.1}, kShares[4] = {0.6, 0.6, 0.87, 0.89};
-    static const double kParts[4] = {0.02, 0.01, 0.03, 0.06};  // us a part of a row
-    constexpr double kLaunch = 1.5, kJoinBytes = 3.2e6;  // us, bytes a us
-    const double kUnit = kUnits[dim], kBytes = D == 512 ? 4.6e6 : 5.2e6;
-    a.own_tiles = (int)((per_item + tile - 1) / tile);
-    a.joined = joined;
-    a.pre_tiles = a.prefix_slot < 0 || a.joined ? 0 : (int)((rows + tile - 1) / tile);
-    const int64_t pre = tiles_of(pre_keys);
-    int64_t items[kMaxItems], most = 1;
-    for (int i = 0; i < a.n_items; ++i) {
-        items[i] = std::max<int64_t>(1, tiles_of(own[i]) + (a.joined ? pre : 0));
-        most = std::max(most, items[i]);
-    }
-    const double cp = cost(std::min<int64_t>(rows, tile)), co = cost(std::min<int64_t>(per_item, tile));
-    const double share = kShares[dim] / 256;
-    int64_t all_own = 0;
-    for (int i = 0; i < a.n_items; ++i) all_own += own[i];
-    // (the 64-row tiles of one item that head_dim 256 and 512 have do not meet in the L2)
-    const double floor = (double)(all_own * (D >= 256 ? a.own_tiles : 1) + pre_keys) * hkv * D * 4 / kBytes;
-    const bool ragged = !a.joined && a.own_tiles == 1;
-    // ranges of an item of t tiles: even ones, or of `per` tiles where items differ
-    const auto ranges = [](int64_t t, int64_t per) { return std::max<int64_t>(1, (t + per - 1) / per); };
-    double best = 1e30;
-    int64_t best_pre = 1, best_per = most;
-    for (int64_t per = 1;; per = std::min(most, per + 1 + per / 4)) {
-        const int64_t splits = ranges(most, per);
-        if (splits <= kMaxSharedParts) {
-            double work = 0, units = 0;
-            for (int i = 0; i < a.n_items; ++i) {
-                const double u = (double)(ragged ? ranges(items[i], per) : splits);
-                units += u * a.own_tiles;
-                work += (items[i] * co + u * kUnit) * a.own_tiles;
-            }
-            for (int64_t pp = 1;; pp = std::min(pre, pp + 1 + pp / 4)) {
-                const int64_t ps = a.pre_tiles ? ranges(pre, pp) : 0;
-                const double c = (units + a.pre_tiles * ps) * hkv / 256;  // units on a CU, whole ones
-                if (ps <= kMaxSharedParts && (c <= kMaxSharedUnits / 256 || splits + ps <= 2)) {
-                    double all = hkv * (work + a.pre_tiles * (pre * cp + ps * kUnit)) * share;
-                    if (c > 1) all *= std::ceil(c) / c;
-                    const double longest = std::max((double)std::min(per, most) * co, a.pre_tiles ? pp * cp : 0.0) + kUnit;
-                    const int64_t parts = splits + ps;
-                    double t = std::max(all, longest);
-                    t = std::max(t, floor) + kLaunch;
-                    if (parts > 1) t += kJoins[dim] + kParts[dim] * parts + (double)rows * hkv * parts * D * 8 / kJoinBytes;
-                    if (t < best) best = t, best_pre = ps, best_per = per;
-                }
-                if (!a.pre_tiles || pp >= pre) break;
-            }
-        }
-        if (per >= most) break;
-    }
-    a.pre_splits = (int)best_pre;
-    a.own_splits = (int)ranges(most, best_per);
-    a.own_per = a.own_wgs = 0;
-    if (ragged && a.own_splits > 1) {
-        a.own_per = (int)best_per;
-        for (int i = 0; i < a.n_items; ++i) a.own_wgs += (int)ranges(items[i], best_per);
-    }
-    a.parts = a.pre_splits + a.own_splits;
-    return best;
-}
-
-// The shape of a call on the prefill's tiles (PrefillArgs: row blocks and key parts of a
-// workgroup, key ranges), for items whose rows see `keys` keys at most, `all` together, and its
-// time, us: the chain of 32-key blocks that a wave walks, in rounds of 256 workgroups that
-// overlap where LDS holds more than one to a CU, and the merge of ranges. Fitted to 5000 calls
-// (1 to 8 items of 16 to 2200 rows, 300 to 20000 keys, every shape, 1 to 32 ranges), which the
-// times meet with 4 to 8 % (rms); the shape taken is 1.5 % slower than the best on average, the
-// prefill's rule for shorter chunks 10 %.
-double chunk_shape(SharedChunkArgs &a, int D, int64_t keys, int64_t all) {
-    struct Shape {
-        int rw, parts;
-        double block, paged, more;  // us a block, the same for PAGED, ... times workgroups on a CU
-        double base, merge, bytes;  // us, us, bytes a us of the partials
-    };
-    static const Shape kShapes[4][4] = {
-        {{4, 1, 0.67, 0.85, 0.62, 5.7, 2.3, 3.1e6}, {2, 2, 0.67, 0.9, 0.65, 6.3, 2.2, 2.7e6},
-         {2, 4, 0.96, 1.2, 1.0, 6.9, 1.9, 1.6e6}, {1, 4, 0.74, 0, 0.76, 6.0, 2.1, 1.9e6}},
-        {{4, 1, 0.78, 1.0, 0.73, 7.2, 2.0, 3.6e6}, {2, 2, 0.82, 1.08, 0.75, 7.5, 1.9, 3.0e6},
-         {2, 4, 1.25, 1.55, 1.0, 8.5, 1.6, 2.0e6}, {1, 4, 1.05, 0, 1.0, 7.2, 1.3, 1.6e6}},
-        {{4, 1, 1.19, 1.42, 1.0, 9.0, 2.2, 3.9e6}, {2, 2, 1.25, 1.55, 1.0, 11.1, 1.1, 2.9e6}},
-        {{4, 1, 2.0, 2.25, 1.0, 15.0, 1.0, 4.4e6}},
-    };
-    const int hkv = a.kv.kv_heads, dim = D == 64 ? 0 : D == 128 ? 1 : D == 256 ? 2 : 3;
-    const bool paged = a.kv.layout == KVRT_LAYOUT_PAGED;
-    const int64_t rows = (int64_t)a.group * a.qn, blocks = (keys + kPfKeys - 1) / kPfKeys;
-    const double read = (double)all * hkv * D * 4 / 5.2e6;
-    double best = 1e30;
-    for (const Shape &s : kShapes[dim]) {
-        const int64_t tiles = s.rw ? (rows + 32 * s.rw - 1) / (32 * s.rw) : 0;
-        if (s.rw == 0 || (paged && s.paged == 0) || tiles > 65535) continue;  // (a grid's third dimension)
-        for (int64_t nks = 1; nks == 1 || (nks <= 32 && nks * 2 <= blocks); nks += 1 + nks / 4) {
-            const int64_t chain = ((blocks + nks - 1) / nks + s.parts - 1) / s.parts;
-            const int64_t round = (tiles * hkv * a.n_items * nks + 255) / 256;
-            const double walk = chain * (paged ? s.paged : s.block) * std::max(1.0, round * s.more);
-            // (up to head_dim 128 they overlap in part)
-            double t = std::max(walk, read) + (D <= 128 ? 0.2 : 0.0) * std::min(walk, read) + s.base;
-            if (nks > 1) t += s.merge + (double)rows * a.n_items * hkv * nks * D * 8 / s.bytes;
-            if (t < best) best = t, a.row_waves = s.rw, a.key_parts = s.parts, a.n_ksplit = (int)nks;
-        }
-    }
-    return best;
-}
+// Bytes of partials that a call may grow the workspace for (of 20 thousand random calls 1 in 84
+// would take more, the model finds them 0.07 % longer on average).
+constexpr size_t kMaxSharedRoom = (size_t)256 << 20;
 
 }  // namespace
 
@@ -2349,22 +2235,19 @@ int kvrt_attend_prefill_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32
     a.key_parts = parts;
     // Key ranges: as many as keep the grid within one round of 256 workgroups
     // (Q 291 at head_dim 512 over 2339 keys, 4 streams: 156 us unsplit, 99 / 87 /
-    // 121 us with 2 / 3 / 4 ranges). Not inside a capture that would need a
-    // larger workspace. KVRT_PF_KSPLIT=1 turns it off, n >= 2 forces n ranges.
+    // 121 us with 2 / 3 / 4 ranges). Not where that needs a larger workspace
+    // than there is and can be. KVRT_PF_KSPLIT=1 turns it off, n >= 2 forces n ranges.
     a.n_ksplit = 1;
     const int64_t want = ksplit_env > 0 ? ksplit_env : std::min<int64_t>(256 / wgs(rw), block_keys / min_keys);
     const int nks = (int)std::min<int64_t>(want, 16);
     if (nks > 1 && !a.short_heads && (ksplit_env > 0 || block_keys * (nks - 1) / nks >= split_keys)) {
         const size_t po = ((size_t)n * hq * qn * nks * D + 63) / 64 * 64;
         const size_t bytes = po * 4 + (size_t)n * hq * qn * nks * 8 + 256;
-        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-        const bool capturing = hipStreamIsCapturing(c->stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
-        if (bytes <= c->ws_bytes || (!capturing && ensure_workspace(c, bytes) == KVRT_OK)) {
+        if (bytes <= c->ws_bytes || grow_workspace(c, bytes)) {
             a.n_ksplit = nks;
             a.part_o = c->ws;
             a.part_ml = reinterpret_cast<float2 *>(c->ws + po);
         }
-        if (c->poisoned) return KVRT_EDEVICE;
     }
     a.pmask = launch_masks(c, n, slots);
     a.scale_log2 = scale * 1.4426950408889634f;
@@ -2462,81 +2345,45 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
     a.prefix_slot = prefix_slot;
     for (int i = 0; i < n; ++i) a.slots[i] = slots[i];
     a.large = (all_own + pre_keys) * hkv * D * 4 > (int64_t)128 << 20;
-    // the prefix's keys once for the rows of all items, or for each item with its own keys
-    // (also where no row sees the prefix now: a replay may find it otherwise)
-    double time = shared_plan(a, D, pre_keys, own_keys, shared);
-    if (shared && pre_keys > 0) {
-        SharedArgs apart = a;
-        const double t = shared_plan(apart, D, pre_keys, own_keys, false);
-        if (t < time) a = apart, time = t;
-    }
-    // Or, without masks, on the prefill's tiles: 32 rows a wave, as chunks have them. us a call,
-    // joined / apart / on the prefill's tiles, prefix 4096 and 100 rows each, by rows of an
-    // item and KV head: 16 items, 8 KV heads of 128: 1 row 48 / 12 / 28, 16 49 / 27 / 29, 64
-    // 61 / 54 / 43, 256 142 / 192 / 112; 4 items, one KV head of 512: 1 row 16 / 18 / 27, 128
-    // 38 / 35 / 41, 512 65 / 74 / 57.
+    SharedChunkArgs p{};
+    p.kv = a.kv;
+    p.len = a.len;
+    p.q = a.q;
+    p.out = a.out;
+    p.err = a.err;
+    p.n_items = n;
+    p.group = a.group;
+    p.qn = a.qn;
+    p.window = window;
+    p.scale_log2 = a.scale;
+    p.prefix_slot = prefix_slot;
+    p.capacity = cap;
+    p.cap = a.cap;
+    p.inv_cap = a.inv_cap;
+    p.slopes = slopes;
+    for (int i = 0; i < n; ++i) p.slots[i] = slots[i];
     // (A ring holds a block of 32 keys; pages of 8 rows and fewer are the first kernel's, whose
     // 86 us for 4 x 512 queries behind 1400 rows are 99 where every row's page is looked up.)
-    if (!a.pmask && !(s.layout == KVRT_LAYOUT_RING && s.ring_rows < kPfKeys) &&
-        !(s.layout == KVRT_LAYOUT_PAGED && c->cfg.block_size < 16)) {
-        SharedChunkArgs p{};
-        p.kv = a.kv;
-        p.len = a.len;
-        p.q = a.q;
-        p.out = a.out;
-        p.err = a.err;
-        p.n_items = n;
-        p.group = a.group;
-        p.qn = a.qn;
-        p.window = window;
-        p.scale_log2 = a.scale;
-        p.prefix_slot = prefix_slot;
-        p.capacity = cap;
-        p.cap = a.cap;
-        p.inv_cap = a.inv_cap;
-        p.slopes = slopes;
-        for (int i = 0; i < n; ++i) p.slots[i] = slots[i];
-        int64_t keys = 0;  // most keys that the rows of a tile see
-        for (int i = 0; i < n; ++i) keys = std::max<int64_t>(keys, own_keys[i]);
-        keys += pre_keys;
-        if (window > 0) keys = std::min<int64_t>(keys, window + 15);
-        if (chunk_shape(p, D, keys, all_own + pre_keys) < time) {
-            const size_t parts = (size_t)n * hq * qn * p.n_ksplit, po = (parts * D + 63) / 64 * 64;
-            const size_t bytes = p.n_ksplit == 1 ? 0 : po * 4 + parts * 8 + 256;
-            if (bytes > c->ws_bytes) {
-                if (capturing) p.n_ksplit = 1;  // (a workspace that a capture cannot grow)
-                else if ((rc = ensure_workspace(c, bytes)) != KVRT_OK) return rc;
-            }
-            p.part_o = c->ws;
-            p.part_ml = reinterpret_cast<float2 *>(c->ws + po);
-            c->counters.launches += p.n_ksplit > 1 ? 2 : 1;
-            if (launch_shared_chunk(p, D, enq(c)) != hipSuccess) return poison(c);
-            const uint64_t tiles = (per_item + 32 * p.row_waves - 1) / (32 * p.row_waves);
-            const uint64_t read = ((uint64_t)pre_keys * n + all_own) * tiles * hkv;
-            c->counters.attended_keys += read;
-            c->counters.attended_bytes += read * (uint64_t)D * 2 * 2;
-            return KVRT_OK;
-        }
+    const bool tiles_ok = !a.pmask && !(s.layout == KVRT_LAYOUT_RING && s.ring_rows < kPfKeys) &&
+                          !(s.layout == KVRT_LAYOUT_PAGED && c->cfg.block_size < 16);
+    // A workspace that cannot grow (in a capture, or short of memory) takes the divisions that fit.
+    const size_t room = capturing ? c->ws_bytes : std::max(c->ws_bytes, kMaxSharedRoom);
+    bool tiles = plan_shared_call(a, p, D, tiles_ok, pre_keys, own_keys, room);
+    const auto bytes = [&] { return shared_part_bytes(n * hq * qn, tiles ? p.n_ksplit : a.parts, D); };
+    if (bytes() > c->ws_bytes && !grow_workspace(c, bytes()))
+        tiles = plan_shared_call(a, p, D, tiles_ok, pre_keys, own_keys, c->ws_bytes);
+    const int parts = tiles ? p.n_ksplit : a.parts;
+    a.part_o = p.part_o = c->ws;
+    a.part_ml = p.part_ml = reinterpret_cast<float2 *>(c->ws + (size_t)n * hq * qn * parts * D);
+    c->counters.launches += parts > 1 ? 2 : 1;
+    if ((tiles ? launch_shared_chunk(p, D, enq(c)) : launch_shared(a, D, enq(c))) != hipSuccess) return poison(c);
+    uint64_t keys;
+    if (tiles) {
+        keys = ((uint64_t)pre_keys * n + all_own) * ((per_item + 32 * p.row_waves - 1) / (32 * p.row_waves));
+    } else {
+        keys = (uint64_t)pre_keys * (a.joined ? n * a.own_tiles : a.pre_tiles) + (uint64_t)all_own * a.own_tiles;
     }
-    const auto bytes = [&] {
-        const size_t rows = (size_t)n * hq * qn * a.parts;
-        return a.parts == 1 ? 0 : rows * D * 4 + rows * 8 + 256;
-    };
-    if (bytes() > c->ws_bytes) {
-        // a workspace that a capture cannot grow: one walk per row tile, which needs none
-        if (capturing) {
-            a.joined = shared;
-            a.pre_tiles = 0, a.pre_splits = 0, a.own_per = 0, a.own_splits = 1, a.parts = 1;
-        } else if ((rc = ensure_workspace(c, bytes())) != KVRT_OK) {
-            return rc;
-        }
-    }
-    a.part_o = c->ws;
-    a.part_ml = reinterpret_cast<float2 *>(c->ws + (size_t)n * hq * qn * a.parts * D);
-    c->counters.launches += a.parts > 1 ? 2 : 1;
-    if (launch_shared(a, D, enq(c)) != hipSuccess) return poison(c);
-    const uint64_t keys = ((uint64_t)pre_keys * (a.joined ? n * a.own_tiles : a.pre_tiles) +
-                           (uint64_t)all_own * a.own_tiles) * hkv;
+    keys *= hkv;
     c->counters.attended_keys += keys;
     c->counters.attended_bytes += keys * (uint64_t)D * 2 * 2;
     return KVRT_OK;

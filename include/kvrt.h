@@ -592,8 +592,9 @@ int kvrt_attend_talker_async(kvrt_ctx *ctx, int32_t layer, int32_t n, const int3
  * log2 e), as is their quotient. prefix_slot is none of the slots; RING and PAGED
  * layers still hold the oldest keys seen of both, a RING layer's rows those of Q +
  * window - 1 positions (KVRT_ESTATE otherwise). A captured call replays on the
- * lengths it then finds; one whose partials do not fit the context's workspace is
- * captured in an undivided form (one eager call of the shape first sizes it).
+ * lengths it then finds. Partial results of up to 256 MB go to the context's
+ * workspace, which an eager call grows; a captured one, or one that finds no memory,
+ * is divided so that they fit (one eager call of the shape ahead of a capture sizes it).
  * The reference copies the prefix into each session (duplex_kernel/kv_cache.py:41-67)
  * and has no such call. */
 int kvrt_attend_shared_async(kvrt_ctx *ctx, int32_t layer, int32_t n, const int32_t *slots, int32_t prefix_slot,
