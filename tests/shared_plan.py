@@ -75,3 +75,48 @@ def plans(calls: list[dict]) -> list[dict] | None:
                                        c.get("room", 256 << 20), *c["own"]))))
     got = subprocess.run([str(exe)], input="\n".join(text) + "\n", capture_output=True, text=True, check=True)
     return [dict(zip(FIELDS, map(int, line.split()))) for line in got.stdout.splitlines()]
+
+
+def forms(c: dict, p: dict) -> set[tuple]:
+    """The kernels of a call and what they run as: ("chunk", d, layout, row waves, key parts,
+    split), ("unit", d, layout, 16-row blocks a wave, whose keys, past the caches) and ("join", d,
+    groups of a row's parts), as csrc/kvrt_shared_kernel.h and kvrt_shared_chunk.hip choose them."""
+    d, layout, n, rows = c["d"], c.get("layout", "contig"), len(c["own"]), c["hq"] // c["hkv"] * c["q"]
+    if p["tiles"]:
+        return {("chunk", d, layout, p["row_waves"], p["key_parts"], p["ranges"] > 1)}
+    tile = 128 if d <= 128 else 64
+    prefix = c.get("prefix") or 0
+    large = (sum(c["own"]) + prefix) * c["hkv"] * d * 4 > 128 << 20 and layout != "paged"
+
+    def blocks(total, tiles):
+        sizes = {min(total - tile * t, tile) for t in {0, tiles - 1}}
+        return {0 if s <= 16 else 1 if tile == 64 or s <= 64 else 2 for s in sizes}
+
+    got = set()
+    if p["pre_tiles"]:
+        got |= {("unit", d, layout, b, "prefix", large and p["pre_tiles"] == 1) for b in blocks(n * rows, p["pre_tiles"])}
+    whose = "both" if p["joined"] else "own"
+    got |= {("unit", d, layout, b, whose, large and p["own_tiles"] == 1 and not p["joined"]) for b in blocks(rows, p["own_tiles"])}
+    if p["parts"] > 1:
+        groups = 2 if d == 512 else 4 if d == 256 else 8
+        while groups > 1 and p["parts"] <= 8 * (groups // 2):
+            groups //= 2
+        got.add(("join", d, groups))
+    return got
+
+
+def every_form() -> set[tuple]:
+    """All that the kernels are compiled as (a chunk's key ranges and units past the caches apart)."""
+    out = set()
+    for d in (64, 128, 256, 512):
+        for layout in LAYOUTS:
+            shapes = [(4, 1)] + ([(2, 2)] if d <= 256 else []) + ([(2, 4)] if d <= 128 else [])
+            if d <= 128 and layout != "paged":
+                shapes.append((1, 4))
+            out |= {("chunk", d, layout, *s, split) for s in shapes for split in (False, True)}
+            for b in range(3 if d <= 128 else 2):
+                out |= {("unit", d, layout, b, whose, False) for whose in ("prefix", "own", "both")}
+                if layout != "paged":
+                    out |= {("unit", d, layout, b, whose, True) for whose in ("prefix", "own")}
+        out |= {("join", d, g) for g in (1, 2, 4, 8) if g <= (2 if d == 512 else 4 if d == 256 else 8)}
+    return out

@@ -12,13 +12,19 @@ BF16 = torch.bfloat16
 INF = float("inf")
 
 
-def _same_class(s, got, q, scale, *, shared=True, **kw):
+def same_class(s, got, q, scale, *, shared=True, masks=None, **kw):
+    """got against the reference: numbers within its tolerance, the same infinities, NaN for NaN."""
     qn = q.shape[2]
     for i in range(s.n):
         parts = ([s.n] if shared else []) + [i]
         keys, values = (torch.cat([x[j] for j in parts], 1) for x in (s.k, s.v))
         total = keys.shape[1]
-        want, tol = attend(q[i], keys, values, list(range(total - qn, total)), scale, window=s.window, **kw)
+        visible = torch.ones(total, dtype=torch.bool, device="cuda")
+        for j, at in zip(parts, (0, s.k[s.n].shape[1] if shared else 0)):
+            m = masks[j] if masks is not None else None
+            if m is not None:
+                visible[at:at + min(m.numel(), s.k[j].shape[1])] = m[:s.k[j].shape[1]]
+        want, tol = attend(q[i], keys, values, list(range(total - qn, total)), scale, window=s.window, visible=visible, **kw)
         x = got[i].double()
         number = want.isfinite()
         assert bool(((x - want).abs() <= tol)[number].all()), i
@@ -64,9 +70,9 @@ def test_a_seen_infinity_of_v_stays_one(lens, prefix, hq, hkv, d, layout, window
         s.load(i)
     q = torch.randn(s.n, hq, qn, d, generator=gen, device="cuda").to(BF16)
     got = s.rt.attend_shared(0, q, range(s.n), d ** -0.5, prefix_slot=s.n, softcap=cap)
-    _same_class(s, got, q, d ** -0.5, cap=cap)
+    same_class(s, got, q, d ** -0.5, cap=cap)
     got = s.rt.attend_shared(0, q, range(s.n), d ** -0.5, softcap=cap)
-    _same_class(s, got, q, d ** -0.5, shared=False, cap=cap)
+    same_class(s, got, q, d ** -0.5, shared=False, cap=cap)
     assert s.rt.health() == 0
 
 
@@ -82,5 +88,5 @@ def test_a_seen_infinity_of_k(lens, prefix, hq, hkv, d, layout, window, qn, cap)
         s.load(i)
     q = torch.randn(s.n, hq, qn, d, generator=gen, device="cuda").to(BF16)
     got = s.rt.attend_shared(0, q, range(s.n), d ** -0.5, prefix_slot=s.n, softcap=cap)
-    _same_class(s, got, q, d ** -0.5, cap=cap)
+    same_class(s, got, q, d ** -0.5, cap=cap)
     assert s.rt.health() == 0

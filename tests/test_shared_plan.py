@@ -5,7 +5,8 @@ import random
 
 import pytest
 
-from shared_plan import plans
+from shared_forms import SHAPES, call
+from shared_plan import every_form, forms, plans
 
 
 def _plans(calls):
@@ -44,3 +45,11 @@ def test_one_call_grows_the_workspace_to_a_quarter_of_a_gigabyte_at_most():
     calls = [dict(d=512, hkv=1, hq=8, q=q, own=[q + 3] * 4, prefix=1400) for q in range(16, 2049)]
     calls += [dict(d=512, hkv=8, hq=64, q=q, own=[32768] * 16, prefix=16384) for q in (1, 7, 100, 4096)]
     assert max(p["bytes"] for p in _plans(calls)) <= 256 << 20
+
+
+def test_the_gpu_tests_run_every_kernel():
+    """The model picks the kernel, so that a change of its constants moves what a shape covers:
+    tests/test_gpu_shared_forms.py then needs others for the forms named here."""
+    calls = [call(*s) for s in SHAPES]
+    ran = set().union(*(forms(c, p) for c, p in zip(calls, _plans(calls))))
+    assert ran == every_form(), sorted(map(str, every_form() - ran))
