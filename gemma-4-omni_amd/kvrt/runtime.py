@@ -46,6 +46,13 @@ def _check(code: int, where: str) -> None:
         raise KVRTError(code, where)
 
 
+def _int32(x: int) -> int:
+    """x as an index of the C interface: -2, which no layer or slot has, for one that 32 bits do
+    not hold (ctypes would pass its low word)."""
+    x = int(x)
+    return x if -2 ** 31 <= x < 2 ** 31 else -2
+
+
 # Descriptors are a pure function of (data pointer, dtype, shape, strides), so
 # they are cached on that key: a decode loop that reuses its buffers skips the
 # ctypes field writes (~3 us per tensor). The C side reads a descriptor
@@ -338,7 +345,7 @@ class KVRuntime:
         key = tuple(map(int, slots))
         hit = _SLOT_ARRAYS.get(key)
         if hit is None:
-            hit = ((ctypes.c_int32 * len(key))(*key), len(key))
+            hit = ((ctypes.c_int32 * len(key))(*map(_int32, key)), len(key))
             if len(_SLOT_ARRAYS) >= _DESC_CACHE_MAX:
                 _SLOT_ARRAYS.clear()
             _SLOT_ARRAYS[key] = hit
@@ -595,7 +602,7 @@ class KVRuntime:
         self._bind()
         arr, n = self._slots(slots)
         qd, od = tensor_desc(q), tensor_desc(out)
-        _check(self.lib.kvrt_attend_shared_async(self._ctx, layer, n, arr, prefix,
+        _check(self.lib.kvrt_attend_shared_async(self._ctx, _int32(layer), n, arr, _int32(prefix),
                                                  ctypes.byref(qd), ctypes.byref(od), float(scale), float(softcap),
                                                  None if slopes is None else slopes.data_ptr()),
                "kvrt_attend_shared_async")
