@@ -2297,7 +2297,9 @@ int kvrt_attend_shared_async(kvrt_ctx *c, int32_t layer, int32_t n, const int32_
     if (!std::isfinite(scale * kLog2e) || !(softcap >= 0.f) || !std::isfinite(softcap * kLog2e) ||
         reinterpret_cast<uintptr_t>(slopes) % 4 != 0)
         return KVRT_EINVAL;
-    if (softcap > 0.f && !std::isfinite(scale / softcap)) return KVRT_EINVAL;
+    // (the tanh's exponent takes 2 log2 e of the quotient; with one that overflows, a product of 0
+    // would be NaN)
+    if (softcap > 0.f && !std::isfinite(scale / softcap * (2.f * kLog2e))) return KVRT_EINVAL;
     const int P = shared ? c->len_at(prefix_slot, layer) : 0;
     const int window = s.window >= 2 * cap ? 0 : s.window;  // past every distance: none
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;

@@ -590,6 +590,8 @@ class KVRuntime:
                 raise ValueError(f"slopes must be a contiguous fp32 tensor of one slope per query head on {self.device}")
         if prefix_slot is not None and int(prefix_slot) < 0:
             raise ValueError(f"prefix_slot must be a slot or None, got {prefix_slot}")
+        if 0.0 < softcap <= 2.0 ** -150:
+            raise ValueError(f"softcap {softcap} is 0, no cap, in fp32")
         prefix = -1 if prefix_slot is None else int(prefix_slot)
         slots = slots if type(slots) in (list, tuple) else tuple(slots)
         o = torch.empty_like(q) if out is None else out

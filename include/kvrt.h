@@ -589,7 +589,7 @@ int kvrt_attend_talker_async(kvrt_ctx *ctx, int32_t layer, int32_t n, const int3
  * Scores, softmax and sums in fp32, weights in two bf16 terms (2^-17 relative). Any
  * 1 <= Q <= L_i, any Hq / kv_heads; bf16 layers of every layout; a capacity of at
  * most 2^29; n * Hq * Q <= 2^22; scale and softcap finite in log2 units (times
- * log2 e), as is their quotient. prefix_slot is none of the slots; RING and PAGED
+ * log2 e), as is twice their quotient. prefix_slot is none of the slots; RING and PAGED
  * layers still hold the oldest keys seen of both, a RING layer's rows those of Q +
  * window - 1 positions (KVRT_ESTATE otherwise). A captured call replays on the
  * lengths it then finds. Partial results of up to 256 MB go to the context's
