@@ -200,7 +200,7 @@ __device__ __forceinline__ void shared_row(const SharedChunkArgs &a, int item, i
     const int64_t orow = ((int64_t)item * hq + head) * a.qn + qr;
     const uint16_t *q = a.q + orow * D;
     const auto *kg = static_cast<const uint16_t *>(a.kv.k), *vg = static_cast<const uint16_t *>(a.kv.v);
-    const float slope = a.slopes ? a.slopes[head] * 1.4426950408889634f : 0.f;
+    const float slope = a.slopes ? log2_slope(a.slopes[head]) : 0.f;
     // element offset of key k's row, -1 where this row does not see it (or its page is unmapped)
     const auto at = [&](int k) __attribute__((always_inline)) -> int64_t {
         const bool own = k >= own0;
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
     float slope = 0.f;
     if constexpr (SHARED) {
         made = a.cap != 0.f || a.slopes;
-        if (a.slopes) slope = a.slopes[kvh * g + hr] * 1.4426950408889634f;
+        if (a.slopes) slope = log2_slope(a.slopes[kvh * g + hr]);
         asm volatile("" : "+v"(slope));  // loaded ahead of the first DMA
     }
 

@@ -195,7 +195,7 @@ __device__ __forceinline__ void row_again(const SharedUnit &u, int f, int dim0, 
         } else {
             t *= a.scale;
         }
-        if (a.slopes) t = fmaf(a.slopes[head] * 1.4426950408889634f, (float)(key - at), t);
+        if (a.slopes) t = fmaf(log2_slope(a.slopes[head]), (float)(key - at), t);
         const float p = off < 0 ? 0.f : __builtin_amdgcn_exp2f(t - m);
         const uint32_t some = (uint32_t)__ballot(off >= 0);
 #pragma clang loop unroll(disable)
@@ -259,7 +259,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
         const uint16_t *qp = a.q + (((int64_t)item * (a.kv.kv_heads * a.group) + head) * a.qn + qr) * D + 8 * grp;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) qop[s][c] = *reinterpret_cast<const uint4 *>(qp + 32 * c);
-        slope[s] = a.slopes ? a.slopes[head] * 1.4426950408889634f : 0.f;
+        slope[s] = a.slopes ? log2_slope(a.slopes[head]) : 0.f;
     }
     // masks of the two slots: length, and word `lane & 15`
     int plen_p = 0, plen_o = 0;

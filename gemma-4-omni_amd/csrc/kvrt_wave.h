@@ -184,6 +184,13 @@ __device__ __forceinline__ void cap_scores(T &x, float by, float cap) {
     }
 }
 
+// A head's slope in log2 units. A finite one stays finite: an infinity times the distance 0 of a
+// query's own key would be NaN.
+__device__ __forceinline__ float log2_slope(float s) {
+    const float x = s * 1.4426950408889634f;
+    return fabsf(x) == INFINITY && fabsf(s) != INFINITY ? copysignf(3.4028235e38f, x) : x;
+}
+
 // Sum of n elements of q times k (16-byte aligned rows, n a multiple of 32), for rows that are
 // made without matrix instructions.
 __device__ __forceinline__ float dot_rows(const uint16_t *q, const uint16_t *k, int n) {
