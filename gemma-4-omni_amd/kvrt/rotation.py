@@ -96,6 +96,7 @@ class HeadRotation:
         self._turns = torch.tensor([ctypes.c_int64(t).value for t in turns], dtype=torch.int64, device=self.device)
         self._axis = torch.tensor(which or [0], dtype=torch.uint8, device=self.device)
         self.q_weight, self.k_weight = copy(q_weight), copy(k_weight)
+        torch.cuda.current_stream(self.device).synchronize()  # (calls come on any stream)
         c = L.KvrtRotation()
         c.turns, c.axis = self._turns.data_ptr(), self._axis.data_ptr()
         c.q_weight, c.k_weight = (None if w is None else w.data_ptr() for w in (self.q_weight, self.k_weight))
