@@ -324,7 +324,8 @@ int kvrt_reset_slot_async(kvrt_ctx *ctx, int32_t slot);
 /* Per-slot prefix-attention mask: key position k < P is visible only where
  * mask[k] != 0; positions >= P are unaffected. Applies on every layer of the
  * slot, on top of causal and window visibility, in kvrt_attend_decode_async,
- * kvrt_append_attend_async and kvrt_attend_prefill_async. mask is a DEVICE
+ * kvrt_append_attend_async, kvrt_attend_prefill_async and kvrt_attend_shared_async
+ * (there of the prefix slot too). mask is a DEVICE
  * tensor [1, P] or [P] of KVRT_INT64 (the reference's dtype), KVRT_INT32 or
  * KVRT_BOOL, 0 <= P <= KVRT_MAX_PREFIX_MASK; NULL or P = 0 clears the mask.
  * It is read on the bound stream, so the caller keeps it alive until the
