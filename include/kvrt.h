@@ -593,7 +593,7 @@ int kvrt_attend_talker_async(kvrt_ctx *ctx, int32_t layer, int32_t n, const int3
  * log2 e), as is twice their quotient. prefix_slot is none of the slots; RING and PAGED
  * layers still hold the oldest keys seen of both, a RING layer's rows those of Q +
  * window - 1 positions (KVRT_ESTATE otherwise). A captured call replays on the
- * lengths it then finds. Partial results of up to 256 MB go to the context's
+ * lengths it then finds. Partial results of up to 1 GiB go to the context's
  * workspace, which an eager call grows; a captured one, or one that finds no memory,
  * is divided so that they fit (one eager call of the shape ahead of a capture sizes it).
  * The reference copies the prefix into each session (duplex_kernel/kv_cache.py:41-67)

@@ -72,7 +72,7 @@ def plans(calls: list[dict]) -> list[dict] | None:
         prefix = c.get("prefix")
         text.append(" ".join(map(str, (c["d"], c["hkv"], c["hq"] // c["hkv"], len(c["own"]), c["q"], LAYOUTS[c.get("layout", "contig")],
                                        c.get("window", 0), int(c.get("tiles", True)), -1 if prefix is None else prefix,
-                                       c.get("room", 256 << 20), *c["own"]))))
+                                       c.get("room", 1 << 30), *c["own"]))))
     got = subprocess.run([str(exe)], input="\n".join(text) + "\n", capture_output=True, text=True, check=True)
     return [dict(zip(FIELDS, map(int, line.split()))) for line in got.stdout.splitlines()]
 

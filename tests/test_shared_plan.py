@@ -41,10 +41,10 @@ def test_partials_take_no_more_than_the_room_there_is():
             assert not p["tiles"]
 
 
-def test_one_call_grows_the_workspace_to_a_quarter_of_a_gigabyte_at_most():
+def test_one_call_grows_the_workspace_to_a_gigabyte_at_most():
     calls = [dict(d=512, hkv=1, hq=8, q=q, own=[q + 3] * 4, prefix=1400) for q in range(16, 2049)]
     calls += [dict(d=512, hkv=8, hq=64, q=q, own=[32768] * 16, prefix=16384) for q in (1, 7, 100, 4096)]
-    assert max(p["bytes"] for p in _plans(calls)) <= 256 << 20
+    assert max(p["bytes"] for p in _plans(calls)) <= 1 << 30
 
 
 def test_the_gpu_tests_run_every_kernel():
