@@ -415,9 +415,9 @@ __global__ __launch_bounds__(64 * RW * KS) void prefill_kernel(std::conditional_
             if constexpr (LAYOUT == KVRT_LAYOUT_PAGED) {
                 // A block starts at a multiple of 32 in its slot (or has one row to read, a last
                 // one again) and a page holds 16 rows or more: the halves of a block lie in one
-                // page each, and a row's place is an addition (4 x 512 queries behind 1400 rows,
-                // head_dim 128: 66 us, 99 with every row's page looked up; 4 x 291, head_dim
-                // 512: 81 and 123).
+                // page each, and a row's place is an addition (kernel times under the profiler:
+                // 4 x 512 queries behind 1400 rows, head_dim 128 66 us, 99 with every row's
+                // page looked up; 4 x 291, head_dim 512 81 and 123).
                 f.first = max(0, kfirst - t0);
                 const int lo = page_row(a.kv, __builtin_amdgcn_readlane(pages, 0), kvh, 0);
                 const int hi = page_row(a.kv, __builtin_amdgcn_readlane(pages, a.kv.block_shift == 4 ? 1 : 0), kvh, 0);

@@ -6,10 +6,12 @@
 // the prefix first, so that the only new work of a block is whose slot it lies in, and, where
 // asked for, the scores' cap and bias. A tile that ends with NaN in a row whose scores are
 // numbers met NaN or infinities in V, and is computed again row by row.
-// Measured: 4 x 512 queries of 16 heads of 128 behind 1400 rows and 577 to 700 of their own 55
-// us, 545 TFLOP/s with P counted once (the tiles of kvrt_shared_kernel.h 75 and a join of 11;
-// the same chunk over prefixes cloned into each session 54); 2 x 291 capped ones over 2000 22
-// and a merge of 4.6. Bound by matrix and vector instructions that in part follow each other.
+// Measured: 4 x 512 queries of 16 heads of 128 behind 1400 rows and 577 to 700 of their own 52 us
+// a call, 575 TFLOP/s with P counted once (on the tiles of kvrt_shared_kernel.h, which calls with
+// masks take, 80); on pages 58; with an infinity in the prefix's V 4.7 ms. 2 x 291 capped ones
+// over 2000 24.5, not capped 20.3. The matrix cores work for 50 % of the waves' life and vector
+// instructions for 51 %: two waves on a SIMD that follow each other. The capped chunk has one
+// wave on a SIMD, 17 % matrix, 35 % vector instructions and 36 % waits.
 #include "kvrt_prefill.h"
 
 namespace kvrt {

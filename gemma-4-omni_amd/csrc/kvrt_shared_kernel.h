@@ -36,12 +36,17 @@
 // each of the 64 banks once, and every operand's address is one register (at head_dim 64
 // and 128 two, by kx) and a constant.
 //
-// What bounds it: with many sessions or keys the bytes (64 sessions, one row each, 8 KV heads
-// of 128, behind 4096 rows: 245 MB in 48.6 us, 5.0 TB/s, and 4.6 us of joins; 16 paged ones
-// behind 1024: 119 MB in 28 us, 4.2 TB/s; a copy of 1 GiB 5.1). With few, the chain of a
-// unit: launch, lengths, first bytes, 0.8 us a tile of 16 rows at head_dim 128 (2.4 of 64 rows
-// at 512, where a tile's reads from LDS last as long), and the join's launch (four sessions
-// behind 2048 rows: 7.1 + 3.6 us).
+// What bounds it (kernel times under the profiler): with many sessions or keys the bytes (64
+// sessions, one row each, 8 KV heads of 128, behind 4096 rows: 245 MB in 48.3 us, 5.1 TB/s, and
+// 4.6 us of joins; 16 paged ones behind 1024: 119 MB in 28.6 us, 4.2 TB/s; a copy of 1 GiB 5.1).
+// With few, the chain of a unit: launch, lengths, first bytes, 0.8 us a tile of 16 rows at
+// head_dim 128, and the join's launch (four sessions behind 2048 rows: 7.4 + 3.5 us). At 512 a
+// tile of 64 rows takes 2.4 us, with one wave on a SIMD: of a wave's life 13 % are matrix
+// instructions and 12 % vector ones, the LDS is busy for 14 to 19 %, 35 % pass in waits for
+// loads and LDS reads and 37 % between instructions.
+//
+// A unit whose V holds a seen infinity adds its rows up again one by one: 64 sessions behind
+// 4096 rows with one in the prefix 4.6 ms.
 #pragma once
 
 #include "kvrt_shared.h"

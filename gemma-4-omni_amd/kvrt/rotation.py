@@ -43,16 +43,19 @@ class HeadRotation:
     """Norms and position rotation of one layer's heads.
 
     ``inv_freq``: angular frequencies (radians a position), a multiple of 8 of them and
-    at most ``head_dim`` / 2 (none: nothing turns); a zero leaves its pair as it is.
+    at most ``head_dim`` / 2 (none: nothing turns); a zero leaves its pair as it is, times
+    ``scaling``.
     Pair f is dims (f, f + len(inv_freq)), with ``adjacent`` (2f, 2f + 1); dims past
     all pairs pass. ``axes``: for each frequency the axis (0 to 3) whose position turns
     it, in sections or alternating; default one axis. ``norm``: the kinds that are
     RMS-normed, "none", "qk" or "qkv", with ``eps`` in the root; ``q_weight``,
     ``k_weight`` [head_dim] multiply the normed heads (default ones; values have none).
-    ``scaling`` multiplies cosines and sines.
+    ``scaling`` multiplies cosines and sines. Dims that are neither normed nor turned leave
+    bit for bit.
 
-    Tables and weights are copied to ``device``; the copies ``q_weight`` and
-    ``k_weight`` (fp32, or None) may be written to in place.
+    Inference only: no gradient is recorded, of inputs that require one either. Tables and
+    weights are copied to ``device``; the copies ``q_weight`` and ``k_weight`` (fp32, or
+    None) may be written to in place.
     """
 
     def __init__(self, head_dim: int, inv_freq: Sequence[float] | torch.Tensor, *,

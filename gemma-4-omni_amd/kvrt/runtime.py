@@ -578,7 +578,8 @@ class KVRuntime:
         GPU) adds slopes[h] * (key - query position) to them. The prefix-attention masks
         of the prefix slot and of the slots hold. bf16 layers, decode steps and chunks.
         NaN and infinities in rows that a query does not see do not reach it; an infinity
-        in V that it sees stays one."""
+        in V that it sees stays one. Inference only: no gradient is recorded, of a q that
+        requires one either."""
         require_cuda(q, "q")
         for t, name in ((q, "q"), (out, "out")):
             if t is not None and t.device != self.device:

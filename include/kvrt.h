@@ -325,9 +325,9 @@ int kvrt_reset_slot_async(kvrt_ctx *ctx, int32_t slot);
  * mask[k] != 0; positions >= P are unaffected. Applies on every layer of the
  * slot, on top of causal and window visibility, in kvrt_attend_decode_async,
  * kvrt_append_attend_async, kvrt_attend_prefill_async and kvrt_attend_shared_async
- * (there of the prefix slot too). mask is a DEVICE
- * tensor [1, P] or [P] of KVRT_INT64 (the reference's dtype), KVRT_INT32 or
- * KVRT_BOOL, 0 <= P <= KVRT_MAX_PREFIX_MASK; NULL or P = 0 clears the mask.
+ * (there of the prefix slot too). mask is a DEVICE tensor [1, P] or [P] of
+ * KVRT_INT64 (the reference's dtype), KVRT_INT32 or KVRT_BOOL, 0 <= P <=
+ * KVRT_MAX_PREFIX_MASK; NULL or P = 0 clears the mask.
  * It is read on the bound stream, so the caller keeps it alive until the
  * call's work has run. Clones and copies carry the mask; kvrt_truncate
  * refuses lengths below P; kvrt_rollover_async keeps positions
@@ -587,7 +587,8 @@ int kvrt_attend_talker_async(kvrt_ctx *ctx, int32_t layer, int32_t n, const int3
  * zeros, and rows that a query does not see do not reach it whatever they hold.
  * An infinity in V that a query sees gives that infinity, or NaN beside one of the
  * other sign (one whose weight is below fp32's range may also be missed).
- * Scores, softmax and sums in fp32, weights in two bf16 terms (2^-17 relative). Any
+ * Scores, softmax and sums in fp32, weights in two bf16 terms (2^-17 relative); a
+ * score capped at up to 64 is off by up to softcap * 2^-22. Any
  * 1 <= Q <= L_i, any Hq / kv_heads; bf16 layers of every layout; a capacity of at
  * most 2^29; n * Hq * Q <= 2^22; scale and softcap finite in log2 units (times
  * log2 e), as is twice their quotient. prefix_slot is none of the slots; RING and PAGED
@@ -815,12 +816,15 @@ int kvrt_rotation_turns(const double *inv_freq, int32_t n, uint64_t *turns);
  *   y = x * weight / sqrt(mean(x^2) + eps)              where the kind is normed
  *   (y_a, y_b) -> (y_a c - y_b s, y_b c + y_a s)        query and key heads, n_freq pairs
  * with c, s = scaling * (cos, sin)(position * inv_freq), all in fp32, rounded to bf16
- * once; value heads have no weight and do not turn. positions: device KVRT_INT32 or
+ * once; value heads have no weight and do not turn. What is neither normed nor turned
+ * (value heads, dims from 2 n_freq on) leaves bit for bit. Sines and cosines err by up to
+ * 2^-21 absolute, at positions up to 2^31. positions: device KVRT_INT32 or
  * KVRT_INT64 [n_axes, n, Q], any strides, values within int32 (an int64's low word is
  * taken); not read where n_freq is 0. An output may be its input itself, otherwise
- * outputs share no memory with inputs or each other. Context-free: runs on the current device and the given stream, allocates
- * nothing, returns KVRT_EINVAL (nothing enqueued) for arguments it does not take and
- * KVRT_EDEVICE when the launch fails.
+ * outputs share no memory with inputs or each other. Context-free: runs on the
+ * current device and the given stream, allocates nothing, returns KVRT_EINVAL
+ * (nothing enqueued) for arguments it does not take and KVRT_EDEVICE when the launch
+ * fails.
  * Replaces the listener's and talker's norm and rotation launches of each layer
  * (kernel_rmsnorm_bf16 and kernel_rope_bf16,
  * native/gemma4_listener_microbatch/gemma4_listener_kernels.cuh:145-500; the
