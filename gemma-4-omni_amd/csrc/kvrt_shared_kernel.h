@@ -157,9 +157,10 @@ struct SharedUnit {
 // number, 2^(score - m); those that are not numbers are stored. Keys over lanes and halves of the
 // dims over halves of the wave for the scores; dims over lanes for the values. The arguments are
 // read again here, so that the loop over the tiles holds no registers for a row that may never
-// come.
+// come. kept: the unit's queries, where answers have taken their place in memory.
 template <int D, int LAYOUT, int DIMS>
-__device__ __forceinline__ void row_again(const SharedUnit &u, int f, int dim0, float m, float sum, int lane) {
+__device__ __forceinline__ void row_again(const SharedUnit &u, const uint16_t *kept, int f, int dim0, float m, float sum,
+                                          int lane) {
     constexpr int E = (DIMS + 63) / 64;  // dims per lane
     uint64_t args = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
     asm volatile("" : "+s"(args));
@@ -179,6 +180,7 @@ __device__ __forceinline__ void row_again(const SharedUnit &u, int f, int dim0, 
     const int64_t row = ((int64_t)item * (a.kv.kv_heads * a.group) + head) * a.qn + qr;
     const auto *kg = static_cast<const uint16_t *>(a.kv.k), *vg = static_cast<const uint16_t *>(a.kv.v);
     const int half = D / 2 * (lane >> 5);
+    const uint16_t *q = a.parts == 1 && a.out == a.q ? kept + (f - u.row0) * D : a.q + row * D;
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
@@ -192,7 +194,7 @@ __device__ __forceinline__ void row_again(const SharedUnit &u, int f, int dim0, 
         bool seen = key >= lo && key <= min(at, last) && (a.window == 0 || key > at - a.window);
         if (a.pmask && key < a.pmask[slot].len) seen &= (a.pmask[slot].bits[(key >> 5) & (kPrefixWords - 1)] >> (key & 31) & 1u) != 0;
         const int64_t off = seen ? row_offset<LAYOUT>(kv, slot, u.kvh, key, D) : -1;  // (-1: its page is not mapped)
-        float t = pair<OpSum, 32>(dot_rows(a.q + row * D + half, kg + (off < 0 ? 0 : off) + half, D / 2));
+        float t = pair<OpSum, 32>(dot_rows(q + half, kg + (off < 0 ? 0 : off) + half, D / 2));
         if (a.cap != 0.f) {
             float one[1] = {t};
             cap_scores<1>(one, a.inv_cap, a.cap);
@@ -227,7 +229,7 @@ __device__ __forceinline__ void row_again(const SharedUnit &u, int f, int dim0, 
 // they are computed and not stored: a branch would part the matrix instructions); 0: the
 // unit has one, which all waves share.
 template <int D, int LAYOUT, int BLOCKS>
-__device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUnit &u, uint8_t *lds) {
+__device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUnit &u, uint8_t *lds, int *again) {
     using S = SharedShape<D>;
     constexpr bool WIDE = BLOCKS > 0;
     constexpr int RS = WIDE ? BLOCKS : 1;
@@ -569,11 +571,44 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
         }
     }
     if (bad) a.err[0] = 1;
+    // A seen infinity times a weight's two terms is NaN where the low one is 0 or below (inf * 0,
+    // inf - inf), and the infinity by definition. Outputs that are not numbers, of rows whose
+    // scores are, are added up again with whole weights and stored over. The rows of block s:
+    auto odd_rows = [&](int s) __attribute__((always_inline)) {
+        float none[4] = {};  // one NaN where an output is no number
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) none[i] = fmaf(o[s][b][i], 0.f, none[i]);
+        none[0] += none[1] + (none[2] + none[3]);
+        const uint64_t odd = __ballot(none[0] != none[0] && l[s] == l[s]);
+        const int left = u.nrows - 16 * (WIDE ? wave + 4 * s : 0);
+        return (uint32_t)(odd | odd >> 16 | odd >> 32 | odd >> 48) & (left >= 16 ? 0xffffu : (1u << max(left, 0)) - 1u);
+    };
+#pragma unroll
+    for (int s = 0; s < RS; ++s) l[s] = pair<OpSum, 32>(pair<OpSum, 16>(l[s]));
+    if (a.parts == 1 && a.out == a.q) {  // (the same for all units: answers go where the queries are)
+        uint32_t odd = 0;
+#pragma unroll
+        for (int s = 0; s < RS; ++s) odd |= odd_rows(s);
+        if (odd != 0) *again = 1;
+        __syncthreads();  // (and every wave has read its last tile)
+        if (*again != 0) {
+            for (int i = 8 * threadIdx.x; i < u.nrows * D; i += 8 * 256) {
+                int item, rem, qr, hr;
+                udivmod_uniform(u.row0 + i / D, per_item, item, rem);
+                udivmod_uniform(rem, a.group, qr, hr);
+                const uint16_t *from =
+                    a.q + (((int64_t)item * (a.kv.kv_heads * a.group) + u.kvh * a.group + hr) * a.qn + qr) * D + i % D;
+                *reinterpret_cast<uint4 *>(lds + 2 * i) = *reinterpret_cast<const uint4 *>(from);
+            }
+            __syncthreads();
+        }
+    }
 #pragma unroll
     for (int s = 0; s < RS; ++s) {
         const int r = 16 * (WIDE ? wave + 4 * s : 0) + col;
-        const float sum = pair<OpSum, 32>(pair<OpSum, 16>(l[s]));
-        l[s] = sum;
+        const float sum = l[s];
         if (r >= u.nrows) continue;
         const int f = u.row0 + r;
         if (a.parts == 1) {
@@ -596,26 +631,15 @@ __device__ __forceinline__ void shared_unit(const SharedArgs &a, const SharedUni
             if (grp == 0 && b0 == 0) a.part_ml[at] = make_float2(m[s], sum);
         }
     }
-    // A seen infinity times a weight's two terms is NaN where the low one is 0 or below (inf * 0,
-    // inf - inf), and the infinity by definition. Outputs that are not numbers, of rows whose
-    // scores are, are added up again with whole weights and stored over.
 #pragma unroll
     for (int s = 0; s < RS; ++s) {
-        float none[4] = {};  // one NaN where an output is no number
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) none[i] = fmaf(o[s][b][i], 0.f, none[i]);
-        none[0] += none[1] + (none[2] + none[3]);
-        const uint64_t odd = __ballot(none[0] != none[0] && l[s] == l[s]);
-        if (__builtin_expect_with_probability(odd == 0, 1, 0.9999)) continue;
-        const int row0 = 16 * (WIDE ? wave + 4 * s : 0);
-        uint32_t left = (uint32_t)(odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xffffu;  // rows of the block
-        left &= u.nrows - row0 >= 16 ? 0xffffu : (1u << max(u.nrows - row0, 0)) - 1u;
+        uint32_t left = odd_rows(s);
+        if (__builtin_expect_with_probability(left == 0, 1, 0.9999)) continue;
         wait_vmem<0>();  // the rows' first answers are stored
         for (; left != 0; left &= left - 1) {
             const int c = __builtin_ctz(left);
-            row_again<D, LAYOUT, 16 * NB>(u, u.row0 + row0 + c, 16 * b0, __shfl(m[s], c), __shfl(l[s], c), lane);
+            row_again<D, LAYOUT, 16 * NB>(u, reinterpret_cast<const uint16_t *>(lds), u.row0 + 16 * (WIDE ? wave + 4 * s : 0) + c,
+                                          16 * b0, __shfl(m[s], c), __shfl(l[s], c), lane);
         }
     }
 }
@@ -625,6 +649,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void shared_at
     using S = SharedShape<D>;
     constexpr int TILE = shared_tile(D);
     __shared__ __align__(16) uint8_t lds[S::STAGES * S::STAGE];
+    __shared__ int again;  // rows are added up again
+    static_assert(TILE * D * 2 <= S::STAGES * S::STAGE, "a unit's queries fit the stages");
+    if (threadIdx.x == 0) again = 0;
     const int lane = threadIdx.x & 63;
     const int hkv = a.kv.kv_heads, per_item = a.group * a.qn;
     const int capacity = a.capacity;
@@ -708,9 +735,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void shared_at
     const int tiles = u.pre.tiles + u.own.tiles, per = (tiles + splits - 1) / splits;
     u.x0 = min(ks * per, tiles);
     u.x1 = min(u.x0 + per, tiles);
-    if (u.nrows <= 16) shared_unit<D, LAYOUT, 0>(a, u, lds);
-    else if (TILE == 64 || u.nrows <= 64) shared_unit<D, LAYOUT, 1>(a, u, lds);
-    else shared_unit<D, LAYOUT, TILE / 64>(a, u, lds);
+    if (u.nrows <= 16) shared_unit<D, LAYOUT, 0>(a, u, lds, &again);
+    else if (TILE == 64 || u.nrows <= 64) shared_unit<D, LAYOUT, 1>(a, u, lds, &again);
+    else shared_unit<D, LAYOUT, TILE / 64>(a, u, lds, &again);
 }
 
 // Joins the partials of every row. A row's parts are dealt to GROUPS groups of D / 4

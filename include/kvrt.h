@@ -586,7 +586,8 @@ int kvrt_attend_talker_async(kvrt_ctx *ctx, int32_t layer, int32_t n, const int3
  * prefix_slot and of the slots on their own rows); a row that sees no key becomes
  * zeros, and rows that a query does not see do not reach it whatever they hold.
  * An infinity in V that a query sees gives that infinity, or NaN beside one of the
- * other sign (one whose weight is below fp32's range may also be missed).
+ * other sign (one whose weight is below fp32's range may also be missed). out may be q
+ * itself, and otherwise shares no memory with it.
  * Scores, softmax and sums in fp32, weights in two bf16 terms (2^-17 relative); a
  * score capped at up to 64 is off by up to softcap * 2^-22. Any
  * 1 <= Q <= L_i, any Hq / kv_heads; bf16 layers of every layout; a capacity of at

@@ -15,14 +15,13 @@ PROGRAM = r"""
 using namespace kvrt;
 int main() {
     int D, hkv, group, n, q, layout, window, tiles_ok;
-    long long pre, room, own[64], x;
+    long long pre, room, x;
     while (std::scanf("%d %d %d %d %d %d %d %d %lld %lld", &D, &hkv, &group, &n, &q, &layout, &window, &tiles_ok, &pre, &room) == 10) {
         int64_t rows[64];
         for (int i = 0; i < n; ++i) {
             if (std::scanf("%lld", &x) != 1) return 1;
             rows[i] = x;
         }
-        (void)own;
         SharedArgs a{};
         SharedChunkArgs p{};
         a.kv.kv_heads = p.kv.kv_heads = hkv;
@@ -44,16 +43,18 @@ FIELDS = ("tiles", "row_waves", "key_parts", "ranges", "joined", "pre_tiles", "p
           "own_per", "own_wgs", "parts", "bytes")
 
 _exe: Path | None = None
+_dir: tempfile.TemporaryDirectory | None = None  # (gone with the process)
 
 
 def _program() -> Path | None:
     """The compiled program, once a process; None without a host compiler or HIP's headers."""
-    global _exe
+    global _exe, _dir
     if _exe is None:
         gxx = shutil.which("g++")
         if gxx is None or not Path("/opt/rocm/include/hip/hip_runtime.h").exists():
             return None
-        where = Path(tempfile.mkdtemp(prefix="kvrt_plan_"))
+        _dir = tempfile.TemporaryDirectory(prefix="kvrt_plan_")
+        where = Path(_dir.name)
         (where / "plan.cpp").write_text(PROGRAM)
         subprocess.run([gxx, "-std=c++17", "-O2", "-w", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", f"-I{ROOT / 'include'}",
                         f"-I{ROOT / 'gemma-4-omni_amd' / 'csrc'}", str(where / "plan.cpp"), "-o", str(where / "plan")], check=True)

@@ -63,4 +63,8 @@ def test_infinities_in_every_kernel(shape):
     q = torch.randn(n, hq, qn, d, generator=gen, device="cuda").to(BF16)
     got = s.rt.attend_shared(0, q, range(n), d ** -0.5, prefix_slot=None if prefix is None else n)
     same_class(s, got, q, d ** -0.5, shared=prefix is not None, masks=masks)
+    # the answer in the queries' place
+    place = q.clone()
+    again = s.rt.attend_shared(0, place, range(n), d ** -0.5, prefix_slot=None if prefix is None else n, out=place)
+    assert again is place and torch.equal(place.view(torch.int16), got.view(torch.int16))
     assert s.rt.health() == 0
